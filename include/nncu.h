@@ -370,6 +370,160 @@ int nncu_logits_batch_dev(const nncu_weight* lm_head, const float* hidden, int32
  * first place is the answer. Device pointers, asynchronous on `stream`. */
 int nncu_argmax_rows_dev(const float* x, size_t x_stride, int32_t n_rows, uint32_t n, int32_t* out, void* stream);
 
+/* ---- serving from a paged cache held in 4 bits ------------------------------
+ * No counterpart in libnnc, which serves one sequence from one contiguous
+ * cache: these serve many requests of different lengths from one pool of
+ * pages. A step of a layer is, in order: nncu_paged_step_dev (once a step),
+ * the projections (the gemvs above), nncu_rope_axes_dev, nncu_kv4_append_dev,
+ * nncu_kv4_attention_dev. The requests' tokens lie one after another in q, k,
+ * v and out (request r's from q_start[r]). Every array is a device pointer,
+ * every call asynchronous on `stream` and without allocation; lengths, tables
+ * and slots are read on the device only, so a captured graph replays them.
+ * The calls are described by structs that a caller fills once and keeps. */
+
+/* The tables of one step, built on the GPU from the requests' lengths.
+ *
+ * In: request r holds `held[r]` pages (block_table[r][0 .. held[r])), has
+ * past[r] tokens in the cache and gets n_new[r] more; n_new[r] < 0 ends it and
+ * gives its pages back. The free pages are ring[(head + i) % n_pages], i <
+ * count, with queue = {head, count}.
+ *
+ * Requests take the pages they lack, ceil((past + n_new) / page_size) - held,
+ * from the ring's head in their order. One that would pass max_blocks pages,
+ * whose tokens would pass max_tok, or for which (with all requests before it)
+ * the ring does not suffice is not served: it keeps its pages, its length
+ * stays, its tokens have no slot. Ended requests' pages join the ring's tail.
+ *
+ * Out: held_out[n_req], queue_out[4] = {head, count, pages that were missing,
+ * tokens of the step}, new entries of block_table (others stay as they are),
+ * seq_len[n_req] (past + n_new; past where not served; 0 where ended),
+ * q_start[n_req + 1], and for every place t of the token buffer positions[t]
+ * (0 past the end), slots[t] = page * page_size + position % page_size (-1: no
+ * slot) and token_req[t] (-1 past the end). held_out and queue_out must not be
+ * held and queue (a caller swaps the two from step to step). */
+#define NNCU_PAGED_MAX_REQ 8192
+typedef struct nncu_paged_step
+{
+	int32_t n_req, page_size, n_pages, max_blocks, max_tok;
+	int32_t table_stride; /* entries between two requests' rows of block_table */
+	const int32_t* past;
+	const int32_t* n_new;
+	const int32_t* held;
+	const int32_t* queue;
+	int32_t* ring;
+	int32_t* block_table;
+	int32_t* held_out;
+	int32_t* queue_out;
+	int32_t* seq_len;
+	int32_t* q_start;
+	int32_t* positions;
+	int32_t* slots;
+	int32_t* token_req;
+} nncu_paged_step;
+int nncu_paged_step_dev(const nncu_paged_step* s, void* stream);
+
+/* Per-head RMS norm (where a gain is given) and rotation of the packed tokens'
+ * q and k rows, every token at a position of its own, with one to four
+ * position axes (text: one; images and video: time, height, width).
+ * positions[a * pos_stride + t] is axis a's position of token t; pair i of the
+ * n_rot / 2 pairs turns by the float product positions * inv_freq[i] of its
+ * axis. section[a] pairs belong to axis a: one axis's after the other's, or
+ * with `interleaved` in turn (pair i to axis i % n_axes while i / n_axes <
+ * section[i % n_axes], otherwise to axis 0). NNCU_ROPE_NEOX pairs i and i +
+ * n_rot / 2, NNCU_ROPE_NORM 2i and 2i + 1; values past n_rot are only normed.
+ * Rows are n_head * head_dim (n_kv * head_dim) floats, strides in floats. The
+ * output may be the input. k (and k_out) NULL: q only, or the reverse. */
+typedef struct nncu_rope_axes
+{
+	int32_t n_tok, n_head, n_kv, head_dim, n_rot, rope_mode;
+	int32_t n_axes, interleaved;
+	int32_t section[4];
+	float eps;
+	const int32_t* positions;
+	size_t pos_stride;
+	const float* inv_freq; /* n_rot / 2 */
+	const float* q_gamma;  /* head_dim, or NULL: no norm */
+	const float* k_gamma;
+	const float* q;
+	const float* k;
+	float* q_out;
+	float* k_out;
+	size_t q_stride, k_stride, q_out_stride, k_out_stride;
+} nncu_rope_axes;
+int nncu_rope_axes_dev(const nncu_rope_axes* r, void* stream);
+
+/* One layer's pool of pages, 16-byte aligned, nncu_kv4_bytes long. A chunk
+ * [page][KV head] holds page_size keys: K codes, V codes (page_size * head_dim
+ * / 2 bytes each), K scales, V scales (bf16, head_dim / 32 a key). Values come
+ * in groups of 32 with one scale s: value = s * code, code -8 .. 7. s is the
+ * value of largest magnitude, with its sign, over -8, rounded to bf16, its
+ * magnitude held between 2^-17 and 2^11 (larger values saturate); the code is
+ * rint(x * (1 / s)), clamped. Eight bits of s times a code are exact in
+ * 16-bit floats. A group with a NaN or an infinity reads as NaN.
+ * A key's codes are head_dim / 32 units of 16 bytes, group g of the key at
+ * offset k of its page in unit g ^ ((k * head_dim / 256) % (head_dim / 32)).
+ * Word w of a unit has values 8w .. 8w + 7, nibble n (from the low end) the
+ * value 8w + 2 (n % 4) + n / 4, as code + 8. */
+typedef struct nncu_kv4_pool
+{
+	void* pages;
+	int32_t n_pages;
+	int32_t page_size; /* 16, 32, 64, 128 or 256 keys */
+	int32_t n_kv;
+	int32_t head_dim;  /* 64, 128 or 256 */
+} nncu_kv4_pool;
+int nncu_kv4_bytes(const nncu_kv4_pool* pool, size_t* bytes);
+
+/* Rows of n_tok tokens: k and v [n_tok][n_kv * head_dim] floats, strides in
+ * floats, token t's at slots[t]. A negative slot (or one outside the pool) is
+ * skipped by the append; reading it gives zeros. Slots of one append differ.
+ * k or v NULL: the other only. */
+typedef struct nncu_kv4_rows
+{
+	nncu_kv4_pool pool;
+	int32_t n_tok;
+	const int32_t* slots;
+	float* k; /* read by the append, written by the read */
+	float* v;
+	size_t k_stride, v_stride;
+} nncu_kv4_rows;
+int nncu_kv4_append_dev(const nncu_kv4_rows* rows, void* stream);
+int nncu_kv4_read_dev(const nncu_kv4_rows* rows, void* stream);
+
+/* Causal attention of the packed tokens over the pool: request r's new tokens
+ * q_start[r] .. q_start[r + 1) are the last of its seq_len[r] keys (appended
+ * before this call), so token t of n sits at position seq_len - n + t and sees
+ * the keys up to itself, `window` at most (0: all). scale, softcap as in
+ * nncu_attn_params. Query head h reads KV head h / (n_head / n_kv); rows are
+ * n_head * head_dim floats, strides in floats. A token that sees no key gets
+ * zeros; keys on pages outside the pool are not seen. max_new bounds the new
+ * tokens of one request and n_tok their sum: tokens past either are left out
+ * (their output rows are not written). What a request that
+ * nncu_paged_step_dev did not serve gets is of no use: its tokens are not in
+ * the cache.
+ *
+ * The workspace (nncu_kv4_workspace_bytes of the same struct) is cleared by
+ * the caller once; a call leaves it ready for the next. Calls that may
+ * overlap need one each. */
+typedef struct nncu_kv4_attn
+{
+	nncu_kv4_pool pool;
+	int32_t n_req, n_tok, n_head, max_new, max_blocks, window;
+	float scale, softcap;
+	const int32_t* block_table; /* [n_req], table_stride entries apart */
+	size_t table_stride;
+	const int32_t* seq_len;
+	const int32_t* q_start; /* n_req + 1 */
+	const float* q;
+	size_t q_stride;
+	float* out;
+	size_t out_stride;
+	void* workspace;
+	size_t workspace_bytes;
+} nncu_kv4_attn;
+int nncu_kv4_workspace_bytes(const nncu_kv4_attn* a, size_t* bytes);
+int nncu_kv4_attention_dev(const nncu_kv4_attn* a, void* stream);
+
 /* One layer's decode / verify attention that allocates nothing: the same
  * K1 + K2 kernels as nncu_attention_batch_dev for one job, with every buffer
  * the caller's. No counterpart in the reference, whose CPU path never

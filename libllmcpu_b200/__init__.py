@@ -34,7 +34,9 @@ __all__ = [
     "attn_block_dev", "attn_merge_dev", "attn_finish_dev", "rmsnorm_gamma_multi_dev", "rmsnorm_dev",
     "rope_dev", "softcap_dev", "gemv_bf16w_dev", "gemv_q8_0_dev", "gemv_q4_s_dev", "block_sums_dev",
     "gemv_bf16w_argmax_dev", "Weight", "AttnWeights", "weight", "W_BF16", "W_Q8_0", "W_Q4_S", "logits_batch_dev",
-    "argmax_rows_dev", "EXPORTS",
+    "argmax_rows_dev", "PagedStep", "paged_step", "paged_step_dev", "RopeAxes", "rope_axes", "rope_axes_dev",
+    "Kv4Pool", "kv4_pool", "kv4_bytes", "Kv4Rows", "kv4_rows", "kv4_append_dev", "kv4_read_dev", "Kv4Attn",
+    "kv4_attn", "kv4_workspace_bytes", "kv4_attention_dev", "EXPORTS",
 ]
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -62,7 +64,8 @@ EXPORTS = [
     "nncu_gemv_bf16w_f32x_batch_dev", "nncu_gemv_q8_0_f32x_batch_dev", "nncu_gemv_q4_s_f32x_batch_dev",
     "nncu_block_sums_dev", "nncu_gemv_bf16w_argmax_dev", "nncu_attention_forward_dev", "nncu_logits_batch_dev",
     "nncu_attention_forward_batch_dev",
-    "nncu_argmax_rows_dev",
+    "nncu_argmax_rows_dev", "nncu_paged_step_dev", "nncu_rope_axes_dev", "nncu_kv4_bytes", "nncu_kv4_append_dev",
+    "nncu_kv4_read_dev", "nncu_kv4_workspace_bytes", "nncu_kv4_attention_dev",
 ]
 GROUP_HANDLE_BYTES = 64
 
@@ -130,6 +133,48 @@ class KVLayerInfo(C.Structure):
 class KVState(C.Structure):
     _fields_ = [("cur_pos", C.c_int32), ("kv_written", C.c_int32), ("max_rewind", C.c_int32),
                 ("n_ctx", C.c_int32), ("bytes", C.c_size_t)]
+
+
+class PagedStep(C.Structure):
+    """nncu_paged_step (include/nncu.h): one step's tables from the requests' lengths."""
+
+    _fields_ = [(n, C.c_int32) for n in ("n_req", "page_size", "n_pages", "max_blocks", "max_tok", "table_stride")] + \
+               [(n, C.c_void_p) for n in ("past", "n_new", "held", "queue", "ring", "block_table", "held_out",
+                                          "queue_out", "seq_len", "q_start", "positions", "slots", "token_req")]
+
+
+class RopeAxes(C.Structure):
+    """nncu_rope_axes (include/nncu.h): per-head norm and rotation by per-token positions."""
+
+    _fields_ = [(n, C.c_int32) for n in ("n_tok", "n_head", "n_kv", "head_dim", "n_rot", "rope_mode", "n_axes",
+                                         "interleaved")] + \
+               [("section", C.c_int32 * 4), ("eps", C.c_float), ("positions", C.c_void_p), ("pos_stride", C.c_size_t)] + \
+               [(n, C.c_void_p) for n in ("inv_freq", "q_gamma", "k_gamma", "q", "k", "q_out", "k_out")] + \
+               [(n, C.c_size_t) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")]
+
+
+class Kv4Pool(C.Structure):
+    """nncu_kv4_pool (include/nncu.h): one layer's pages of 4-bit keys and values."""
+
+    _fields_ = [("pages", C.c_void_p)] + [(n, C.c_int32) for n in ("n_pages", "page_size", "n_kv", "head_dim")]
+
+
+class Kv4Rows(C.Structure):
+    """nncu_kv4_rows (include/nncu.h): rows to append to the pool or to read from it."""
+
+    _fields_ = [("pool", Kv4Pool), ("n_tok", C.c_int32), ("slots", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_stride", C.c_size_t), ("v_stride", C.c_size_t)]
+
+
+class Kv4Attn(C.Structure):
+    """nncu_kv4_attn (include/nncu.h): packed requests' attention over the pool."""
+
+    _fields_ = [("pool", Kv4Pool)] + \
+               [(n, C.c_int32) for n in ("n_req", "n_tok", "n_head", "max_new", "max_blocks", "window")] + \
+               [("scale", C.c_float), ("softcap", C.c_float), ("block_table", C.c_void_p),
+                ("table_stride", C.c_size_t), ("seq_len", C.c_void_p), ("q_start", C.c_void_p), ("q", C.c_void_p),
+                ("q_stride", C.c_size_t), ("out", C.c_void_p), ("out_stride", C.c_size_t),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class PerfPhase(C.Structure):
@@ -229,6 +274,13 @@ def lib() -> C.CDLL:
     L.nncu_attention_forward_batch_dev.argtypes = [vp, i32, i32, vp, C.POINTER(AttnParams), C.POINTER(AttnWeights),
                                                    vp, vp, vp]
     L.nncu_argmax_rows_dev.argtypes = [vp, sz, i32, C.c_uint32, vp, vp]
+    L.nncu_paged_step_dev.argtypes = [C.POINTER(PagedStep), vp]
+    L.nncu_rope_axes_dev.argtypes = [C.POINTER(RopeAxes), vp]
+    L.nncu_kv4_bytes.argtypes = [C.POINTER(Kv4Pool), C.POINTER(sz)]
+    L.nncu_kv4_append_dev.argtypes = [C.POINTER(Kv4Rows), vp]
+    L.nncu_kv4_read_dev.argtypes = [C.POINTER(Kv4Rows), vp]
+    L.nncu_kv4_workspace_bytes.argtypes = [C.POINTER(Kv4Attn), C.POINTER(sz)]
+    L.nncu_kv4_attention_dev.argtypes = [C.POINTER(Kv4Attn), vp]
     L.nncu_host_register.argtypes = [vp, sz]
     L.nncu_host_unregister.argtypes = [vp]
     L.nncu_sync.argtypes = [vp, vp]
@@ -465,6 +517,118 @@ def argmax_rows_dev(x, n_rows: int, n: int, out, x_stride=None, stream=None) -> 
     """nncu_argmax_rows_dev: greedy verify's argmax of each row."""
     _check(lib().nncu_argmax_rows_dev(_ptr(x), int(x_stride if x_stride is not None else n), int(n_rows), int(n),
                                       _ptr(out), _stream(stream)))
+
+
+# ---- serving from a paged cache held in 4 bits ------------------------------------------
+# The descriptions are filled once from device tensors (or raw pointers), which
+# they keep alive, and passed to their call step after step.
+
+def _fill(s, **kw):
+    for name, v in kw.items():
+        setattr(s, name, v if isinstance(v, (int, float, C.Structure, C.Array)) else _ptr(v))
+    s._keep = kw
+    return s
+
+
+def _stride(x, given, row: int) -> int:
+    """The floats from one row of x to the next: as given, a tensor's own, or rows side by side."""
+    if given is not None:
+        return int(given)
+    if x is None or isinstance(x, (int, np.ndarray)) or x.ndim < 2:
+        return row
+    if x.stride(-1) != 1:
+        raise ValueError("the values of a row lie side by side")
+    return int(x.stride(0)) if x.shape[0] > 1 else row
+
+
+def paged_step(n_req: int, page_size: int, n_pages: int, max_blocks: int, max_tok: int, table_stride=None,
+               **arrays) -> PagedStep:
+    """An nncu_paged_step over int32 device arrays (past, n_new, held, queue,
+    ring, block_table, held_out, queue_out, seq_len, q_start, positions,
+    slots, token_req)."""
+    return _fill(PagedStep(), n_req=n_req, page_size=page_size, n_pages=n_pages, max_blocks=max_blocks,
+                 max_tok=max_tok, table_stride=_stride(arrays.get("block_table"), table_stride, max_blocks), **arrays)
+
+
+def paged_step_dev(s: PagedStep, stream=None) -> None:
+    """nncu_paged_step_dev: block tables, lengths, positions and slots of a step."""
+    _check(lib().nncu_paged_step_dev(C.byref(s), _stream(stream)))
+
+
+def rope_axes(n_tok: int, n_head: int, n_kv: int, head_dim: int, positions, inv_freq, q=None, k=None, q_out=None,
+              k_out=None, n_rot=None, rope_mode: int = ROPE_NEOX, sections=None, interleaved: int = 0, pos_stride=None,
+              q_gamma=None, k_gamma=None, eps: float = 1e-6, q_stride=None, k_stride=None, q_out_stride=None,
+              k_out_stride=None) -> RopeAxes:
+    """An nncu_rope_axes; positions int32 [n_axes][n_tok] (or [n_tok]), sections
+    the pairs of each axis; q_out, k_out default to q and k (in place)."""
+    n_rot = head_dim if n_rot is None else n_rot
+    sections = [n_rot // 2] if sections is None else [int(x) for x in sections]
+    q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
+    return _fill(RopeAxes(), n_tok=n_tok, n_head=n_head, n_kv=n_kv, head_dim=head_dim, n_rot=n_rot,
+                 rope_mode=rope_mode, n_axes=len(sections), interleaved=int(interleaved),
+                 section=(C.c_int32 * 4)(*sections[:4]), eps=eps, positions=positions,
+                 pos_stride=_stride(positions, pos_stride, n_tok), inv_freq=inv_freq, q_gamma=q_gamma,
+                 k_gamma=k_gamma, q=q, k=k, q_out=q_out, k_out=k_out,
+                 q_stride=_stride(q, q_stride, n_head * head_dim), k_stride=_stride(k, k_stride, n_kv * head_dim),
+                 q_out_stride=_stride(q_out, q_out_stride, n_head * head_dim),
+                 k_out_stride=_stride(k_out, k_out_stride, n_kv * head_dim))
+
+
+def rope_axes_dev(r: RopeAxes, stream=None) -> None:
+    """nncu_rope_axes_dev: the packed tokens' q and k normed and rotated."""
+    _check(lib().nncu_rope_axes_dev(C.byref(r), _stream(stream)))
+
+
+def kv4_pool(pages, n_pages: int, page_size: int, n_kv: int, head_dim: int) -> Kv4Pool:
+    """One layer's pool over `pages` (a uint8 device array of kv4_bytes)."""
+    return _fill(Kv4Pool(), pages=pages, n_pages=n_pages, page_size=page_size, n_kv=n_kv, head_dim=head_dim)
+
+
+def kv4_bytes(n_pages: int, page_size: int, n_kv: int, head_dim: int) -> int:
+    """Bytes of a layer's pool."""
+    n = C.c_size_t()
+    _check(lib().nncu_kv4_bytes(C.byref(Kv4Pool(None, n_pages, page_size, n_kv, head_dim)), C.byref(n)))
+    return n.value
+
+
+def kv4_rows(pool: Kv4Pool, slots, n_tok: int, k=None, v=None, k_stride=None, v_stride=None) -> Kv4Rows:
+    """An nncu_kv4_rows: token t's k and v rows at slots[t]."""
+    row = pool.n_kv * pool.head_dim
+    return _fill(Kv4Rows(), pool=pool, n_tok=n_tok, slots=slots, k=k, v=v, k_stride=_stride(k, k_stride, row),
+                 v_stride=_stride(v, v_stride, row))
+
+
+def kv4_append_dev(rows: Kv4Rows, stream=None) -> None:
+    """nncu_kv4_append_dev: rows quantised into their slots."""
+    _check(lib().nncu_kv4_append_dev(C.byref(rows), _stream(stream)))
+
+
+def kv4_read_dev(rows: Kv4Rows, stream=None) -> None:
+    """nncu_kv4_read_dev: the values that the slots hold."""
+    _check(lib().nncu_kv4_read_dev(C.byref(rows), _stream(stream)))
+
+
+def kv4_attn(pool: Kv4Pool, n_req: int, n_tok: int, n_head: int, max_new: int, max_blocks: int, block_table, seq_len,
+             q_start, q, out, scale=None, softcap: float = 0.0, window: int = 0, table_stride=None, q_stride=None,
+             out_stride=None, workspace=None, workspace_bytes: int = 0) -> Kv4Attn:
+    """An nncu_kv4_attn; give it a cleared workspace of kv4_workspace_bytes(a)."""
+    row = n_head * pool.head_dim
+    return _fill(Kv4Attn(), pool=pool, n_req=n_req, n_tok=n_tok, n_head=n_head, max_new=max_new,
+                 max_blocks=max_blocks, window=window, scale=1.0 / float(np.sqrt(pool.head_dim)) if scale is None else scale,
+                 softcap=softcap, block_table=block_table, table_stride=_stride(block_table, table_stride, max_blocks),
+                 seq_len=seq_len, q_start=q_start, q=q, q_stride=_stride(q, q_stride, row), out=out,
+                 out_stride=_stride(out, out_stride, row), workspace=workspace, workspace_bytes=workspace_bytes)
+
+
+def kv4_workspace_bytes(a: Kv4Attn) -> int:
+    n = C.c_size_t()
+    _check(lib().nncu_kv4_workspace_bytes(C.byref(a), C.byref(n)))
+    return n.value
+
+
+def kv4_attention_dev(a: Kv4Attn, stream=None) -> None:
+    """nncu_kv4_attention_dev: decode, verify and prompt attention over the pool."""
+    _check(lib().nncu_kv4_attention_dev(C.byref(a), _stream(stream)))
 
 
 def job(layer: int, p: AttnParams, q, k, v, out, seq: int = 0) -> AttnJob:

@@ -1,0 +1,628 @@
+// k_paged.cu -- the paged cache's small operators: a step's tables from the
+// requests' lengths, the rotation by per-token positions with several axes,
+// and the 4-bit cache's write and read-back. (The attention over it:
+// k_kv4_attn.cu.)
+#include <cuda_runtime.h>
+
+#include <cstdio>
+
+#include "kv4.cuh"
+
+namespace nncu
+{
+namespace
+{
+
+// ---- a step's tables ---------------------------------------------------------------
+//
+// Everything follows from three running sums over the requests: of their new
+// tokens, of the pages they lack and of the pages they give back. Every CTA
+// forms all three (12 bytes a request from L2, a scan in shared memory)
+// instead of waiting for another one, then handles its share of the tokens,
+// the new pages and the returned pages: one launch, no workspace.
+
+constexpr int STEP_THREADS = 512;
+constexpr int SAT = 1 << 30; // running sums of absurd lengths stop here instead of wrapping
+
+__device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, SAT); }
+
+// Inclusive running sum over the CTA's threads; `total` gets the sum of all.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total)
+{
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+	for (int o = 1; o < 32; o <<= 1)
+	{
+		const int u = __shfl_up_sync(0xffffffffu, v, o);
+		if (lane >= o) v = sat_add(v, u);
+	}
+	__syncthreads(); // the previous call's sums have been read
+	if (lane == 31) warp_sums[warp] = v;
+	__syncthreads();
+	int before = 0, all = 0;
+#pragma unroll
+	for (int w = 0; w < STEP_THREADS / 32; ++w)
+	{
+		const int s = warp_sums[w];
+		if (w < warp) before = sat_add(before, s);
+		all = sat_add(all, s);
+	}
+	total = all;
+	return sat_add(before, v);
+}
+
+// The last i of [0, n] with a[i] <= x (a rising, a[0] <= x).
+__device__ __forceinline__ int last_at_most(const int* a, int n, int x)
+{
+	int lo = 0, hi = n;
+	while (lo < hi)
+	{
+		const int mid = (lo + hi + 1) >> 1;
+		if (a[mid] <= x)
+			lo = mid;
+		else
+			hi = mid - 1;
+	}
+	return lo;
+}
+
+__global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_paged_step s)
+{
+	extern __shared__ int sm[];
+	const int n = s.n_req;
+	int* tok = sm;             // [n + 1] running sum of new tokens
+	int* lack = sm + (n + 1);  // [n + 1] ... of pages to take
+	int* back = lack + n + 1;  // [n + 1] ... of pages given back
+	__shared__ int warp_sums[STEP_THREADS / 32];
+	const long long room = (long long)s.max_blocks * s.page_size;
+
+	if (threadIdx.x == 0) tok[0] = lack[0] = back[0] = 0;
+	int c_tok = 0, c_lack = 0, c_back = 0;
+	for (int i0 = 0; i0 < n; i0 += STEP_THREADS)
+	{
+		const int i = i0 + (int)threadIdx.x;
+		int nn = 0, past = 0, held = 0, t;
+		if (i < n)
+		{
+			nn = s.n_new[i];
+			past = s.past[i];
+			held = max(0, min(s.held[i], s.max_blocks));
+		}
+		const bool ends = nn < 0;
+		const int q_end = sat_add(c_tok, block_scan(min(max(nn, 0), SAT), warp_sums, t));
+		c_tok = sat_add(c_tok, t);
+		const bool fits = !ends && past >= 0 && (long long)past + nn <= room && q_end <= s.max_tok;
+		const int need = fits ? max(0, (int)(((long long)past + nn + s.page_size - 1) / s.page_size) - held) : 0;
+		const int l_end = sat_add(c_lack, block_scan(need, warp_sums, t));
+		c_lack = sat_add(c_lack, t);
+		const int b_end = sat_add(c_back, block_scan(ends ? held : 0, warp_sums, t));
+		c_back = sat_add(c_back, t);
+		if (i < n) tok[i + 1] = q_end, lack[i + 1] = l_end, back[i + 1] = b_end;
+	}
+	__syncthreads();
+
+	const int np = s.n_pages;
+	const int count = max(0, min(s.queue[1], np));
+	const int head = ((s.queue[0] % np) + np) % np;
+	const int taken = lack[last_at_most(lack, n, count)];
+	const auto served = [&](int r, int nn, int past) {
+		const int need = lack[r + 1] - lack[r];
+		return nn >= 0 && past >= 0 && (long long)past + nn <= room && tok[r + 1] <= s.max_tok &&
+		       (need == 0 || lack[r + 1] <= count);
+	};
+	const int step = gridDim.x * STEP_THREADS, me = blockIdx.x * STEP_THREADS + (int)threadIdx.x;
+
+	for (int r = me; r < n; r += step)
+	{
+		const int nn = s.n_new[r], past = s.past[r], held = max(0, min(s.held[r], s.max_blocks));
+		const bool ok = served(r, nn, past);
+		s.held_out[r] = nn < 0 ? 0 : held + (ok ? lack[r + 1] - lack[r] : 0);
+		s.seq_len[r] = nn < 0 ? 0 : ok ? past + nn : past;
+		s.q_start[r] = tok[r];
+	}
+	if (me == 0)
+	{
+		s.q_start[n] = tok[n];
+		s.queue_out[0] = (head + taken) % np;
+		s.queue_out[1] = count - taken + back[n];
+		s.queue_out[2] = lack[n] - taken;
+		s.queue_out[3] = tok[n];
+	}
+	for (int x = me; x < taken; x += step) // the new pages' entries
+	{
+		const int r = last_at_most(lack, n - 1, x);
+		const int b = max(0, min(s.held[r], s.max_blocks)) + x - lack[r];
+		s.block_table[(size_t)r * s.table_stride + b] = s.ring[(head + x) % np];
+	}
+	for (int x = me; x < back[n]; x += step) // the returned pages, behind the free ones
+	{
+		const int r = last_at_most(back, n - 1, x);
+		s.ring[((long long)head + count + x) % np] = s.block_table[(size_t)r * s.table_stride + x - back[r]];
+	}
+	for (int t = me; t < s.max_tok; t += step)
+	{
+		int pos = 0, slot = -1, req = -1;
+		if (t < tok[n])
+		{
+			req = last_at_most(tok, n - 1, t);
+			const int nn = s.n_new[req], past = s.past[req];
+			pos = past + t - tok[req];
+			if (served(req, nn, past))
+			{
+				const int held = max(0, min(s.held[req], s.max_blocks)), b = pos / s.page_size;
+				const int page = b < held ? s.block_table[(size_t)req * s.table_stride + b]
+				                          : s.ring[(head + lack[req] + b - held) % np];
+				slot = page * s.page_size + pos % s.page_size;
+			}
+		}
+		s.positions[t] = pos;
+		s.slots[t] = slot;
+		s.token_req[t] = req;
+	}
+}
+
+// ---- norm and rotation by per-token positions ---------------------------------------
+//
+// Memory bound: 8 bytes a value. One CTA per token: its angles (their cosines
+// and sines) serve all its heads, so they are formed once, in shared memory,
+// while the first head vectors are already on their way. A head vector is
+// spread over LPV lanes; a lane's item is the 2 VEC values that turn together
+// (NEOX: VEC at e and VEC at e + n_rot / 2), so no exchange between lanes is
+// needed but the norm's sum.
+
+constexpr int ROPE_THREADS = 256;
+
+struct RopeArgs
+{
+	nncu_rope_axes r;
+	int half;
+};
+
+template <int VEC>
+struct RopeVec
+{
+	float v[2 * VEC];
+};
+
+template <int VEC>
+__device__ __forceinline__ void rope_load(RopeVec<VEC>& x, const float* p, int a, int b)
+{
+	if constexpr (VEC == 4)
+	{
+		const float4 u = *reinterpret_cast<const float4*>(p + a), w = *reinterpret_cast<const float4*>(p + b);
+		x.v[0] = u.x, x.v[1] = u.y, x.v[2] = u.z, x.v[3] = u.w;
+		x.v[4] = w.x, x.v[5] = w.y, x.v[6] = w.z, x.v[7] = w.w;
+	}
+	else
+		x.v[0] = p[a], x.v[1] = p[b];
+}
+
+template <int VEC>
+__device__ __forceinline__ void rope_store(const RopeVec<VEC>& x, float* p, int a, int b)
+{
+	if constexpr (VEC == 4)
+	{
+		*reinterpret_cast<float4*>(p + a) = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+		*reinterpret_cast<float4*>(p + b) = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
+	}
+	else
+		p[a] = x.v[0], p[b] = x.v[1];
+}
+
+// IPL items a lane, LPV lanes a vector (a power of two).
+template <int VEC, int IPL, int LPV>
+__global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeArgs g)
+{
+	const nncu_rope_axes& r = g.r;
+	__shared__ float2 turn[256]; // cos, sin of the token's pairs
+	constexpr int VPC = ROPE_THREADS / LPV; // vectors in flight a CTA
+	const int t = blockIdx.x, half = g.half, D = r.head_dim, items = D / (2 * VEC);
+	const int lane = threadIdx.x % LPV;
+	const bool neox = r.rope_mode == NNCU_ROPE_NEOX;
+	const int nq = r.q ? r.n_head : 0, n_vec = nq + (r.k ? r.n_kv : 0);
+
+	// where item i's two runs of VEC values begin
+	const auto place = [&](int i, int& a, int& b) {
+		if (neox && i < half / VEC)
+			a = i * VEC, b = a + half;
+		else
+			a = 2 * VEC * i, b = a + VEC;
+	};
+	const auto source = [&](int w) {
+		return w < nq ? r.q + (size_t)t * r.q_stride + (size_t)w * D
+		              : r.k + (size_t)t * r.k_stride + (size_t)(w - nq) * D;
+	};
+	RopeVec<VEC> x[IPL];
+	const auto load = [&](int w) {
+		const float* p = source(w);
+#pragma unroll
+		for (int j = 0; j < IPL; ++j)
+		{
+			const int i = lane + j * LPV;
+			int a, b;
+			place(i, a, b);
+			if (i < items) rope_load<VEC>(x[j], p, a, b);
+		}
+	};
+	int w = threadIdx.x / LPV;
+	if (w < n_vec) load(w);
+
+	for (int i = threadIdx.x; i < half; i += ROPE_THREADS)
+	{
+		int axis = 0;
+		if (r.interleaved)
+		{
+			const int a = i % r.n_axes;
+			axis = i / r.n_axes < r.section[a] ? a : 0;
+		}
+		else
+			for (int e = r.section[0]; axis + 1 < r.n_axes && i >= e; e += r.section[axis]) ++axis;
+		const float angle = (float)r.positions[axis * r.pos_stride + t] * r.inv_freq[i];
+		float sn, cs;
+		sincosf(angle, &sn, &cs);
+		turn[i] = make_float2(cs, sn);
+	}
+	__syncthreads();
+
+	for (; w < n_vec; w += VPC)
+	{
+		const float* gamma = w < nq ? r.q_gamma : r.k_gamma;
+		if (gamma)
+		{
+			float ss = 0.0f;
+#pragma unroll
+			for (int j = 0; j < IPL; ++j)
+				if (lane + j * LPV < items)
+#pragma unroll
+					for (int e = 0; e < 2 * VEC; ++e) ss = fmaf(x[j].v[e], x[j].v[e], ss);
+			// the lanes of one vector leave the loop together, so they name each other alone
+			const unsigned mask = LPV == 32 ? 0xffffffffu
+			                                : ((1u << (LPV & 31)) - 1u) << ((threadIdx.x & 31) / LPV * LPV);
+#pragma unroll
+			for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+			const float sc = 1.0f / sqrtf(ss / (float)D + r.eps);
+#pragma unroll
+			for (int j = 0; j < IPL; ++j)
+			{
+				const int i = lane + j * LPV;
+				int a, b;
+				place(i, a, b);
+				if (i < items)
+				{
+					RopeVec<VEC> gm;
+					rope_load<VEC>(gm, gamma, a, b);
+#pragma unroll
+					for (int e = 0; e < 2 * VEC; ++e) x[j].v[e] = x[j].v[e] * sc * gm.v[e];
+				}
+			}
+		}
+		float* y = w < nq ? r.q_out + (size_t)t * r.q_out_stride + (size_t)w * D
+		                  : r.k_out + (size_t)t * r.k_out_stride + (size_t)(w - nq) * D;
+#pragma unroll
+		for (int j = 0; j < IPL; ++j)
+		{
+			const int i = lane + j * LPV;
+			int a, b;
+			place(i, a, b);
+			if (i >= items) continue;
+			if (i < half / VEC)
+			{
+#pragma unroll
+				for (int e = 0; e < VEC; ++e)
+				{
+					// NEOX: values e and e + VEC of the item; NORM: 2e and 2e + 1
+					const float2 cs = turn[i * VEC + e];
+					float& u = x[j].v[neox ? e : 2 * e];
+					float& v = x[j].v[neox ? e + VEC : 2 * e + 1];
+					const float u0 = u, v0 = v;
+					u = u0 * cs.x - v0 * cs.y;
+					v = u0 * cs.y + v0 * cs.x;
+				}
+			}
+			rope_store<VEC>(x[j], y, a, b);
+		}
+		if (w + VPC < n_vec) load(w + VPC);
+	}
+}
+
+template <int VEC>
+int launch_rope_axes(const RopeArgs& g, cudaStream_t st)
+{
+	const int items = g.r.head_dim / (2 * VEC);
+	const unsigned grid = (unsigned)g.r.n_tok;
+	if (items <= 8)
+		rope_axes_kernel<VEC, 1, 8><<<grid, ROPE_THREADS, 0, st>>>(g);
+	else if (items <= 16)
+		rope_axes_kernel<VEC, 1, 16><<<grid, ROPE_THREADS, 0, st>>>(g);
+	else if (items <= 32)
+		rope_axes_kernel<VEC, 1, 32><<<grid, ROPE_THREADS, 0, st>>>(g);
+	else if (items <= 64)
+		rope_axes_kernel<VEC, 2, 32><<<grid, ROPE_THREADS, 0, st>>>(g);
+	else if (VEC == 1)
+		rope_axes_kernel<1, 8, 32><<<grid, ROPE_THREADS, 0, st>>>(g);
+	note_launches(1);
+	return (int)cudaGetLastError();
+}
+
+// ---- the 4-bit cache's write -----------------------------------------------------------
+//
+// Memory bound: 4 bytes a value in, 0.5625 out. A group of 32 values is 8
+// lanes with a 16-byte load each; its extremes meet in three exchanges, its
+// scale and reciprocal are formed by every lane, a pair of lanes builds one
+// 32-bit word. blockIdx.y: K or V.
+
+constexpr int ROWS_THREADS = 256;
+constexpr int ROWS_ITEMS = 4; // 16-byte loads in flight a thread
+
+struct RowsArgs
+{
+	uint8_t* pages;
+	int n_pages, page, n_kv, D, n_tok;
+	const int* slots;
+	float* x[2];
+	size_t stride[2];
+	int first; // 0: from K; 1: V only
+};
+
+// Where a token's row of one KV head sits: its codes and its scales.
+__device__ __forceinline__ bool rows_at(const RowsArgs& a, int which, int slot, int h, int& off, uint8_t*& codes,
+                                        uint16_t*& scales)
+{
+	const int pg = slot / a.page;
+	if (slot < 0 || pg >= a.n_pages) return false;
+	off = slot - pg * a.page;
+	const int cb = kv4_codes_bytes(a.page, a.D), sb = kv4_scales_bytes(a.page, a.D);
+	uint8_t* chunk = a.pages + ((size_t)pg * a.n_kv + h) * kv4_chunk_bytes(a.page, a.D);
+	codes = chunk + which * cb + off * (a.D / 2);
+	scales = reinterpret_cast<uint16_t*>(chunk + 2 * cb + which * sb) + off * (a.D / KV4_GROUP);
+	return true;
+}
+
+__global__ void __launch_bounds__(ROWS_THREADS) kv4_append_kernel(const RowsArgs a)
+{
+	const int which = a.first + blockIdx.y;
+	const float* __restrict__ src = a.x[which];
+	const size_t stride = a.stride[which];
+	const int per_tok = a.n_kv * a.D / 4; // 16-byte pieces a token
+	const long long total = (long long)a.n_tok * per_tok;
+	const long long base = (long long)blockIdx.x * (ROWS_THREADS * ROWS_ITEMS) + threadIdx.x;
+	float4 v[ROWS_ITEMS];
+	int slot[ROWS_ITEMS], piece[ROWS_ITEMS];
+#pragma unroll
+	for (int j = 0; j < ROWS_ITEMS; ++j)
+	{
+		const long long i = base + (long long)j * ROWS_THREADS;
+		slot[j] = -1;
+		piece[j] = 0;
+		v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+		if (i < total)
+		{
+			const int t = (int)(i / per_tok);
+			piece[j] = (int)(i - (long long)t * per_tok);
+			slot[j] = a.slots[t];
+			v[j] = *reinterpret_cast<const float4*>(src + (size_t)t * stride + 4 * (size_t)piece[j]);
+		}
+	}
+#pragma unroll
+	for (int j = 0; j < ROWS_ITEMS; ++j)
+	{
+		// (whole warps: a group's 8 lanes always work on one row)
+		const float x[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+		float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+		uint32_t bits = 0; // the largest magnitude's bits, NaN's included (the extremes above pass NaNs by)
+#pragma unroll
+		for (int e = 0; e < 4; ++e) bits = max(bits, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+		for (int o = 1; o < 8; o <<= 1)
+		{
+			hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+			lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+			bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+		}
+		const bool bad = bits >= 0x7f800000u;
+		float s = __bfloat162float(__float2bfloat16_rn((hi >= -lo ? hi : lo) * -0.125f));
+		s = copysignf(fminf(fmaxf(fabsf(s), KV4_SCALE_MIN), KV4_SCALE_MAX), s);
+		const float inv = __frcp_rn(s);
+		uint32_t w = 0;
+		const int l8 = threadIdx.x & 7; // this lane's four values of the group's 32: 4 l8 ..
+#pragma unroll
+		for (int e = 0; e < 4; ++e)
+		{
+			const int c = bad ? 0 : (int)fminf(fmaxf(rintf(x[e] * inv), -8.0f), 7.0f);
+			w |= (uint32_t)(c + 8) << (4 * kv4_nibble(4 * (l8 & 1) + e));
+		}
+		w |= __shfl_xor_sync(0xffffffffu, w, 1);
+		const int h = piece[j] / (a.D / 4), g = piece[j] % (a.D / 4) / 8;
+		int off;
+		uint8_t* codes;
+		uint16_t* scales;
+		if (rows_at(a, which, slot[j], h, off, codes, scales))
+		{
+			if (!(l8 & 1)) *reinterpret_cast<uint32_t*>(codes + 16 * kv4_unit(off, g, a.D) + 2 * l8) = w;
+			if (l8 == 0) scales[g] = bad ? (uint16_t)0x7fc0u : (uint16_t)(__float_as_uint(s) >> 16);
+		}
+	}
+}
+
+// ---- and its reading back: a thread takes one word (8 values) -----------------------------
+
+__global__ void __launch_bounds__(ROWS_THREADS) kv4_read_kernel(const RowsArgs a)
+{
+	const int which = a.first + blockIdx.y;
+	const int per_tok = a.n_kv * a.D / 8;
+	const long long i = (long long)blockIdx.x * ROWS_THREADS + threadIdx.x;
+	if (i >= (long long)a.n_tok * per_tok) return;
+	const int t = (int)(i / per_tok), word = (int)(i - (long long)t * per_tok);
+	const int h = word / (a.D / 8), in = word % (a.D / 8), g = in / 4;
+	float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+	int off;
+	uint8_t* codes;
+	uint16_t* scales;
+	if (rows_at(a, which, a.slots[t], h, off, codes, scales))
+	{
+		const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + 16 * kv4_unit(off, g, a.D) + 4 * (in & 3));
+		const float s = bf16_bits_to_float(scales[g]);
+#pragma unroll
+		for (int e = 0; e < 8; ++e) y[e] = s * (float)((int)((w >> (4 * kv4_nibble(e))) & 15u) - 8);
+	}
+	float4* dst = reinterpret_cast<float4*>(a.x[which] + (size_t)t * a.stride[which] + 8 * (size_t)word);
+	dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+	dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+}
+
+int refuse(const char* msg) { return set_error(NNCU_ERR_INVALID_ARGUMENT, msg); }
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Checks of a rows call; 1: nothing to do.
+int rows_args(const nncu_kv4_rows* r, const char* what, RowsArgs& a)
+{
+	char msg[160];
+	if (!r) return refuse("kv4 rows: NULL argument");
+	const int rc = kv4_check_pool(&r->pool, what);
+	if (rc != NNCU_OK) return rc;
+	const size_t row = (size_t)r->pool.n_kv * r->pool.head_dim;
+	msg[0] = 0;
+	if (r->n_tok < 0)
+		snprintf(msg, sizeof msg, "%s: negative n_tok", what);
+	else if (r->n_tok > 0 && (!r->slots || (!r->k && !r->v)))
+		snprintf(msg, sizeof msg, "%s: NULL slots or rows", what);
+	else if (!aligned16(r->k) || !aligned16(r->v) || (r->k && r->k_stride % 4) || (r->v && r->v_stride % 4))
+		snprintf(msg, sizeof msg, "%s: rows must be 16-byte aligned", what);
+	else if (r->n_tok > 1 && ((r->k && r->k_stride < row) || (r->v && r->v_stride < row)))
+		snprintf(msg, sizeof msg, "%s: strides shorter than a row", what);
+	if (msg[0]) return refuse(msg);
+	a = RowsArgs{static_cast<uint8_t*>(r->pool.pages), r->pool.n_pages, r->pool.page_size, r->pool.n_kv,
+	             r->pool.head_dim, r->n_tok, r->slots, {r->k, r->v}, {r->k_stride, r->v_stride}, r->k ? 0 : 1};
+	return NNCU_OK;
+}
+
+} // namespace
+
+int kv4_check_pool(const nncu_kv4_pool* p, const char* what, bool need_pages)
+{
+	char msg[160];
+	msg[0] = 0;
+	if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+		snprintf(msg, sizeof msg, "%s: head_dim %d (64, 128 and 256 are served)", what, (int)p->head_dim);
+	else if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
+		snprintf(msg, sizeof msg, "%s: page_size %d (16, 32, 64, 128 or 256)", what, (int)p->page_size);
+	else if (p->n_pages <= 0 || p->n_kv <= 0 || (long long)p->n_pages * p->page_size > INT32_MAX || p->n_kv > 65535)
+		snprintf(msg, sizeof msg, "%s: bad n_pages or n_kv", what);
+	else if (need_pages && (!p->pages || !aligned16(p->pages)))
+		snprintf(msg, sizeof msg, "%s: pages NULL or not 16-byte aligned", what);
+	return msg[0] ? refuse(msg) : NNCU_OK;
+}
+
+} // namespace nncu
+
+using namespace nncu;
+
+extern "C" int nncu_paged_step_dev(const nncu_paged_step* s, void* stream)
+{
+	if (!s) return refuse("paged step: NULL argument");
+	if (s->n_req <= 0 || s->n_req > NNCU_PAGED_MAX_REQ) return refuse("paged step: n_req out of range");
+	if (s->page_size <= 0 || s->n_pages <= 0 || s->max_blocks <= 0 || s->max_tok < 0 || s->max_tok > (1 << 28) ||
+	    (long long)s->n_pages * s->page_size > INT32_MAX || (long long)s->max_blocks * s->page_size > INT32_MAX ||
+	    s->n_pages > (1 << 29))
+		return refuse("paged step: bad page_size, n_pages, max_blocks or max_tok");
+	if (s->table_stride < s->max_blocks) return refuse("paged step: table rows shorter than max_blocks");
+	if (!s->past || !s->n_new || !s->held || !s->queue || !s->ring || !s->block_table || !s->held_out ||
+	    !s->queue_out || !s->seq_len || !s->q_start || (s->max_tok > 0 && (!s->positions || !s->slots || !s->token_req)))
+		return refuse("paged step: NULL array");
+	if (s->held_out == s->held || s->queue_out == s->queue)
+		return refuse("paged step: held_out and queue_out must not be the inputs");
+	const size_t smem = 3 * sizeof(int) * ((size_t)s->n_req + 1);
+	if (smem > 48 * 1024)
+	{
+		const cudaError_t ce = cudaFuncSetAttribute(paged_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+		                                            3 * (int)sizeof(int) * (NNCU_PAGED_MAX_REQ + 1));
+		if (ce != cudaSuccess) return set_cuda_error((int)ce, "paged step shared memory");
+	}
+	// four tokens a thread; every CTA repeats the sums, so no more than that asks for
+	const int work = s->max_tok > s->n_req ? s->max_tok : s->n_req;
+	const int grid = (work + 4 * STEP_THREADS - 1) / (4 * STEP_THREADS);
+	paged_step_kernel<<<grid < 296 ? grid : 296, STEP_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(*s);
+	note_launches(1);
+	const int e = (int)cudaGetLastError();
+	return e ? set_cuda_error(e, "paged step launch") : NNCU_OK;
+}
+
+extern "C" int nncu_rope_axes_dev(const nncu_rope_axes* r, void* stream)
+{
+	if (!r) return refuse("rope axes: NULL argument");
+	if (r->n_tok < 0 || (!r->q && !r->k)) return refuse("rope axes: negative n_tok or no rows");
+	if (r->head_dim <= 0 || r->head_dim > 512 || r->head_dim % 2) return refuse("rope axes: head_dim must be even, up to 512");
+	if (r->n_rot < 0 || r->n_rot % 2 || r->n_rot > r->head_dim) return refuse("rope axes: n_rot must be even, up to head_dim");
+	if (r->rope_mode != NNCU_ROPE_NEOX && r->rope_mode != NNCU_ROPE_NORM) return refuse("rope axes: unknown rope mode");
+	if (r->n_axes < 1 || r->n_axes > 4) return refuse("rope axes: one to four axes");
+	long long pairs = 0;
+	for (int a = 0; a < r->n_axes; ++a)
+	{
+		if (r->section[a] < 0) return refuse("rope axes: negative section");
+		pairs += r->section[a];
+	}
+	if (pairs != r->n_rot / 2) return refuse("rope axes: the sections must have n_rot / 2 pairs together");
+	if (r->interleaved)
+		for (int a = 1; a < r->n_axes; ++a)
+			if (r->section[a] > 0 && (long long)(r->section[a] - 1) * r->n_axes + a >= r->n_rot / 2)
+				return refuse("rope axes: an interleaved section passes the last pair");
+	if ((r->q && (!r->q_out || r->n_head <= 0)) || (r->k && (!r->k_out || r->n_kv <= 0)))
+		return refuse("rope axes: NULL output or no heads");
+	if (r->n_rot > 0 && (!r->positions || !r->inv_freq)) return refuse("rope axes: NULL positions or frequencies");
+	if (r->n_tok > 1 && r->n_axes > 1 && r->pos_stride < (size_t)r->n_tok)
+		return refuse("rope axes: pos_stride shorter than the tokens");
+	const size_t qrow = (size_t)r->n_head * r->head_dim, krow = (size_t)r->n_kv * r->head_dim;
+	if (r->n_tok > 1 && ((r->q && (r->q_stride < qrow || r->q_out_stride < qrow)) ||
+	                     (r->k && (r->k_stride < krow || r->k_out_stride < krow))))
+		return refuse("rope axes: strides shorter than a row");
+	if ((r->q && r->q == r->q_out && r->q_stride != r->q_out_stride) ||
+	    (r->k && r->k == r->k_out && r->k_stride != r->k_out_stride))
+		return refuse("rope axes: in place with two strides");
+	if (r->n_tok == 0) return NNCU_OK;
+	const RopeArgs g{*r, r->n_rot / 2};
+	// 16-byte accesses where every run of four values allows them
+	const bool vec = r->head_dim % 8 == 0 && r->n_rot % 8 == 0 && aligned16(r->q) && aligned16(r->k) &&
+	                 aligned16(r->q_out) && aligned16(r->k_out) && aligned16(r->q_gamma) && aligned16(r->k_gamma) &&
+	                 (!r->q || (r->q_stride % 4 == 0 && r->q_out_stride % 4 == 0)) &&
+	                 (!r->k || (r->k_stride % 4 == 0 && r->k_out_stride % 4 == 0));
+	const auto st = static_cast<cudaStream_t>(stream);
+	const int e = vec ? launch_rope_axes<4>(g, st) : launch_rope_axes<1>(g, st);
+	return e ? set_cuda_error(e, "rope axes launch") : NNCU_OK;
+}
+
+extern "C" int nncu_kv4_bytes(const nncu_kv4_pool* pool, size_t* bytes)
+{
+	if (!pool || !bytes) return refuse("kv4 bytes: NULL argument");
+	const int rc = kv4_check_pool(pool, "kv4 bytes", false);
+	if (rc != NNCU_OK) return rc;
+	*bytes = kv4_chunk_bytes(pool->page_size, pool->head_dim) * pool->n_kv * pool->n_pages;
+	return NNCU_OK;
+}
+
+extern "C" int nncu_kv4_append_dev(const nncu_kv4_rows* rows, void* stream)
+{
+	RowsArgs a;
+	const int rc = rows_args(rows, "kv4 append", a);
+	if (rc != NNCU_OK || a.n_tok == 0) return rc;
+	const long long pieces = (long long)a.n_tok * a.n_kv * a.D / 4;
+	const dim3 grid((unsigned)((pieces + ROWS_THREADS * ROWS_ITEMS - 1) / (ROWS_THREADS * ROWS_ITEMS)),
+	                a.x[0] && a.x[1] ? 2u : 1u);
+	kv4_append_kernel<<<grid, ROWS_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
+	note_launches(1);
+	const int e = (int)cudaGetLastError();
+	return e ? set_cuda_error(e, "kv4 append launch") : NNCU_OK;
+}
+
+extern "C" int nncu_kv4_read_dev(const nncu_kv4_rows* rows, void* stream)
+{
+	RowsArgs a;
+	const int rc = rows_args(rows, "kv4 read", a);
+	if (rc != NNCU_OK || a.n_tok == 0) return rc;
+	const long long words = (long long)a.n_tok * a.n_kv * a.D / 8;
+	const dim3 grid((unsigned)((words + ROWS_THREADS - 1) / ROWS_THREADS), a.x[0] && a.x[1] ? 2u : 1u);
+	kv4_read_kernel<<<grid, ROWS_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
+	note_launches(1);
+	const int e = (int)cudaGetLastError();
+	return e ? set_cuda_error(e, "kv4 read launch") : NNCU_OK;
+}
