@@ -523,6 +523,10 @@ typedef struct nncu_kv4_attn
 } nncu_kv4_attn;
 int nncu_kv4_workspace_bytes(const nncu_kv4_attn* a, size_t* bytes);
 int nncu_kv4_attention_dev(const nncu_kv4_attn* a, void* stream);
+/* Wait for `stream` and report whether a kernel of a call with this workspace
+ * had a bounded wait run out (NNCU_ERR_TIMEOUT: those outputs are void); the
+ * workspace is then cleared. */
+int nncu_kv4_check(const nncu_kv4_attn* a, void* stream);
 
 /* One layer's decode / verify attention that allocates nothing: the same
  * K1 + K2 kernels as nncu_attention_batch_dev for one job, with every buffer

@@ -36,7 +36,7 @@ __all__ = [
     "gemv_bf16w_argmax_dev", "Weight", "AttnWeights", "weight", "W_BF16", "W_Q8_0", "W_Q4_S", "logits_batch_dev",
     "argmax_rows_dev", "PagedStep", "paged_step", "paged_step_dev", "RopeAxes", "rope_axes", "rope_axes_dev",
     "Kv4Pool", "kv4_pool", "kv4_bytes", "Kv4Rows", "kv4_rows", "kv4_append_dev", "kv4_read_dev", "Kv4Attn",
-    "kv4_attn", "kv4_workspace_bytes", "kv4_attention_dev", "EXPORTS",
+    "kv4_attn", "kv4_workspace_bytes", "kv4_attention_dev", "kv4_check", "EXPORTS",
 ]
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -66,6 +66,7 @@ EXPORTS = [
     "nncu_attention_forward_batch_dev",
     "nncu_argmax_rows_dev", "nncu_paged_step_dev", "nncu_rope_axes_dev", "nncu_kv4_bytes", "nncu_kv4_append_dev",
     "nncu_kv4_read_dev", "nncu_kv4_workspace_bytes", "nncu_kv4_attention_dev",
+    "nncu_kv4_check",
 ]
 GROUP_HANDLE_BYTES = 64
 
@@ -281,6 +282,7 @@ def lib() -> C.CDLL:
     L.nncu_kv4_read_dev.argtypes = [C.POINTER(Kv4Rows), vp]
     L.nncu_kv4_workspace_bytes.argtypes = [C.POINTER(Kv4Attn), C.POINTER(sz)]
     L.nncu_kv4_attention_dev.argtypes = [C.POINTER(Kv4Attn), vp]
+    L.nncu_kv4_check.argtypes = [C.POINTER(Kv4Attn), vp]
     L.nncu_host_register.argtypes = [vp, sz]
     L.nncu_host_unregister.argtypes = [vp]
     L.nncu_sync.argtypes = [vp, vp]
@@ -629,6 +631,11 @@ def kv4_workspace_bytes(a: Kv4Attn) -> int:
 def kv4_attention_dev(a: Kv4Attn, stream=None) -> None:
     """nncu_kv4_attention_dev: decode, verify and prompt attention over the pool."""
     _check(lib().nncu_kv4_attention_dev(C.byref(a), _stream(stream)))
+
+
+def kv4_check(a: Kv4Attn, stream=None) -> None:
+    """nncu_kv4_check: wait for `stream`; raise (ERR_TIMEOUT) if a kernel using a's workspace timed out."""
+    _check(lib().nncu_kv4_check(C.byref(a), _stream(stream)))
 
 
 def job(layer: int, p: AttnParams, q, k, v, out, seq: int = 0) -> AttnJob:

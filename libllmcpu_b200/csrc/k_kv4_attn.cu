@@ -1,5 +1,32 @@
 // k_kv4_attn.cu -- attention of packed requests over the paged 4-bit cache
-// (nncu_kv4_attention_dev): decode, verify and prompt.
+// (nncu_kv4_attention_dev).
+//
+// Work. A segment is (request, KV head, row group): 8 R query rows (token x
+// grouped head) that read the same keys. Its keys are walked in tiles of 64;
+// the segments' tiles, one request after another, are cut into equal runs,
+// one per CTA, whatever the requests' lengths: every CTA finds its run from
+// the lengths on the device (a scan over the requests), so one launch serves
+// any batch and a captured graph follows new lengths. A run is a few pieces of
+// segments; a piece that is a whole segment writes the output, another leaves
+// its unnormalised sum with its maximum and weight in the workspace, and the
+// CTA that adds the last piece of a segment joins them in order.
+//
+// A CTA is four computing warps, 16 keys of a tile each, with a softmax state
+// of their own until the piece's end, and one warp that keeps a ring of tiles
+// coming (bulk copies of the pages' codes and scales, looked up in the block
+// table 32 entries at a time).
+//
+// Mathematics. Codes feed the tensor cores without being scaled first: for a
+// group of 32 values (one scale s) q.k = s (sum q u - 8 sum q), u = code + 8.
+// Masking a word of codes leaves u in the low bits of a 16-bit lane, which
+// read as a float is u x 2^-24 (or x 2^-20 one nibble up): an exact operand,
+// with no conversion. The group's sum then takes its scale in 32 bits. V's
+// codes cannot wait for their scale (the sum runs over keys): 16 + u, built by
+// the mask, times s minus 24 s is s (u - 8) in one rounding, and 8 bits of
+// scale times 4 of code are exact in a 16-bit float. q and the weights p go in
+// as two 16-bit halves each (22 bits), accumulated in 32: the result is as
+// close to the exact one as 32-bit arithmetic. p carries 2^15 so that small
+// weights keep their digits.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
@@ -12,80 +39,728 @@ namespace nncu
 namespace
 {
 
-constexpr int SIMPLE_WARPS = 4;
+constexpr int TILE = 64;               // keys a tile
+constexpr int CW = 4;                  // computing warps, 16 keys of a tile each
+constexpr int THREADS = (CW + 1) * 32; // and the loading warp
+constexpr int STAGES = 4;
+constexpr int MIN_TILES = 2;           // a run is at least this long, while tiles are few
+constexpr float P_SCALE_LOG2 = 15.0f;
 
-// One CTA per (token, query head); the warps take keys in turn, every lane
-// D / 32 neighbouring values, and join their softmax states at the end.
-template <int D>
-__global__ void __launch_bounds__(SIMPLE_WARPS * 32) kv4_simple_kernel(const Kv4Args a)
+// What a launch keeps in the workspace: an error word, a counter per CTA (of
+// the segment that begins in the CTA's run and does not end there), and two
+// partial results per CTA (of its first and its last piece).
+struct Ws
 {
-	constexpr int E = D / 32, U = D / KV4_GROUP;
-	__shared__ float so[SIMPLE_WARPS][D], sm[SIMPLE_WARPS], sl[SIMPLE_WARPS];
-	const int t = blockIdx.x, h = blockIdx.y, hk = h / a.group;
-	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-	// the request of this token (the last whose first token is not past it)
-	int lo = 0, hi = a.n_req - 1;
-	while (lo < hi)
+	int* err;
+	int* counters;
+	float* parts;
+};
+
+template <int D, int R>
+struct Shape
+{
+	static constexpr int U = D / KV4_GROUP, ROWS = 8 * R;
+	static constexpr int CODES = TILE * D / 2, SCALES = TILE * U * 2;
+	static constexpr int STAGE = 2 * (CODES + SCALES);
+	static constexpr int RED_ROW = D + 4;                   // floats a row of the joining buffer
+	static constexpr bool Q_REGS = D * R <= 128;            // q's operands in registers (or in shared memory)
+	static constexpr int SM_RED = STAGES * STAGE;           // [CW][ROWS][RED_ROW]
+	static constexpr int SM_Q = SM_RED + CW * ROWS * RED_ROW * 4;
+	static constexpr int SM_ML = SM_Q + (Q_REGS ? 0 : D / 16 * R * 512); // [CW][ROWS] (maximum, weight)
+	static constexpr int SM_BAR = SM_ML + CW * ROWS * 8;
+	static constexpr int SMEM = SM_BAR + 256;
+	static constexpr int PART = ROWS * (D + 2);             // floats a partial result
+	static constexpr int CTAS = D == 256 ? 2 : 3;           // per SM
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1)
+{
+	asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+	    : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+	    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 matrix of 16-bit values, transposed across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+	uint32_t y;
+	asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+	return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// x, y as 16-bit halves: hi the rounded values, lo what they leave.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo)
+{
+	const __half2 h = __floats2half2_rn(x, y);
+	const float2 f = __half22float2(h);
+	hi = half2_bits(h);
+	lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// One segment's rows and the tiles of its keys.
+struct Segment
+{
+	Kv4Request x;
+	int r, hk, row0, rows;   // request, KV head, first row of the group, rows of the request (token x grouped head)
+	int tile0, tiles;        // first tile and their number, for every segment of the request
+	int first, last;         // keys of the request's new tokens together
+};
+
+__device__ __forceinline__ void segment_tiles(const Kv4Args& a, Segment& s, int r)
+{
+	s.r = r;
+	s.x = kv4_request(a, r);
+	s.rows = s.x.n_new * a.group;
+	s.last = min(s.x.pos0 + s.x.n_new - 1, s.x.keys - 1);
+	s.first = a.window > 0 ? max(0, s.x.pos0 - a.window + 1) : 0;
+	s.tile0 = s.first / TILE;
+	s.tiles = s.rows == 0 ? 0 : s.last < s.first ? 1 : s.last / TILE - s.tile0 + 1;
+}
+
+// Equal runs of `total` tiles over n CTAs: the first total % n one longer.
+struct Runs
+{
+	long long per, rem;
+	__device__ __forceinline__ long long begin(int c) const { return c * per + min((long long)c, rem); }
+	__device__ __forceinline__ int owner(long long t) const
 	{
-		const int mid = (lo + hi + 1) >> 1;
-		if (a.q_start[mid] <= t)
-			lo = mid;
-		else
-			hi = mid - 1;
+		return t < rem * (per + 1) ? (int)(t / (per + 1)) : (int)(rem + (t - rem * (per + 1)) / per);
 	}
-	const Kv4Request x = kv4_request(a, lo);
-	if (t < x.q0 || t - x.q0 >= x.n_new) return;
-	const int pos = x.pos0 + t - x.q0;
-	const int last = min(pos, x.keys - 1), first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-	float q[E], o[E], m = -CUDART_INF_F, l = 0.0f;
-	const float* qp = a.q + (size_t)t * a.q_stride + (size_t)h * D + lane * E;
-#pragma unroll
-	for (int e = 0; e < E; ++e) q[e] = qp[e], o[e] = 0.0f;
-	const int v0 = lane * E, g = v0 / KV4_GROUP;
-	const int cb = kv4_codes_bytes(a.page, D), sb = kv4_scales_bytes(a.page, D);
-	for (int k = first + warp; k <= last; k += SIMPLE_WARPS)
+};
+
+template <int D, int R>
+__global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kernel(const Kv4Args a, const Ws ws)
+{
+	using L = Shape<D, R>;
+	constexpr int U = L::U, J = U / 2, ROWS = L::ROWS;
+	extern __shared__ __align__(128) unsigned char smem[];
+	float* red = reinterpret_cast<float*>(smem + L::SM_RED);
+	uint4* qsm = reinterpret_cast<uint4*>(smem + L::SM_Q);
+	float2* ml = reinterpret_cast<float2*>(smem + L::SM_ML);
+	uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::SM_BAR);
+	uint64_t* empty = full + STAGES;
+	int* loaded = reinterpret_cast<int*>(empty + STAGES); // [STAGES]: which 16-key parts of the tile came
+	volatile int* abort_ = loaded + STAGES;
+	int* last_piece = loaded + STAGES + 1;
+	long long* scan = reinterpret_cast<long long*>(loaded + STAGES + 4); // warp sums, then the start
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+	if (tid == 0)
 	{
-		const int pg = a.table[(size_t)lo * a.table_stride + (k >> a.page_shift)];
-		if (pg < 0 || pg >= a.n_pages) continue;
-		const int off = k & (a.page - 1);
-		const uint8_t* chunk = a.pages + ((size_t)pg * a.n_kv + hk) * kv4_chunk_bytes(a.page, D);
-		const uint8_t* row = chunk + off * (D / 2) + 16 * kv4_unit(off, g, D) + (v0 % KV4_GROUP) / 8 * 4;
-		const uint16_t* sc = reinterpret_cast<const uint16_t*>(chunk + 2 * cb) + off * U + g;
-		const uint32_t kw = *reinterpret_cast<const uint32_t*>(row), vw = *reinterpret_cast<const uint32_t*>(row + cb);
-		const float ks = bf16_bits_to_float(sc[0]), vs = bf16_bits_to_float(sc[sb / 2]);
-		float s = 0.0f;
-#pragma unroll
-		for (int e = 0; e < E; ++e)
-			s = fmaf(q[e], ks * (float)((int)((kw >> (4 * kv4_nibble((v0 + e) & 7))) & 15u) - 8), s);
-		s = warp_sum(s) * a.scale;
-		if (a.softcap > 0.0f) s = a.softcap * tanhf(s / a.softcap);
-		const float mn = fmaxf(m, s);
-		const float c = mn == -CUDART_INF_F ? 0.0f : expf(m - mn), p = mn == -CUDART_INF_F ? 0.0f : expf(s - mn);
-		l = l * c + p;
-#pragma unroll
-		for (int e = 0; e < E; ++e)
-			o[e] = o[e] * c + p * (vs * (float)((int)((vw >> (4 * kv4_nibble((v0 + e) & 7))) & 15u) - 8));
-		m = mn;
+		for (int s = 0; s < STAGES; ++s)
+		{
+			mbar_init(&full[s], 1);
+			mbar_init(&empty[s], CW);
+		}
+		*abort_ = 0;
+		fence_barrier_init();
 	}
+
+	// ---- this CTA's run: a scan of the requests' tiles, each thread a few requests ----
+	const int each = (a.n_req + THREADS - 1) / THREADS;
+	const auto cost = [&](const Segment& s) {
+		return (long long)s.tiles * a.n_kv * ((s.rows + ROWS - 1) / ROWS);
+	};
+	long long mine = 0;
+	for (int r = tid * each; r < min(a.n_req, (tid + 1) * each); ++r)
+	{
+		Segment s;
+		segment_tiles(a, s, r);
+		mine += cost(s);
+	}
+	long long before = mine;
 #pragma unroll
-	for (int e = 0; e < E; ++e) so[warp][v0 + e] = o[e];
-	if (lane == 0) sm[warp] = m, sl[warp] = l;
+	for (int o = 1; o < 32; o <<= 1)
+	{
+		const long long u = __shfl_up_sync(0xffffffffu, before, o);
+		if (lane >= o) before += u;
+	}
+	if (lane == 31) scan[warp] = before;
 	__syncthreads();
-	float mm = -CUDART_INF_F, ll = 0.0f;
-	for (int w = 0; w < SIMPLE_WARPS; ++w) mm = fmaxf(mm, sm[w]);
-	float f[SIMPLE_WARPS];
-	for (int w = 0; w < SIMPLE_WARPS; ++w)
+	long long total = 0;
+	before -= mine;
+	for (int w = 0; w <= CW; ++w)
 	{
-		f[w] = sm[w] == -CUDART_INF_F ? 0.0f : expf(sm[w] - mm);
-		ll += f[w] * sl[w];
+		if (w < warp) before += scan[w];
+		total += scan[w];
 	}
-	for (int d = threadIdx.x; d < D; d += blockDim.x)
+	const int n_ctas = (int)min((long long)gridDim.x, max(1ll, total / MIN_TILES));
+	const Runs runs{total / n_ctas, total % n_ctas};
+	if ((int)blockIdx.x >= n_ctas || total == 0) return;
+	const long long run0 = runs.begin(blockIdx.x);
+	__syncthreads();
+	if (before <= run0 && run0 < before + mine)
 	{
-		float y = 0.0f;
-		for (int w = 0; w < SIMPLE_WARPS; ++w)
-			if (f[w] != 0.0f) y += f[w] * so[w][d];
-		a.out[(size_t)t * a.out_stride + (size_t)h * D + d] = ll != 0.0f ? y / ll : 0.0f;
+		long long at = before;
+		for (int r = tid * each;; ++r)
+		{
+			Segment s;
+			segment_tiles(a, s, r);
+			const long long c = cost(s);
+			if (run0 < at + c)
+			{
+				scan[0] = r;
+				scan[1] = run0 - at;
+				break;
+			}
+			at += c;
+		}
 	}
+	__syncthreads();
+	const int start_req = (int)scan[0];
+	const long long start_off = scan[1];
+	int left = (int)(runs.begin(blockIdx.x + 1) - run0);
+
+	// the pieces of the run, one after another (the same for every warp)
+	Segment s;
+	segment_tiles(a, s, start_req);
+	int groups = (s.rows + ROWS - 1) / ROWS;
+	int seg = (int)(start_off / s.tiles), tile = (int)(start_off % s.tiles); // segment of the request, tile of the segment
+	long long seg_at = run0 - tile;                                          // the segment's first tile among all
+	const auto next_piece = [&](int done) {
+		left -= done;
+		seg_at += s.tiles;
+		tile = 0;
+		if (left > 0 && ++seg == a.n_kv * groups)
+		{
+			seg = 0;
+			int r = s.r;
+			do segment_tiles(a, s, ++r);
+			while (s.rows == 0);
+			groups = (s.rows + ROWS - 1) / ROWS;
+		}
+	};
+
+	if (warp == CW)
+	{
+		// ---- the loading warp: lane = 4 x part of the tile + {K codes, V codes, K scales, V scales} ----
+		const int parts = min(TILE, a.page), n_parts = TILE / parts; // keys a part, parts a tile
+		const int what = lane & 3, part = lane >> 2;
+		const int cb = kv4_codes_bytes(a.page, D), sb = kv4_scales_bytes(a.page, D);
+		const uint32_t bytes = what < 2 ? parts * (D / 2) : parts * U * 2;
+		const int src0 = what < 2 ? what * cb : 2 * cb + (what - 2) * sb;
+		const int dst0 = what < 2 ? what * L::CODES : 2 * L::CODES + (what - 2) * L::SCALES;
+		const int row_bytes = what < 2 ? D / 2 : U * 2;
+		int it = 0;
+		while (left > 0)
+		{
+			const int n = min(left, s.tiles - tile), hk = seg / groups;
+			const int* table = a.table + (size_t)s.r * a.table_stride;
+			int ids = -1, base = -1; // 32 entries of the table from page `base`
+			for (int t = tile; t < tile + n; ++t, ++it)
+			{
+				const int stage = it % STAGES;
+				if (it >= STAGES && !*abort_ && !mbar_wait_bounded(&empty[stage], ((it / STAGES) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY))
+					*abort_ = 1;
+				__syncwarp();
+				const bool stop = __shfl_sync(0xffffffffu, *abort_, 0) != 0; // one answer for the warp
+				const int key0 = (s.tile0 + t) * TILE, page0 = key0 >> a.page_shift;
+				if (base < 0 || page0 + n_parts > base + 32)
+				{
+					base = page0;
+					ids = base + lane < a.max_blocks ? table[base + lane] : -1;
+				}
+				const int k0 = key0 + part * parts; // this lane's part: its first key
+				const int id = __shfl_sync(0xffffffffu, ids, page0 - base + (part < n_parts ? part : 0));
+				const bool get = !stop && part < n_parts && id >= 0 && id < a.n_pages && k0 <= s.last && k0 + parts > s.first;
+				const unsigned got = __ballot_sync(0xffffffffu, get);
+				if (lane == 0)
+				{
+					int mask = 0;
+					for (int p = 0; p < n_parts; ++p)
+						if (got >> (4 * p) & 1) mask |= ((1 << (parts / 16)) - 1) << (p * (parts / 16));
+					loaded[stage] = mask;
+					mbar_arrive_expect_tx(&full[stage], __popc(got) / 4 * 2 * (uint32_t)(parts * (D / 2) + parts * U * 2));
+				}
+				__syncwarp();
+				if (get)
+				{
+					const int off = k0 & (a.page - 1);
+					bulk_g2s(smem + stage * L::STAGE + dst0 + part * parts * row_bytes,
+					         a.pages + ((size_t)id * a.n_kv + hk) * kv4_chunk_bytes(a.page, D) + src0 + off * row_bytes, bytes,
+					         &full[stage]);
+				}
+			}
+			next_piece(n);
+		}
+		// after a wait that ran out nobody may have waited for the copies in flight: not to leave before they landed
+		if (*abort_)
+			for (int i = max(0, it - STAGES); i < it; ++i)
+				mbar_wait_bounded(&full[i % STAGES], (i / STAGES) & 1, nullptr, 0);
+		return;
+	}
+
+	// ---- the computing warps ----
+	const int c4 = lane & 3, i8 = lane >> 2;
+	// K: this lane's two rows of the products, keys ka and ka + 8 of the warp's 16; V: keys c4 + 4 kk
+	const int ka = warp * 16 + (i8 >> 1) + 4 * (i8 & 1);
+	const int k_off = ka * (D / 2) + 4 * c4, k_swz = (ka * D / 256) & (U - 1);
+	int v_off[2];
+#pragma unroll
+	for (int kk = 0; kk < 2; ++kk)
+	{
+		const int key = warp * 16 + c4 + 4 * kk;
+		v_off[kk] = key * (D / 2) + 16 * (((i8 >> 2) * J) ^ ((key * D / 256) & (U - 1))) + 4 * (i8 & 3);
+	}
+	int it = 0;
+	while (left > 0)
+	{
+		const int n = min(left, s.tiles - tile), hk = seg / groups;
+		s.row0 = (seg - hk * groups) * ROWS;
+
+		// q's rows as operands: column i8 of row tile r is row s.row0 + 8 r + i8
+		uint32_t qf[L::Q_REGS ? D / 16 * R * 4 : 1];
+		float q0[R][U][2], mult[R][2]; // -8 x the group's sum of q; what turns a product into a base-2 score
+		int kf[R][2], kl[R][2];        // keys that columns 2 c4 and 2 c4 + 1 see
+		float m[R][2], l[R][2];
+		int all_from = 0, all_to = INT_MAX; // keys that every row sees
+#pragma unroll
+		for (int r = 0; r < R; ++r)
+		{
+			const int row = s.row0 + 8 * r + i8;
+			const bool real = row < s.rows;
+			const float* qp = nullptr;
+			if (real)
+			{
+				const int t = row / a.group;
+				qp = a.q + (size_t)(s.x.q0 + t) * a.q_stride + (size_t)(hk * a.group + row - t * a.group) * D + 8 * c4;
+			}
+			float v[U][8], top = 0.0f;
+#pragma unroll
+			for (int g = 0; g < U; ++g)
+			{
+				const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+				const float4 x = real ? *reinterpret_cast<const float4*>(qp + 32 * g) : z;
+				const float4 y = real ? *reinterpret_cast<const float4*>(qp + 32 * g + 4) : z;
+				v[g][0] = x.x, v[g][1] = x.y, v[g][2] = x.z, v[g][3] = x.w;
+				v[g][4] = y.x, v[g][5] = y.y, v[g][6] = y.z, v[g][7] = y.w;
+#pragma unroll
+				for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[g][e]));
+			}
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+			top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+			// the power of two that brings the row's largest value to [2^14, 2^15)
+			const int ex = top > 0.0f ? max(-100, min(100, ilogbf(top))) : 0;
+			const float f = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
+			float sum[U];
+#pragma unroll
+			for (int g = 0; g < U; ++g)
+			{
+				sum[g] = 0.0f;
+#pragma unroll
+				for (int h = 0; h < 2; ++h)
+				{
+					uint32_t b[4]; // hi of values 4h, 4h+1 | 4h+2, 4h+3 (a nibble up: / 16), lo of both
+					const float w = f * 0.0625f;
+					split2(v[g][4 * h] * f, v[g][4 * h + 1] * f, b[0], b[2]);
+					split2(v[g][4 * h + 2] * w, v[g][4 * h + 3] * w, b[1], b[3]);
+					float2 p = __half22float2(bits_half2(b[0])), q = __half22float2(bits_half2(b[2]));
+					sum[g] += (p.x + q.x) + (p.y + q.y);
+					p = __half22float2(bits_half2(b[1])), q = __half22float2(bits_half2(b[3]));
+					sum[g] += 16.0f * ((p.x + q.x) + (p.y + q.y));
+					if constexpr (L::Q_REGS)
+					{
+#pragma unroll
+						for (int e = 0; e < 4; ++e) qf[((2 * g + h) * R + r) * 4 + e] = b[e];
+					}
+					else if ((g & (CW - 1)) == warp)
+						qsm[((2 * g + h) * R + r) * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+				}
+				sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+				sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+			}
+#pragma unroll
+			for (int e = 0; e < 2; ++e)
+			{
+				const int from = (2 * c4 + e) * 4;
+#pragma unroll
+				for (int g = 0; g < U; ++g) q0[r][g][e] = __shfl_sync(0xffffffffu, sum[g], from) * (-8.0f * 0x1p-24f);
+				mult[r][e] = a.scale * 0x1p24f / __shfl_sync(0xffffffffu, f, from);
+				const int row2 = s.row0 + 8 * r + 2 * c4 + e;
+				const int pos = s.x.pos0 + row2 / a.group;
+				kf[r][e] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+				kl[r][e] = row2 < s.rows ? min(pos, s.x.keys - 1) : -1;
+				m[r][e] = -CUDART_INF_F;
+				l[r][e] = 0.0f;
+				if (row2 < s.rows)
+				{
+					all_from = max(all_from, kf[r][e]);
+					all_to = min(all_to, kl[r][e]);
+				}
+			}
+		}
+#pragma unroll
+		for (int o = 1; o < 4; o <<= 1)
+		{
+			all_from = max(all_from, __shfl_xor_sync(0xffffffffu, all_from, o));
+			all_to = min(all_to, __shfl_xor_sync(0xffffffffu, all_to, o));
+		}
+		if constexpr (!L::Q_REGS) named_sync(1, CW * 32);
+
+		float o[J * 4][R][4];
+#pragma unroll
+		for (int x = 0; x < J * 4; ++x)
+#pragma unroll
+			for (int r = 0; r < R; ++r)
+#pragma unroll
+				for (int e = 0; e < 4; ++e) o[x][r][e] = 0.0f;
+		bool bad = false; // a visible V scale that is no number
+
+		for (int t = tile; t < tile + n; ++t, ++it)
+		{
+			const int stage = it % STAGES;
+			if (!*abort_ && !mbar_wait_bounded(&full[stage], (it / STAGES) & 1, ws.err, DEVERR_WAIT_FULL)) *abort_ = 1;
+			const unsigned char* st = smem + stage * L::STAGE;
+			const int key0 = (s.tile0 + t) * TILE + warp * 16;
+			if (loaded[stage] >> warp & 1)
+			{
+				// ---- scores of 16 keys ----
+				float sc[R][4];
+#pragma unroll
+				for (int r = 0; r < R; ++r)
+#pragma unroll
+					for (int e = 0; e < 4; ++e) sc[r][e] = 0.0f;
+				const uint16_t* ks = reinterpret_cast<const uint16_t*>(st + 2 * L::CODES) + ka * U;
+#pragma unroll
+				for (int g = 0; g < U; ++g)
+				{
+					const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + k_off + 16 * (g ^ k_swz));
+					const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + k_off + 16 * (g ^ k_swz) + 8 * (D / 2));
+					const float s0 = bf16_bits_to_float(ks[g]), s1 = bf16_bits_to_float(ks[g + 8 * U]);
+					const uint32_t x0 = w0 >> 8, x1 = w1 >> 8;
+#pragma unroll
+					for (int r = 0; r < R; ++r)
+					{
+						float d[4] = {q0[r][g][0], q0[r][g][1], q0[r][g][0], q0[r][g][1]};
+						uint4 b, e;
+						if constexpr (L::Q_REGS)
+						{
+							const uint32_t* p = &qf[(2 * g * R + r) * 4];
+							b = make_uint4(p[0], p[1], p[2], p[3]);
+							p += R * 4;
+							e = make_uint4(p[0], p[1], p[2], p[3]);
+						}
+						else
+						{
+							b = qsm[(2 * g * R + r) * 32 + lane];
+							e = qsm[((2 * g + 1) * R + r) * 32 + lane];
+						}
+						const uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u;
+						mma16816(d, w0 & lo, w1 & lo, w0 & hi, w1 & hi, b.x, b.y);
+						mma16816(d, w0 & lo, w1 & lo, w0 & hi, w1 & hi, b.z, b.w);
+						mma16816(d, x0 & lo, x1 & lo, x0 & hi, x1 & hi, e.x, e.y);
+						mma16816(d, x0 & lo, x1 & lo, x0 & hi, x1 & hi, e.z, e.w);
+						sc[r][0] = fmaf(d[0], s0, sc[r][0]);
+						sc[r][1] = fmaf(d[1], s0, sc[r][1]);
+						sc[r][2] = fmaf(d[2], s1, sc[r][2]);
+						sc[r][3] = fmaf(d[3], s1, sc[r][3]);
+					}
+				}
+				// ---- weights ----
+				const bool edge = key0 < all_from || key0 + 15 > all_to;
+				const int kx = key0 + (ka & 15);
+				uint32_t ph[R][2], pl[R][2]; // [keys 0-7 | 8-15], transposed: the second product's operand
+#pragma unroll
+				for (int r = 0; r < R; ++r)
+				{
+					float alpha[2], ref[2];
+#pragma unroll
+					for (int e = 0; e < 2; ++e)
+					{
+						float x0 = sc[r][e] * mult[r][e], x1 = sc[r][e + 2] * mult[r][e];
+						if (a.softcap > 0.0f)
+						{
+							x0 = a.softcap * tanhf(x0 / a.softcap);
+							x1 = a.softcap * tanhf(x1 / a.softcap);
+						}
+						x0 *= 1.4426950408889634f;
+						x1 *= 1.4426950408889634f;
+						if (edge)
+						{
+							if (kx < kf[r][e] || kx > kl[r][e]) x0 = -CUDART_INF_F;
+							if (kx + 8 < kf[r][e] || kx + 8 > kl[r][e]) x1 = -CUDART_INF_F;
+						}
+						float top = fmaxf(x0, x1);
+#pragma unroll
+						for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+						const float mn = fmaxf(m[r][e], top);
+						ref[e] = mn == -CUDART_INF_F ? 0.0f : mn - P_SCALE_LOG2;
+						alpha[e] = mn == m[r][e] ? 1.0f : ex2(m[r][e] - mn);
+						m[r][e] = mn;
+						sc[r][e] = ex2(x0 - ref[e]);
+						sc[r][e + 2] = ex2(x1 - ref[e]);
+						l[r][e] = fmaf(l[r][e], alpha[e], sc[r][e] + sc[r][e + 2]);
+					}
+					if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f))
+					{
+#pragma unroll
+						for (int x = 0; x < J * 4; ++x)
+						{
+							o[x][r][0] *= alpha[0];
+							o[x][r][1] *= alpha[1];
+							o[x][r][2] *= alpha[0];
+							o[x][r][3] *= alpha[1];
+						}
+					}
+#pragma unroll
+					for (int h = 0; h < 2; ++h)
+					{
+						uint32_t hi, lo;
+						split2(sc[r][2 * h], sc[r][2 * h + 1], hi, lo);
+						ph[r][h] = transpose8(hi);
+						pl[r][h] = transpose8(lo);
+					}
+				}
+				// ---- values: keys c4 + 4 kk of the warp's 16, J words of codes each ----
+				const unsigned char* sv = st + L::CODES;
+				const uint16_t* vs = reinterpret_cast<const uint16_t*>(st + 2 * L::CODES + L::SCALES);
+#pragma unroll
+				for (int j = 0; j < J; ++j)
+				{
+					__half2 s2[2], b2[2]; // the scales of key pairs (0, 1) and (2, 3), and -24 times them
+					uint32_t lo[2], hi[2];
+#pragma unroll
+					for (int pr = 0; pr < 2; ++pr)
+					{
+						float f[2];
+						uint32_t w[2];
+#pragma unroll
+						for (int e = 0; e < 2; ++e)
+						{
+							const int kk = 2 * pr + e, key = warp * 16 + c4 + 4 * kk;
+							w[e] = *reinterpret_cast<const uint32_t*>(sv + (v_off[e] ^ (16 * j)) + pr * 8 * (D / 2));
+							f[e] = bf16_bits_to_float(vs[key * U + (i8 >> 2) * J + j]);
+							if (!(fabsf(f[e]) <= KV4_SCALE_MAX))
+							{
+								// no number (or, past the request's keys, whatever was there): its weight's product
+								// would be none either, also where the weight is zero
+								const int k = key0 + c4 + 4 * kk;
+								bad |= k >= s.first && k <= s.last;
+								f[e] = 0.0f;
+							}
+						}
+						s2[pr] = __floats2half2_rn(f[0], f[1]);
+						b2[pr] = __hmul2(s2[pr], __float2half2_rn(-24.0f));
+						lo[pr] = __byte_perm(w[0], w[1], 0x5410);
+						hi[pr] = __byte_perm(w[0], w[1], 0x7632);
+					}
+#pragma unroll
+					for (int x = 0; x < 4; ++x)
+					{
+						// nibble x to bits 6-9 of each half: 16 + u
+						const auto widen = [&](uint32_t w, int pr) {
+							const uint32_t sh = x == 0 ? w << 6 : x == 1 ? w << 2 : x == 2 ? w >> 2 : w >> 6;
+							return half2_bits(__hfma2(bits_half2((sh & 0x03C003C0u) | 0x4C004C00u), s2[pr], b2[pr]));
+						};
+						const uint32_t a0 = widen(lo[0], 0), a1 = widen(hi[0], 0), a2 = widen(lo[1], 1), a3 = widen(hi[1], 1);
+#pragma unroll
+						for (int r = 0; r < R; ++r)
+						{
+							mma16816(o[j * 4 + x][r], a0, a1, a2, a3, ph[r][0], ph[r][1]);
+							mma16816(o[j * 4 + x][r], a0, a1, a2, a3, pl[r][0], pl[r][1]);
+						}
+					}
+				}
+			}
+			__syncwarp();
+			if (lane == 0) mbar_arrive(&empty[stage]);
+		}
+
+		// ---- the piece's end: the four warps' states joined ----
+#pragma unroll
+		for (int r = 0; r < R; ++r)
+#pragma unroll
+			for (int e = 0; e < 2; ++e)
+			{
+#pragma unroll
+				for (int w = 4; w < 32; w <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], w);
+				if (i8 == 0) ml[warp * ROWS + 8 * r + 2 * c4 + e] = make_float2(m[r][e], l[r][e]);
+			}
+		const bool any_bad = named_sync_or(1, CW * 32, bad);
+#pragma unroll
+		for (int r = 0; r < R; ++r)
+#pragma unroll
+			for (int e = 0; e < 2; ++e)
+			{
+				const int col = 8 * r + 2 * c4 + e;
+				float top = ml[col].x;
+#pragma unroll
+				for (int w = 1; w < CW; ++w) top = fmaxf(top, ml[w * ROWS + col].x);
+				const float f = m[r][e] == top ? 1.0f : ex2(m[r][e] - top);
+				float* dst = red + (warp * ROWS + col) * L::RED_ROW + 32 * ((i8 >> 2) * J) + 8 * (i8 & 3);
+#pragma unroll
+				for (int j = 0; j < J; ++j)
+				{
+					float4 y[2];
+					y[0] = make_float4(o[4 * j][r][e] * f, o[4 * j][r][e + 2] * f, o[4 * j + 1][r][e] * f, o[4 * j + 1][r][e + 2] * f);
+					y[1] = make_float4(o[4 * j + 2][r][e] * f, o[4 * j + 2][r][e + 2] * f, o[4 * j + 3][r][e] * f,
+					                   o[4 * j + 3][r][e + 2] * f);
+					reinterpret_cast<float4*>(dst + 32 * j)[0] = y[0];
+					reinterpret_cast<float4*>(dst + 32 * j)[1] = y[1];
+				}
+			}
+		// (the weights of a row, for the threads that finish it below)
+		constexpr int QUADS = D / 4, MINE = ROWS * QUADS / (CW * 32);
+		float top[MINE], sum[MINE];
+#pragma unroll
+		for (int x = 0; x < MINE; ++x)
+		{
+			const int row = (tid + x * CW * 32) / QUADS;
+			top[x] = ml[row].x;
+#pragma unroll
+			for (int w = 1; w < CW; ++w) top[x] = fmaxf(top[x], ml[w * ROWS + row].x);
+			sum[x] = 0.0f;
+#pragma unroll
+			for (int w = 0; w < CW; ++w)
+			{
+				const float2 y = ml[w * ROWS + row];
+				sum[x] = fmaf(y.y, y.x == top[x] ? 1.0f : ex2(y.x - top[x]), sum[x]);
+			}
+		}
+		named_sync(1, CW * 32);
+		const bool whole = tile == 0 && n == s.tiles;
+		const int c_first = whole ? 0 : runs.owner(seg_at), c_last = whole ? 0 : runs.owner(seg_at + s.tiles - 1);
+		// where CTA c's piece of this segment lies: behind its first, if the segment begins inside its run
+		const auto slot = [&](int c) {
+			return ws.parts + (size_t)(2 * c + (c == c_first && runs.begin(c) < seg_at)) * L::PART;
+		};
+#pragma unroll
+		for (int x = 0; x < MINE; ++x)
+		{
+			const int item = tid + x * CW * 32, row = item / QUADS, d = item % QUADS * 4;
+			float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+			for (int w = 0; w < CW; ++w)
+			{
+				const float4 z = *reinterpret_cast<const float4*>(red + (w * ROWS + row) * L::RED_ROW + d);
+				y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+			}
+			const int rr = s.row0 + row;
+			if (any_bad && rr < s.rows)
+			{
+				// a row that sees a value that is no number has none in the group
+				const int pos = s.x.pos0 + rr / a.group;
+				const int from = max(a.window > 0 ? max(0, pos - a.window + 1) : 0, (s.tile0 + tile) * TILE);
+				const int to = min(min(pos, s.x.keys - 1), (s.tile0 + tile + n) * TILE - 1);
+				for (int k = from; k <= to; ++k)
+				{
+					const int id = a.table[(size_t)s.r * a.table_stride + (k >> a.page_shift)];
+					if (id < 0 || id >= a.n_pages) continue;
+					const uint8_t* chunk = a.pages + ((size_t)id * a.n_kv + hk) * kv4_chunk_bytes(a.page, D);
+					const uint16_t* vs = reinterpret_cast<const uint16_t*>(chunk + 2 * kv4_codes_bytes(a.page, D) +
+					                                                       kv4_scales_bytes(a.page, D));
+					const float f = bf16_bits_to_float(vs[(k & (a.page - 1)) * U + d / KV4_GROUP]);
+					if (!(fabsf(f) <= KV4_SCALE_MAX)) y.x = y.y = y.z = y.w = CUDART_NAN_F;
+				}
+			}
+			if (whole)
+			{
+				if (rr < s.rows)
+				{
+					const float inv = sum[x] == 0.0f ? 0.0f : 1.0f / sum[x];
+					const int tk = rr / a.group;
+					*reinterpret_cast<float4*>(a.out + (size_t)(s.x.q0 + tk) * a.out_stride +
+					                           (size_t)(hk * a.group + rr - tk * a.group) * D + d) =
+						make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+				}
+			}
+			else
+			{
+				float* p = slot(blockIdx.x);
+				*reinterpret_cast<float4*>(p + row * D + d) = y;
+				if (d == 0) *reinterpret_cast<float2*>(p + ROWS * D + 2 * row) = make_float2(top[x], sum[x]);
+			}
+		}
+		if (!whole)
+		{
+			__threadfence();
+			named_sync(1, CW * 32);
+			if (tid == 0)
+			{
+				const int was = atomicAdd(&ws.counters[c_first], 1);
+				*last_piece = was == c_last - c_first;
+				if (*last_piece) ws.counters[c_first] = 0; // ready for the next call
+			}
+			named_sync(1, CW * 32);
+			if (*last_piece)
+			{
+				// the last piece of the segment: all of them joined, in order
+				__threadfence();
+				for (int item = tid; item < ROWS * QUADS; item += CW * 32)
+				{
+					const int row = item / QUADS, d = item % QUADS * 4, rr = s.row0 + row;
+					if (rr >= s.rows) continue;
+					float mx = -CUDART_INF_F, w = 0.0f;
+					for (int c = c_first; c <= c_last; ++c) mx = fmaxf(mx, __ldcg(slot(c) + ROWS * D + 2 * row));
+					float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+					for (int c = c_first; c <= c_last; ++c)
+					{
+						const float* p = slot(c);
+						const float2 z = __ldcg(reinterpret_cast<const float2*>(p + ROWS * D + 2 * row));
+						const float4 u = __ldcg(reinterpret_cast<const float4*>(p + row * D + d));
+						const float f = z.x == mx ? 1.0f : ex2(z.x - mx);
+						w = fmaf(z.y, f, w);
+						y.x = fmaf(u.x, f, y.x), y.y = fmaf(u.y, f, y.y), y.z = fmaf(u.z, f, y.z), y.w = fmaf(u.w, f, y.w);
+					}
+					const float inv = w == 0.0f ? 0.0f : 1.0f / w;
+					const int tk = rr / a.group;
+					*reinterpret_cast<float4*>(a.out + (size_t)(s.x.q0 + tk) * a.out_stride +
+					                           (size_t)(hk * a.group + rr - tk * a.group) * D + d) =
+						make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+				}
+			}
+		}
+		next_piece(n);
+	}
+}
+
+constexpr int MAX_SMS = 192;
+
+template <int D, int R>
+constexpr size_t ws_bytes(int sms)
+{
+	const size_t ctas = (size_t)sms * Shape<D, R>::CTAS;
+	return 256 + (ctas * 4 + 255) / 256 * 256 + ctas * 2 * Shape<D, R>::PART * 4;
+}
+
+int num_sms()
+{
+	static int known[64] = {};
+	int dev = 0;
+	if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+	if (known[dev] == 0 && cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+		return 0;
+	return known[dev];
+}
+
+template <int D, int R>
+int launch_decode4(const Kv4Args& a, void* workspace, cudaStream_t st)
+{
+	using L = Shape<D, R>;
+	static bool configured[64] = {};
+	int dev = 0;
+	cudaGetDevice(&dev);
+	if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+	auto kernel = kv4_decode_kernel<D, R>;
+	if (!configured[dev])
+	{
+		const cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+		if (ce != cudaSuccess) return (int)ce;
+		configured[dev] = true;
+	}
+	const int ctas = num_sms() * L::CTAS;
+	if (ctas == 0) return (int)cudaErrorInvalidDevice;
+	unsigned char* w = static_cast<unsigned char*>(workspace);
+	const Ws ws{reinterpret_cast<int*>(w), reinterpret_cast<int*>(w + 256),
+	            reinterpret_cast<float*>(w + 256 + ((size_t)ctas * 4 + 255) / 256 * 256)};
+	kernel<<<ctas, THREADS, L::SMEM, st>>>(a, ws);
+	note_launches(1);
+	return (int)cudaGetLastError();
 }
 
 int refuse(const char* msg) { return set_error(NNCU_ERR_INVALID_ARGUMENT, msg); }
@@ -116,8 +791,25 @@ extern "C" int nncu_kv4_workspace_bytes(const nncu_kv4_attn* a, size_t* bytes)
 	const int rc = check_shape(a, false);
 	if (rc != NNCU_OK) return rc;
 	if (!bytes) return refuse("kv4 workspace: NULL argument");
-	*bytes = 256;
+	// enough for every variant of the head_dim on any device of this kind
+	*bytes = a->pool.head_dim == 64 ? ws_bytes<64, 4>(MAX_SMS) : a->pool.head_dim == 128 ? ws_bytes<128, 2>(MAX_SMS)
+	                                                                                    : ws_bytes<256, 1>(MAX_SMS);
 	return NNCU_OK;
+}
+
+extern "C" int nncu_kv4_check(const nncu_kv4_attn* a, void* stream)
+{
+	if (!a || !a->workspace || a->workspace_bytes < 256) return refuse("kv4 check: NULL argument or workspace");
+	const auto st = static_cast<cudaStream_t>(stream);
+	int err = 0;
+	cudaError_t ce = cudaMemcpyAsync(&err, a->workspace, sizeof err, cudaMemcpyDeviceToHost, st);
+	if (ce == cudaSuccess) ce = cudaStreamSynchronize(st);
+	if (ce != cudaSuccess) return set_cuda_error((int)ce, "kv4 check");
+	if (err == 0) return NNCU_OK;
+	ce = cudaMemsetAsync(a->workspace, 0, a->workspace_bytes, st);
+	if (ce == cudaSuccess) ce = cudaStreamSynchronize(st);
+	if (ce != cudaSuccess) return set_cuda_error((int)ce, "kv4 check");
+	return set_error(NNCU_ERR_TIMEOUT, "kv4 attention: a kernel's bounded wait ran out; its outputs are void");
 }
 
 extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
@@ -151,14 +843,15 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 	                p->max_new, p->max_blocks, p->window, p->scale, p->softcap, p->block_table, p->table_stride,
 	                p->seq_len, p->q_start, p->q, p->q_stride, p->out, p->out_stride};
 	const auto st = static_cast<cudaStream_t>(stream);
-	const dim3 grid((unsigned)p->n_tok, (unsigned)p->n_head);
-	switch (p->pool.head_dim)
-	{
-	case 64: kv4_simple_kernel<64><<<grid, SIMPLE_WARPS * 32, 0, st>>>(a); break;
-	case 128: kv4_simple_kernel<128><<<grid, SIMPLE_WARPS * 32, 0, st>>>(a); break;
-	default: kv4_simple_kernel<256><<<grid, SIMPLE_WARPS * 32, 0, st>>>(a); break;
-	}
-	note_launches(1);
-	const int e = (int)cudaGetLastError();
+	const long long rows = (long long)a.group * p->max_new;
+	int e;
+	if (a.D == 256)
+		e = launch_decode4<256, 1>(a, p->workspace, st);
+	else if (a.D == 128)
+		e = rows <= 8 ? launch_decode4<128, 1>(a, p->workspace, st) : launch_decode4<128, 2>(a, p->workspace, st);
+	else
+		e = rows <= 8    ? launch_decode4<64, 1>(a, p->workspace, st)
+		    : rows <= 16 ? launch_decode4<64, 2>(a, p->workspace, st)
+		                 : launch_decode4<64, 4>(a, p->workspace, st);
 	return e ? set_cuda_error(e, "kv4 attention launch") : NNCU_OK;
 }

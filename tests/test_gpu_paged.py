@@ -364,7 +364,7 @@ class Attn:
 def test_attention(nncu, torch_cuda, case, slack):
     a = Attn(torch_cuda, nncu, case, slack=slack)
     nncu.kv4_attention_dev(a.call)
-    torch_cuda.cuda.synchronize()
+    nncu.kv4_check(a.call)
     a.check(a.out)
 
 

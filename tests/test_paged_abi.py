@@ -99,7 +99,7 @@ def test_nothing_to_do_is_no_error(L):
 
 def test_null_structs_are_refused(L):
     for f in (L.nncu_paged_step_dev, L.nncu_rope_axes_dev, L.nncu_kv4_append_dev, L.nncu_kv4_read_dev,
-              L.nncu_kv4_attention_dev):
+              L.nncu_kv4_attention_dev, L.nncu_kv4_check):
         refused(f(None, None), L, "NULL")
 
 
