@@ -21,9 +21,9 @@
 // Masking a word of codes leaves u in the low bits of a 16-bit lane, which
 // read as a float is u x 2^-24 (or x 2^-20 one nibble up): an exact operand,
 // with no conversion. The group's sum then takes its scale in 32 bits. V's
-// codes cannot wait for their scale (the sum runs over keys): 16 + u, built by
-// the mask, times s minus 24 s is s (u - 8) in one rounding, and 8 bits of
-// scale times 4 of code are exact in a 16-bit float. q and the weights p go in
+// codes cannot wait for their scale (the sum runs over keys): the mask makes
+// 1024 + u (or 64 + u), less 1032 (72) that is the code, and 8 bits of scale
+// times 4 of code are exact in a 16-bit float. q and the weights p go in
 // as two 16-bit halves each (22 bits), accumulated in 32: the result is as
 // close to the exact one as 32-bit arithmetic. p carries 2^15 so that small
 // weights keep their digits.
@@ -42,9 +42,13 @@ namespace
 constexpr int TILE = 64;               // keys a tile
 constexpr int CW = 4;                  // computing warps, 16 keys of a tile each
 constexpr int THREADS = (CW + 1) * 32; // and the loading warp
-constexpr int STAGES = 4;
+constexpr int STAGES = 3;              // tiles in the ring: what arrives while one is worked on
 constexpr int MIN_TILES = 2;           // a run is at least this long, while tiles are few
-constexpr float P_SCALE_LOG2 = 15.0f;
+// A row's weights are taken against a held score, 2^11 at it, which moves only
+// when a score passes it by more than 2^4: then no weight passes 2^15, within a
+// 16-bit float, and weights of 2^-24 of the largest keep 11 bits and more.
+constexpr float P_SCALE = 11.0f, P_TOP = 15.0f;
+constexpr float NONE = 1e30f; // P_SCALE - held score of a row that has seen no key yet
 
 // What a launch keeps in the workspace: an error word, a counter per CTA (of
 // the segment that begins in the CTA's run and does not end there), and two
@@ -63,14 +67,17 @@ struct Shape
 	static constexpr int CODES = TILE * D / 2, SCALES = TILE * U * 2;
 	static constexpr int STAGE = 2 * (CODES + SCALES);
 	static constexpr int RED_ROW = D + 4;                   // floats a row of the joining buffer
-	static constexpr bool Q_REGS = D * R <= 128;            // q's operands in registers (or in shared memory)
 	static constexpr int SM_RED = STAGES * STAGE;           // [CW][ROWS][RED_ROW]
-	static constexpr int SM_Q = SM_RED + CW * ROWS * RED_ROW * 4;
-	static constexpr int SM_ML = SM_Q + (Q_REGS ? 0 : D / 16 * R * 512); // [CW][ROWS] (maximum, weight)
+	static constexpr int SM_Q = SM_RED + CW * ROWS * RED_ROW * 4; // q's operands [D / 16][R][32 lanes] of 16 bytes
+	static constexpr int SM_Q0 = SM_Q + D / 16 * R * 512;   // -8 x the groups' sums of q [R][U][8 rows]
+	static constexpr int SM_ML = SM_Q0 + R * U * 32;        // [CW][ROWS] (maximum, weight)
 	static constexpr int SM_BAR = SM_ML + CW * ROWS * 8;
 	static constexpr int SMEM = SM_BAR + 256;
+	static_assert(SM_BAR % 16 == 0 && SM_Q % 16 == 0 && SM_RED % 16 == 0 && SCALES % 16 == 0, "aligned for their accesses");
+	static_assert(2 * STAGES * 8 + (STAGES + 2) * 4 <= 128, "barriers and words before the scan");
 	static constexpr int PART = ROWS * (D + 2);             // floats a partial result
-	static constexpr int CTAS = D == 256 ? 2 : 3;           // per SM
+	static constexpr int CTAS = D * R <= 128 ? 4 : D == 256 ? 2 : 3; // per SM
+	static_assert(192 * CTAS * 4 <= 4096, "a counter per CTA");
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -99,6 +106,33 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 	const float2 f = __half22float2(h);
 	hi = half2_bits(h);
 	lo = half2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// N neighbouring scales.
+template <int N>
+__device__ __forceinline__ void load_scales(float (&f)[N], const unsigned char* p)
+{
+	if constexpr (N == 1)
+		f[0] = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(p));
+	else
+	{
+		uint32_t w[N / 2];
+		if constexpr (N == 2)
+			w[0] = *reinterpret_cast<const uint32_t*>(p);
+		else if constexpr (N == 4)
+		{
+			const uint2 x = *reinterpret_cast<const uint2*>(p);
+			w[0] = x.x, w[1] = x.y;
+		}
+		else
+		{
+			const uint4 x = *reinterpret_cast<const uint4*>(p);
+			w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+		}
+#pragma unroll
+		for (int i = 0; i < N / 2; ++i)
+			f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+	}
 }
 
 // One segment's rows and the tiles of its keys.
@@ -140,13 +174,14 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 	extern __shared__ __align__(128) unsigned char smem[];
 	float* red = reinterpret_cast<float*>(smem + L::SM_RED);
 	uint4* qsm = reinterpret_cast<uint4*>(smem + L::SM_Q);
+	float* q0 = reinterpret_cast<float*>(smem + L::SM_Q0);
 	float2* ml = reinterpret_cast<float2*>(smem + L::SM_ML);
 	uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::SM_BAR);
 	uint64_t* empty = full + STAGES;
 	int* loaded = reinterpret_cast<int*>(empty + STAGES); // [STAGES]: which 16-key parts of the tile came
 	volatile int* abort_ = loaded + STAGES;
 	int* last_piece = loaded + STAGES + 1;
-	long long* scan = reinterpret_cast<long long*>(loaded + STAGES + 4); // warp sums, then the start
+	long long* scan = reinterpret_cast<long long*>(smem + L::SM_BAR + 128); // warp sums, then the start
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
 	if (tid == 0)
@@ -298,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 	const int c4 = lane & 3, i8 = lane >> 2;
 	// K: this lane's two rows of the products, keys ka and ka + 8 of the warp's 16; V: keys c4 + 4 kk
 	const int ka = warp * 16 + (i8 >> 1) + 4 * (i8 & 1);
-	const int k_off = ka * (D / 2) + 4 * c4, k_swz = (ka * D / 256) & (U - 1);
+	const int k_off = ka * (D / 2) + 16 * ((ka * D / 256) & (U - 1)) + 4 * c4;
 	int v_off[2];
 #pragma unroll
 	for (int kk = 0; kk < 2; ++kk)
@@ -306,6 +341,9 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 		const int key = warp * 16 + c4 + 4 * kk;
 		v_off[kk] = key * (D / 2) + 16 * (((i8 >> 2) * J) ^ ((key * D / 256) & (U - 1))) + 4 * (i8 & 3);
 	}
+	// scores in base 2 (with a soft-cap: its argument, and what multiplies its value)
+	const float scale2 = a.softcap > 0.0f ? a.scale * 0x1p24f / a.softcap : a.scale * (0x1p24f * 1.4426950408889634f);
+	const float softcap2 = a.softcap * 1.4426950408889634f;
 	int it = 0;
 	while (left > 0)
 	{
@@ -313,10 +351,9 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 		s.row0 = (seg - hk * groups) * ROWS;
 
 		// q's rows as operands: column i8 of row tile r is row s.row0 + 8 r + i8
-		uint32_t qf[L::Q_REGS ? D / 16 * R * 4 : 1];
-		float q0[R][U][2], mult[R][2]; // -8 x the group's sum of q; what turns a product into a base-2 score
-		int kf[R][2], kl[R][2];        // keys that columns 2 c4 and 2 c4 + 1 see
-		float m[R][2], l[R][2];
+		float mult[R][2];              // what turns a product into a base-2 score
+		int at[R][2];                  // positions of columns 2 c4 and 2 c4 + 1 (-1: no row)
+		float held[R][2], l[R][2];     // P_SCALE - held score, sum of the weights
 		int all_from = 0, all_to = INT_MAX; // keys that every row sees
 #pragma unroll
 		for (int r = 0; r < R; ++r)
@@ -362,34 +399,26 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 					sum[g] += (p.x + q.x) + (p.y + q.y);
 					p = __half22float2(bits_half2(b[1])), q = __half22float2(bits_half2(b[3]));
 					sum[g] += 16.0f * ((p.x + q.x) + (p.y + q.y));
-					if constexpr (L::Q_REGS)
-					{
-#pragma unroll
-						for (int e = 0; e < 4; ++e) qf[((2 * g + h) * R + r) * 4 + e] = b[e];
-					}
-					else if ((g & (CW - 1)) == warp)
+					if ((g & (CW - 1)) == warp)
 						qsm[((2 * g + h) * R + r) * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
 				}
 				sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
 				sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+				if ((g & (CW - 1)) == warp && c4 == 0) q0[(r * U + g) * 8 + i8] = sum[g] * (-8.0f * 0x1p-24f);
 			}
 #pragma unroll
 			for (int e = 0; e < 2; ++e)
 			{
 				const int from = (2 * c4 + e) * 4;
-#pragma unroll
-				for (int g = 0; g < U; ++g) q0[r][g][e] = __shfl_sync(0xffffffffu, sum[g], from) * (-8.0f * 0x1p-24f);
-				mult[r][e] = a.scale * 0x1p24f / __shfl_sync(0xffffffffu, f, from);
+				mult[r][e] = scale2 / __shfl_sync(0xffffffffu, f, from);
 				const int row2 = s.row0 + 8 * r + 2 * c4 + e;
-				const int pos = s.x.pos0 + row2 / a.group;
-				kf[r][e] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-				kl[r][e] = row2 < s.rows ? min(pos, s.x.keys - 1) : -1;
-				m[r][e] = -CUDART_INF_F;
+				at[r][e] = row2 < s.rows ? s.x.pos0 + row2 / a.group : -1;
+				held[r][e] = NONE;
 				l[r][e] = 0.0f;
 				if (row2 < s.rows)
 				{
-					all_from = max(all_from, kf[r][e]);
-					all_to = min(all_to, kl[r][e]);
+					all_from = max(all_from, a.window > 0 ? at[r][e] - a.window + 1 : 0);
+					all_to = min(all_to, min(at[r][e], s.x.keys - 1));
 				}
 			}
 		}
@@ -399,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 			all_from = max(all_from, __shfl_xor_sync(0xffffffffu, all_from, o));
 			all_to = min(all_to, __shfl_xor_sync(0xffffffffu, all_to, o));
 		}
-		if constexpr (!L::Q_REGS) named_sync(1, CW * 32);
+		named_sync(1, CW * 32);
 
 		float o[J * 4][R][4];
 #pragma unroll
@@ -408,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 			for (int r = 0; r < R; ++r)
 #pragma unroll
 				for (int e = 0; e < 4; ++e) o[x][r][e] = 0.0f;
-		bool bad = false; // a visible V scale that is no number
+		__half2 odd = __float2half2_rn(0.0f); // no number once a V scale was none
 
 		for (int t = tile; t < tile + n; ++t, ++it)
 		{
@@ -424,87 +453,92 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 				for (int r = 0; r < R; ++r)
 #pragma unroll
 					for (int e = 0; e < 4; ++e) sc[r][e] = 0.0f;
-				const uint16_t* ks = reinterpret_cast<const uint16_t*>(st + 2 * L::CODES) + ka * U;
+				float ks[2][U];
+				load_scales<U>(ks[0], st + 2 * L::CODES + ka * (2 * U));
+				load_scales<U>(ks[1], st + 2 * L::CODES + (ka + 8) * (2 * U));
 #pragma unroll
 				for (int g = 0; g < U; ++g)
 				{
-					const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + k_off + 16 * (g ^ k_swz));
-					const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + k_off + 16 * (g ^ k_swz) + 8 * (D / 2));
-					const float s0 = bf16_bits_to_float(ks[g]), s1 = bf16_bits_to_float(ks[g + 8 * U]);
+					const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + (k_off ^ (16 * g)));
+					const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + (k_off ^ (16 * g)) + 8 * (D / 2));
 					const uint32_t x0 = w0 >> 8, x1 = w1 >> 8;
 #pragma unroll
 					for (int r = 0; r < R; ++r)
 					{
-						float d[4] = {q0[r][g][0], q0[r][g][1], q0[r][g][0], q0[r][g][1]};
-						uint4 b, e;
-						if constexpr (L::Q_REGS)
-						{
-							const uint32_t* p = &qf[(2 * g * R + r) * 4];
-							b = make_uint4(p[0], p[1], p[2], p[3]);
-							p += R * 4;
-							e = make_uint4(p[0], p[1], p[2], p[3]);
-						}
-						else
-						{
-							b = qsm[(2 * g * R + r) * 32 + lane];
-							e = qsm[((2 * g + 1) * R + r) * 32 + lane];
-						}
+						float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+						const uint4 b = qsm[(2 * g * R + r) * 32 + lane], e = qsm[((2 * g + 1) * R + r) * 32 + lane];
+						const float2 z = *reinterpret_cast<const float2*>(q0 + (r * U + g) * 8 + 2 * c4);
 						const uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u;
 						mma16816(d, w0 & lo, w1 & lo, w0 & hi, w1 & hi, b.x, b.y);
 						mma16816(d, w0 & lo, w1 & lo, w0 & hi, w1 & hi, b.z, b.w);
 						mma16816(d, x0 & lo, x1 & lo, x0 & hi, x1 & hi, e.x, e.y);
 						mma16816(d, x0 & lo, x1 & lo, x0 & hi, x1 & hi, e.z, e.w);
-						sc[r][0] = fmaf(d[0], s0, sc[r][0]);
-						sc[r][1] = fmaf(d[1], s0, sc[r][1]);
-						sc[r][2] = fmaf(d[2], s1, sc[r][2]);
-						sc[r][3] = fmaf(d[3], s1, sc[r][3]);
+						sc[r][0] = fmaf(d[0] + z.x, ks[0][g], sc[r][0]);
+						sc[r][1] = fmaf(d[1] + z.y, ks[0][g], sc[r][1]);
+						sc[r][2] = fmaf(d[2] + z.x, ks[1][g], sc[r][2]);
+						sc[r][3] = fmaf(d[3] + z.y, ks[1][g], sc[r][3]);
 					}
 				}
 				// ---- weights ----
 				const bool edge = key0 < all_from || key0 + 15 > all_to;
-				const int kx = key0 + (ka & 15);
 				uint32_t ph[R][2], pl[R][2]; // [keys 0-7 | 8-15], transposed: the second product's operand
+				if (a.softcap > 0.0f)
+				{
+#pragma unroll
+					for (int r = 0; r < R; ++r)
+#pragma unroll
+						for (int e = 0; e < 4; ++e) sc[r][e] = tanhf(sc[r][e] * mult[r][e & 1]) * softcap2;
+				}
+				else
+				{
+#pragma unroll
+					for (int r = 0; r < R; ++r)
+#pragma unroll
+						for (int e = 0; e < 4; ++e) sc[r][e] *= mult[r][e & 1];
+				}
+				if (edge)
+				{
+					const int kx = key0 + (ka & 15), end = s.x.keys;
+#pragma unroll
+					for (int r = 0; r < R; ++r)
+#pragma unroll
+						for (int e = 0; e < 4; ++e)
+						{
+							const int k = kx + (e & 2 ? 8 : 0), pos = at[r][e & 1];
+							if (k > pos || k >= end || (a.window > 0 && k <= pos - a.window)) sc[r][e] = -CUDART_INF_F;
+						}
+				}
 #pragma unroll
 				for (int r = 0; r < R; ++r)
 				{
-					float alpha[2], ref[2];
-#pragma unroll
-					for (int e = 0; e < 2; ++e)
+					const float t0 = fmaxf(sc[r][0], sc[r][2]) + held[r][0], t1 = fmaxf(sc[r][1], sc[r][3]) + held[r][1];
+					if (__any_sync(0xffffffffu, fmaxf(t0, t1) > P_TOP))
 					{
-						float x0 = sc[r][e] * mult[r][e], x1 = sc[r][e + 2] * mult[r][e];
-						if (a.softcap > 0.0f)
-						{
-							x0 = a.softcap * tanhf(x0 / a.softcap);
-							x1 = a.softcap * tanhf(x1 / a.softcap);
-						}
-						x0 *= 1.4426950408889634f;
-						x1 *= 1.4426950408889634f;
-						if (edge)
-						{
-							if (kx < kf[r][e] || kx > kl[r][e]) x0 = -CUDART_INF_F;
-							if (kx + 8 < kf[r][e] || kx + 8 > kl[r][e]) x1 = -CUDART_INF_F;
-						}
-						float top = fmaxf(x0, x1);
 #pragma unroll
-						for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-						const float mn = fmaxf(m[r][e], top);
-						ref[e] = mn == -CUDART_INF_F ? 0.0f : mn - P_SCALE_LOG2;
-						alpha[e] = mn == m[r][e] ? 1.0f : ex2(m[r][e] - mn);
-						m[r][e] = mn;
-						sc[r][e] = ex2(x0 - ref[e]);
-						sc[r][e + 2] = ex2(x1 - ref[e]);
-						l[r][e] = fmaf(l[r][e], alpha[e], sc[r][e] + sc[r][e + 2]);
+						for (int e = 0; e < 2; ++e)
+						{
+							float top = fmaxf(sc[r][e], sc[r][e + 2]);
+#pragma unroll
+							for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+							if (top + held[r][e] > P_TOP)
+							{
+								const float alpha = ex2(P_SCALE - top - held[r][e]);
+								held[r][e] = P_SCALE - top;
+								l[r][e] *= alpha;
+#pragma unroll
+								for (int x = 0; x < J * 4; ++x)
+								{
+									o[x][r][e] *= alpha;
+									o[x][r][e + 2] *= alpha;
+								}
+							}
+						}
 					}
-					if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f))
-					{
 #pragma unroll
-						for (int x = 0; x < J * 4; ++x)
-						{
-							o[x][r][0] *= alpha[0];
-							o[x][r][1] *= alpha[1];
-							o[x][r][2] *= alpha[0];
-							o[x][r][3] *= alpha[1];
-						}
+					for (int e = 0; e < 4; ++e)
+					{
+						sc[r][e] = ex2(sc[r][e] + held[r][e & 1]);
+						l[r][e & 1] += sc[r][e];
 					}
 #pragma unroll
 					for (int h = 0; h < 2; ++h)
@@ -516,45 +550,43 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 					}
 				}
 				// ---- values: keys c4 + 4 kk of the warp's 16, J words of codes each ----
-				const unsigned char* sv = st + L::CODES;
-				const uint16_t* vs = reinterpret_cast<const uint16_t*>(st + 2 * L::CODES + L::SCALES);
+				float vs[4][J];
+#pragma unroll
+				for (int kk = 0; kk < 4; ++kk)
+				{
+					const int k = c4 + 4 * kk;
+					load_scales<J>(vs[kk], st + 2 * L::CODES + L::SCALES + ((warp * 16 + k) * U + (i8 >> 2) * J) * 2);
+					if (edge && (key0 + k < s.first || key0 + k > s.last)) // whatever was there
+#pragma unroll
+						for (int j = 0; j < J; ++j) vs[kk][j] = 0.0f;
+				}
 #pragma unroll
 				for (int j = 0; j < J; ++j)
 				{
-					__half2 s2[2], b2[2]; // the scales of key pairs (0, 1) and (2, 3), and -24 times them
+					__half2 s2[2]; // the scales of key pairs (0, 1) and (2, 3)
 					uint32_t lo[2], hi[2];
 #pragma unroll
 					for (int pr = 0; pr < 2; ++pr)
 					{
-						float f[2];
-						uint32_t w[2];
-#pragma unroll
-						for (int e = 0; e < 2; ++e)
-						{
-							const int kk = 2 * pr + e, key = warp * 16 + c4 + 4 * kk;
-							w[e] = *reinterpret_cast<const uint32_t*>(sv + (v_off[e] ^ (16 * j)) + pr * 8 * (D / 2));
-							f[e] = bf16_bits_to_float(vs[key * U + (i8 >> 2) * J + j]);
-							if (!(fabsf(f[e]) <= KV4_SCALE_MAX))
-							{
-								// no number (or, past the request's keys, whatever was there): its weight's product
-								// would be none either, also where the weight is zero
-								const int k = key0 + c4 + 4 * kk;
-								bad |= k >= s.first && k <= s.last;
-								f[e] = 0.0f;
-							}
-						}
-						s2[pr] = __floats2half2_rn(f[0], f[1]);
-						b2[pr] = __hmul2(s2[pr], __float2half2_rn(-24.0f));
-						lo[pr] = __byte_perm(w[0], w[1], 0x5410);
-						hi[pr] = __byte_perm(w[0], w[1], 0x7632);
+						const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + L::CODES + (v_off[0] ^ (16 * j)) + pr * 8 * (D / 2));
+						const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + L::CODES + (v_off[1] ^ (16 * j)) + pr * 8 * (D / 2));
+						s2[pr] = __floats2half2_rn(vs[2 * pr][j], vs[2 * pr + 1][j]);
+						// a scale that is no number (finite ones are within range) marks `odd` for good, and goes in as
+						// a number: zero weights must stay zero for the rows that do not see its key
+						odd = __hfma2(s2[pr], __float2half2_rn(0.0f), odd);
+						s2[pr] = __hmax2(__hmin2(s2[pr], __float2half2_rn(KV4_SCALE_MAX)), __float2half2_rn(-KV4_SCALE_MAX));
+						lo[pr] = __byte_perm(w0, w1, 0x5410);
+						hi[pr] = __byte_perm(w0, w1, 0x7632);
 					}
 #pragma unroll
 					for (int x = 0; x < 4; ++x)
 					{
-						// nibble x to bits 6-9 of each half: 16 + u
+						// nibble x of each half: 1024 + u or 64 + u by the mask, less 1032 or 72, times the scale: all exact
 						const auto widen = [&](uint32_t w, int pr) {
-							const uint32_t sh = x == 0 ? w << 6 : x == 1 ? w << 2 : x == 2 ? w >> 2 : w >> 6;
-							return half2_bits(__hfma2(bits_half2((sh & 0x03C003C0u) | 0x4C004C00u), s2[pr], b2[pr]));
+							const uint32_t v = x >= 2 ? w >> 8 : w;
+							const uint32_t h = x & 1 ? (v & 0x00F000F0u) | 0x54005400u : (v & 0x000F000Fu) | 0x64006400u;
+							const __half2 c = __hadd2(bits_half2(h), __float2half2_rn(x & 1 ? -72.0f : -1032.0f));
+							return half2_bits(__hmul2(c, s2[pr]));
 						};
 						const uint32_t a0 = widen(lo[0], 0), a1 = widen(hi[0], 0), a2 = widen(lo[1], 1), a3 = widen(hi[1], 1);
 #pragma unroll
@@ -571,6 +603,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 		}
 
 		// ---- the piece's end: the four warps' states joined ----
+		float m[R][2];
 #pragma unroll
 		for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -578,9 +611,10 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 			{
 #pragma unroll
 				for (int w = 4; w < 32; w <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], w);
+				m[r][e] = held[r][e] == NONE ? -CUDART_INF_F : P_SCALE - held[r][e];
 				if (i8 == 0) ml[warp * ROWS + 8 * r + 2 * c4 + e] = make_float2(m[r][e], l[r][e]);
 			}
-		const bool any_bad = named_sync_or(1, CW * 32, bad);
+		const bool any_bad = named_sync_or(1, CW * 32, __hisnan(__low2half(odd)) || __hisnan(__high2half(odd)));
 #pragma unroll
 		for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -720,12 +754,14 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 }
 
 constexpr int MAX_SMS = 192;
+// the counters' place is the same for every variant: one workspace serves them all in turn
+constexpr size_t WS_PARTS = 256 + 4096;
 
 template <int D, int R>
 constexpr size_t ws_bytes(int sms)
 {
 	const size_t ctas = (size_t)sms * Shape<D, R>::CTAS;
-	return 256 + (ctas * 4 + 255) / 256 * 256 + ctas * 2 * Shape<D, R>::PART * 4;
+	return WS_PARTS + ctas * 2 * Shape<D, R>::PART * 4;
 }
 
 int num_sms()
@@ -754,10 +790,10 @@ int launch_decode4(const Kv4Args& a, void* workspace, cudaStream_t st)
 		configured[dev] = true;
 	}
 	const int ctas = num_sms() * L::CTAS;
-	if (ctas == 0) return (int)cudaErrorInvalidDevice;
+	if (ctas == 0 || ctas > MAX_SMS * L::CTAS) return (int)cudaErrorInvalidDevice;
 	unsigned char* w = static_cast<unsigned char*>(workspace);
 	const Ws ws{reinterpret_cast<int*>(w), reinterpret_cast<int*>(w + 256),
-	            reinterpret_cast<float*>(w + 256 + ((size_t)ctas * 4 + 255) / 256 * 256)};
+	            reinterpret_cast<float*>(w + WS_PARTS)};
 	kernel<<<ctas, THREADS, L::SMEM, st>>>(a, ws);
 	note_launches(1);
 	return (int)cudaGetLastError();
@@ -792,8 +828,12 @@ extern "C" int nncu_kv4_workspace_bytes(const nncu_kv4_attn* a, size_t* bytes)
 	if (rc != NNCU_OK) return rc;
 	if (!bytes) return refuse("kv4 workspace: NULL argument");
 	// enough for every variant of the head_dim on any device of this kind
-	*bytes = a->pool.head_dim == 64 ? ws_bytes<64, 4>(MAX_SMS) : a->pool.head_dim == 128 ? ws_bytes<128, 2>(MAX_SMS)
-	                                                                                    : ws_bytes<256, 1>(MAX_SMS);
+	*bytes = a->pool.head_dim == 64    ? ws_bytes<64, 4>(MAX_SMS)
+	         : a->pool.head_dim == 128 ? ws_bytes<128, 2>(MAX_SMS)
+	                                   : ws_bytes<256, 1>(MAX_SMS);
+	static_assert(ws_bytes<64, 4>(1) >= ws_bytes<64, 2>(1) && ws_bytes<64, 4>(1) >= ws_bytes<64, 1>(1) &&
+	                  ws_bytes<128, 2>(1) >= ws_bytes<128, 1>(1),
+	              "the largest variant");
 	return NNCU_OK;
 }
 

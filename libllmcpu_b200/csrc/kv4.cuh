@@ -13,7 +13,7 @@ namespace nncu
 
 constexpr int KV4_GROUP = 32;              // values that share a scale
 constexpr float KV4_SCALE_MIN = 0x1p-17f;  // below: an 11-bit product would not be exact in a 16-bit float
-constexpr float KV4_SCALE_MAX = 0x1p11f;   // above: 24 times the scale (the unpacking's constant) would overflow one
+constexpr float KV4_SCALE_MAX = 0x1p11f;   // -8 times it is 2^14: well within one
 
 // Bytes of one (page, KV head): K codes, V codes, K scales, V scales.
 __host__ __device__ constexpr int kv4_codes_bytes(int page, int D) { return page * D / 2; }

@@ -386,6 +386,19 @@ def test_attention_again_is_the_same(nncu, torch_cuda, case):
     assert all(torch.equal(o, outs[0]) for o in outs[1:])
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_one_workspace_for_all_row_counts(nncu, torch_cuda, d):
+    """Decode, verify and prompt calls share a workspace in turn."""
+    torch = torch_cuda
+    cases = [Attn(torch, nncu, ([(900, n), (333, n)], 2, 4, d, 64, 0, 0.0), seed=n) for n in (1, 3, 60, 8)]
+    ws = max((a.ws for a in cases), key=lambda w: w.numel())
+    for a in cases + cases[::-1] + cases:
+        a.call.workspace, a.call.workspace_bytes = ws.data_ptr(), ws.numel()
+        a.out.fill_(5.0)
+        nncu.kv4_attention_dev(a.call)
+        a.check(a.out)
+
+
 @pytest.mark.parametrize("k_scale", [1e-4, 30.0])
 def test_attention_of_flat_and_sharp_scores(nncu, torch_cuda, k_scale):
     """Near-equal weights, and one key that outweighs all others. Scores reach
