@@ -1,5 +1,6 @@
 // k_kv4_attn.cu -- attention of packed requests over the paged 4-bit cache
-// (nncu_kv4_attention_dev).
+// (nncu_kv4_attention_dev): the entry, and the kernel for requests with few
+// query rows (decode, verify; prompts: k_kv4_prompt.cu).
 //
 // Work. A segment is (request, KV head, row group): 8 R query rows (token x
 // grouped head) that read the same keys. Its keys are walked in tiles of 64;
@@ -43,6 +44,7 @@ constexpr int TILE = 64;               // keys a tile
 constexpr int CW = 4;                  // computing warps, 16 keys of a tile each
 constexpr int THREADS = (CW + 1) * 32; // and the loading warp
 constexpr int STAGES = 3;              // tiles in the ring: what arrives while one is worked on
+constexpr int FEW_ROWS = 32;           // requests with more query rows a KV head go to k_kv4_prompt.cu
 constexpr int MIN_TILES = 2;           // a run is at least this long, while tiles are few
 // A row's weights are taken against a held score, 2^11 at it, which moves only
 // when a score passes it by more than 2^4: then no weight passes 2^15, within a
@@ -149,6 +151,7 @@ __device__ __forceinline__ void segment_tiles(const Kv4Args& a, Segment& s, int 
 	s.r = r;
 	s.x = kv4_request(a, r);
 	s.rows = s.x.n_new * a.group;
+	if (s.rows > FEW_ROWS) s.rows = 0; // the tensor-core kernel's
 	s.last = min(s.x.pos0 + s.x.n_new - 1, s.x.keys - 1);
 	s.first = a.window > 0 ? max(0, s.x.pos0 - a.window + 1) : 0;
 	s.tile0 = s.first / TILE;
@@ -761,7 +764,14 @@ template <int D, int R>
 constexpr size_t ws_bytes(int sms)
 {
 	const size_t ctas = (size_t)sms * Shape<D, R>::CTAS;
-	return WS_PARTS + ctas * 2 * Shape<D, R>::PART * 4;
+	return (WS_PARTS + ctas * 2 * Shape<D, R>::PART * 4 + 255) / 256 * 256;
+}
+size_t ws_bytes(int D) // enough for every variant of the head_dim on any device of this kind
+{
+	static_assert(ws_bytes<64, 4>(1) >= ws_bytes<64, 2>(1) && ws_bytes<64, 4>(1) >= ws_bytes<64, 1>(1) &&
+	                  ws_bytes<128, 2>(1) >= ws_bytes<128, 1>(1),
+	              "the largest variant");
+	return D == 64 ? ws_bytes<64, 4>(MAX_SMS) : D == 128 ? ws_bytes<128, 2>(MAX_SMS) : ws_bytes<256, 1>(MAX_SMS);
 }
 
 int num_sms()
@@ -827,13 +837,10 @@ extern "C" int nncu_kv4_workspace_bytes(const nncu_kv4_attn* a, size_t* bytes)
 	const int rc = check_shape(a, false);
 	if (rc != NNCU_OK) return rc;
 	if (!bytes) return refuse("kv4 workspace: NULL argument");
-	// enough for every variant of the head_dim on any device of this kind
-	*bytes = a->pool.head_dim == 64    ? ws_bytes<64, 4>(MAX_SMS)
-	         : a->pool.head_dim == 128 ? ws_bytes<128, 2>(MAX_SMS)
-	                                   : ws_bytes<256, 1>(MAX_SMS);
-	static_assert(ws_bytes<64, 4>(1) >= ws_bytes<64, 2>(1) && ws_bytes<64, 4>(1) >= ws_bytes<64, 1>(1) &&
-	                  ws_bytes<128, 2>(1) >= ws_bytes<128, 1>(1),
-	              "the largest variant");
+	*bytes = ws_bytes(a->pool.head_dim);
+	const long long group = a->n_head / a->pool.n_kv;
+	if (group * a->max_new > FEW_ROWS)
+		*bytes = kv4_prompt_ws_end(a->pool.head_dim, *bytes, a->n_req, group * a->n_tok, a->pool.n_kv);
 	return NNCU_OK;
 }
 
@@ -884,6 +891,7 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 	                p->seq_len, p->q_start, p->q, p->q_stride, p->out, p->out_stride};
 	const auto st = static_cast<cudaStream_t>(stream);
 	const long long rows = (long long)a.group * p->max_new;
+	// (a call that may have prompts still decodes the requests with few rows here)
 	int e;
 	if (a.D == 256)
 		e = launch_decode4<256, 1>(a, p->workspace, st);
@@ -893,5 +901,6 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 		e = rows <= 8    ? launch_decode4<64, 1>(a, p->workspace, st)
 		    : rows <= 16 ? launch_decode4<64, 2>(a, p->workspace, st)
 		                 : launch_decode4<64, 4>(a, p->workspace, st);
+	if (!e && rows > FEW_ROWS) e = launch_kv4_prompt(a, p->workspace, ws_bytes(a.D), FEW_ROWS, stream);
 	return e ? set_cuda_error(e, "kv4 attention launch") : NNCU_OK;
 }

@@ -1,0 +1,885 @@
+// k_kv4_prompt.cu -- attention over the paged 4-bit cache for requests with
+// many query rows (prompts, chunks of prompts), on the 5th-generation tensor
+// cores. (Few rows: k_kv4_attn.cu.)
+//
+// Work. A block is (request, KV head, 128 NQ query rows; a row is token x
+// grouped head, so the heads that share a KV head share its keys' unpacking).
+// A block's keys are walked in tiles of 64. A planning kernel (one CTA) lists
+// the blocks of the requests from their lengths on the device, cuts those
+// with long spans into pieces of about half an SM's share, and the attention
+// kernel takes one (piece, KV head) per CTA. Pieces of one block meet in the
+// workspace; the last one joins them in order.
+//
+// Mathematics. 8 bits of scale times 4 of code are exact in a 16-bit float, so
+// K and V go to the tensor cores as they are; q and the softmax weights go as
+// two 16-bit halves each (22 bits), accumulated in 32:
+//
+//   S  = Qhi K^T + Qlo K^T   tcgen05.mma, M 128 x N 64, operands in shared memory
+//   O += Phi V  + Plo V      tcgen05.mma, M 128 x N D, P from TMEM over its own S
+//
+// which is twice a 16-bit attention's products for 32-bit results. A row's q
+// is scaled by a power of two to fill the 16-bit range, undone in the softmax;
+// weights are taken against a held score, 2^11 at it, that moves only when a
+// score passes it by 2^4.
+//
+// Roles (512 threads): warp 0 brings the pages' codes and scales (bulk copies
+// into a ring of half tiles: K of tile u, V of tile u - 1, ...); warp 1 owns
+// TMEM and issues the products; warps 4-7 unpack half tiles into 16-bit
+// operands (128-byte swizzled); warps 8-11 and 12-15 do the softmax of Q tile
+// A and B, one row a thread, and write the output. Two S buffers a Q tile: the
+// softmax of tile u + 1 runs while P V of tile u and S of tile u + 2 are
+// computed. Every wait is bounded; after one that ran out the CTA records an
+// error and steps through without waiting.
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include "kv4.cuh"
+#include "tc.cuh"
+
+namespace nncu
+{
+namespace
+{
+
+constexpr int BN = 64;           // keys a tile
+constexpr int PT = 512;          // threads
+constexpr int SHARES = 2 * 148;  // pieces are about total / SHARES tiles long, and not under MIN_PIECE
+constexpr int MIN_PIECE = 8;
+constexpr float HELD = 11.0f, HELD_TOP = 15.0f; // see k_kv4_attn.cu
+constexpr int PLAN_THREADS = 1024;
+
+template <int D>
+struct PShape
+{
+	static constexpr int U = D / KV4_GROUP, NQ = D == 256 ? 1 : 2, BR = 128 * NQ, PANELS = D / 64;
+	static constexpr int Q_PANEL = 128 * 128, Q_HALF = PANELS * Q_PANEL; // 128 rows x 64 values; one 16-bit half of a Q tile
+	static constexpr int KV_PANEL = BN * 128, KV_TILE = PANELS * KV_PANEL;
+	static constexpr int KS = D == 256 ? 1 : 2; // unpacked K tiles, and V tiles
+	static constexpr int CODES = BN * D / 2, SCALES = BN * U * 2, RAW = CODES + SCALES, RAW_STAGES = D == 256 ? 3 : 4;
+	static constexpr int SM_Q = 0, SM_K = SM_Q + NQ * 2 * Q_HALF, SM_V = SM_K + KS * KV_TILE;
+	static constexpr int SM_RAW = SM_V + KS * KV_TILE, SM_BAR = SM_RAW + RAW_STAGES * RAW;
+	static constexpr int SMEM = SM_BAR + 512 + 1024;
+	static_assert(SMEM <= 227 * 1024 && SM_BAR % 16 == 0 && RAW % 16 == 0, "shared memory");
+	// TMEM: S of Q tile X, buffer b at 128 X + 64 b (its P: 32 columns of high halves, 32 of low), O behind
+	static constexpr uint32_t T_O = NQ * 128, COLS = 512;
+	static_assert(NQ * (128 + D) <= 512, "TMEM");
+	static constexpr size_t PART = (size_t)BR * (D + 2); // floats a partial result: [D / 4][BR] of 4, then [BR] of 2
+};
+
+// A run of a block's key tiles, as the planning kernel lists it.
+struct Piece
+{
+	int r, row0;        // request, first row of the block
+	int tile0, tiles;   // of the piece
+	int first, n;       // first piece of the block, its number of pieces
+	int block, split0;  // the block (its counter); of a split block's pieces: the partial results before this one
+};
+
+// What the planning kernel leaves for the attention kernel.
+struct PlanHead
+{
+	int n_pieces;
+};
+
+struct PromptWs
+{
+	int* err;
+	PlanHead* head;
+	int* blk0;       // [n_req + 1] blocks before request r
+	int* tiles;      // [blocks] tiles of a block
+	Piece* pieces;
+	int* counters;   // [blocks][n_kv]
+	float* parts;
+	int max_blocks, max_pieces;
+};
+
+struct Block
+{
+	Kv4Request x;
+	int rows, row0;
+	int lo, hi; // tiles [lo, hi] of all rows
+};
+
+// The tiles of rows [row0, row0 + n) of a request; lo > hi: no keys.
+__device__ __forceinline__ void row_tiles(const Kv4Args& a, const Kv4Request& x, int rows, int row0, int n, int& lo, int& hi)
+{
+	lo = 1;
+	hi = 0;
+	if (row0 >= rows) return;
+	const int p0 = x.pos0 + row0 / a.group, p1 = x.pos0 + (min(rows, row0 + n) - 1) / a.group;
+	const int first = a.window > 0 ? max(0, p0 - a.window + 1) : 0, last = min(p1, x.keys - 1);
+	if (last < first) return;
+	lo = first / BN;
+	hi = last / BN;
+}
+
+__device__ __forceinline__ int prompt_rows(const Kv4Args& a, const Kv4Request& x, int min_rows)
+{
+	const int rows = x.n_new * a.group;
+	return rows > min_rows ? rows : 0;
+}
+
+// Inclusive running sum over the CTA, and the total.
+__device__ __forceinline__ int plan_scan(int v, int* sums, int& total)
+{
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+	for (int o = 1; o < 32; o <<= 1)
+	{
+		const int u = __shfl_up_sync(0xffffffffu, v, o);
+		if (lane >= o) v += u;
+	}
+	__syncthreads();
+	if (lane == 31) sums[warp] = v;
+	__syncthreads();
+	int before = 0, all = 0;
+	for (int w = 0; w < PLAN_THREADS / 32; ++w)
+	{
+		if (w < warp) before += sums[w];
+		all += sums[w];
+	}
+	total = all;
+	return before + v;
+}
+
+template <int BR>
+__global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const Kv4Args a, const PromptWs ws, int min_rows)
+{
+	__shared__ int sums[PLAN_THREADS / 32];
+	const int tid = threadIdx.x;
+	int at = 0, total;
+	for (int r0 = 0; r0 < a.n_req; r0 += PLAN_THREADS)
+	{
+		const int r = r0 + tid;
+		int nb = 0;
+		if (r < a.n_req) nb = (prompt_rows(a, kv4_request(a, r), min_rows) + BR - 1) / BR;
+		const int end = at + plan_scan(nb, sums, total);
+		if (r < a.n_req) ws.blk0[r + 1] = min(end, ws.max_blocks);
+		at += total;
+	}
+	if (tid == 0) ws.blk0[0] = 0;
+	__syncthreads();
+	const int blocks = min(at, ws.max_blocks);
+	const auto find = [&](int b) {
+		int lo = 0, hi = a.n_req - 1;
+		while (lo < hi)
+		{
+			const int mid = (lo + hi + 1) >> 1;
+			if (ws.blk0[mid] <= b)
+				lo = mid;
+			else
+				hi = mid - 1;
+		}
+		return lo;
+	};
+	// the blocks' tiles, and what a piece may have of them
+	int mine = 0;
+	for (int b = tid; b < blocks; b += PLAN_THREADS)
+	{
+		const int r = find(b);
+		const Kv4Request x = kv4_request(a, r);
+		int lo, hi;
+		row_tiles(a, x, prompt_rows(a, x, min_rows), (b - ws.blk0[r]) * BR, BR, lo, hi);
+		const int n = max(1, hi - lo + 1); // (a block without keys still writes its zeros)
+		ws.tiles[b] = n;
+		mine += n;
+	}
+	plan_scan(mine, sums, total);
+	const int longest = max(MIN_PIECE, (int)(((long long)total * a.n_kv + SHARES - 1) / SHARES));
+	int pieces = 0, split = 0;
+	for (int b0 = 0; b0 < blocks; b0 += PLAN_THREADS)
+	{
+		const int b = b0 + tid, n = b < blocks ? ws.tiles[b] : 0, np = (n + longest - 1) / longest;
+		int t1, t2;
+		const int p1 = pieces + plan_scan(np, sums, t1), s1 = split + plan_scan(np > 1 ? np : 0, sums, t2);
+		pieces += t1;
+		split += t2;
+		if (b < blocks)
+		{
+			const int r = find(b), row0 = (b - ws.blk0[r]) * BR;
+			const Kv4Request x = kv4_request(a, r);
+			int lo, hi;
+			row_tiles(a, x, prompt_rows(a, x, min_rows), row0, BR, lo, hi);
+			const int first = p1 - np, each = (n + np - 1) / np;
+			for (int i = 0; i < np && first + i < ws.max_pieces; ++i)
+				ws.pieces[first + i] = Piece{r, row0, (lo > hi ? 0 : lo) + i * each, min(each, n - i * each), first, np, b,
+				                             s1 - np + i};
+			for (int h = 0; h < a.n_kv; ++h) ws.counters[(size_t)b * a.n_kv + h] = 0;
+		}
+	}
+	if (tid == 0) ws.head->n_pieces = min(pieces, ws.max_pieces);
+}
+
+// 32 consecutive 32-bit columns into this thread's TMEM lane.
+__device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t* v)
+{
+	float f[32];
+#pragma unroll
+	for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+	tmem_st32(taddr, f);
+}
+
+// D (+)= A B with A in TMEM.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc)
+{
+	asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+	             "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+	             "r"(a), "l"(b), "r"(id), "r"(acc)
+	             : "memory");
+}
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack_half2(float x, float y)
+{
+	const __half2 h = __floats2half2_rn(x, y);
+	return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+template <int D>
+__global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, const PromptWs ws, int min_rows)
+{
+	using L = PShape<D>;
+	constexpr int U = L::U, NQ = L::NQ, KS = L::KS, RS = L::RAW_STAGES;
+	const int pid = (int)blockIdx.x / a.n_kv, hk = (int)blockIdx.x % a.n_kv;
+	const int n_pieces = ws.head->n_pieces;
+	if (pid >= n_pieces) return;
+	const Piece pc = ws.pieces[n_pieces - 1 - pid]; // a request's last rows see the most keys: first
+	extern __shared__ unsigned char smem_raw[];
+	unsigned char* smem =
+		reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+	uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::SM_BAR);
+	uint64_t* raw_full = bars;          // [4] a half tile's codes and scales are here
+	uint64_t* raw_empty = bars + 4;     // [4] the unpacking warps have read them
+	uint64_t* k_full = bars + 8;        // [2] an unpacked K tile
+	uint64_t* k_empty = bars + 10;      // [2] its products are done
+	uint64_t* v_full = bars + 12;       // [2]
+	uint64_t* v_empty = bars + 14;      // [2]
+	uint64_t* s_full = bars + 16;       // [2 Q tiles][2 buffers]
+	uint64_t* p_full = bars + 20;       // [2 Q tiles][2 buffers]: P in TMEM (and O rescaled)
+	uint64_t* pv_done = bars + 24;      // [2] one phase per P V of the Q tile
+	uint64_t* o_done = bars + 26;       // [2] its last P V is done
+	uint64_t* q_ready = bars + 28;      // Q's halves are in shared memory
+	uint64_t* mma_done = bars + 29;     // every product issued is done
+	uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
+	volatile int* flags = reinterpret_cast<volatile int*>(bars + 31); // [0] abort, [1] a V scale was no number
+	int* shared_last = reinterpret_cast<int*>(bars + 32);
+	int* loaded = reinterpret_cast<int*>(bars + 33); // [16] by tile: which 16-key parts of it are in the cache
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+	const Kv4Request x = kv4_request(a, pc.r);
+	const int rows = prompt_rows(a, x, min_rows);
+	// each Q tile's key tiles within the piece; none: lo > hi
+	int lo[2] = {1, 1}, hi[2] = {0, 0};
+#pragma unroll
+	for (int X = 0; X < NQ; ++X)
+	{
+		row_tiles(a, x, rows, pc.row0 + 128 * X, 128, lo[X], hi[X]);
+		lo[X] = max(lo[X], pc.tile0);
+		hi[X] = min(hi[X], pc.tile0 + pc.tiles - 1);
+	}
+	const bool any = lo[0] <= hi[0] || (NQ == 2 && lo[1] <= hi[1]);
+	const int u_lo = pc.tile0, n_u = any ? pc.tiles : 0;
+
+	if (threadIdx.x == 0)
+	{
+		for (int s = 0; s < 4; ++s)
+		{
+			mbar_init(&raw_full[s], 1);
+			mbar_init(&raw_empty[s], 4);
+			mbar_init(&s_full[s], 1);
+			mbar_init(&p_full[s], 128);
+		}
+		for (int s = 0; s < 2; ++s)
+		{
+			mbar_init(&k_full[s], 128);
+			mbar_init(&k_empty[s], 1);
+			mbar_init(&v_full[s], 128);
+			mbar_init(&v_empty[s], 1);
+			mbar_init(&pv_done[s], 1);
+			mbar_init(&o_done[s], 1);
+		}
+		mbar_init(q_ready, NQ * 128);
+		mbar_init(mma_done, 1);
+		flags[0] = flags[1] = 0;
+		fence_barrier_init();
+	}
+	if (warp == 1) tmem_alloc(tmem_slot, L::COLS);
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	const uint32_t tmem = *tmem_slot;
+
+	// registers to the softmax (the launch gives every thread 128: 128 x (40 + 104 + 2 x 184) = 512 x 128)
+	if (warp < 4)
+	{
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 40;" ::: "memory");
+		if (warp == 0)
+		{
+			// ---- codes and scales: lane = 2 x part of the tile + {codes, scales} ----
+			const int parts = min(BN, a.page), n_parts = BN / parts;
+			const int what = lane & 1, part = lane >> 1;
+			const int row_bytes = what ? U * 2 : D / 2;
+			const int cb = kv4_codes_bytes(a.page, D), sb = kv4_scales_bytes(a.page, D);
+			const int* table = a.table + (size_t)pc.r * a.table_stride;
+			const int last = min(x.pos0 + x.n_new - 1, x.keys - 1);
+			int ids = -1, base = -1, h = 0;
+			int id[2] = {-1, -1}; // this lane's page of the K tile and of the V tile behind it
+			unsigned got[2] = {0, 0};
+			const auto load = [&](int v, int u) {
+				const int s = h % RS;
+				if (h >= RS && !flags[0] && !mbar_wait_bounded(&raw_empty[s], ((h / RS) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY))
+					flags[0] = 1;
+				__syncwarp();
+				if (__shfl_sync(0xffffffffu, flags[0], 0)) return false;
+				const int k0 = (u_lo + u) * BN + part * parts;
+				if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], __popc(got[v]) / 2 * (uint32_t)(parts * (D / 2 + U * 2)));
+				__syncwarp();
+				if (got[v] >> lane & 1)
+				{
+					const int off = k0 & (a.page - 1);
+					bulk_g2s(smem + L::SM_RAW + s * L::RAW + (what ? L::CODES : 0) + part * parts * row_bytes,
+					         a.pages + ((size_t)id[v] * a.n_kv + hk) * kv4_chunk_bytes(a.page, D) +
+					             (what ? 2 * cb + v * sb : v * cb) + off * row_bytes,
+					         parts * row_bytes, &raw_full[s]);
+				}
+				++h;
+				return true;
+			};
+			bool ok = true;
+			for (int u = 0; ok && u <= n_u; ++u)
+			{
+				if (u > 0) id[1] = id[0], got[1] = got[0];
+				if (u < n_u)
+				{
+					const int page0 = ((u_lo + u) * BN) >> a.page_shift;
+					if (base < 0 || page0 + n_parts > base + 32)
+					{
+						base = page0;
+						ids = base + lane < a.max_blocks ? table[base + lane] : -1;
+					}
+					id[0] = __shfl_sync(0xffffffffu, ids, page0 - base + (part < n_parts ? part : 0));
+					const bool get = part < n_parts && id[0] >= 0 && id[0] < a.n_pages && (u_lo + u) * BN + part * parts <= last;
+					got[0] = __ballot_sync(0xffffffffu, get);
+					if (lane == 0)
+					{
+						int mask = 0;
+						for (int p = 0; p < n_parts; ++p)
+							if (got[0] >> (2 * p) & 1) mask |= ((1 << (parts / 16)) - 1) << (p * (parts / 16));
+						loaded[u & 15] = mask;
+					}
+					ok = load(0, u);
+				}
+				if (ok && u > 0) ok = load(1, u - 1);
+			}
+			// not to leave (after a wait that ran out) while a copy may still land here
+			for (int i = max(0, h - RS); i < h; ++i) mbar_wait_bounded(&raw_full[i % RS], (i / RS) & 1, nullptr, 0);
+			__syncwarp();
+		}
+		else if (warp == 1)
+		{
+			if (lane == 0)
+			{
+				constexpr uint32_t ID_S = tc_idesc(128, BN, false, false, false);
+				constexpr uint32_t ID_PV = tc_idesc(128, D, false, false, true);
+				const uint64_t dq = sdesc(smem_u32(smem + L::SM_Q), 16, 1024);
+				const uint64_t dk = sdesc(smem_u32(smem + L::SM_K), 16, 1024);
+				const uint64_t dv = sdesc(smem_u32(smem + L::SM_V), L::KV_PANEL, 1024);
+				const auto has = [&](int X, int t) { return X ? (NQ == 2 && t >= lo[1] && t <= hi[1]) : (t >= lo[0] && t <= hi[0]); };
+				int ns[2] = {0, 0}, np[2] = {0, 0}; // S issued, P consumed, per Q tile
+				const auto wait = [&](uint64_t* bar, int phase) {
+					return !flags[0] && mbar_wait_bounded(bar, (uint32_t)(phase & 1), ws.err, DEVERR_WAIT_FULL);
+				};
+				const auto issue_s = [&](int X, int u) {
+					const int b = ns[X] & 1;
+					const uint32_t d = tmem + 128 * X + 64 * b;
+					const uint64_t q = dq + (uint64_t)(2 * X) * (L::Q_HALF >> 4), k = dk + (uint64_t)(u % KS) * (L::KV_TILE >> 4);
+#pragma unroll
+					for (int i = 0; i < D / 16; ++i)
+					{
+						const uint64_t qo = (uint64_t)((i >> 2) * (L::Q_PANEL >> 4) + (i & 3) * 2);
+						const uint64_t ko = (uint64_t)((i >> 2) * (L::KV_PANEL >> 4) + (i & 3) * 2);
+						mma_f16(d, q + qo, k + ko, ID_S, i > 0);
+						mma_f16(d, q + qo + (L::Q_HALF >> 4), k + ko, ID_S, 1);
+					}
+					mma_commit(&s_full[2 * X + b]);
+					++ns[X];
+				};
+				bool ok = n_u == 0 || wait(q_ready, 0);
+				for (int u = 0; ok && u < min(2, n_u); ++u)
+				{
+					ok = wait(&k_full[u % KS], u / KS);
+					if (!ok) break;
+					tc_fence_after();
+					for (int X = 0; X < NQ; ++X)
+						if (has(X, u_lo + u)) issue_s(X, u);
+					mma_commit(&k_empty[u % KS]);
+				}
+				for (int u = 0; ok && u < n_u; ++u)
+				{
+					const int t = u_lo + u, s = u % KS;
+					ok = wait(&v_full[s], u / KS);
+					const bool ahead = u + 2 < n_u;
+					bool k_ready = false;
+					for (int X = 0; ok && X < NQ; ++X)
+					{
+						if (has(X, t))
+						{
+							const int b = np[X] & 1;
+							ok = wait(&p_full[2 * X + b], np[X] >> 1);
+							if (!ok) break;
+							tc_fence_after();
+							const uint32_t d = tmem + L::T_O + D * X, p = tmem + 128 * X + 64 * b;
+							const uint64_t v = dv + (uint64_t)s * (L::KV_TILE >> 4);
+#pragma unroll
+							for (int i = 0; i < BN / 16; ++i)
+							{
+								mma_ts(d, p + 8 * i, v + 128 * i, ID_PV, np[X] > 0 || i > 0);
+								mma_ts(d, p + 32 + 8 * i, v + 128 * i, ID_PV, 1);
+							}
+							mma_commit(&pv_done[X]);
+							if (t == (X ? hi[1] : hi[0])) mma_commit(&o_done[X]);
+							++np[X];
+						}
+						if (X == NQ - 1) mma_commit(&v_empty[s]);
+						if (ahead && has(X, t + 2))
+						{
+							if (!k_ready)
+							{
+								ok = wait(&k_full[(u + 2) % KS], (u + 2) / KS);
+								if (!ok) break;
+								tc_fence_after();
+								k_ready = true;
+							}
+							issue_s(X, u + 2);
+						}
+					}
+					if (!ok) break;
+					if (ahead)
+					{
+						if (!k_ready) ok = wait(&k_full[(u + 2) % KS], (u + 2) / KS);
+						mma_commit(&k_empty[(u + 2) % KS]);
+					}
+				}
+				if (!ok) flags[0] = 1;
+				mma_commit(mma_done);
+				mbar_wait_bounded(mma_done, 0, nullptr, 0);
+			}
+			__syncwarp();
+		}
+	}
+	else if (warp < 8)
+	{
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 104;" ::: "memory");
+		// ---- unpacking: a thread takes words (8 codes) of a half tile ----
+		const int tid = threadIdx.x - 128;
+		constexpr int WPR = D / 8, WORDS = BN * WPR / 128; // words a row; a thread's of a half tile
+		int h = 0;
+		const auto unpack = [&](int v, int u) {
+			const int rs = h % RS, s = u % KS;
+			uint64_t* empty = v ? v_empty : k_empty;
+			bool ok = !flags[0] && mbar_wait_bounded(&raw_full[rs], (h / RS) & 1, ws.err, DEVERR_WAIT_FULL);
+			ok = ok && (u < KS || (!flags[0] && mbar_wait_bounded(&empty[s], ((u / KS) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY)));
+			if (!__all_sync(0xffffffffu, ok))
+			{
+				flags[0] = 1;
+				return false;
+			}
+			const unsigned char* raw = smem + L::SM_RAW + rs * L::RAW;
+			unsigned char* dst = smem + (v ? L::SM_V : L::SM_K) + s * L::KV_TILE;
+			const int key0 = (u_lo + u) * BN;
+#pragma unroll 4
+			for (int i = 0; i < WORDS; ++i)
+			{
+				const int at = tid + 128 * i, row = at / WPR, w = at % WPR;
+				const int g = kv4_unit(row, w >> 2, D), chunk = 4 * g + (w & 3); // 8 values: 16 bytes unpacked
+				uint32_t c = *reinterpret_cast<const uint32_t*>(raw + 4 * at);
+				float f = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(raw + L::CODES + (row * U + g) * 2));
+				if (v && !(fabsf(f) <= KV4_SCALE_MAX))
+				{
+					// no number (or whatever lies past the keys): zero weights must stay zero. Rows that see such a key
+					// of theirs get none at the end.
+					const int key = key0 + row;
+					if (key < x.keys) flags[1] = 1;
+					f = 0.0f;
+				}
+				const __half2 sc = __float2half2_rn(f);
+				uint32_t y[4];
+#pragma unroll
+				for (int e = 0; e < 4; ++e)
+				{
+					const uint32_t z = e >= 2 ? c >> 8 : c;
+					uint32_t m = e & 1 ? (z & 0x00F000F0u) | 0x54005400u : (z & 0x000F000Fu) | 0x64006400u;
+					const __half2 q = __hmul2(__hadd2(*reinterpret_cast<__half2*>(&m), __float2half2_rn(e & 1 ? -72.0f : -1032.0f)), sc);
+					y[e] = *reinterpret_cast<const uint32_t*>(&q);
+				}
+				*reinterpret_cast<uint4*>(dst + (chunk >> 3) * L::KV_PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
+					make_uint4(y[0], y[1], y[2], y[3]);
+			}
+			fence_async_shared();
+			mbar_arrive(v ? &v_full[s] : &k_full[s]);
+			__syncwarp();
+			if (lane == 0) mbar_arrive(&raw_empty[rs]);
+			++h;
+			return true;
+		};
+		bool ok = true;
+		for (int u = 0; ok && u <= n_u; ++u)
+		{
+			if (u < n_u) ok = unpack(0, u);
+			if (ok && u > 0) ok = unpack(1, u - 1);
+		}
+	}
+	else
+	{
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 184;" ::: "memory");
+		const int X = (warp - 8) >> 2, wq = warp & 3, r = wq * 32 + lane;
+		if (X < NQ)
+		{
+			const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
+			const uint32_t ts0 = tmem + 128 * X + lane_off, to = tmem + L::T_O + D * X + lane_off;
+			const int row = pc.row0 + 128 * X + r, tok = row / a.group;
+			const bool real = row < rows;
+			const size_t head = (size_t)(hk * a.group + row - tok * a.group) * D;
+			const int qp = x.pos0 + tok;
+			const int kf = a.window > 0 ? max(0, qp - a.window + 1) : 0, kl = real ? min(qp, x.keys - 1) : -1;
+
+			// ---- this row of Q, as two 16-bit halves ----
+			const float* q = a.q + (size_t)(x.q0 + tok) * a.q_stride + head;
+			float top = 0.0f;
+			if (real)
+#pragma unroll 8
+				for (int d = 0; d < D; d += 4)
+				{
+					const float4 y = *reinterpret_cast<const float4*>(q + d);
+					top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+				}
+			const int ex = top > 0.0f ? max(-100, min(100, ilogbf(top))) : 0;
+			const float f = __uint_as_float((uint32_t)(127 + 13 - ex) << 23); // the largest to [2^13, 2^14)
+			unsigned char* qs = smem + L::SM_Q + X * 2 * L::Q_HALF;
+#pragma unroll 4
+			for (int c = 0; c < D / 8; ++c)
+			{
+				float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z = y;
+				if (real)
+				{
+					y = *reinterpret_cast<const float4*>(q + 8 * c);
+					z = *reinterpret_cast<const float4*>(q + 8 * c + 4);
+				}
+				const float v[8] = {y.x * f, y.y * f, y.z * f, y.w * f, z.x * f, z.y * f, z.z * f, z.w * f};
+				uint32_t h[4], l[4];
+#pragma unroll
+				for (int e = 0; e < 4; ++e)
+				{
+					h[e] = pack_half2(v[2 * e], v[2 * e + 1]);
+					const float2 b = unpack_half2(h[e]);
+					l[e] = pack_half2(v[2 * e] - b.x, v[2 * e + 1] - b.y);
+				}
+				unsigned char* dst = qs + (c >> 3) * L::Q_PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+				*reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+				*reinterpret_cast<uint4*>(dst + L::Q_HALF) = make_uint4(l[0], l[1], l[2], l[3]);
+			}
+			fence_async_shared();
+			mbar_arrive(q_ready);
+
+			// ---- the softmax, O kept in scale ----
+			const float mult = (a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f) / f;
+			const float cap2 = a.softcap * 1.4426950408889634f;
+			float held = 1e30f, l = 0.0f; // HELD - held score (1e30: no key seen)
+			bool ok = true;
+			int n = 0;
+			const int t_lo = X ? lo[1] : lo[0], t_hi = X ? hi[1] : hi[0];
+			for (int t = t_lo; t <= t_hi; ++t, ++n)
+			{
+				const int b = n & 1;
+				const uint32_t ts = ts0 + 64 * b;
+				ok = ok && !flags[0] && mbar_wait_bounded(&s_full[2 * X + b], (uint32_t)((n >> 1) & 1), ws.err, DEVERR_WAIT_FULL);
+				if (!__all_sync(0xffffffffu, ok))
+				{
+					ok = false;
+					break;
+				}
+				tc_fence_after();
+				float s[BN];
+				tmem_ld32(ts, s);
+				tmem_ld32(ts + 32, s + 32);
+				tmem_wait_ld();
+				if (a.softcap > 0.0f)
+				{
+#pragma unroll
+					for (int c = 0; c < BN; ++c) s[c] = tanhf(s[c] * mult) * cap2;
+				}
+				const float sl = a.softcap > 0.0f ? 1.0f : mult;
+				const int key0 = t * BN, here = loaded[(t - u_lo) & 15];
+				if (key0 < kf || key0 + BN - 1 > kl || here != 15)
+				{
+#pragma unroll
+					for (int c = 0; c < BN; ++c)
+						if (key0 + c < kf || key0 + c > kl || !(here >> (c >> 4) & 1)) s[c] = -CUDART_INF_F;
+				}
+				// weights against the held score; `over`: the largest exponent
+				float sum[4];
+				const auto write_p = [&](float h) {
+					float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+					for (int i = 0; i < 4; ++i) sum[i] = 0.0f;
+					uint32_t lo32[32];
+					uint32_t hi32[32];
+#pragma unroll
+					for (int c = 0; c < BN; c += 2)
+					{
+						const float e0 = fmaf(s[c], sl, h), e1 = fmaf(s[c + 1], sl, h);
+						mx[(c >> 1) & 3] = fmaxf(mx[(c >> 1) & 3], fmaxf(e0, e1));
+						const float p0 = ex2(e0), p1 = ex2(e1);
+						sum[(c >> 1) & 3] += p0 + p1;
+						hi32[c >> 1] = pack_half2(p0, p1);
+						const float2 y = unpack_half2(hi32[c >> 1]);
+						lo32[c >> 1] = pack_half2(p0 - y.x, p1 - y.y);
+					}
+					st32u(ts, hi32);
+					st32u(ts + 32, lo32);
+					return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+				};
+				float alpha = 1.0f;
+				bool move;
+				if (__any_sync(0xffffffffu, held == 1e30f))
+				{
+					// a row's first keys: the tile's maximum first
+					float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+					for (int c = 0; c < BN; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c] * sl);
+					const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+					move = m + held > HELD_TOP;
+					if (move)
+					{
+						alpha = ex2(HELD - m - held); // (none seen before: 0)
+						held = HELD - m;
+					}
+					write_p(held);
+				}
+				else
+				{
+					const float over = write_p(held);
+					move = over > HELD_TOP;
+					if (__any_sync(0xffffffffu, move))
+					{
+						if (move)
+						{
+							alpha = ex2(HELD - over);
+							held += HELD - over;
+						}
+						write_p(held);
+					}
+				}
+				if (__any_sync(0xffffffffu, move) && n > 0)
+				{
+					// O must hold every P V before this tile's. (S of this tile completed after P V of tile n - 2, so
+					// pv_done is at most one phase behind and its parity does not alias.)
+					const bool done = !flags[0] && mbar_wait_bounded(&pv_done[X], (uint32_t)((n - 1) & 1), ws.err, DEVERR_WAIT_FULL);
+					if (!__all_sync(0xffffffffu, done))
+					{
+						ok = false;
+						break;
+					}
+					tc_fence_after();
+#pragma unroll
+					for (int c = 0; c < D; c += 32)
+					{
+						float o[32];
+						tmem_ld32(to + c, o);
+						tmem_wait_ld();
+#pragma unroll
+						for (int i = 0; i < 32; ++i) o[i] *= alpha;
+						tmem_st32(to + c, o);
+					}
+				}
+				tmem_wait_st();
+				l = fmaf(l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+				tc_fence_before();
+				mbar_arrive(&p_full[2 * X + b]);
+			}
+			if (!ok) flags[0] = 1;
+			if (ok && n > 0) ok = !flags[0] && mbar_wait_bounded(&o_done[X], 0, ws.err, DEVERR_WAIT_FULL);
+			ok = __all_sync(0xffffffffu, ok);
+			tc_fence_after();
+
+			// ---- the row's output, or its part of it ----
+			const bool spoilt = flags[1] != 0;
+			const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+			float* out = a.out + (size_t)(x.q0 + tok) * a.out_stride + head;
+			const auto slot = [&](int i) { // piece i of the block
+				return ws.parts + ((size_t)(pc.split0 - (n_pieces - 1 - pid - pc.first) + i) * a.n_kv + hk) * L::PART;
+			};
+			const int my = n_pieces - 1 - pid - pc.first;
+#pragma unroll 1
+			for (int c = 0; c < D; c += 32)
+			{
+				float o[32];
+				if (n > 0)
+				{
+					tmem_ld32(to + c, o);
+					tmem_wait_ld();
+				}
+				else
+#pragma unroll
+					for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+				if (spoilt && real)
+				{
+					// (32 columns are one group of values)
+					const int from = max(kf, pc.tile0 * BN), to_ = min(kl, (pc.tile0 + pc.tiles) * BN - 1);
+					for (int k = from; k <= to_; ++k)
+					{
+						const int id = a.table[(size_t)pc.r * a.table_stride + (k >> a.page_shift)];
+						if (id < 0 || id >= a.n_pages) continue;
+						const uint8_t* chunk = a.pages + ((size_t)id * a.n_kv + hk) * kv4_chunk_bytes(a.page, D);
+						const uint16_t* vs = reinterpret_cast<const uint16_t*>(chunk + 2 * kv4_codes_bytes(a.page, D) +
+						                                                       kv4_scales_bytes(a.page, D));
+						const float f2 = bf16_bits_to_float(vs[(k & (a.page - 1)) * U + c / KV4_GROUP]);
+						if (!(fabsf(f2) <= KV4_SCALE_MAX))
+#pragma unroll
+							for (int i = 0; i < 32; ++i) o[i] = CUDART_NAN_F;
+					}
+				}
+				if (pc.n == 1)
+				{
+					if (real)
+#pragma unroll
+						for (int i = 0; i < 32; i += 4)
+							*reinterpret_cast<float4*>(out + c + i) =
+								make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+				}
+				else
+				{
+					float4* p = reinterpret_cast<float4*>(slot(my)) + (c / 4) * L::BR + 128 * X + r;
+#pragma unroll
+					for (int i = 0; i < 32; i += 4) p[(i / 4) * L::BR] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+				}
+			}
+			if (pc.n > 1)
+			{
+				reinterpret_cast<float2*>(slot(my) + (size_t)L::BR * D)[128 * X + r] =
+					make_float2(held == 1e30f ? -CUDART_INF_F : HELD - held, l);
+				__threadfence();
+				named_sync(1, NQ * 128);
+				if (threadIdx.x == 256) *shared_last = atomicAdd(&ws.counters[(size_t)pc.block * a.n_kv + hk], 1) == pc.n - 1;
+				named_sync(1, NQ * 128);
+				if (*shared_last)
+				{
+					__threadfence();
+					float m = -CUDART_INF_F, w = 0.0f;
+					for (int i = 0; i < pc.n; ++i)
+						m = fmaxf(m, __ldcg(reinterpret_cast<const float2*>(slot(i) + (size_t)L::BR * D) + 128 * X + r).x);
+					for (int i = 0; i < pc.n; ++i)
+					{
+						const float2 z = __ldcg(reinterpret_cast<const float2*>(slot(i) + (size_t)L::BR * D) + 128 * X + r);
+						w = fmaf(z.y, z.x == m ? 1.0f : ex2(z.x - m), w);
+					}
+					const float winv = w == 0.0f ? 0.0f : 1.0f / w;
+#pragma unroll 1
+					for (int c = 0; c < D; c += 32)
+					{
+						float o[32];
+#pragma unroll
+						for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+						for (int i = 0; i < pc.n; ++i)
+						{
+							const float zx = __ldcg(reinterpret_cast<const float2*>(slot(i) + (size_t)L::BR * D) + 128 * X + r).x;
+							const float g = zx == m ? 1.0f : ex2(zx - m);
+							const float4* p = reinterpret_cast<const float4*>(slot(i)) + (c / 4) * L::BR + 128 * X + r;
+#pragma unroll
+							for (int e = 0; e < 8; ++e)
+							{
+								const float4 y = __ldcg(p + e * L::BR);
+								o[4 * e] = fmaf(y.x, g, o[4 * e]), o[4 * e + 1] = fmaf(y.y, g, o[4 * e + 1]);
+								o[4 * e + 2] = fmaf(y.z, g, o[4 * e + 2]), o[4 * e + 3] = fmaf(y.w, g, o[4 * e + 3]);
+							}
+						}
+						if (real)
+#pragma unroll
+							for (int e = 0; e < 32; e += 4)
+								*reinterpret_cast<float4*>(out + c + e) =
+									make_float4(o[e] * winv, o[e + 1] * winv, o[e + 2] * winv, o[e + 3] * winv);
+					}
+				}
+			}
+		}
+	}
+	tc_fence_before();
+	__syncthreads();
+	if (warp == 1)
+	{
+		tc_fence_after();
+		tmem_dealloc(tmem, L::COLS);
+	}
+}
+
+size_t up(size_t x) { return (x + 255) / 256 * 256; }
+
+// The workspace's parts behind `base` (which may be NULL: sizes only).
+template <int D>
+size_t prompt_ws(unsigned char* base, size_t at, int n_req, long long rows, int n_kv, PromptWs& ws)
+{
+	using L = PShape<D>;
+	// every block but a request's last is full; a block cut into n pieces holds more than n - 1 shares
+	const long long blocks = rows / L::BR + n_req, pieces = blocks + SHARES;
+	ws.max_blocks = (int)blocks;
+	ws.max_pieces = (int)pieces;
+	const auto take = [&](size_t bytes) {
+		unsigned char* p = base + at;
+		at += up(bytes);
+		return p;
+	};
+	ws.err = reinterpret_cast<int*>(base);
+	ws.head = reinterpret_cast<PlanHead*>(take(sizeof(PlanHead)));
+	ws.blk0 = reinterpret_cast<int*>(take(4 * ((size_t)n_req + 1)));
+	ws.tiles = reinterpret_cast<int*>(take(4 * (size_t)blocks));
+	ws.pieces = reinterpret_cast<Piece*>(take(sizeof(Piece) * (size_t)pieces));
+	ws.counters = reinterpret_cast<int*>(take(4 * (size_t)blocks * n_kv));
+	ws.parts = reinterpret_cast<float*>(take((size_t)2 * SHARES * L::PART * 4));
+	return at;
+}
+
+template <int D>
+int launch(const Kv4Args& a, unsigned char* workspace, size_t at, int min_rows, cudaStream_t st)
+{
+	using L = PShape<D>;
+	static bool configured[64] = {};
+	int dev = 0;
+	cudaGetDevice(&dev);
+	if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+	auto kernel = kv4_prompt_kernel<D>;
+	if (!configured[dev])
+	{
+		const cudaError_t ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+		if (ce != cudaSuccess) return (int)ce;
+		configured[dev] = true;
+	}
+	PromptWs ws;
+	prompt_ws<D>(workspace, at, a.n_req, (long long)a.n_tok * a.group, a.n_kv, ws);
+	kv4_plan_kernel<L::BR><<<1, PLAN_THREADS, 0, st>>>(a, ws, min_rows);
+	kernel<<<(unsigned)ws.max_pieces * (unsigned)a.n_kv, PT, L::SMEM, st>>>(a, ws, min_rows);
+	note_launches(2);
+	return (int)cudaGetLastError();
+}
+
+} // namespace
+
+size_t kv4_prompt_ws_end(int D, size_t at, int n_req, long long rows, int n_kv)
+{
+	PromptWs ws;
+	return D == 64    ? prompt_ws<64>(nullptr, at, n_req, rows, n_kv, ws)
+	       : D == 128 ? prompt_ws<128>(nullptr, at, n_req, rows, n_kv, ws)
+	                  : prompt_ws<256>(nullptr, at, n_req, rows, n_kv, ws);
+}
+
+int launch_kv4_prompt(const Kv4Args& a, void* workspace, size_t at, int min_rows, void* stream)
+{
+	unsigned char* w = static_cast<unsigned char*>(workspace);
+	const auto st = static_cast<cudaStream_t>(stream);
+	return a.D == 64    ? launch<64>(a, w, at, min_rows, st)
+	       : a.D == 128 ? launch<128>(a, w, at, min_rows, st)
+	                    : launch<256>(a, w, at, min_rows, st);
+}
+
+} // namespace nncu

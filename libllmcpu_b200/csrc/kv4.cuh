@@ -78,4 +78,10 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4Args& a, int r)
 // NNCU_OK or the refusal (k_paged.cu).
 int kv4_check_pool(const nncu_kv4_pool* p, const char* what, bool need_pages = true);
 
+// The tensor-core kernel for requests with more than min_rows query rows
+// (k_kv4_prompt.cu), its workspace from byte `at` of the call's; and where
+// that ends for n_req requests with `rows` query rows a KV head together.
+int launch_kv4_prompt(const Kv4Args& a, void* workspace, size_t at, int min_rows, void* stream);
+size_t kv4_prompt_ws_end(int D, size_t at, int n_req, long long rows, int n_kv);
+
 } // namespace nncu
