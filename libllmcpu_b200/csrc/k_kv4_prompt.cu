@@ -219,12 +219,37 @@ __device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t* v)
 	tmem_st32(taddr, f);
 }
 
-// D (+)= A B with A in TMEM.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc)
+// The products are issued by a whole warp, converged, and executed by its
+// elected lane: the operands' descriptors then stay in the warp's uniform
+// registers. (From a branch that one lane takes, each product cost 130 to 260
+// cycles of moving them there, whatever its size.)
+__device__ __forceinline__ uint32_t elect_one()
 {
-	asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-	             "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-	             "r"(a), "l"(b), "r"(id), "r"(acc)
+	uint32_t r;
+	asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+	return r;
+}
+// D (+)= A B, both in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t lead)
+{
+	asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+	             "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+	             "l"(a), "l"(b), "r"(id), "r"(acc), "r"(lead)
+	             : "memory");
+}
+// A in TMEM
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t lead)
+{
+	asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+	             "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+	             "r"(a), "l"(b), "r"(id), "r"(acc), "r"(lead)
+	             : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead)
+{
+	asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+	             "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+	             "r"(lead)
 	             : "memory");
 }
 
@@ -379,93 +404,100 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 		}
 		else if (warp == 1)
 		{
-			if (lane == 0)
-			{
-				constexpr uint32_t ID_S = tc_idesc(128, BN, false, false, false);
-				constexpr uint32_t ID_PV = tc_idesc(128, D, false, false, true);
-				const uint64_t dq = sdesc(smem_u32(smem + L::SM_Q), 16, 1024);
-				const uint64_t dk = sdesc(smem_u32(smem + L::SM_K), 16, 1024);
-				const uint64_t dv = sdesc(smem_u32(smem + L::SM_V), L::KV_PANEL, 1024);
-				const auto has = [&](int X, int t) { return X ? (NQ == 2 && t >= lo[1] && t <= hi[1]) : (t >= lo[0] && t <= hi[0]); };
-				int ns[2] = {0, 0}, np[2] = {0, 0}; // S issued, P consumed, per Q tile
-				const auto wait = [&](uint64_t* bar, int phase) {
-					return !flags[0] && mbar_wait_bounded(bar, (uint32_t)(phase & 1), ws.err, DEVERR_WAIT_FULL);
-				};
-				const auto issue_s = [&](int X, int u) {
-					const int b = ns[X] & 1;
-					const uint32_t d = tmem + 128 * X + 64 * b;
-					const uint64_t q = dq + (uint64_t)(2 * X) * (L::Q_HALF >> 4), k = dk + (uint64_t)(u % KS) * (L::KV_TILE >> 4);
+			constexpr uint32_t ID_S = tc_idesc(128, BN, false, false, false);
+			constexpr uint32_t ID_PV = tc_idesc(128, D, false, false, true);
+			const uint32_t lead = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+			const uint64_t dq = sdesc(smem_u32(smem + L::SM_Q), 16, 1024);
+			const uint64_t dk = sdesc(smem_u32(smem + L::SM_K), 16, 1024);
+			const uint64_t dv = sdesc(smem_u32(smem + L::SM_V), L::KV_PANEL, 1024);
+			// the same for every lane, and known to be
+			const int nu = __shfl_sync(0xffffffffu, n_u, 0);
+			int from[2], to[2];
 #pragma unroll
-					for (int i = 0; i < D / 16; ++i)
-					{
-						const uint64_t qo = (uint64_t)((i >> 2) * (L::Q_PANEL >> 4) + (i & 3) * 2);
-						const uint64_t ko = (uint64_t)((i >> 2) * (L::KV_PANEL >> 4) + (i & 3) * 2);
-						mma_f16(d, q + qo, k + ko, ID_S, i > 0);
-						mma_f16(d, q + qo + (L::Q_HALF >> 4), k + ko, ID_S, 1);
-					}
-					mma_commit(&s_full[2 * X + b]);
-					++ns[X];
-				};
-				bool ok = n_u == 0 || wait(q_ready, 0);
-				for (int u = 0; ok && u < min(2, n_u); ++u)
+			for (int X = 0; X < 2; ++X)
+				from[X] = __shfl_sync(0xffffffffu, lo[X] - u_lo, 0), to[X] = __shfl_sync(0xffffffffu, hi[X] - u_lo, 0);
+			const auto has = [&](int X, int u) { return u >= from[X] && u <= to[X]; };
+			int ns[2] = {0, 0}, np[2] = {0, 0}; // S issued, P consumed, per Q tile
+			const auto wait = [&](uint64_t* bar, int phase) {
+				const bool w = !flags[0] && mbar_wait_bounded(bar, (uint32_t)(phase & 1), ws.err, DEVERR_WAIT_FULL);
+				return __all_sync(0xffffffffu, w) != 0;
+			};
+			const auto issue_s = [&](int X, int u) {
+				const int b = ns[X] & 1;
+				const uint32_t d = tm + 128 * X + 64 * b;
+				const uint64_t q = dq + (uint64_t)(2 * X) * (L::Q_HALF >> 4), k = dk + (uint64_t)(u % KS) * (L::KV_TILE >> 4);
+#pragma unroll
+				for (int i = 0; i < D / 16; ++i)
 				{
-					ok = wait(&k_full[u % KS], u / KS);
-					if (!ok) break;
-					tc_fence_after();
-					for (int X = 0; X < NQ; ++X)
-						if (has(X, u_lo + u)) issue_s(X, u);
-					mma_commit(&k_empty[u % KS]);
+					const uint64_t qo = (uint64_t)((i >> 2) * (L::Q_PANEL >> 4) + (i & 3) * 2);
+					const uint64_t ko = (uint64_t)((i >> 2) * (L::KV_PANEL >> 4) + (i & 3) * 2);
+					mma_ss(d, q + qo, k + ko, ID_S, i > 0, lead);
+					mma_ss(d, q + qo + (L::Q_HALF >> 4), k + ko, ID_S, 1, lead);
 				}
-				for (int u = 0; ok && u < n_u; ++u)
+				commit(&s_full[2 * X + b], lead);
+				++ns[X];
+			};
+			bool ok = nu == 0 || wait(q_ready, 0);
+			for (int u = 0; ok && u < min(2, nu); ++u)
+			{
+				ok = wait(&k_full[u % KS], u / KS);
+				if (!ok) break;
+				tc_fence_after();
+#pragma unroll
+				for (int X = 0; X < NQ; ++X)
+					if (has(X, u)) issue_s(X, u);
+				commit(&k_empty[u % KS], lead);
+			}
+			for (int u = 0; ok && u < nu; ++u)
+			{
+				const int s = u % KS;
+				ok = wait(&v_full[s], u / KS);
+				const bool ahead = u + 2 < nu;
+				bool k_ready = false;
+#pragma unroll
+				for (int X = 0; X < NQ; ++X)
 				{
-					const int t = u_lo + u, s = u % KS;
-					ok = wait(&v_full[s], u / KS);
-					const bool ahead = u + 2 < n_u;
-					bool k_ready = false;
-					for (int X = 0; ok && X < NQ; ++X)
+					if (ok && has(X, u))
 					{
-						if (has(X, t))
+						const int b = np[X] & 1;
+						ok = wait(&p_full[2 * X + b], np[X] >> 1);
+						if (ok)
 						{
-							const int b = np[X] & 1;
-							ok = wait(&p_full[2 * X + b], np[X] >> 1);
-							if (!ok) break;
 							tc_fence_after();
-							const uint32_t d = tmem + L::T_O + D * X, p = tmem + 128 * X + 64 * b;
+							const uint32_t d = tm + L::T_O + D * X, p = tm + 128 * X + 64 * b;
 							const uint64_t v = dv + (uint64_t)s * (L::KV_TILE >> 4);
 #pragma unroll
 							for (int i = 0; i < BN / 16; ++i)
 							{
-								mma_ts(d, p + 8 * i, v + 128 * i, ID_PV, np[X] > 0 || i > 0);
-								mma_ts(d, p + 32 + 8 * i, v + 128 * i, ID_PV, 1);
+								mma_ts(d, p + 8 * i, v + 128 * i, ID_PV, i > 0 ? 1 : np[X] > 0, lead);
+								mma_ts(d, p + 32 + 8 * i, v + 128 * i, ID_PV, 1, lead);
 							}
-							mma_commit(&pv_done[X]);
-							if (t == (X ? hi[1] : hi[0])) mma_commit(&o_done[X]);
+							commit(&pv_done[X], lead);
+							if (u == to[X]) commit(&o_done[X], lead);
 							++np[X];
 						}
-						if (X == NQ - 1) mma_commit(&v_empty[s]);
-						if (ahead && has(X, t + 2))
-						{
-							if (!k_ready)
-							{
-								ok = wait(&k_full[(u + 2) % KS], (u + 2) / KS);
-								if (!ok) break;
-								tc_fence_after();
-								k_ready = true;
-							}
-							issue_s(X, u + 2);
-						}
 					}
-					if (!ok) break;
-					if (ahead)
+					if (X == NQ - 1) commit(&v_empty[s], lead);
+					if (ok && ahead && has(X, u + 2))
 					{
-						if (!k_ready) ok = wait(&k_full[(u + 2) % KS], (u + 2) / KS);
-						mma_commit(&k_empty[(u + 2) % KS]);
+						if (!k_ready)
+						{
+							ok = wait(&k_full[(u + 2) % KS], (u + 2) / KS);
+							tc_fence_after();
+							k_ready = true;
+						}
+						if (ok) issue_s(X, u + 2);
 					}
 				}
-				if (!ok) flags[0] = 1;
-				mma_commit(mma_done);
-				mbar_wait_bounded(mma_done, 0, nullptr, 0);
+				if (ok && ahead)
+				{
+					if (!k_ready) ok = wait(&k_full[(u + 2) % KS], (u + 2) / KS);
+					commit(&k_empty[(u + 2) % KS], lead);
+				}
 			}
+			if (!ok) flags[0] = 1;
+			commit(mma_done, lead);
+			mbar_wait_bounded(mma_done, 0, nullptr, 0);
 			__syncwarp();
 		}
 	}
