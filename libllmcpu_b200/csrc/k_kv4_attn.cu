@@ -17,17 +17,16 @@
 // coming (bulk copies of the pages' codes and scales, looked up in the block
 // table 32 entries at a time).
 //
-// Mathematics. Codes feed the tensor cores without being scaled first: for a
-// group of 32 values (one scale s) q.k = s (sum q u - 8 sum q), u = code + 8.
-// Masking a word of codes leaves u in the low bits of a 16-bit lane, which
-// read as a float is u x 2^-24 (or x 2^-20 one nibble up): an exact operand,
-// with no conversion. The group's sum then takes its scale in 32 bits. V's
-// codes cannot wait for their scale (the sum runs over keys): the mask makes
-// 1024 + u (or 64 + u), less 1032 (72) that is the code, and 8 bits of scale
-// times 4 of code are exact in a 16-bit float. q and the weights p go in
-// as two 16-bit halves each (22 bits), accumulated in 32: the result is as
-// close to the exact one as 32-bit arithmetic. p carries 2^15 so that small
-// weights keep their digits.
+// Mathematics. For a group of 32 values (one scale s) q.k = s sum q c: the
+// codes c go to the tensor cores unscaled (a mask and a subtraction make them
+// 16-bit floats) and the group's sum takes its scale in 32 bits. V's codes
+// cannot wait for their scale (the sum runs over keys), but 8 bits of scale
+// times 4 of code are exact in a 16-bit float. q and the weights p go in as
+// two 16-bit halves each (22 bits), accumulated in 32: the result is as close
+// to the exact one as 32-bit arithmetic. (Codes as denormal floats, straight
+// from a mask, would save the subtraction, but the products' adder aligns by
+// exponents and cuts off the bits that the denormals lack: 3e-6 instead of
+// 1e-6 of the output.)
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
@@ -71,8 +70,7 @@ struct Shape
 	static constexpr int RED_ROW = D + 4;                   // floats a row of the joining buffer
 	static constexpr int SM_RED = STAGES * STAGE;           // [CW][ROWS][RED_ROW]
 	static constexpr int SM_Q = SM_RED + CW * ROWS * RED_ROW * 4; // q's operands [D / 16][R][32 lanes] of 16 bytes
-	static constexpr int SM_Q0 = SM_Q + D / 16 * R * 512;   // -8 x the groups' sums of q [R][U][8 rows]
-	static constexpr int SM_ML = SM_Q0 + R * U * 32;        // [CW][ROWS] (maximum, weight)
+	static constexpr int SM_ML = SM_Q + D / 16 * R * 512;   // [CW][ROWS] (maximum, weight)
 	static constexpr int SM_BAR = SM_ML + CW * ROWS * 8;
 	static constexpr int SMEM = SM_BAR + 256;
 	static_assert(SM_BAR % 16 == 0 && SM_Q % 16 == 0 && SM_RED % 16 == 0 && SCALES % 16 == 0, "aligned for their accesses");
@@ -137,6 +135,15 @@ __device__ __forceinline__ void load_scales(float (&f)[N], const unsigned char* 
 	}
 }
 
+// Nibbles x and x + 4 of a word as codes: the mask makes 1024 + u (or 64 + u,
+// one nibble up) in the two halves, less 1032 (72): exact.
+__device__ __forceinline__ __half2 codes2(uint32_t w, int x)
+{
+	const uint32_t v = x >= 2 ? w >> 8 : w;
+	const uint32_t h = x & 1 ? (v & 0x00F000F0u) | 0x54005400u : (v & 0x000F000Fu) | 0x64006400u;
+	return __hadd2(bits_half2(h), __float2half2_rn(x & 1 ? -72.0f : -1032.0f));
+}
+
 // One segment's rows and the tiles of its keys.
 struct Segment
 {
@@ -177,7 +184,6 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 	extern __shared__ __align__(128) unsigned char smem[];
 	float* red = reinterpret_cast<float*>(smem + L::SM_RED);
 	uint4* qsm = reinterpret_cast<uint4*>(smem + L::SM_Q);
-	float* q0 = reinterpret_cast<float*>(smem + L::SM_Q0);
 	float2* ml = reinterpret_cast<float2*>(smem + L::SM_ML);
 	uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::SM_BAR);
 	uint64_t* empty = full + STAGES;
@@ -345,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 		v_off[kk] = key * (D / 2) + 16 * (((i8 >> 2) * J) ^ ((key * D / 256) & (U - 1))) + 4 * (i8 & 3);
 	}
 	// scores in base 2 (with a soft-cap: its argument, and what multiplies its value)
-	const float scale2 = a.softcap > 0.0f ? a.scale * 0x1p24f / a.softcap : a.scale * (0x1p24f * 1.4426950408889634f);
+	const float scale2 = a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
 	const float softcap2 = a.softcap * 1.4426950408889634f;
 	int it = 0;
 	while (left > 0)
@@ -386,29 +392,17 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 			// the power of two that brings the row's largest value to [2^14, 2^15)
 			const int ex = top > 0.0f ? max(-100, min(100, ilogbf(top))) : 0;
 			const float f = __uint_as_float((uint32_t)(127 + 14 - ex) << 23);
-			float sum[U];
 #pragma unroll
 			for (int g = 0; g < U; ++g)
-			{
-				sum[g] = 0.0f;
 #pragma unroll
 				for (int h = 0; h < 2; ++h)
 				{
-					uint32_t b[4]; // hi of values 4h, 4h+1 | 4h+2, 4h+3 (a nibble up: / 16), lo of both
-					const float w = f * 0.0625f;
+					if ((g & (CW - 1)) != warp) continue;
+					uint32_t b[4]; // high halves of values 4h, 4h+1 | 4h+2, 4h+3, low halves
 					split2(v[g][4 * h] * f, v[g][4 * h + 1] * f, b[0], b[2]);
-					split2(v[g][4 * h + 2] * w, v[g][4 * h + 3] * w, b[1], b[3]);
-					float2 p = __half22float2(bits_half2(b[0])), q = __half22float2(bits_half2(b[2]));
-					sum[g] += (p.x + q.x) + (p.y + q.y);
-					p = __half22float2(bits_half2(b[1])), q = __half22float2(bits_half2(b[3]));
-					sum[g] += 16.0f * ((p.x + q.x) + (p.y + q.y));
-					if ((g & (CW - 1)) == warp)
-						qsm[((2 * g + h) * R + r) * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
+					split2(v[g][4 * h + 2] * f, v[g][4 * h + 3] * f, b[1], b[3]);
+					qsm[((2 * g + h) * R + r) * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
 				}
-				sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
-				sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
-				if ((g & (CW - 1)) == warp && c4 == 0) q0[(r * U + g) * 8 + i8] = sum[g] * (-8.0f * 0x1p-24f);
-			}
 #pragma unroll
 			for (int e = 0; e < 2; ++e)
 			{
@@ -464,22 +458,22 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 				{
 					const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + (k_off ^ (16 * g)));
 					const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + (k_off ^ (16 * g)) + 8 * (D / 2));
-					const uint32_t x0 = w0 >> 8, x1 = w1 >> 8;
+					uint32_t k0[4], k1[4]; // the codes of both keys, pair by pair
+#pragma unroll
+					for (int x = 0; x < 4; ++x) k0[x] = half2_bits(codes2(w0, x)), k1[x] = half2_bits(codes2(w1, x));
 #pragma unroll
 					for (int r = 0; r < R; ++r)
 					{
 						float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 						const uint4 b = qsm[(2 * g * R + r) * 32 + lane], e = qsm[((2 * g + 1) * R + r) * 32 + lane];
-						const float2 z = *reinterpret_cast<const float2*>(q0 + (r * U + g) * 8 + 2 * c4);
-						const uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u;
-						mma16816(d, w0 & lo, w1 & lo, w0 & hi, w1 & hi, b.x, b.y);
-						mma16816(d, w0 & lo, w1 & lo, w0 & hi, w1 & hi, b.z, b.w);
-						mma16816(d, x0 & lo, x1 & lo, x0 & hi, x1 & hi, e.x, e.y);
-						mma16816(d, x0 & lo, x1 & lo, x0 & hi, x1 & hi, e.z, e.w);
-						sc[r][0] = fmaf(d[0] + z.x, ks[0][g], sc[r][0]);
-						sc[r][1] = fmaf(d[1] + z.y, ks[0][g], sc[r][1]);
-						sc[r][2] = fmaf(d[2] + z.x, ks[1][g], sc[r][2]);
-						sc[r][3] = fmaf(d[3] + z.y, ks[1][g], sc[r][3]);
+						mma16816(d, k0[0], k1[0], k0[1], k1[1], b.x, b.y);
+						mma16816(d, k0[0], k1[0], k0[1], k1[1], b.z, b.w);
+						mma16816(d, k0[2], k1[2], k0[3], k1[3], e.x, e.y);
+						mma16816(d, k0[2], k1[2], k0[3], k1[3], e.z, e.w);
+						sc[r][0] = fmaf(d[0], ks[0][g], sc[r][0]);
+						sc[r][1] = fmaf(d[1], ks[0][g], sc[r][1]);
+						sc[r][2] = fmaf(d[2], ks[1][g], sc[r][2]);
+						sc[r][3] = fmaf(d[3], ks[1][g], sc[r][3]);
 					}
 				}
 				// ---- weights ----
@@ -584,13 +578,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 #pragma unroll
 					for (int x = 0; x < 4; ++x)
 					{
-						// nibble x of each half: 1024 + u or 64 + u by the mask, less 1032 or 72, times the scale: all exact
-						const auto widen = [&](uint32_t w, int pr) {
-							const uint32_t v = x >= 2 ? w >> 8 : w;
-							const uint32_t h = x & 1 ? (v & 0x00F000F0u) | 0x54005400u : (v & 0x000F000Fu) | 0x64006400u;
-							const __half2 c = __hadd2(bits_half2(h), __float2half2_rn(x & 1 ? -72.0f : -1032.0f));
-							return half2_bits(__hmul2(c, s2[pr]));
-						};
+						const auto widen = [&](uint32_t w, int pr) { return half2_bits(__hmul2(codes2(w, x), s2[pr])); };
 						const uint32_t a0 = widen(lo[0], 0), a1 = widen(hi[0], 0), a2 = widen(lo[1], 1), a3 = widen(hi[1], 1);
 #pragma unroll
 						for (int r = 0; r < R; ++r)
