@@ -33,6 +33,8 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "kv4.cuh"
 #include "tc.cuh"
 
@@ -210,39 +212,38 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const Kv4Args a,
 	if (tid == 0) ws.head->n_pieces = min(pieces, ws.max_pieces);
 }
 
-// 32 consecutive 32-bit columns into this thread's TMEM lane.
-__device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t* v)
-{
-	float f[32];
-#pragma unroll
-	for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
-	tmem_st32(taddr, f);
-}
-
 // The products are issued by a whole warp, converged, and executed by its
-// elected lane: the operands' descriptors then stay in the warp's uniform
-// registers. (From a branch that one lane takes, each product cost 130 to 260
-// cycles of moving them there, whatever its size.)
+// elected lane; every condition on their way is a vote, whose result the
+// compiler knows to be one for the warp. The operands' descriptors then live
+// in the warp's uniform registers. (From a branch that one lane takes, or
+// under conditions that might differ between lanes, each product cost 80 to
+// 260 cycles of moving them there, whatever its size.)
+__device__ __forceinline__ bool uni(bool c) { return __any_sync(0xffffffffu, c) != 0; }
 __device__ __forceinline__ uint32_t elect_one()
 {
 	uint32_t r;
 	asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
 	return r;
 }
-// D (+)= A B, both in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t lead)
+// D (+)= A B, both in shared memory: a, b the low words of their descriptors
+// (address and leading offset), which share the high word.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t id, uint32_t acc,
+                                       uint32_t lead)
 {
-	asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-	             "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-	             "l"(a), "l"(b), "r"(id), "r"(acc), "r"(lead)
+	asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+	             "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\t"
+	             "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}" ::"r"(d),
+	             "r"(a), "r"(b), "r"(high), "r"(id), "r"(acc), "r"(lead)
 	             : "memory");
 }
 // A in TMEM
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t lead)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t id, uint32_t acc,
+                                       uint32_t lead)
 {
-	asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-	             "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-	             "r"(a), "l"(b), "r"(id), "r"(acc), "r"(lead)
+	asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+	             "mov.b64 y, {%2, %3};\n\t"
+	             "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d),
+	             "r"(a), "r"(b), "r"(high), "r"(id), "r"(acc), "r"(lead)
 	             : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead)
@@ -335,11 +336,12 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = *tmem_slot;
+	if (tmem != 0) flags[0] = 1, atomicCAS(ws.err, 0, DEVERR_PLAN); // (cannot be: see the products' warp)
 
-	// registers to the softmax (the launch gives every thread 128: 128 x (40 + 104 + 2 x 184) = 512 x 128)
+	// registers to the softmax (the launch gives every thread 128: 128 x (72 + 104 + 2 x 168) = 512 x 128)
 	if (warp < 4)
 	{
-		asm volatile("setmaxnreg.dec.sync.aligned.u32 40;" ::: "memory");
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
 		if (warp == 0)
 		{
 			// ---- codes and scales: lane = 2 x part of the tile + {codes, scales} ----
@@ -406,39 +408,34 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 		{
 			constexpr uint32_t ID_S = tc_idesc(128, BN, false, false, false);
 			constexpr uint32_t ID_PV = tc_idesc(128, D, false, false, true);
-			const uint32_t lead = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
-			const uint64_t dq = sdesc(smem_u32(smem + L::SM_Q), 16, 1024);
-			const uint64_t dk = sdesc(smem_u32(smem + L::SM_K), 16, 1024);
-			const uint64_t dv = sdesc(smem_u32(smem + L::SM_V), L::KV_PANEL, 1024);
-			// the same for every lane, and known to be
-			const int nu = __shfl_sync(0xffffffffu, n_u, 0);
-			int from[2], to[2];
-#pragma unroll
-			for (int X = 0; X < 2; ++X)
-				from[X] = __shfl_sync(0xffffffffu, lo[X] - u_lo, 0), to[X] = __shfl_sync(0xffffffffu, hi[X] - u_lo, 0);
-			const auto has = [&](int X, int u) { return u >= from[X] && u <= to[X]; };
+			const uint32_t lead = elect_one();
+			constexpr uint32_t tm = 0; // (512 columns are all there are: the allocation starts at the first)
+			const uint32_t dq = (uint32_t)sdesc(smem_u32(smem + L::SM_Q), 16, 1024);
+			const uint32_t dk = (uint32_t)sdesc(smem_u32(smem + L::SM_K), 16, 1024);
+			const uint32_t dv = (uint32_t)sdesc(smem_u32(smem + L::SM_V), L::KV_PANEL, 1024);
+			const uint32_t high = (uint32_t)(sdesc(0, 16, 1024) >> 32);
+			const auto has = [&](int X, int u) { return uni(u + u_lo >= lo[X] && u + u_lo <= hi[X]); };
 			int ns[2] = {0, 0}, np[2] = {0, 0}; // S issued, P consumed, per Q tile
 			const auto wait = [&](uint64_t* bar, int phase) {
 				const bool w = !flags[0] && mbar_wait_bounded(bar, (uint32_t)(phase & 1), ws.err, DEVERR_WAIT_FULL);
 				return __all_sync(0xffffffffu, w) != 0;
 			};
+			// (the low halves first: the adder cuts a sum off at its size, and while only they are in it that is small)
 			const auto issue_s = [&](int X, int u) {
-				const int b = ns[X] & 1;
-				const uint32_t d = tm + 128 * X + 64 * b;
-				const uint64_t q = dq + (uint64_t)(2 * X) * (L::Q_HALF >> 4), k = dk + (uint64_t)(u % KS) * (L::KV_TILE >> 4);
+				const bool odd = uni(ns[X] & 1);
+				const uint32_t d = tm + 128 * X + (odd ? 64 : 0);
+				const uint32_t q = dq + 2 * X * (L::Q_HALF >> 4), k = dk + (u % KS) * (L::KV_TILE >> 4);
 #pragma unroll
-				for (int i = 0; i < D / 16; ++i)
-				{
-					const uint64_t qo = (uint64_t)((i >> 2) * (L::Q_PANEL >> 4) + (i & 3) * 2);
-					const uint64_t ko = (uint64_t)((i >> 2) * (L::KV_PANEL >> 4) + (i & 3) * 2);
-					mma_ss(d, q + qo, k + ko, ID_S, i > 0, lead);
-					mma_ss(d, q + qo + (L::Q_HALF >> 4), k + ko, ID_S, 1, lead);
-				}
-				commit(&s_full[2 * X + b], lead);
+				for (int half = 1; half >= 0; --half)
+#pragma unroll
+					for (int i = 0; i < D / 16; ++i)
+						mma_ss(d, q + half * (L::Q_HALF >> 4) + (i >> 2) * (L::Q_PANEL >> 4) + (i & 3) * 2,
+						       k + (i >> 2) * (L::KV_PANEL >> 4) + (i & 3) * 2, high, ID_S, half == 0 || i > 0, lead);
+				commit(&s_full[2 * X + odd], lead);
 				++ns[X];
 			};
-			bool ok = nu == 0 || wait(q_ready, 0);
-			for (int u = 0; ok && u < min(2, nu); ++u)
+			bool ok = uni(n_u == 0) || wait(q_ready, 0);
+			for (int u = 0; u < 2 && uni(ok && u < n_u); ++u)
 			{
 				ok = wait(&k_full[u % KS], u / KS);
 				if (!ok) break;
@@ -448,32 +445,33 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 					if (has(X, u)) issue_s(X, u);
 				commit(&k_empty[u % KS], lead);
 			}
-			for (int u = 0; ok && u < nu; ++u)
+			for (int u = 0; uni(ok && u < n_u); ++u)
 			{
 				const int s = u % KS;
 				ok = wait(&v_full[s], u / KS);
-				const bool ahead = u + 2 < nu;
+				const bool ahead = uni(u + 2 < n_u);
 				bool k_ready = false;
 #pragma unroll
 				for (int X = 0; X < NQ; ++X)
 				{
 					if (ok && has(X, u))
 					{
-						const int b = np[X] & 1;
-						ok = wait(&p_full[2 * X + b], np[X] >> 1);
+						const bool odd = uni(np[X] & 1);
+						ok = wait(&p_full[2 * X + odd], np[X] >> 1);
 						if (ok)
 						{
 							tc_fence_after();
-							const uint32_t d = tm + L::T_O + D * X, p = tm + 128 * X + 64 * b;
-							const uint64_t v = dv + (uint64_t)s * (L::KV_TILE >> 4);
+							const uint32_t d = tm + L::T_O + D * X, p = tm + 128 * X + (odd ? 64 : 0);
+							const uint32_t v = dv + s * (L::KV_TILE >> 4);
+							const bool more = uni(np[X] > 0);
 #pragma unroll
 							for (int i = 0; i < BN / 16; ++i)
 							{
-								mma_ts(d, p + 8 * i, v + 128 * i, ID_PV, i > 0 ? 1 : np[X] > 0, lead);
-								mma_ts(d, p + 32 + 8 * i, v + 128 * i, ID_PV, 1, lead);
+								mma_ts(d, p + 8 * i, v + 128 * i, high, ID_PV, i > 0 ? 1 : more, lead);
+								mma_ts(d, p + 32 + 8 * i, v + 128 * i, high, ID_PV, 1, lead);
 							}
 							commit(&pv_done[X], lead);
-							if (u == to[X]) commit(&o_done[X], lead);
+							if (uni(u + u_lo == hi[X])) commit(&o_done[X], lead);
 							++np[X];
 						}
 					}
@@ -508,7 +506,9 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 		const int tid = threadIdx.x - 128;
 		constexpr int WPR = D / 8, WORDS = BN * WPR / 128; // words a row; a thread's of a half tile
 		int h = 0;
-		const auto unpack = [&](int v, int u) {
+		const auto unpack = [&](auto which, int u) {
+			constexpr bool V = decltype(which)::value;
+			constexpr int v = V;
 			const int rs = h % RS, s = u % KS;
 			uint64_t* empty = v ? v_empty : k_empty;
 			bool ok = !flags[0] && mbar_wait_bounded(&raw_full[rs], (h / RS) & 1, ws.err, DEVERR_WAIT_FULL);
@@ -521,34 +521,49 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			const unsigned char* raw = smem + L::SM_RAW + rs * L::RAW;
 			unsigned char* dst = smem + (v ? L::SM_V : L::SM_K) + s * L::KV_TILE;
 			const int key0 = (u_lo + u) * BN;
-#pragma unroll 4
-			for (int i = 0; i < WORDS; ++i)
-			{
-				const int at = tid + 128 * i, row = at / WPR, w = at % WPR;
-				const int g = kv4_unit(row, w >> 2, D), chunk = 4 * g + (w & 3); // 8 values: 16 bytes unpacked
-				uint32_t c = *reinterpret_cast<const uint32_t*>(raw + 4 * at);
-				float f = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(raw + L::CODES + (row * U + g) * 2));
-				if (v && !(fabsf(f) <= KV4_SCALE_MAX))
-				{
-					// no number (or whatever lies past the keys): zero weights must stay zero. Rows that see such a key
-					// of theirs get none at the end.
-					const int key = key0 + row;
-					if (key < x.keys) flags[1] = 1;
-					f = 0.0f;
-				}
-				const __half2 sc = __float2half2_rn(f);
-				uint32_t y[4];
+			bool odd = false;
+			constexpr int BATCH = WORDS < 8 ? WORDS : 8; // read before any is written: the stores could be to their place
 #pragma unroll
-				for (int e = 0; e < 4; ++e)
+			for (int i0 = 0; i0 < WORDS; i0 += BATCH)
+			{
+				uint32_t c[BATCH];
+				float f[BATCH];
+#pragma unroll
+				for (int i = 0; i < BATCH; ++i)
 				{
-					const uint32_t z = e >= 2 ? c >> 8 : c;
-					uint32_t m = e & 1 ? (z & 0x00F000F0u) | 0x54005400u : (z & 0x000F000Fu) | 0x64006400u;
-					const __half2 q = __hmul2(__hadd2(*reinterpret_cast<__half2*>(&m), __float2half2_rn(e & 1 ? -72.0f : -1032.0f)), sc);
-					y[e] = *reinterpret_cast<const uint32_t*>(&q);
+					const int at = tid + 128 * (i0 + i), row = at / WPR, g = kv4_unit(row, at % WPR >> 2, D);
+					c[i] = *reinterpret_cast<const uint32_t*>(raw + 4 * at);
+					f[i] = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(raw + L::CODES + (row * U + g) * 2));
 				}
-				*reinterpret_cast<uint4*>(dst + (chunk >> 3) * L::KV_PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
-					make_uint4(y[0], y[1], y[2], y[3]);
+#pragma unroll
+				for (int i = 0; i < BATCH; ++i)
+				{
+					const int at = tid + 128 * (i0 + i), row = at / WPR, w = at % WPR;
+					const int chunk = 4 * kv4_unit(row, w >> 2, D) + (w & 3); // 8 values: 16 bytes unpacked
+					if constexpr (V)
+					{
+						// no number (or whatever lies past the keys): zero weights must stay zero. Rows that see such a
+						// key of theirs get none at the end.
+						const bool fine = fabsf(f[i]) <= KV4_SCALE_MAX;
+						odd |= !fine && key0 + row < x.keys;
+						f[i] = fine ? f[i] : 0.0f;
+					}
+					const __half2 sc = __float2half2_rn(f[i]);
+					uint32_t y[4];
+#pragma unroll
+					for (int e = 0; e < 4; ++e)
+					{
+						const uint32_t z = e >= 2 ? c[i] >> 8 : c[i];
+						uint32_t m = e & 1 ? (z & 0x00F000F0u) | 0x54005400u : (z & 0x000F000Fu) | 0x64006400u;
+						const __half2 q =
+							__hmul2(__hadd2(*reinterpret_cast<__half2*>(&m), __float2half2_rn(e & 1 ? -72.0f : -1032.0f)), sc);
+						y[e] = *reinterpret_cast<const uint32_t*>(&q);
+					}
+					*reinterpret_cast<uint4*>(dst + (chunk >> 3) * L::KV_PANEL + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
+						make_uint4(y[0], y[1], y[2], y[3]);
+				}
 			}
+			if (odd) flags[1] = 1;
 			fence_async_shared();
 			mbar_arrive(v ? &v_full[s] : &k_full[s]);
 			__syncwarp();
@@ -559,13 +574,13 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 		bool ok = true;
 		for (int u = 0; ok && u <= n_u; ++u)
 		{
-			if (u < n_u) ok = unpack(0, u);
-			if (ok && u > 0) ok = unpack(1, u - 1);
+			if (u < n_u) ok = unpack(std::false_type{}, u);
+			if (ok && u > 0) ok = unpack(std::true_type{}, u - 1);
 		}
 	}
 	else
 	{
-		asm volatile("setmaxnreg.inc.sync.aligned.u32 184;" ::: "memory");
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
 		const int X = (warp - 8) >> 2, wq = warp & 3, r = wq * 32 + lane;
 		if (X < NQ)
 		{
@@ -573,44 +588,62 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			const uint32_t ts0 = tmem + 128 * X + lane_off, to = tmem + L::T_O + D * X + lane_off;
 			const int row = pc.row0 + 128 * X + r, tok = row / a.group;
 			const bool real = row < rows;
-			const size_t head = (size_t)(hk * a.group + row - tok * a.group) * D;
 			const int qp = x.pos0 + tok;
 			const int kf = a.window > 0 ? max(0, qp - a.window + 1) : 0, kl = real ? min(qp, x.keys - 1) : -1;
 
-			// ---- this row of Q, as two 16-bit halves ----
-			const float* q = a.q + (size_t)(x.q0 + tok) * a.q_stride + head;
-			float top = 0.0f;
-			if (real)
-#pragma unroll 8
-				for (int d = 0; d < D; d += 4)
-				{
-					const float4 y = *reinterpret_cast<const float4*>(q + d);
-					top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-				}
-			const int ex = top > 0.0f ? max(-100, min(100, ilogbf(top))) : 0;
-			const float f = __uint_as_float((uint32_t)(127 + 13 - ex) << 23); // the largest to [2^13, 2^14)
+			// ---- the warp's 32 rows of Q, as two 16-bit halves: whole rows, LPR lanes each ----
+			constexpr int LPR = D / 4 < 32 ? D / 4 : 32, VPL = D / 4 / LPR, RPI = 32 / LPR;
+			constexpr int BATCH = 8 / VPL; // row loads in flight
 			unsigned char* qs = smem + L::SM_Q + X * 2 * L::Q_HALF;
-#pragma unroll 4
-			for (int c = 0; c < D / 8; ++c)
+			float f = 1.0f; // this thread's row's factor
+#pragma unroll 1
+			for (int i0 = 0; i0 < 32; i0 += RPI * BATCH)
 			{
-				float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z = y;
-				if (real)
-				{
-					y = *reinterpret_cast<const float4*>(q + 8 * c);
-					z = *reinterpret_cast<const float4*>(q + 8 * c + 4);
-				}
-				const float v[8] = {y.x * f, y.y * f, y.z * f, y.w * f, z.x * f, z.y * f, z.z * f, z.w * f};
-				uint32_t h[4], l[4];
+				float4 y[BATCH][VPL];
 #pragma unroll
-				for (int e = 0; e < 4; ++e)
+				for (int i = 0; i < BATCH; ++i)
 				{
-					h[e] = pack_half2(v[2 * e], v[2 * e + 1]);
-					const float2 b = unpack_half2(h[e]);
-					l[e] = pack_half2(v[2 * e] - b.x, v[2 * e + 1] - b.y);
+					const int rw = pc.row0 + 128 * X + wq * 32 + i0 + i * RPI + lane / LPR, tk = rw / a.group;
+					const float* q = a.q + (size_t)(x.q0 + tk) * a.q_stride + (size_t)(hk * a.group + rw - tk * a.group) * D;
+#pragma unroll
+					for (int j = 0; j < VPL; ++j)
+						y[i][j] = rw < rows ? *reinterpret_cast<const float4*>(q + 4 * (lane % LPR + j * LPR))
+						                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 				}
-				unsigned char* dst = qs + (c >> 3) * L::Q_PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-				*reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-				*reinterpret_cast<uint4*>(dst + L::Q_HALF) = make_uint4(l[0], l[1], l[2], l[3]);
+				float tops[BATCH];
+#pragma unroll
+				for (int i = 0; i < BATCH; ++i)
+				{
+					tops[i] = 0.0f;
+#pragma unroll
+					for (int j = 0; j < VPL; ++j)
+						tops[i] = fmaxf(tops[i], fmaxf(fmaxf(fabsf(y[i][j].x), fabsf(y[i][j].y)), fmaxf(fabsf(y[i][j].z), fabsf(y[i][j].w))));
+				}
+#pragma unroll
+				for (int o = LPR / 2; o > 0; o >>= 1)
+#pragma unroll
+					for (int i = 0; i < BATCH; ++i) tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], o));
+#pragma unroll
+				for (int i = 0; i < BATCH; ++i)
+				{
+					const float top = tops[i];
+					const int ex = top > 0.0f ? max(-100, min(100, ilogbf(top))) : 0;
+					const float g = __uint_as_float((uint32_t)(127 + 13 - ex) << 23); // the largest to [2^13, 2^14)
+					const int first = i0 + i * RPI, rr = wq * 32 + first + lane / LPR;
+					const float g2 = __shfl_sync(0xffffffffu, g, (lane - first) * LPR & 31);
+					if (lane >= first && lane < first + RPI) f = g2;
+#pragma unroll
+					for (int j = 0; j < VPL; ++j)
+					{
+						const float4 z = make_float4(y[i][j].x * g, y[i][j].y * g, y[i][j].z * g, y[i][j].w * g);
+						const uint32_t h0 = pack_half2(z.x, z.y), h1 = pack_half2(z.z, z.w);
+						const float2 b0 = unpack_half2(h0), b1 = unpack_half2(h1);
+						const int c = (lane % LPR + j * LPR) >> 1; // the 16-byte chunk: this lane has one half of it
+						unsigned char* dst = qs + (c >> 3) * L::Q_PANEL + rr * 128 + (((c & 7) ^ (rr & 7)) << 4) + (lane & 1) * 8;
+						*reinterpret_cast<uint2*>(dst) = make_uint2(h0, h1);
+						*reinterpret_cast<uint2*>(dst + L::Q_HALF) = make_uint2(pack_half2(z.x - b0.x, z.y - b0.y), pack_half2(z.z - b1.x, z.w - b1.y));
+					}
+				}
 			}
 			fence_async_shared();
 			mbar_arrive(q_ready);
@@ -656,21 +689,25 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 					float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
 					for (int i = 0; i < 4; ++i) sum[i] = 0.0f;
-					uint32_t lo32[32];
-					uint32_t hi32[32];
 #pragma unroll
-					for (int c = 0; c < BN; c += 2)
+					for (int c0 = 0; c0 < BN; c0 += 32)
 					{
-						const float e0 = fmaf(s[c], sl, h), e1 = fmaf(s[c + 1], sl, h);
-						mx[(c >> 1) & 3] = fmaxf(mx[(c >> 1) & 3], fmaxf(e0, e1));
-						const float p0 = ex2(e0), p1 = ex2(e1);
-						sum[(c >> 1) & 3] += p0 + p1;
-						hi32[c >> 1] = pack_half2(p0, p1);
-						const float2 y = unpack_half2(hi32[c >> 1]);
-						lo32[c >> 1] = pack_half2(p0 - y.x, p1 - y.y);
+						float ph[16], pl[16]; // pairs of 16-bit halves
+#pragma unroll
+						for (int c = c0; c < c0 + 32; c += 2)
+						{
+							const float e0 = fmaf(s[c], sl, h), e1 = fmaf(s[c + 1], sl, h);
+							mx[(c >> 1) & 3] = fmaxf(mx[(c >> 1) & 3], fmaxf(e0, e1));
+							const float p0 = ex2(e0), p1 = ex2(e1);
+							sum[(c >> 1) & 3] += p0 + p1;
+							const uint32_t w = pack_half2(p0, p1);
+							const float2 y = unpack_half2(w);
+							ph[(c - c0) >> 1] = __uint_as_float(w);
+							pl[(c - c0) >> 1] = __uint_as_float(pack_half2(p0 - y.x, p1 - y.y));
+						}
+						tmem_st<16>(ts + c0 / 2, ph);
+						tmem_st<16>(ts + 32 + c0 / 2, pl);
 					}
-					st32u(ts, hi32);
-					st32u(ts + 32, lo32);
 					return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 				};
 				float alpha = 1.0f;
@@ -739,7 +776,33 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			// ---- the row's output, or its part of it ----
 			const bool spoilt = flags[1] != 0;
 			const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-			float* out = a.out + (size_t)(x.q0 + tok) * a.out_stride + head;
+			// (this Q tile is not read any more, nor, after the barrier, still being written: O goes out through its
+			// place, whole rows at a time)
+			named_sync(2 + X, 128);
+			unsigned char* os = smem + L::SM_Q + X * 2 * L::Q_HALF + wq * 32 * (D * 4);
+			const auto stage_out = [&](int c, const float (&o)[32], float by) {
+#pragma unroll
+				for (int i = 0; i < 32; i += 4)
+					*reinterpret_cast<float4*>(os + lane * (D * 4) + ((((c + i) / 4) ^ (lane & 7)) << 4)) =
+						make_float4(o[i] * by, o[i + 1] * by, o[i + 2] * by, o[i + 3] * by);
+			};
+			const auto rows_out = [&]() {
+				__syncwarp();
+#pragma unroll 4
+				for (int i = 0; i < 32; i += RPI)
+				{
+					const int in = i + lane / LPR, rw = pc.row0 + 128 * X + wq * 32 + in, tk = rw / a.group;
+					if (rw >= rows) continue;
+					float* dst = a.out + (size_t)(x.q0 + tk) * a.out_stride + (size_t)(hk * a.group + rw - tk * a.group) * D;
+#pragma unroll
+					for (int j = 0; j < VPL; ++j)
+					{
+						const int c = lane % LPR + j * LPR;
+						*reinterpret_cast<float4*>(dst + 4 * c) =
+							*reinterpret_cast<const float4*>(os + in * (D * 4) + ((c ^ (in & 7)) << 4));
+					}
+				}
+			};
 			const auto slot = [&](int i) { // piece i of the block
 				return ws.parts + ((size_t)(pc.split0 - (n_pieces - 1 - pid - pc.first) + i) * a.n_kv + hk) * L::PART;
 			};
@@ -774,13 +837,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 					}
 				}
 				if (pc.n == 1)
-				{
-					if (real)
-#pragma unroll
-						for (int i = 0; i < 32; i += 4)
-							*reinterpret_cast<float4*>(out + c + i) =
-								make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-				}
+					stage_out(c, o, inv);
 				else
 				{
 					float4* p = reinterpret_cast<float4*>(slot(my)) + (c / 4) * L::BR + 128 * X + r;
@@ -788,7 +845,9 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 					for (int i = 0; i < 32; i += 4) p[(i / 4) * L::BR] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
 				}
 			}
-			if (pc.n > 1)
+			if (pc.n == 1)
+				rows_out();
+			else
 			{
 				reinterpret_cast<float2*>(slot(my) + (size_t)L::BR * D)[128 * X + r] =
 					make_float2(held == 1e30f ? -CUDART_INF_F : HELD - held, l);
@@ -827,12 +886,9 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 								o[4 * e + 2] = fmaf(y.z, g, o[4 * e + 2]), o[4 * e + 3] = fmaf(y.w, g, o[4 * e + 3]);
 							}
 						}
-						if (real)
-#pragma unroll
-							for (int e = 0; e < 32; e += 4)
-								*reinterpret_cast<float4*>(out + c + e) =
-									make_float4(o[e] * winv, o[e + 1] * winv, o[e + 2] * winv, o[e + 3] * winv);
+						stage_out(c, o, winv);
 					}
+					rows_out();
 				}
 			}
 		}
