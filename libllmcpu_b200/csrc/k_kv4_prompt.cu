@@ -49,6 +49,11 @@ constexpr int SHARES = 2 * 148;  // pieces are about total / SHARES tiles long, 
 constexpr int MIN_PIECE = 8;
 constexpr float HELD = 11.0f, HELD_TOP = 15.0f; // see k_kv4_attn.cu
 constexpr int PLAN_THREADS = 1024;
+// Each product cuts the accumulator off at 24 bits, always towards zero: over
+// a long run of tiles that adds up (6e-6 of the output after 50 tiles). So O
+// starts anew every FRESH tiles, and the threads add up what it held, rounded
+// to nearest, in the CTA's part of the workspace (one per SM: a CTA fills it).
+constexpr int FRESH = 6, MAX_SMS = 192;
 
 template <int D>
 struct PShape
@@ -92,6 +97,7 @@ struct PromptWs
 	Piece* pieces;
 	int* counters;   // [blocks][n_kv]
 	float* parts;
+	float* sums;     // [MAX_SMS][D / 4][BR] of 4: what O held before it started anew
 	int max_blocks, max_pieces;
 };
 
@@ -294,6 +300,9 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 	int* loaded = reinterpret_cast<int*>(bars + 33); // [16] by tile: which 16-key parts of it are in the cache
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+	uint32_t sm;
+	asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
+	sm = min(sm, (uint32_t)MAX_SMS - 1);
 	const Kv4Request x = kv4_request(a, pc.r);
 	const int rows = prompt_rows(a, x, min_rows);
 	// each Q tile's key tiles within the piece; none: lo > hi
@@ -463,7 +472,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 							tc_fence_after();
 							const uint32_t d = tm + L::T_O + D * X, p = tm + 128 * X + (odd ? 64 : 0);
 							const uint32_t v = dv + s * (L::KV_TILE >> 4);
-							const bool more = uni(np[X] > 0);
+							const bool more = uni(np[X] % FRESH > 0);
 #pragma unroll
 							for (int i = 0; i < BN / 16; ++i)
 							{
@@ -652,6 +661,30 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			const float mult = (a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f) / f;
 			const float cap2 = a.softcap * 1.4426950408889634f;
 			float held = 1e30f, l = 0.0f; // HELD - held score (1e30: no key seen)
+			// O's earlier parts, relative to sums_held
+			float4* sums = reinterpret_cast<float4*>(ws.sums + (size_t)sm * L::BR * D) + 128 * X + r;
+			float sums_held = 0.0f;
+			bool have_sums = false;
+			const auto add_up = [&](float now) {
+				const float by = have_sums ? ex2(now - sums_held) : 0.0f;
+#pragma unroll
+				for (int c = 0; c < D; c += 32)
+				{
+					float o[32];
+					tmem_ld32(to + c, o);
+					float4 y[8];
+#pragma unroll
+					for (int i = 0; i < 8; ++i)
+						y[i] = have_sums ? __ldcg(sums + (c / 4 + i) * L::BR) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+					tmem_wait_ld();
+#pragma unroll
+					for (int i = 0; i < 8; ++i)
+						__stcg(sums + (c / 4 + i) * L::BR,
+						       make_float4(fmaf(y[i].x, by, o[4 * i]), fmaf(y[i].y, by, o[4 * i + 1]), fmaf(y[i].z, by, o[4 * i + 2]),
+						                   fmaf(y[i].w, by, o[4 * i + 3])));
+				}
+				have_sums = true;
+			};
 			bool ok = true;
 			int n = 0;
 			const int t_lo = X ? lo[1] : lo[0], t_hi = X ? hi[1] : hi[0];
@@ -710,6 +743,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 					}
 					return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 				};
+				const float before = held; // what O is relative to
 				float alpha = 1.0f;
 				bool move;
 				if (__any_sync(0xffffffffu, held == 1e30f))
@@ -741,7 +775,8 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 						write_p(held);
 					}
 				}
-				if (__any_sync(0xffffffffu, move) && n > 0)
+				const bool fresh = n > 0 && n % FRESH == 0;
+				if (fresh || (__any_sync(0xffffffffu, move) && n > 0))
 				{
 					// O must hold every P V before this tile's. (S of this tile completed after P V of tile n - 2, so
 					// pv_done is at most one phase behind and its parity does not alias.)
@@ -752,16 +787,22 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 						break;
 					}
 					tc_fence_after();
-#pragma unroll
-					for (int c = 0; c < D; c += 32)
+					if (fresh)
 					{
-						float o[32];
-						tmem_ld32(to + c, o);
-						tmem_wait_ld();
-#pragma unroll
-						for (int i = 0; i < 32; ++i) o[i] *= alpha;
-						tmem_st32(to + c, o);
+						add_up(before);
+						sums_held = before;
 					}
+					else
+#pragma unroll
+						for (int c = 0; c < D; c += 32)
+						{
+							float o[32];
+							tmem_ld32(to + c, o);
+							tmem_wait_ld();
+#pragma unroll
+							for (int i = 0; i < 32; ++i) o[i] *= alpha;
+							tmem_st32(to + c, o);
+						}
 				}
 				tmem_wait_st();
 				l = fmaf(l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
@@ -819,6 +860,17 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 				else
 #pragma unroll
 					for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+				if (have_sums)
+				{
+					const float by = ex2(held - sums_held);
+#pragma unroll
+					for (int i = 0; i < 8; ++i)
+					{
+						const float4 y = __ldcg(sums + (c / 4 + i) * L::BR);
+						o[4 * i] = fmaf(y.x, by, o[4 * i]), o[4 * i + 1] = fmaf(y.y, by, o[4 * i + 1]);
+						o[4 * i + 2] = fmaf(y.z, by, o[4 * i + 2]), o[4 * i + 3] = fmaf(y.w, by, o[4 * i + 3]);
+					}
+				}
 				if (spoilt && real)
 				{
 					// (32 columns are one group of values)
@@ -925,6 +977,7 @@ size_t prompt_ws(unsigned char* base, size_t at, int n_req, long long rows, int 
 	ws.pieces = reinterpret_cast<Piece*>(take(sizeof(Piece) * (size_t)pieces));
 	ws.counters = reinterpret_cast<int*>(take(4 * (size_t)blocks * n_kv));
 	ws.parts = reinterpret_cast<float*>(take((size_t)2 * SHARES * L::PART * 4));
+	ws.sums = reinterpret_cast<float*>(take((size_t)MAX_SMS * L::BR * D * 4));
 	return at;
 }
 

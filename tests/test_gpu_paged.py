@@ -399,6 +399,16 @@ def test_one_workspace_for_all_row_counts(nncu, torch_cuda, d):
         a.check(a.out)
 
 
+@pytest.mark.parametrize("case", [([(2100, 70), (1500, 45)], 1, 4, 128, 64, 0, 0.0), ([(1400, 40)], 2, 2, 256, 16, 0, 0.0),
+                                  ([(2600, 90), (40, 33)], 1, 4, 64, 32, 1100, 0.0)])
+def test_prompts_over_long_spans(nncu, torch_cuda, case):
+    """Spans of many tiles: sums that start anew on their way, and pieces that meet."""
+    a = Attn(torch_cuda, nncu, case)
+    nncu.kv4_attention_dev(a.call)
+    nncu.kv4_check(a.call)
+    a.check(a.out)
+
+
 @pytest.mark.parametrize("k_scale", [1e-4, 30.0])
 def test_attention_of_flat_and_sharp_scores(nncu, torch_cuda, k_scale):
     """Near-equal weights, and one key that outweighs all others. Scores reach
