@@ -232,8 +232,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeArgs 
 		return w < nq ? r.q + (size_t)t * r.q_stride + (size_t)w * D
 		              : r.k + (size_t)t * r.k_stride + (size_t)(w - nq) * D;
 	};
-	RopeVec<VEC> x[IPL];
-	const auto load = [&](int w) {
+	RopeVec<VEC> x[IPL], ahead[IPL];
+	const auto load = [&](RopeVec<VEC> (&x)[IPL], int w) {
 		const float* p = source(w);
 #pragma unroll
 		for (int j = 0; j < IPL; ++j)
@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeArgs 
 		}
 	};
 	int w = threadIdx.x / LPV;
-	if (w < n_vec) load(w);
+	if (w < n_vec) load(x, w);
+	if (w + VPC < n_vec) load(ahead, w + VPC);
 
 	for (int i = threadIdx.x; i < half; i += ROPE_THREADS)
 	{
@@ -321,7 +322,9 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeArgs 
 			}
 			rope_store<VEC>(x[j], y, a, b);
 		}
-		if (w + VPC < n_vec) load(w + VPC);
+#pragma unroll
+		for (int j = 0; j < IPL; ++j) x[j] = ahead[j];
+		if (w + 2 * VPC < n_vec) load(ahead, w + 2 * VPC);
 	}
 }
 
@@ -352,55 +355,66 @@ int launch_rope_axes(const RopeArgs& g, cudaStream_t st)
 // 32-bit word. blockIdx.y: K or V.
 
 constexpr int ROWS_THREADS = 256;
-constexpr int ROWS_ITEMS = 4; // 16-byte loads in flight a thread
+constexpr int ROWS_ITEMS = 4;           // 16-byte pieces in flight a thread
+constexpr long long ROWS_MOST = 1 << 30; // pieces of one launch, so that 32 bits number them
 
 struct RowsArgs
 {
 	uint8_t* pages;
-	int n_pages, page, n_kv, D, n_tok;
+	int n_pages, page_shift, n_kv, d_shift, n_tok;
+	uint32_t per_tok;  // 16-byte pieces a token
+	uint32_t div_m;    // piece / per_tok = piece * div_m >> div_s (pieces below 2^31)
+	int div_s;
 	const int* slots;
 	float* x[2];
 	size_t stride[2];
 	int first; // 0: from K; 1: V only
 };
 
+// Piece i: its token, and the piece within the token's row.
+__device__ __forceinline__ void rows_split(const RowsArgs& a, uint32_t i, uint32_t& t, uint32_t& piece)
+{
+	t = (uint32_t)(((uint64_t)i * a.div_m) >> a.div_s);
+	piece = i - t * a.per_tok;
+}
+
 // Where a token's row of one KV head sits: its codes and its scales.
 __device__ __forceinline__ bool rows_at(const RowsArgs& a, int which, int slot, int h, int& off, uint8_t*& codes,
                                         uint16_t*& scales)
 {
-	const int pg = slot / a.page;
+	const int pg = slot >> a.page_shift, page = 1 << a.page_shift, D = 1 << a.d_shift;
 	if (slot < 0 || pg >= a.n_pages) return false;
-	off = slot - pg * a.page;
-	const int cb = kv4_codes_bytes(a.page, a.D), sb = kv4_scales_bytes(a.page, a.D);
-	uint8_t* chunk = a.pages + ((size_t)pg * a.n_kv + h) * kv4_chunk_bytes(a.page, a.D);
-	codes = chunk + which * cb + off * (a.D / 2);
-	scales = reinterpret_cast<uint16_t*>(chunk + 2 * cb + which * sb) + off * (a.D / KV4_GROUP);
+	off = slot & (page - 1);
+	const int cb = kv4_codes_bytes(page, D), sb = kv4_scales_bytes(page, D);
+	uint8_t* chunk = a.pages + ((size_t)pg * a.n_kv + h) * kv4_chunk_bytes(page, D);
+	codes = chunk + which * cb + off * (D / 2);
+	scales = reinterpret_cast<uint16_t*>(chunk + 2 * cb + which * sb) + off * (D / KV4_GROUP);
 	return true;
 }
 
 __global__ void __launch_bounds__(ROWS_THREADS) kv4_append_kernel(const RowsArgs a)
 {
-	const int which = a.first + blockIdx.y;
+	const int which = a.first + blockIdx.y, D = 1 << a.d_shift;
 	const float* __restrict__ src = a.x[which];
 	const size_t stride = a.stride[which];
-	const int per_tok = a.n_kv * a.D / 4; // 16-byte pieces a token
-	const long long total = (long long)a.n_tok * per_tok;
-	const long long base = (long long)blockIdx.x * (ROWS_THREADS * ROWS_ITEMS) + threadIdx.x;
+	const uint32_t total = (uint32_t)a.n_tok * a.per_tok;
+	const uint32_t base = blockIdx.x * (ROWS_THREADS * ROWS_ITEMS) + threadIdx.x;
 	float4 v[ROWS_ITEMS];
-	int slot[ROWS_ITEMS], piece[ROWS_ITEMS];
+	int slot[ROWS_ITEMS];
+	uint32_t piece[ROWS_ITEMS];
 #pragma unroll
 	for (int j = 0; j < ROWS_ITEMS; ++j)
 	{
-		const long long i = base + (long long)j * ROWS_THREADS;
+		const uint32_t i = base + j * ROWS_THREADS;
 		slot[j] = -1;
 		piece[j] = 0;
 		v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 		if (i < total)
 		{
-			const int t = (int)(i / per_tok);
-			piece[j] = (int)(i - (long long)t * per_tok);
+			uint32_t t;
+			rows_split(a, i, t, piece[j]);
 			slot[j] = a.slots[t];
-			v[j] = *reinterpret_cast<const float4*>(src + (size_t)t * stride + 4 * (size_t)piece[j]);
+			v[j] = __ldcs(reinterpret_cast<const float4*>(src + (size_t)t * stride + 4 * (size_t)piece[j]));
 		}
 	}
 #pragma unroll
@@ -432,42 +446,60 @@ __global__ void __launch_bounds__(ROWS_THREADS) kv4_append_kernel(const RowsArgs
 			w |= (uint32_t)(c + 8) << (4 * kv4_nibble(4 * (l8 & 1) + e));
 		}
 		w |= __shfl_xor_sync(0xffffffffu, w, 1);
-		const int h = piece[j] / (a.D / 4), g = piece[j] % (a.D / 4) / 8;
+		const int h = piece[j] >> (a.d_shift - 2), g = (piece[j] & (D / 4 - 1)) / 8;
 		int off;
 		uint8_t* codes;
 		uint16_t* scales;
 		if (rows_at(a, which, slot[j], h, off, codes, scales))
 		{
-			if (!(l8 & 1)) *reinterpret_cast<uint32_t*>(codes + 16 * kv4_unit(off, g, a.D) + 2 * l8) = w;
+			if (!(l8 & 1)) *reinterpret_cast<uint32_t*>(codes + 16 * kv4_unit(off, g, D) + 2 * l8) = w;
 			if (l8 == 0) scales[g] = bad ? (uint16_t)0x7fc0u : (uint16_t)(__float_as_uint(s) >> 16);
 		}
 	}
 }
 
-// ---- and its reading back: a thread takes one word (8 values) -----------------------------
+// ---- and its reading back: a piece is 4 values, half a word ------------------------------
 
 __global__ void __launch_bounds__(ROWS_THREADS) kv4_read_kernel(const RowsArgs a)
 {
-	const int which = a.first + blockIdx.y;
-	const int per_tok = a.n_kv * a.D / 8;
-	const long long i = (long long)blockIdx.x * ROWS_THREADS + threadIdx.x;
-	if (i >= (long long)a.n_tok * per_tok) return;
-	const int t = (int)(i / per_tok), word = (int)(i - (long long)t * per_tok);
-	const int h = word / (a.D / 8), in = word % (a.D / 8), g = in / 4;
-	float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-	int off;
-	uint8_t* codes;
-	uint16_t* scales;
-	if (rows_at(a, which, a.slots[t], h, off, codes, scales))
-	{
-		const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + 16 * kv4_unit(off, g, a.D) + 4 * (in & 3));
-		const float s = bf16_bits_to_float(scales[g]);
+	const int which = a.first + blockIdx.y, D = 1 << a.d_shift;
+	const uint32_t total = (uint32_t)a.n_tok * a.per_tok;
+	const uint32_t base = blockIdx.x * (ROWS_THREADS * ROWS_ITEMS) + threadIdx.x;
+	uint32_t t[ROWS_ITEMS], piece[ROWS_ITEMS], w[ROWS_ITEMS];
+	int slot[ROWS_ITEMS];
+	float s[ROWS_ITEMS];
 #pragma unroll
-		for (int e = 0; e < 8; ++e) y[e] = s * (float)((int)((w >> (4 * kv4_nibble(e))) & 15u) - 8);
+	for (int j = 0; j < ROWS_ITEMS; ++j)
+	{
+		const uint32_t i = base + j * ROWS_THREADS;
+		rows_split(a, i < total ? i : 0, t[j], piece[j]);
+		slot[j] = a.slots[t[j]];
 	}
-	float4* dst = reinterpret_cast<float4*>(a.x[which] + (size_t)t * a.stride[which] + 8 * (size_t)word);
-	dst[0] = make_float4(y[0], y[1], y[2], y[3]);
-	dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+#pragma unroll
+	for (int j = 0; j < ROWS_ITEMS; ++j)
+	{
+		const int h = piece[j] >> (a.d_shift - 2), in = piece[j] & (D / 4 - 1), g = in / 8;
+		int off;
+		uint8_t* codes;
+		uint16_t* scales;
+		w[j] = 0;
+		s[j] = 0.0f;
+		if (rows_at(a, which, slot[j], h, off, codes, scales))
+		{
+			w[j] = *reinterpret_cast<const uint32_t*>(codes + 16 * kv4_unit(off, g, D) + 4 * ((in >> 1) & 3));
+			s[j] = bf16_bits_to_float(scales[g]);
+		}
+	}
+#pragma unroll
+	for (int j = 0; j < ROWS_ITEMS; ++j)
+	{
+		if (base + j * ROWS_THREADS >= total) continue;
+		float y[4];
+#pragma unroll
+		for (int e = 0; e < 4; ++e) y[e] = s[j] * (float)((int)((w[j] >> (4 * kv4_nibble(4 * (piece[j] & 1) + e))) & 15u) - 8);
+		__stcs(reinterpret_cast<float4*>(a.x[which] + (size_t)t[j] * a.stride[which] + 4 * (size_t)piece[j]),
+		       make_float4(y[0], y[1], y[2], y[3]));
+	}
 }
 
 int refuse(const char* msg) { return set_error(NNCU_ERR_INVALID_ARGUMENT, msg); }
@@ -492,9 +524,37 @@ int rows_args(const nncu_kv4_rows* r, const char* what, RowsArgs& a)
 	else if (r->n_tok > 1 && ((r->k && r->k_stride < row) || (r->v && r->v_stride < row)))
 		snprintf(msg, sizeof msg, "%s: strides shorter than a row", what);
 	if (msg[0]) return refuse(msg);
-	a = RowsArgs{static_cast<uint8_t*>(r->pool.pages), r->pool.n_pages, r->pool.page_size, r->pool.n_kv,
-	             r->pool.head_dim, r->n_tok, r->slots, {r->k, r->v}, {r->k_stride, r->v_stride}, r->k ? 0 : 1};
+	const auto log2i = [](int x) {
+		int s = 0;
+		while ((1 << s) < x) ++s;
+		return s;
+	};
+	const uint32_t per_tok = (uint32_t)(row / 4);
+	int s = 0; // ceil(log2 per_tok): the multiplier 2^(31 + s) / per_tok, rounded up, fits 32 bits and divides exactly
+	while ((1ull << s) < per_tok) ++s;
+	a = RowsArgs{static_cast<uint8_t*>(r->pool.pages), r->pool.n_pages, log2i(r->pool.page_size), r->pool.n_kv,
+	             log2i(r->pool.head_dim), r->n_tok, per_tok, (uint32_t)(((1ull << (31 + s)) + per_tok - 1) / per_tok),
+	             31 + s, r->slots, {r->k, r->v}, {r->k_stride, r->v_stride}, r->k ? 0 : 1};
 	return NNCU_OK;
+}
+
+// The rows in launches of at most ROWS_MOST pieces.
+template <typename K>
+int launch_rows(K kernel, RowsArgs a, cudaStream_t st)
+{
+	const int most = (int)(ROWS_MOST / a.per_tok), all = a.n_tok;
+	for (int t0 = 0; t0 < all; t0 += most)
+	{
+		a.n_tok = all - t0 < most ? all - t0 : most;
+		const uint32_t pieces = (uint32_t)a.n_tok * a.per_tok;
+		const dim3 grid((pieces + ROWS_THREADS * ROWS_ITEMS - 1) / (ROWS_THREADS * ROWS_ITEMS), a.x[0] && a.x[1] ? 2u : 1u);
+		kernel<<<grid, ROWS_THREADS, 0, st>>>(a);
+		note_launches(1);
+		a.slots += a.n_tok;
+		for (int w = 0; w < 2; ++w)
+			if (a.x[w]) a.x[w] += (size_t)a.n_tok * a.stride[w];
+	}
+	return (int)cudaGetLastError();
 }
 
 } // namespace
@@ -507,7 +567,7 @@ int kv4_check_pool(const nncu_kv4_pool* p, const char* what, bool need_pages)
 		snprintf(msg, sizeof msg, "%s: head_dim %d (64, 128 and 256 are served)", what, (int)p->head_dim);
 	else if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
 		snprintf(msg, sizeof msg, "%s: page_size %d (16, 32, 64, 128 or 256)", what, (int)p->page_size);
-	else if (p->n_pages <= 0 || p->n_kv <= 0 || (long long)p->n_pages * p->page_size > INT32_MAX || p->n_kv > 65535)
+	else if (p->n_pages <= 0 || p->n_kv <= 0 || (long long)p->n_pages * p->page_size > INT32_MAX || (long long)p->n_kv * p->head_dim > (1 << 24))
 		snprintf(msg, sizeof msg, "%s: bad n_pages or n_kv", what);
 	else if (need_pages && (!p->pages || !aligned16(p->pages)))
 		snprintf(msg, sizeof msg, "%s: pages NULL or not 16-byte aligned", what);
@@ -605,12 +665,7 @@ extern "C" int nncu_kv4_append_dev(const nncu_kv4_rows* rows, void* stream)
 	RowsArgs a;
 	const int rc = rows_args(rows, "kv4 append", a);
 	if (rc != NNCU_OK || a.n_tok == 0) return rc;
-	const long long pieces = (long long)a.n_tok * a.n_kv * a.D / 4;
-	const dim3 grid((unsigned)((pieces + ROWS_THREADS * ROWS_ITEMS - 1) / (ROWS_THREADS * ROWS_ITEMS)),
-	                a.x[0] && a.x[1] ? 2u : 1u);
-	kv4_append_kernel<<<grid, ROWS_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
-	note_launches(1);
-	const int e = (int)cudaGetLastError();
+	const int e = launch_rows(kv4_append_kernel, a, static_cast<cudaStream_t>(stream));
 	return e ? set_cuda_error(e, "kv4 append launch") : NNCU_OK;
 }
 
@@ -619,10 +674,6 @@ extern "C" int nncu_kv4_read_dev(const nncu_kv4_rows* rows, void* stream)
 	RowsArgs a;
 	const int rc = rows_args(rows, "kv4 read", a);
 	if (rc != NNCU_OK || a.n_tok == 0) return rc;
-	const long long words = (long long)a.n_tok * a.n_kv * a.D / 8;
-	const dim3 grid((unsigned)((words + ROWS_THREADS - 1) / ROWS_THREADS), a.x[0] && a.x[1] ? 2u : 1u);
-	kv4_read_kernel<<<grid, ROWS_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
-	note_launches(1);
-	const int e = (int)cudaGetLastError();
+	const int e = launch_rows(kv4_read_kernel, a, static_cast<cudaStream_t>(stream));
 	return e ? set_cuda_error(e, "kv4 read launch") : NNCU_OK;
 }
