@@ -163,14 +163,16 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 
 // ---- norm and rotation by per-token positions ---------------------------------------
 //
-// Memory bound: 8 bytes a value. One CTA per token: its angles (their cosines
-// and sines) serve all its heads, so they are formed once, in shared memory,
-// while the first head vectors are already on their way. A head vector is
-// spread over LPV lanes; a lane's item is the 2 VEC values that turn together
-// (NEOX: VEC at e and VEC at e + n_rot / 2), so no exchange between lanes is
-// needed but the norm's sum.
+// Memory bound: 8 bytes a value. A CTA takes tokens in turn; a token's angles
+// (their cosines and sines) serve all its heads, so they are formed once, in
+// shared memory, while the first head vectors are already on their way, and
+// then held in registers, as the gains are: a head vector is spread over LPV
+// lanes, and a lane has the same places of every vector. Its item is the 2 VEC
+// values that turn together (NEOX: VEC at e and VEC at e + n_rot / 2), so no
+// exchange between lanes is needed but the norm's sum.
 
 constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_CTAS = 4 * 148; // what fits on the SMs at once: more tokens are taken in turn
 
 struct RopeArgs
 {
@@ -210,159 +212,166 @@ __device__ __forceinline__ void rope_store(const RopeVec<VEC>& x, float* p, int 
 }
 
 // IPL items a lane, LPV lanes a vector (a power of two).
-template <int VEC, int IPL, int LPV>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeArgs g)
+template <int VEC, int IPL, int LPV, bool NEOX>
+__global__ void __launch_bounds__(ROPE_THREADS, VEC * IPL <= 4 ? 4 : 2) rope_axes_kernel(const RopeArgs g)
 {
 	const nncu_rope_axes& r = g.r;
-	__shared__ float2 turn[256]; // cos, sin of the token's pairs
+	__shared__ float2 turn[2][256]; // cos, sin of a token's pairs
 	constexpr int VPC = ROPE_THREADS / LPV; // vectors in flight a CTA
-	const int t = blockIdx.x, half = g.half, D = r.head_dim, items = D / (2 * VEC);
-	const int lane = threadIdx.x % LPV;
-	const bool neox = r.rope_mode == NNCU_ROPE_NEOX;
+	const int half = g.half, D = r.head_dim, items = D / (2 * VEC), turning = half / VEC;
+	const int lane = threadIdx.x % LPV, slot = threadIdx.x / LPV;
 	const int nq = r.q ? r.n_head : 0, n_vec = nq + (r.k ? r.n_kv : 0);
 
-	// where item i's two runs of VEC values begin
-	const auto place = [&](int i, int& a, int& b) {
-		if (neox && i < half / VEC)
-			a = i * VEC, b = a + half;
+	// where this lane's items' two runs of VEC values begin (those past n_rot: two halves of the rest), and the gains
+	int a[IPL], b[IPL];
+	RopeVec<VEC> gq[IPL], gk[IPL];
+#pragma unroll
+	for (int j = 0; j < IPL; ++j)
+	{
+		const int i = lane + j * LPV;
+		if (!NEOX)
+			a[j] = 2 * VEC * i, b[j] = a[j] + VEC;
+		else if (i < turning)
+			a[j] = i * VEC, b[j] = a[j] + half;
 		else
-			a = 2 * VEC * i, b = a + VEC;
-	};
-	const auto source = [&](int w) {
-		return w < nq ? r.q + (size_t)t * r.q_stride + (size_t)w * D
-		              : r.k + (size_t)t * r.k_stride + (size_t)(w - nq) * D;
-	};
-	RopeVec<VEC> x[IPL], ahead[IPL];
-	const auto load = [&](RopeVec<VEC> (&x)[IPL], int w) {
-		const float* p = source(w);
+			a[j] = half + i * VEC, b[j] = a[j] + D / 2 - half;
+#pragma unroll
+		for (int e = 0; e < 2 * VEC; ++e) gq[j].v[e] = gk[j].v[e] = 1.0f;
+		if (r.q_gamma && i < items) rope_load<VEC>(gq[j], r.q_gamma, a[j], b[j]);
+		if (r.k_gamma && i < items) rope_load<VEC>(gk[j], r.k_gamma, a[j], b[j]);
+	}
+	const auto load = [&](RopeVec<VEC> (&x)[IPL], int t, int w) {
+		const float* p = w < nq ? r.q + (size_t)t * r.q_stride + (size_t)w * D
+		                        : r.k + (size_t)t * r.k_stride + (size_t)(w - nq) * D;
 #pragma unroll
 		for (int j = 0; j < IPL; ++j)
-		{
-			const int i = lane + j * LPV;
-			int a, b;
-			place(i, a, b);
-			if (i < items) rope_load<VEC>(x[j], p, a, b);
-		}
+			if (lane + j * LPV < items) rope_load<VEC>(x[j], p, a[j], b[j]);
 	};
-	int w = threadIdx.x / LPV;
-	if (w < n_vec) load(x, w);
-	if (w + VPC < n_vec) load(ahead, w + VPC);
-
-	for (int i = threadIdx.x; i < half; i += ROPE_THREADS)
+	int buf = 0;
+	for (int t = blockIdx.x; t < r.n_tok; t += gridDim.x, buf ^= 1)
 	{
-		int axis = 0;
-		if (r.interleaved)
+		RopeVec<VEC> x[IPL], ahead[IPL];
+		int w = slot;
+		if (w < n_vec) load(x, t, w);
+		for (int i = threadIdx.x; i < half; i += ROPE_THREADS)
 		{
-			const int a = i % r.n_axes;
-			axis = i / r.n_axes < r.section[a] ? a : 0;
+			int axis = 0;
+			if (r.interleaved)
+			{
+				const int m = i % r.n_axes;
+				axis = i / r.n_axes < r.section[m] ? m : 0;
+			}
+			else
+				for (int e = r.section[0]; axis + 1 < r.n_axes && i >= e; e += r.section[axis]) ++axis;
+			const float angle = (float)r.positions[axis * r.pos_stride + t] * r.inv_freq[i];
+			float sn, cs;
+			sincosf(angle, &sn, &cs);
+			turn[buf][i] = make_float2(cs, sn);
 		}
-		else
-			for (int e = r.section[0]; axis + 1 < r.n_axes && i >= e; e += r.section[axis]) ++axis;
-		const float angle = (float)r.positions[axis * r.pos_stride + t] * r.inv_freq[i];
-		float sn, cs;
-		sincosf(angle, &sn, &cs);
-		turn[i] = make_float2(cs, sn);
-	}
-	__syncthreads();
+		if (w + VPC < n_vec) load(ahead, t, w + VPC);
+		__syncthreads(); // (two buffers: who comes here again has read this one long since)
+		float2 cs[IPL][VEC];
+#pragma unroll
+		for (int j = 0; j < IPL; ++j)
+#pragma unroll
+			for (int e = 0; e < VEC; ++e)
+				cs[j][e] = lane + j * LPV < turning ? turn[buf][(lane + j * LPV) * VEC + e] : make_float2(1.0f, 0.0f);
 
-	for (; w < n_vec; w += VPC)
-	{
-		const float* gamma = w < nq ? r.q_gamma : r.k_gamma;
-		if (gamma)
+		for (; w < n_vec; w += VPC)
 		{
-			float ss = 0.0f;
+			const bool is_q = w < nq;
+			if (is_q ? r.q_gamma != nullptr : r.k_gamma != nullptr)
+			{
+				float ss = 0.0f;
 #pragma unroll
-			for (int j = 0; j < IPL; ++j)
-				if (lane + j * LPV < items)
+				for (int j = 0; j < IPL; ++j)
+					if (lane + j * LPV < items)
 #pragma unroll
-					for (int e = 0; e < 2 * VEC; ++e) ss = fmaf(x[j].v[e], x[j].v[e], ss);
-			// the lanes of one vector leave the loop together, so they name each other alone
-			const unsigned mask = LPV == 32 ? 0xffffffffu
-			                                : ((1u << (LPV & 31)) - 1u) << ((threadIdx.x & 31) / LPV * LPV);
+						for (int e = 0; e < 2 * VEC; ++e) ss = fmaf(x[j].v[e], x[j].v[e], ss);
+				// the lanes of one vector leave the loop together, so they name each other alone
+				const unsigned mask = LPV == 32 ? 0xffffffffu
+				                                : ((1u << (LPV & 31)) - 1u) << ((threadIdx.x & 31) / LPV * LPV);
 #pragma unroll
-			for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-			const float sc = 1.0f / sqrtf(ss / (float)D + r.eps);
+				for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+				const float sc = 1.0f / sqrtf(ss / (float)D + r.eps);
+#pragma unroll
+				for (int j = 0; j < IPL; ++j)
+#pragma unroll
+					for (int e = 0; e < 2 * VEC; ++e) x[j].v[e] = x[j].v[e] * sc * (is_q ? gq[j].v[e] : gk[j].v[e]);
+			}
+			float* y = is_q ? r.q_out + (size_t)t * r.q_out_stride + (size_t)w * D
+			                : r.k_out + (size_t)t * r.k_out_stride + (size_t)(w - nq) * D;
 #pragma unroll
 			for (int j = 0; j < IPL; ++j)
 			{
-				const int i = lane + j * LPV;
-				int a, b;
-				place(i, a, b);
-				if (i < items)
+				if (lane + j * LPV >= items) continue;
+				if (lane + j * LPV < turning)
 				{
-					RopeVec<VEC> gm;
-					rope_load<VEC>(gm, gamma, a, b);
 #pragma unroll
-					for (int e = 0; e < 2 * VEC; ++e) x[j].v[e] = x[j].v[e] * sc * gm.v[e];
+					for (int e = 0; e < VEC; ++e)
+					{
+						// NEOX: values e and e + VEC of the item; NORM: 2e and 2e + 1
+						float& u = x[j].v[NEOX ? e : 2 * e];
+						float& v = x[j].v[NEOX ? e + VEC : 2 * e + 1];
+						const float u0 = u, v0 = v;
+						u = u0 * cs[j][e].x - v0 * cs[j][e].y;
+						v = u0 * cs[j][e].y + v0 * cs[j][e].x;
+					}
 				}
+				rope_store<VEC>(x[j], y, a[j], b[j]);
 			}
+#pragma unroll
+			for (int j = 0; j < IPL; ++j) x[j] = ahead[j];
+			if (w + 2 * VPC < n_vec) load(ahead, t, w + 2 * VPC);
 		}
-		float* y = w < nq ? r.q_out + (size_t)t * r.q_out_stride + (size_t)w * D
-		                  : r.k_out + (size_t)t * r.k_out_stride + (size_t)(w - nq) * D;
-#pragma unroll
-		for (int j = 0; j < IPL; ++j)
-		{
-			const int i = lane + j * LPV;
-			int a, b;
-			place(i, a, b);
-			if (i >= items) continue;
-			if (i < half / VEC)
-			{
-#pragma unroll
-				for (int e = 0; e < VEC; ++e)
-				{
-					// NEOX: values e and e + VEC of the item; NORM: 2e and 2e + 1
-					const float2 cs = turn[i * VEC + e];
-					float& u = x[j].v[neox ? e : 2 * e];
-					float& v = x[j].v[neox ? e + VEC : 2 * e + 1];
-					const float u0 = u, v0 = v;
-					u = u0 * cs.x - v0 * cs.y;
-					v = u0 * cs.y + v0 * cs.x;
-				}
-			}
-			rope_store<VEC>(x[j], y, a, b);
-		}
-#pragma unroll
-		for (int j = 0; j < IPL; ++j) x[j] = ahead[j];
-		if (w + 2 * VPC < n_vec) load(ahead, w + 2 * VPC);
 	}
+}
+
+template <int VEC, int IPL, int LPV>
+void launch_rope_as(const RopeArgs& g, cudaStream_t st)
+{
+	const unsigned grid = (unsigned)(g.r.n_tok < ROPE_CTAS ? g.r.n_tok : ROPE_CTAS);
+	if (g.r.rope_mode == NNCU_ROPE_NEOX)
+		rope_axes_kernel<VEC, IPL, LPV, true><<<grid, ROPE_THREADS, 0, st>>>(g);
+	else
+		rope_axes_kernel<VEC, IPL, LPV, false><<<grid, ROPE_THREADS, 0, st>>>(g);
 }
 
 template <int VEC>
 int launch_rope_axes(const RopeArgs& g, cudaStream_t st)
 {
 	const int items = g.r.head_dim / (2 * VEC);
-	const unsigned grid = (unsigned)g.r.n_tok;
 	if (items <= 8)
-		rope_axes_kernel<VEC, 1, 8><<<grid, ROPE_THREADS, 0, st>>>(g);
+		launch_rope_as<VEC, 1, 8>(g, st);
 	else if (items <= 16)
-		rope_axes_kernel<VEC, 1, 16><<<grid, ROPE_THREADS, 0, st>>>(g);
+		launch_rope_as<VEC, 1, 16>(g, st);
 	else if (items <= 32)
-		rope_axes_kernel<VEC, 1, 32><<<grid, ROPE_THREADS, 0, st>>>(g);
+		launch_rope_as<VEC, 1, 32>(g, st);
 	else if (items <= 64)
-		rope_axes_kernel<VEC, 2, 32><<<grid, ROPE_THREADS, 0, st>>>(g);
+		launch_rope_as<VEC, 2, 32>(g, st);
 	else if (VEC == 1)
-		rope_axes_kernel<1, 8, 32><<<grid, ROPE_THREADS, 0, st>>>(g);
+		launch_rope_as<1, 8, 32>(g, st);
 	note_launches(1);
 	return (int)cudaGetLastError();
 }
 
 // ---- the 4-bit cache's write -----------------------------------------------------------
 //
-// Memory bound: 4 bytes a value in, 0.5625 out. A group of 32 values is 8
-// lanes with a 16-byte load each; its extremes meet in three exchanges, its
-// scale and reciprocal are formed by every lane, a pair of lanes builds one
-// 32-bit word. blockIdx.y: K or V.
+// Memory bound: 4 bytes a value in, 0.5625 out. A lane takes 8 values, which
+// become one 32-bit word, four lanes a group of 32: its largest magnitude (with
+// its sign as the lowest bit, so that the positive one wins a tie) meets in two
+// exchanges, and every lane forms the scale and its reciprocal. blockIdx.y: K
+// or V.
 
 constexpr int ROWS_THREADS = 256;
-constexpr int ROWS_ITEMS = 4;           // 16-byte pieces in flight a thread
+constexpr int ROWS_ITEMS = 2;           // pieces (8 values, 32 bytes) in flight a thread
 constexpr long long ROWS_MOST = 1 << 30; // pieces of one launch, so that 32 bits number them
 
 struct RowsArgs
 {
 	uint8_t* pages;
 	int n_pages, page_shift, n_kv, d_shift, n_tok;
-	uint32_t per_tok;  // 16-byte pieces a token
+	uint32_t per_tok;  // pieces of 8 values a token
 	uint32_t div_m;    // piece / per_tok = piece * div_m >> div_s (pieces below 2^31)
 	int div_s;
 	const int* slots;
@@ -395,11 +404,11 @@ __device__ __forceinline__ bool rows_at(const RowsArgs& a, int which, int slot, 
 __global__ void __launch_bounds__(ROWS_THREADS) kv4_append_kernel(const RowsArgs a)
 {
 	const int which = a.first + blockIdx.y, D = 1 << a.d_shift;
-	const float* __restrict__ src = a.x[which];
+	const float* __restrict__ src = a.x[which]; // (K and V rows are read, never written)
 	const size_t stride = a.stride[which];
 	const uint32_t total = (uint32_t)a.n_tok * a.per_tok;
 	const uint32_t base = blockIdx.x * (ROWS_THREADS * ROWS_ITEMS) + threadIdx.x;
-	float4 v[ROWS_ITEMS];
+	float x[ROWS_ITEMS][8];
 	int slot[ROWS_ITEMS];
 	uint32_t piece[ROWS_ITEMS];
 #pragma unroll
@@ -408,57 +417,58 @@ __global__ void __launch_bounds__(ROWS_THREADS) kv4_append_kernel(const RowsArgs
 		const uint32_t i = base + j * ROWS_THREADS;
 		slot[j] = -1;
 		piece[j] = 0;
-		v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), w = v;
 		if (i < total)
 		{
 			uint32_t t;
 			rows_split(a, i, t, piece[j]);
 			slot[j] = a.slots[t];
-			v[j] = __ldcs(reinterpret_cast<const float4*>(src + (size_t)t * stride + 4 * (size_t)piece[j]));
+			const float4* p = reinterpret_cast<const float4*>(src + (size_t)t * stride + 8 * (size_t)piece[j]);
+			v = __ldcs(p);
+			w = __ldcs(p + 1);
 		}
+		x[j][0] = v.x, x[j][1] = v.y, x[j][2] = v.z, x[j][3] = v.w;
+		x[j][4] = w.x, x[j][5] = w.y, x[j][6] = w.z, x[j][7] = w.w;
 	}
 #pragma unroll
 	for (int j = 0; j < ROWS_ITEMS; ++j)
 	{
-		// (whole warps: a group's 8 lanes always work on one row)
-		const float x[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-		float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-		uint32_t bits = 0; // the largest magnitude's bits, NaN's included (the extremes above pass NaNs by)
+		// (whole warps: a group's 4 lanes always work on one row)
+		uint32_t top = 0; // magnitude's bits, then 1 where positive
 #pragma unroll
-		for (int e = 0; e < 4; ++e) bits = max(bits, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-		for (int o = 1; o < 8; o <<= 1)
+		for (int e = 0; e < 8; ++e)
 		{
-			hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-			lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-			bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+			const uint32_t u = __float_as_uint(x[j][e]);
+			top = max(top, (u << 1) | (~u >> 31));
 		}
-		const bool bad = bits >= 0x7f800000u;
-		float s = __bfloat162float(__float2bfloat16_rn((hi >= -lo ? hi : lo) * -0.125f));
+		top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+		top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+		const bool bad = (top >> 1) >= 0x7f800000u; // an infinity or a NaN
+		const float m = __uint_as_float((top >> 1) | (~top << 31));
+		float s = __bfloat162float(__float2bfloat16_rn(m * -0.125f));
 		s = copysignf(fminf(fmaxf(fabsf(s), KV4_SCALE_MIN), KV4_SCALE_MAX), s);
 		const float inv = __frcp_rn(s);
-		uint32_t w = 0;
-		const int l8 = threadIdx.x & 7; // this lane's four values of the group's 32: 4 l8 ..
+		uint32_t c[8]; // code + 8 in the low bits: the sum rounds to the nearest whole number, ties to even
 #pragma unroll
-		for (int e = 0; e < 4; ++e)
-		{
-			const int c = bad ? 0 : (int)fminf(fmaxf(rintf(x[e] * inv), -8.0f), 7.0f);
-			w |= (uint32_t)(c + 8) << (4 * kv4_nibble(4 * (l8 & 1) + e));
-		}
-		w |= __shfl_xor_sync(0xffffffffu, w, 1);
-		const int h = piece[j] >> (a.d_shift - 2), g = (piece[j] & (D / 4 - 1)) / 8;
+		for (int e = 0; e < 8; ++e)
+			c[e] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x[j][e], inv), -8.0f), 7.0f), 12582920.0f)) & 15u;
+		uint32_t w = 0;
+#pragma unroll
+		for (int e = 0; e < 8; ++e) w |= c[e] << (4 * kv4_nibble(e));
+		if (bad) w = 0x88888888u;
+		const int h = piece[j] >> (a.d_shift - 3), in = piece[j] & (D / 8 - 1), g = in / 4;
 		int off;
 		uint8_t* codes;
 		uint16_t* scales;
 		if (rows_at(a, which, slot[j], h, off, codes, scales))
 		{
-			if (!(l8 & 1)) *reinterpret_cast<uint32_t*>(codes + 16 * kv4_unit(off, g, D) + 2 * l8) = w;
-			if (l8 == 0) scales[g] = bad ? (uint16_t)0x7fc0u : (uint16_t)(__float_as_uint(s) >> 16);
+			*reinterpret_cast<uint32_t*>(codes + 16 * kv4_unit(off, g, D) + 4 * (in & 3)) = w;
+			if ((in & 3) == 0) scales[g] = bad ? (uint16_t)0x7fc0u : (uint16_t)(__float_as_uint(s) >> 16);
 		}
 	}
 }
 
-// ---- and its reading back: a piece is 4 values, half a word ------------------------------
+// ---- and its reading back: a piece is a word --------------------------------------------
 
 __global__ void __launch_bounds__(ROWS_THREADS) kv4_read_kernel(const RowsArgs a)
 {
@@ -478,7 +488,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) kv4_read_kernel(const RowsArgs a
 #pragma unroll
 	for (int j = 0; j < ROWS_ITEMS; ++j)
 	{
-		const int h = piece[j] >> (a.d_shift - 2), in = piece[j] & (D / 4 - 1), g = in / 8;
+		const int h = piece[j] >> (a.d_shift - 3), in = piece[j] & (D / 8 - 1), g = in / 4;
 		int off;
 		uint8_t* codes;
 		uint16_t* scales;
@@ -486,7 +496,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) kv4_read_kernel(const RowsArgs a
 		s[j] = 0.0f;
 		if (rows_at(a, which, slot[j], h, off, codes, scales))
 		{
-			w[j] = *reinterpret_cast<const uint32_t*>(codes + 16 * kv4_unit(off, g, D) + 4 * ((in >> 1) & 3));
+			w[j] = *reinterpret_cast<const uint32_t*>(codes + 16 * kv4_unit(off, g, D) + 4 * (in & 3));
 			s[j] = bf16_bits_to_float(scales[g]);
 		}
 	}
@@ -494,11 +504,13 @@ __global__ void __launch_bounds__(ROWS_THREADS) kv4_read_kernel(const RowsArgs a
 	for (int j = 0; j < ROWS_ITEMS; ++j)
 	{
 		if (base + j * ROWS_THREADS >= total) continue;
-		float y[4];
+		float y[8];
 #pragma unroll
-		for (int e = 0; e < 4; ++e) y[e] = s[j] * (float)((int)((w[j] >> (4 * kv4_nibble(4 * (piece[j] & 1) + e))) & 15u) - 8);
-		__stcs(reinterpret_cast<float4*>(a.x[which] + (size_t)t[j] * a.stride[which] + 4 * (size_t)piece[j]),
-		       make_float4(y[0], y[1], y[2], y[3]));
+		for (int e = 0; e < 8; ++e)
+			y[e] = s[j] * (__uint_as_float(((w[j] >> (4 * kv4_nibble(e))) & 15u) | 0x4b000000u) - 8388616.0f); // 2^23 + u, less 2^23 + 8
+		float4* p = reinterpret_cast<float4*>(a.x[which] + (size_t)t[j] * a.stride[which] + 8 * (size_t)piece[j]);
+		__stcs(p, make_float4(y[0], y[1], y[2], y[3]));
+		__stcs(p + 1, make_float4(y[4], y[5], y[6], y[7]));
 	}
 }
 
@@ -529,7 +541,7 @@ int rows_args(const nncu_kv4_rows* r, const char* what, RowsArgs& a)
 		while ((1 << s) < x) ++s;
 		return s;
 	};
-	const uint32_t per_tok = (uint32_t)(row / 4);
+	const uint32_t per_tok = (uint32_t)(row / 8);
 	int s = 0; // ceil(log2 per_tok): the multiplier 2^(31 + s) / per_tok, rounded up, fits 32 bits and divides exactly
 	while ((1ull << s) < per_tok) ++s;
 	a = RowsArgs{static_cast<uint8_t*>(r->pool.pages), r->pool.n_pages, log2i(r->pool.page_size), r->pool.n_kv,
