@@ -88,6 +88,15 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 	    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same from nothing: d = A B.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1)
+{
+	asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+	    : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+	    : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // An 8 x 8 matrix of 16-bit values, transposed across the warp.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x)
 {
@@ -137,10 +146,16 @@ __device__ __forceinline__ void load_scales(float (&f)[N], const unsigned char* 
 
 // Nibbles x and x + 4 of a word as codes: the mask makes 1024 + u (or 64 + u,
 // one nibble up) in the two halves, less 1032 (72): exact.
-__device__ __forceinline__ __half2 codes2(uint32_t w, int x)
+struct Masks
+{
+	uint32_t low = 0x000F000Fu, high = 0x00F000F0u, k1024 = 0x64006400u, k64 = 0x54005400u;
+	// kept in registers: as constants, one of the two that an operation needs would be moved there every time
+	__device__ __forceinline__ Masks() { asm volatile("" : "+r"(low), "+r"(high), "+r"(k1024), "+r"(k64)); }
+};
+__device__ __forceinline__ __half2 codes2(const Masks& mk, uint32_t w, int x)
 {
 	const uint32_t v = x >= 2 ? w >> 8 : w;
-	const uint32_t h = x & 1 ? (v & 0x00F000F0u) | 0x54005400u : (v & 0x000F000Fu) | 0x64006400u;
+	const uint32_t h = x & 1 ? (v & mk.high) | mk.k64 : (v & mk.low) | mk.k1024;
 	return __hadd2(bits_half2(h), __float2half2_rn(x & 1 ? -72.0f : -1032.0f));
 }
 
@@ -298,7 +313,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 			for (int t = tile; t < tile + n; ++t, ++it)
 			{
 				const int stage = it % STAGES;
-				if (it >= STAGES && !*abort_ && !mbar_wait_bounded(&empty[stage], ((it / STAGES) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY))
+				if (it >= STAGES && !*abort_ && !kv4_wait(&empty[stage], ((it / STAGES) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY))
 					*abort_ = 1;
 				__syncwarp();
 				const bool stop = __shfl_sync(0xffffffffu, *abort_, 0) != 0; // one answer for the warp
@@ -334,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 		// after a wait that ran out nobody may have waited for the copies in flight: not to leave before they landed
 		if (*abort_)
 			for (int i = max(0, it - STAGES); i < it; ++i)
-				mbar_wait_bounded(&full[i % STAGES], (i / STAGES) & 1, nullptr, 0);
+				kv4_wait(&full[i % STAGES], (i / STAGES) & 1, nullptr, 0);
 		return;
 	}
 
@@ -353,6 +368,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 	// scores in base 2 (with a soft-cap: its argument, and what multiplies its value)
 	const float scale2 = a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
 	const float softcap2 = a.softcap * 1.4426950408889634f;
+	const Masks mk;
 	int it = 0;
 	while (left > 0)
 	{
@@ -434,12 +450,12 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 			for (int r = 0; r < R; ++r)
 #pragma unroll
 				for (int e = 0; e < 4; ++e) o[x][r][e] = 0.0f;
-		__half2 odd = __float2half2_rn(0.0f); // no number once a V scale was none
+		bool bad = false; // a V scale was no number
 
 		for (int t = tile; t < tile + n; ++t, ++it)
 		{
 			const int stage = it % STAGES;
-			if (!*abort_ && !mbar_wait_bounded(&full[stage], (it / STAGES) & 1, ws.err, DEVERR_WAIT_FULL)) *abort_ = 1;
+			if (!*abort_ && !kv4_wait(&full[stage], (it / STAGES) & 1, ws.err, DEVERR_WAIT_FULL)) *abort_ = 1;
 			const unsigned char* st = smem + stage * L::STAGE;
 			const int key0 = (s.tile0 + t) * TILE + warp * 16;
 			if (loaded[stage] >> warp & 1)
@@ -460,13 +476,13 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 					const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + (k_off ^ (16 * g)) + 8 * (D / 2));
 					uint32_t k0[4], k1[4]; // the codes of both keys, pair by pair
 #pragma unroll
-					for (int x = 0; x < 4; ++x) k0[x] = half2_bits(codes2(w0, x)), k1[x] = half2_bits(codes2(w1, x));
+					for (int x = 0; x < 4; ++x) k0[x] = half2_bits(codes2(mk, w0, x)), k1[x] = half2_bits(codes2(mk, w1, x));
 #pragma unroll
 					for (int r = 0; r < R; ++r)
 					{
-						float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+						float d[4];
 						const uint4 b = qsm[(2 * g * R + r) * 32 + lane], e = qsm[((2 * g + 1) * R + r) * 32 + lane];
-						mma16816(d, k0[0], k1[0], k0[1], k1[1], b.x, b.y);
+						mma16816_first(d, k0[0], k1[0], k0[1], k1[1], b.x, b.y);
 						mma16816(d, k0[0], k1[0], k0[1], k1[1], b.z, b.w);
 						mma16816(d, k0[2], k1[2], k0[3], k1[3], e.x, e.y);
 						mma16816(d, k0[2], k1[2], k0[3], k1[3], e.z, e.w);
@@ -550,35 +566,50 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 				float vs[4][J];
 #pragma unroll
 				for (int kk = 0; kk < 4; ++kk)
-				{
-					const int k = c4 + 4 * kk;
-					load_scales<J>(vs[kk], st + 2 * L::CODES + L::SCALES + ((warp * 16 + k) * U + (i8 >> 2) * J) * 2);
-					if (edge && (key0 + k < s.first || key0 + k > s.last)) // whatever was there
+					load_scales<J>(vs[kk], st + 2 * L::CODES + L::SCALES + ((warp * 16 + c4 + 4 * kk) * U + (i8 >> 2) * J) * 2);
+				if (edge)
 #pragma unroll
-						for (int j = 0; j < J; ++j) vs[kk][j] = 0.0f;
+					for (int kk = 0; kk < 4; ++kk)
+						if (key0 + c4 + 4 * kk < s.first || key0 + c4 + 4 * kk > s.last) // whatever was there
+#pragma unroll
+							for (int j = 0; j < J; ++j) vs[kk][j] = 0.0f;
+				__half2 s2[J][2]; // the scales of key pairs (0, 1) and (2, 3)
+				__half2 odd = __float2half2_rn(0.0f);
+#pragma unroll
+				for (int j = 0; j < J; ++j)
+#pragma unroll
+					for (int pr = 0; pr < 2; ++pr)
+					{
+						s2[j][pr] = __floats2half2_rn(vs[2 * pr][j], vs[2 * pr + 1][j]);
+						odd = __hfma2(s2[j][pr], __float2half2_rn(0.0f), odd); // no number where a scale is none (or no 16-bit one)
+					}
+				if (__any_sync(0xffffffffu, __hisnan(__low2half(odd)) || __hisnan(__high2half(odd))))
+				{
+					// goes in as a number: zero weights must stay zero for the rows that do not see its key. (Finite
+					// scales are within these bounds.)
+					bad = true;
+#pragma unroll
+					for (int j = 0; j < J; ++j)
+#pragma unroll
+						for (int pr = 0; pr < 2; ++pr)
+							s2[j][pr] = __hmax2(__hmin2(s2[j][pr], __float2half2_rn(KV4_SCALE_MAX)), __float2half2_rn(-KV4_SCALE_MAX));
 				}
 #pragma unroll
 				for (int j = 0; j < J; ++j)
 				{
-					__half2 s2[2]; // the scales of key pairs (0, 1) and (2, 3)
 					uint32_t lo[2], hi[2];
 #pragma unroll
 					for (int pr = 0; pr < 2; ++pr)
 					{
 						const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + L::CODES + (v_off[0] ^ (16 * j)) + pr * 8 * (D / 2));
 						const uint32_t w1 = *reinterpret_cast<const uint32_t*>(st + L::CODES + (v_off[1] ^ (16 * j)) + pr * 8 * (D / 2));
-						s2[pr] = __floats2half2_rn(vs[2 * pr][j], vs[2 * pr + 1][j]);
-						// a scale that is no number (finite ones are within range) marks `odd` for good, and goes in as
-						// a number: zero weights must stay zero for the rows that do not see its key
-						odd = __hfma2(s2[pr], __float2half2_rn(0.0f), odd);
-						s2[pr] = __hmax2(__hmin2(s2[pr], __float2half2_rn(KV4_SCALE_MAX)), __float2half2_rn(-KV4_SCALE_MAX));
 						lo[pr] = __byte_perm(w0, w1, 0x5410);
 						hi[pr] = __byte_perm(w0, w1, 0x7632);
 					}
 #pragma unroll
 					for (int x = 0; x < 4; ++x)
 					{
-						const auto widen = [&](uint32_t w, int pr) { return half2_bits(__hmul2(codes2(w, x), s2[pr])); };
+						const auto widen = [&](uint32_t w, int pr) { return half2_bits(__hmul2(codes2(mk, w, x), s2[j][pr])); };
 						const uint32_t a0 = widen(lo[0], 0), a1 = widen(hi[0], 0), a2 = widen(lo[1], 1), a3 = widen(hi[1], 1);
 #pragma unroll
 						for (int r = 0; r < R; ++r)
@@ -605,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 				m[r][e] = held[r][e] == NONE ? -CUDART_INF_F : P_SCALE - held[r][e];
 				if (i8 == 0) ml[warp * ROWS + 8 * r + 2 * c4 + e] = make_float2(m[r][e], l[r][e]);
 			}
-		const bool any_bad = named_sync_or(1, CW * 32, __hisnan(__low2half(odd)) || __hisnan(__high2half(odd)));
+		const bool any_bad = named_sync_or(1, CW * 32, bad);
 #pragma unroll
 		for (int r = 0; r < R; ++r)
 #pragma unroll

@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			unsigned got[2] = {0, 0};
 			const auto load = [&](int v, int u) {
 				const int s = h % RS;
-				if (h >= RS && !flags[0] && !mbar_wait_bounded(&raw_empty[s], ((h / RS) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY))
+				if (h >= RS && !flags[0] && !kv4_wait(&raw_empty[s], ((h / RS) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY))
 					flags[0] = 1;
 				__syncwarp();
 				if (__shfl_sync(0xffffffffu, flags[0], 0)) return false;
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 				if (ok && u > 0) ok = load(1, u - 1);
 			}
 			// not to leave (after a wait that ran out) while a copy may still land here
-			for (int i = max(0, h - RS); i < h; ++i) mbar_wait_bounded(&raw_full[i % RS], (i / RS) & 1, nullptr, 0);
+			for (int i = max(0, h - RS); i < h; ++i) kv4_wait(&raw_full[i % RS], (i / RS) & 1, nullptr, 0);
 			__syncwarp();
 		}
 		else if (warp == 1)
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			const auto has = [&](int X, int u) { return uni(u + u_lo >= lo[X] && u + u_lo <= hi[X]); };
 			int ns[2] = {0, 0}, np[2] = {0, 0}; // S issued, P consumed, per Q tile
 			const auto wait = [&](uint64_t* bar, int phase) {
-				const bool w = !flags[0] && mbar_wait_bounded(bar, (uint32_t)(phase & 1), ws.err, DEVERR_WAIT_FULL);
+				const bool w = !flags[0] && kv4_wait(bar, (uint32_t)(phase & 1), ws.err, DEVERR_WAIT_FULL);
 				return __all_sync(0xffffffffu, w) != 0;
 			};
 			// (the low halves first: the adder cuts a sum off at its size, and while only they are in it that is small)
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			}
 			if (!ok) flags[0] = 1;
 			commit(mma_done, lead);
-			mbar_wait_bounded(mma_done, 0, nullptr, 0);
+			kv4_wait(mma_done, 0, nullptr, 0);
 			__syncwarp();
 		}
 	}
@@ -520,8 +520,8 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			constexpr int v = V;
 			const int rs = h % RS, s = u % KS;
 			uint64_t* empty = v ? v_empty : k_empty;
-			bool ok = !flags[0] && mbar_wait_bounded(&raw_full[rs], (h / RS) & 1, ws.err, DEVERR_WAIT_FULL);
-			ok = ok && (u < KS || (!flags[0] && mbar_wait_bounded(&empty[s], ((u / KS) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY)));
+			bool ok = !flags[0] && kv4_wait(&raw_full[rs], (h / RS) & 1, ws.err, DEVERR_WAIT_FULL);
+			ok = ok && (u < KS || (!flags[0] && kv4_wait(&empty[s], ((u / KS) - 1) & 1, ws.err, DEVERR_WAIT_EMPTY)));
 			if (!__all_sync(0xffffffffu, ok))
 			{
 				flags[0] = 1;
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			{
 				const int b = n & 1;
 				const uint32_t ts = ts0 + 64 * b;
-				ok = ok && !flags[0] && mbar_wait_bounded(&s_full[2 * X + b], (uint32_t)((n >> 1) & 1), ws.err, DEVERR_WAIT_FULL);
+				ok = ok && !flags[0] && kv4_wait(&s_full[2 * X + b], (uint32_t)((n >> 1) & 1), ws.err, DEVERR_WAIT_FULL);
 				if (!__all_sync(0xffffffffu, ok))
 				{
 					ok = false;
@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 				{
 					// O must hold every P V before this tile's. (S of this tile completed after P V of tile n - 2, so
 					// pv_done is at most one phase behind and its parity does not alias.)
-					const bool done = !flags[0] && mbar_wait_bounded(&pv_done[X], (uint32_t)((n - 1) & 1), ws.err, DEVERR_WAIT_FULL);
+					const bool done = !flags[0] && kv4_wait(&pv_done[X], (uint32_t)((n - 1) & 1), ws.err, DEVERR_WAIT_FULL);
 					if (!__all_sync(0xffffffffu, done))
 					{
 						ok = false;
@@ -810,7 +810,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 				mbar_arrive(&p_full[2 * X + b]);
 			}
 			if (!ok) flags[0] = 1;
-			if (ok && n > 0) ok = !flags[0] && mbar_wait_bounded(&o_done[X], 0, ws.err, DEVERR_WAIT_FULL);
+			if (ok && n > 0) ok = !flags[0] && kv4_wait(&o_done[X], 0, ws.err, DEVERR_WAIT_FULL);
 			ok = __all_sync(0xffffffffu, ok);
 			tc_fence_after();
 

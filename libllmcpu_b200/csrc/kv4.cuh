@@ -55,6 +55,31 @@ struct Kv4Args
 	size_t out_stride;
 };
 
+// Wait for phase `parity` of `bar`, giving up after WAIT_LIMIT_NS (false, with
+// `code` in the error word where there is one). The thread sleeps up to 1 ms
+// at a time: these kernels have many warps waiting for one another, and short
+// polls would take the issue slots of those that work.
+__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, int* err, int code)
+{
+	const auto poll = [&]() {
+		uint32_t ok;
+		asm volatile("{\n\t.reg .pred p;\n\t"
+		             "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+		             "selp.u32 %0, 1, 0, p;\n\t}"
+		             : "=r"(ok)
+		             : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+		             : "memory");
+		return ok != 0;
+	};
+	if (poll()) return true;
+	const uint64_t t0 = globaltimer_ns();
+	do
+		if (poll()) return true;
+	while (globaltimer_ns() - t0 <= WAIT_LIMIT_NS);
+	if (err) atomicCAS(err, 0, code);
+	return false;
+}
+
 // One request's place in the packed tokens and its keys.
 struct Kv4Request
 {
