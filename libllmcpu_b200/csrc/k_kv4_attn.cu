@@ -44,7 +44,7 @@ constexpr int CW = 4;                  // computing warps, 16 keys of a tile eac
 constexpr int THREADS = (CW + 1) * 32; // and the loading warp
 constexpr int STAGES = 3;              // tiles in the ring: what arrives while one is worked on
 constexpr int FEW_ROWS = 32;           // requests with more query rows a KV head go to k_kv4_prompt.cu
-constexpr int MIN_TILES = 2;           // a run is at least this long, while tiles are few
+constexpr int MIN_TILES = 4;           // a run is at least this long, while tiles are few
 // A row's weights are taken against a held score, 2^11 at it, which moves only
 // when a score passes it by more than 2^4: then no weight passes 2^15, within a
 // 16-bit float, and weights of 2^-24 of the largest keep 11 bits and more.
@@ -187,7 +187,10 @@ struct Runs
 	__device__ __forceinline__ long long begin(int c) const { return c * per + min((long long)c, rem); }
 	__device__ __forceinline__ int owner(long long t) const
 	{
-		return t < rem * (per + 1) ? (int)(t / (per + 1)) : (int)(rem + (t - rem * (per + 1)) / per);
+		const long long u = t - rem * (per + 1); // behind the longer runs
+		const long long x = u < 0 ? t : u, d = u < 0 ? per + 1 : per;
+		const int q = ((x | d) >> 32) == 0 ? (int)((uint32_t)x / (uint32_t)d) : (int)(x / d);
+		return u < 0 ? q : (int)rem + q;
 	}
 };
 
@@ -329,9 +332,13 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 				const unsigned got = __ballot_sync(0xffffffffu, get);
 				if (lane == 0)
 				{
-					int mask = 0;
-					for (int p = 0; p < n_parts; ++p)
-						if (got >> (4 * p) & 1) mask |= ((1 << (parts / 16)) - 1) << (p * (parts / 16));
+					int mask = got ? 15 : 0; // one part: all or nothing
+					if (n_parts > 1)
+					{
+						mask = 0;
+						for (int p = 0; p < n_parts; ++p)
+							if (got >> (4 * p) & 1) mask |= (parts == 32 ? 3 : 1) << (p * (parts / 16));
+					}
 					loaded[stage] = mask;
 					mbar_arrive_expect_tx(&full[stage], __popc(got) / 4 * 2 * (uint32_t)(parts * (D / 2) + parts * U * 2));
 				}
@@ -733,41 +740,55 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 		}
 		if (!whole)
 		{
-			__threadfence();
 			named_sync(1, CW * 32);
 			if (tid == 0)
 			{
-				const int was = atomicAdd(&ws.counters[c_first], 1);
+				// (releases what the barrier has gathered, acquires what the others released)
+				int was;
+				asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(was) : "l"(&ws.counters[c_first]) : "memory");
 				*last_piece = was == c_last - c_first;
 				if (*last_piece) ws.counters[c_first] = 0; // ready for the next call
 			}
 			named_sync(1, CW * 32);
 			if (*last_piece)
 			{
-				// the last piece of the segment: all of them joined, in order
-				__threadfence();
-				for (int item = tid; item < ROWS * QUADS; item += CW * 32)
+				// the last piece of the segment: all of them joined, in order (the largest maximum first: then the
+				// parts' loads wait for nothing but each other's places)
+				float mx[MINE], w[MINE];
+				float4 y[MINE];
+#pragma unroll
+				for (int x = 0; x < MINE; ++x) mx[x] = -CUDART_INF_F, w[x] = 0.0f, y[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+				for (int c = c_first; c <= c_last; ++c)
+#pragma unroll
+					for (int x = 0; x < MINE; ++x)
+						mx[x] = fmaxf(mx[x], __ldcg(slot(c) + ROWS * D + 2 * ((tid + x * CW * 32) / QUADS)));
+#pragma unroll(MINE <= 2 ? 8 : 2)
+				for (int c = c_first; c <= c_last; ++c)
 				{
-					const int row = item / QUADS, d = item % QUADS * 4, rr = s.row0 + row;
-					if (rr >= s.rows) continue;
-					float mx = -CUDART_INF_F, w = 0.0f;
-					for (int c = c_first; c <= c_last; ++c) mx = fmaxf(mx, __ldcg(slot(c) + ROWS * D + 2 * row));
-					float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-					for (int c = c_first; c <= c_last; ++c)
+					const float* p = slot(c);
+#pragma unroll
+					for (int x = 0; x < MINE; ++x)
 					{
-						const float* p = slot(c);
+						const int item = tid + x * CW * 32, row = item / QUADS, d = item % QUADS * 4;
 						const float2 z = __ldcg(reinterpret_cast<const float2*>(p + ROWS * D + 2 * row));
 						const float4 u = __ldcg(reinterpret_cast<const float4*>(p + row * D + d));
-						const float f = z.x == mx ? 1.0f : ex2(z.x - mx);
-						w = fmaf(z.y, f, w);
-						y.x = fmaf(u.x, f, y.x), y.y = fmaf(u.y, f, y.y), y.z = fmaf(u.z, f, y.z), y.w = fmaf(u.w, f, y.w);
+						const float f = z.x == mx[x] ? 1.0f : ex2(z.x - mx[x]);
+						w[x] = fmaf(z.y, f, w[x]);
+						y[x].x = fmaf(u.x, f, y[x].x), y[x].y = fmaf(u.y, f, y[x].y);
+						y[x].z = fmaf(u.z, f, y[x].z), y[x].w = fmaf(u.w, f, y[x].w);
 					}
-					const float inv = w == 0.0f ? 0.0f : 1.0f / w;
+				}
+#pragma unroll
+				for (int x = 0; x < MINE; ++x)
+				{
+					const int item = tid + x * CW * 32, rr = s.row0 + item / QUADS, d = item % QUADS * 4;
+					if (rr >= s.rows) continue;
+					const float inv = w[x] == 0.0f ? 0.0f : 1.0f / w[x];
 					const int tk = rr / a.group;
 					*reinterpret_cast<float4*>(a.out + (size_t)(s.x.q0 + tk) * a.out_stride +
 					                           (size_t)(hk * a.group + rr - tk * a.group) * D + d) =
-						make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+						make_float4(y[x].x * inv, y[x].y * inv, y[x].z * inv, y[x].w * inv);
 				}
 			}
 		}
@@ -787,7 +808,7 @@ constexpr size_t ws_bytes(int sms)
 }
 size_t ws_bytes(int D) // enough for every variant of the head_dim on any device of this kind
 {
-	static_assert(ws_bytes<64, 4>(1) >= ws_bytes<64, 2>(1) && ws_bytes<64, 4>(1) >= ws_bytes<64, 1>(1) &&
+	static_assert(ws_bytes<64, 4>(1) >= ws_bytes<64, 3>(1) && ws_bytes<64, 4>(1) >= ws_bytes<64, 2>(1) && ws_bytes<64, 4>(1) >= ws_bytes<64, 1>(1) &&
 	                  ws_bytes<128, 2>(1) >= ws_bytes<128, 1>(1),
 	              "the largest variant");
 	return D == 64 ? ws_bytes<64, 4>(MAX_SMS) : D == 128 ? ws_bytes<128, 2>(MAX_SMS) : ws_bytes<256, 1>(MAX_SMS);
@@ -919,6 +940,7 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 	else
 		e = rows <= 8    ? launch_decode4<64, 1>(a, p->workspace, st)
 		    : rows <= 16 ? launch_decode4<64, 2>(a, p->workspace, st)
+		    : rows <= 24 ? launch_decode4<64, 3>(a, p->workspace, st)
 		                 : launch_decode4<64, 4>(a, p->workspace, st);
 	if (!e && rows > FEW_ROWS) e = launch_kv4_prompt(a, p->workspace, ws_bytes(a.D), FEW_ROWS, stream);
 	return e ? set_cuda_error(e, "kv4 attention launch") : NNCU_OK;

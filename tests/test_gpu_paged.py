@@ -588,3 +588,14 @@ def test_serving_steps(nncu, torch_cuda, d):
                                        cache[r][1][:, h // group], int(lens[r]) + i, 0, d ** -0.5, 0.0)
                     assert np.abs(got[at + i, h * d:(h + 1) * d] - want).max() <= 1e-5 * vmax, (it, r, i, h)
             at += n
+
+
+def test_the_serving_command(nncu, torch_cuda, capsys):
+    import json
+
+    from libllmcpu_b200 import paged_bench
+
+    assert paged_bench.main(["--model", "llama3.2-1b", "--requests", "5", "--context", "300", "--page", "16",
+                             "--steps", "7", "--tokens", "2"]) == 0
+    line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert set(line["operators_us"]) == {"tables", "rope", "append", "attention"} and line["step_us"] > 0

@@ -119,3 +119,11 @@ def test_strides_come_from_the_tensors():
     assert N.rope_axes(**{**ROPE, "q": y}).q_stride == 520
     with pytest.raises(ValueError):
         N.rope_axes(**{**ROPE, "q": torch.zeros(512, 4).T})
+
+
+def test_paged_bench_parses_its_arguments():
+    from libllmcpu_b200 import paged_bench
+
+    with pytest.raises(SystemExit) as e:
+        paged_bench.main(["--help"])
+    assert e.value.code == 0
