@@ -496,7 +496,8 @@ int nncu_kv4_read_dev(const nncu_kv4_rows* rows, void* stream);
  * the keys up to itself, `window` at most (0: all). scale, softcap as in
  * nncu_attn_params. Query head h reads KV head h / (n_head / n_kv); rows are
  * n_head * head_dim floats, strides in floats. A token that sees no key gets
- * zeros; keys on pages outside the pool are not seen. max_new bounds the new
+ * zeros; keys on pages outside the pool are not seen; a seq_len past its
+ * table row (max_blocks pages) counts as that row's end. max_new bounds the new
  * tokens of one request and n_tok their sum: tokens past either are left out
  * (their output rows are not written). What a request that
  * nncu_paged_step_dev did not serve gets is of no use: its tokens are not in

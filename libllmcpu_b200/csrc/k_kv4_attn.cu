@@ -862,8 +862,13 @@ int check_shape(const nncu_kv4_attn* a, bool need_pages)
 	if (a->n_req < 0 || a->n_tok < 0 || a->max_new < 0 || a->max_blocks < 0 || a->window < 0)
 		return refuse("kv4 attention: negative n_req, n_tok, max_new, max_blocks or window");
 	if (a->n_head <= 0 || a->n_head % a->pool.n_kv) return refuse("kv4 attention: n_head must be a multiple of n_kv");
-	if ((long long)a->max_blocks * a->pool.page_size > INT32_MAX)
+	if ((long long)a->max_blocks * a->pool.page_size > INT32_MAX - 256)
 		return refuse("kv4 attention: max_blocks x page_size passes 2^31");
+	// rows, and the tensor-core kernel's CTAs, are numbered with 32 bits
+	const long long group = a->n_head / a->pool.n_kv, rows = group * a->n_tok;
+	if (rows > INT32_MAX / 2 || group * a->max_new > INT32_MAX / 2 ||
+	    (rows / 128 + a->n_req + 1024) * a->pool.n_kv > INT32_MAX)
+		return refuse("kv4 attention: n_tok, n_req and heads together pass 2^31");
 	return NNCU_OK;
 }
 

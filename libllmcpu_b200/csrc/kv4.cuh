@@ -92,8 +92,8 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4Args& a, int r)
 	const int s = max(0, a.q_start[r]), e = a.q_start[r + 1];
 	const int n = max(0, e - s);
 	x.q0 = s;
-	x.keys = max(0, min(a.seq_len[r], a.max_blocks << a.page_shift));
-	x.pos0 = a.seq_len[r] - n;
+	x.keys = max(0, min(a.seq_len[r], a.max_blocks << a.page_shift)); // (a length past its table row: the row's end)
+	x.pos0 = x.keys - n;
 	x.n_new = max(0, min(min(n, a.max_new), a.n_tok - s));
 	return x;
 }

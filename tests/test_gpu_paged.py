@@ -493,6 +493,21 @@ def test_attention_leaves_out_what_passes_its_bounds(nncu, torch_cuda):
     assert np.abs(got[:7] - a.want[:7]).max() <= 1e-5 * a.vmax and (got[7:] == 5.0).all()
 
 
+@pytest.mark.parametrize("seq,rows", [(2 ** 31 - 1, 64 * 2), (-5, 0), (1000, 64 * 2)])
+def test_lengths_no_table_can_hold(nncu, torch_cuda, seq, rows):
+    """A seq_len past the table row counts as the row's end, a negative one as none: nothing is read beyond."""
+    torch = torch_cuda
+    for new in (1, 50):
+        a = Attn(torch, nncu, ([(128, new)], 1, 4, 128, 64, 100, 0.0))
+        a.call._keep["seq_len"].fill_(seq)
+        nncu.kv4_attention_dev(a.call)
+        nncu.kv4_check(a.call)
+        if rows:
+            a.check(a.out)
+        else:
+            assert float(a.out[:new].abs().max()) == 0.0
+
+
 def test_attention_in_a_graph_follows_new_lengths(nncu, torch_cuda):
     """Lengths are read on the device: a captured call replays with others."""
     torch = torch_cuda

@@ -83,7 +83,7 @@ def test_rows_are_checked(L, change, text):
     (dict(n_head=0), "n_head"), (dict(max_blocks=1 << 26), "max_blocks"), (dict(table_stride=3), "table"),
     (dict(block_table=None), "NULL"), (dict(q=None), "NULL"), (dict(q=A + 4), "aligned"),
     (dict(out_stride=1026), "aligned"), (dict(q_stride=512), "strides"), (dict(softcap=-1.0), "softcap"),
-    (dict(scale=float("nan")), "scale"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=16), "workspace"),
+    (dict(scale=float("nan")), "scale"), (dict(n_tok=1 << 30), "2^31"), (dict(n_req=2000000000), "2^31"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=16), "workspace"),
     (dict(workspace=A + 8), "workspace"),
 ])
 def test_attention_refuses(L, change, text):
