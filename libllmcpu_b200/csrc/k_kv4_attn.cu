@@ -31,7 +31,7 @@
 // values (150 of them unpack), not memory. 64 requests of 512 to 8192 keys,
 // 32/8 heads x 128: 92 us, 2.26 TB/s of the cache; 131072 keys, 8/4 x 256,
 // four tokens: 88 us, 1.7 TB/s; 4096 keys, 32/8 x 128: 15 us (latency).
-// Requests with more than FEW_ROWS query rows a KV head are left to the
+// Requests with many query rows a KV head (few_rows) are left to the
 // tensor-memory kernel: it takes 128 rows or more at a time for the price of
 // one unpacking, this one 8 to 32.
 #include <cuda_runtime.h>
@@ -50,7 +50,16 @@ constexpr int TILE = 64;               // keys a tile
 constexpr int CW = 4;                  // computing warps, 16 keys of a tile each
 constexpr int THREADS = (CW + 1) * 32; // and the loading warp
 constexpr int STAGES = 3;              // tiles in the ring: what arrives while one is worked on
-constexpr int FEW_ROWS = 32;           // requests with more query rows a KV head go to k_kv4_prompt.cu
+// Requests with more query rows a KV head go to k_kv4_prompt.cu. Measured, 16
+// requests over 4000 keys, 8 KV heads (256: 4), here and there: 64 values a
+// head, 128 rows 181 and 212 us; 128, 96 rows 259 and 361, 128 rows 339 and
+// 293; 256, 64 rows 221 and 246, 96 rows 325 and 249.
+constexpr int few_rows(int D) { return D == 64 ? 128 : D == 128 ? 96 : 64; }
+// Several row tiles a segment share the unpacking, single ones make more and
+// shorter segments: 16 requests over 4000 keys, 8 KV heads x 128, 32 rows, two
+// tiles 101 us, one 118; one request, two 34 us, one 24. So several from this
+// many key tiles on (the most that the tables can hold).
+constexpr long long MANY_TILES = 4096;
 constexpr int MIN_TILES = 4;           // a run is at least this long, while tiles are few
 // A row's weights are taken against a held score, 2^11 at it, which moves only
 // when a score passes it by more than 2^4: then no weight passes 2^15, within a
@@ -180,7 +189,7 @@ __device__ __forceinline__ void segment_tiles(const Kv4Args& a, Segment& s, int 
 	s.r = r;
 	s.x = kv4_request(a, r);
 	s.rows = s.x.n_new * a.group;
-	if (s.rows > FEW_ROWS) s.rows = 0; // the tensor-core kernel's
+	if (s.rows > few_rows(a.D)) s.rows = 0; // the tensor-memory kernel's
 	s.last = min(s.x.pos0 + s.x.n_new - 1, s.x.keys - 1);
 	s.first = a.window > 0 ? max(0, s.x.pos0 - a.window + 1) : 0;
 	s.tile0 = s.first / TILE;
@@ -891,7 +900,7 @@ extern "C" int nncu_kv4_workspace_bytes(const nncu_kv4_attn* a, size_t* bytes)
 	if (!bytes) return refuse("kv4 workspace: NULL argument");
 	*bytes = ws_bytes(a->pool.head_dim);
 	const long long group = a->n_head / a->pool.n_kv;
-	if (group * a->max_new > FEW_ROWS)
+	if (group * a->max_new > few_rows(a->pool.head_dim))
 		*bytes = kv4_prompt_ws_end(a->pool.head_dim, *bytes, a->n_req, group * a->n_tok, a->pool.n_kv);
 	return NNCU_OK;
 }
@@ -944,16 +953,21 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 	const auto st = static_cast<cudaStream_t>(stream);
 	const long long rows = (long long)a.group * p->max_new;
 	// (a call that may have prompts still decodes the requests with few rows here)
+	const long long few = rows < few_rows(a.D) ? rows : few_rows(a.D), tiles8 = (few + 7) / 8;
+	const long long span = (long long)a.max_blocks * a.page, seen = (long long)a.window + a.max_new;
+	const long long tiles = (a.window > 0 && seen < span ? seen : span) / TILE * a.n_req * a.n_kv;
 	int e;
 	if (a.D == 256)
 		e = launch_decode4<256, 1>(a, p->workspace, st);
 	else if (a.D == 128)
-		e = rows <= 8 ? launch_decode4<128, 1>(a, p->workspace, st) : launch_decode4<128, 2>(a, p->workspace, st);
+		// (three row tiles: 93 us one by one, 99 as two and one)
+		e = tiles < MANY_TILES || (tiles8 & 1 && tiles8 < 4) ? launch_decode4<128, 1>(a, p->workspace, st)
+		                                                     : launch_decode4<128, 2>(a, p->workspace, st);
 	else
-		e = rows <= 8    ? launch_decode4<64, 1>(a, p->workspace, st)
-		    : rows <= 16 ? launch_decode4<64, 2>(a, p->workspace, st)
-		    : rows <= 24 ? launch_decode4<64, 3>(a, p->workspace, st)
-		                 : launch_decode4<64, 4>(a, p->workspace, st);
-	if (!e && rows > FEW_ROWS) e = launch_kv4_prompt(a, p->workspace, ws_bytes(a.D), FEW_ROWS, stream);
+		e = tiles < MANY_TILES || tiles8 == 1 ? launch_decode4<64, 1>(a, p->workspace, st)
+		    : tiles8 == 2                     ? launch_decode4<64, 2>(a, p->workspace, st)
+		    : tiles8 == 3                     ? launch_decode4<64, 3>(a, p->workspace, st)
+		                                      : launch_decode4<64, 4>(a, p->workspace, st);
+	if (!e && rows > few_rows(a.D)) e = launch_kv4_prompt(a, p->workspace, ws_bytes(a.D), few_rows(a.D), stream);
 	return e ? set_cuda_error(e, "kv4 attention launch") : NNCU_OK;
 }

@@ -666,7 +666,8 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			// ---- the softmax, O kept in scale ----
 			const float mult = (a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f) / f;
 			const float cap2 = a.softcap * 1.4426950408889634f;
-			float held = 1e30f, l = 0.0f; // HELD - held score (1e30: no key seen)
+			// HELD - held score (1e30: no key seen; places without a row: any score, for they never see one)
+			float held = real ? 1e30f : 0.0f, l = 0.0f;
 			// O's earlier parts, relative to sums_held
 			float4* sums = reinterpret_cast<float4*>(ws.sums + (size_t)sm * L::BR * D) + 128 * X + r;
 			float sums_held = 0.0f;

@@ -295,7 +295,14 @@ ATTN_CASES = [
     ([(130, 129)], 3, 1, 128, 64, 0, 0.0),
     ([(4000, 1)] + [(40 + 3 * i, 1) for i in range(30)], 1, 4, 64, 16, 0, 0.0),
     ([(3, 5), (0, 2), (40, 41)], 2, 2, 128, 64, 0, 0.0),  # more tokens than keys: the first see none
+    ([(3, 70), (150, 60)], 2, 2, 128, 64, 0, 0.0),        # the same among many rows
+    ([(200, 24), (200, 25), (90, 1)], 1, 4, 128, 64, 0, 0.0),  # 96 and 100 rows a KV head: one kernel and the other
+    ([(200, 32), (200, 33)], 1, 4, 64, 32, 0, 0.0),
+    ([(200, 16), (200, 17)], 1, 4, 256, 64, 0, 0.0),
 ]
+# enough key tiles for several row tiles a segment: 8, 16, 24, 32 rows and more
+ATTN_MANY = [([(60 + 7 * (i % 9), n) for i in range(300)], 8, g, d, 64, 0, 0.0)
+             for n, g, d in ((2, 2, 64), (3, 4, 64), (4, 4, 64), (5, 4, 64), (9, 4, 64), (4, 4, 128), (5, 4, 128))]
 
 
 class Attn:
@@ -366,6 +373,33 @@ def test_attention(nncu, torch_cuda, case, slack):
     nncu.kv4_attention_dev(a.call)
     nncu.kv4_check(a.call)
     a.check(a.out)
+
+
+@pytest.mark.parametrize("case", ATTN_MANY, ids=lambda c: f"{c[0][0][1]}x{c[2]}-d{c[3]}")
+def test_attention_of_many_requests(nncu, torch_cuda, case):
+    """A few of many requests checked (the table and lengths of all are live; the pool holds what the few see)."""
+    torch = torch_cuda
+    reqs, n_kv, g, d, page, _, _ = case
+    few = Attn(torch, nncu, (reqs[:3],) + case[1:])
+    keep = few.call._keep
+    n, new, mb = len(reqs), reqs[0][1], few.call.max_blocks
+    table = keep["block_table"][:, :mb].repeat(n // 3, 1).contiguous()
+    seq = keep["seq_len"].repeat(n // 3)
+    q = few.call._keep["q"].repeat(n // 3, 1).contiguous()
+    out = torch.zeros_like(q)
+    start = torch.arange(0, n * new + 1, new, dtype=torch.int32, device="cuda")
+    wide = 16 * mb  # a table with room: what the call can know of the lengths
+    roomy = torch.full((n, wide), -1, dtype=torch.int32, device="cuda")
+    roomy[:, :mb] = table
+    call = nncu.kv4_attn(few.call.pool, n_req=n, n_tok=n * new, n_head=n_kv * g, max_new=new, max_blocks=wide,
+                         block_table=roomy, seq_len=seq, q_start=start, q=q, out=out)
+    ws = torch.zeros(nncu.kv4_workspace_bytes(call), dtype=torch.uint8, device="cuda")
+    call.workspace, call.workspace_bytes = ws.data_ptr(), ws.numel()
+    nncu.kv4_attention_dev(call)
+    nncu.kv4_check(call)
+    got = out.view(n // 3, 3 * new, -1)
+    want = torch.as_tensor(few.want, device="cuda")
+    assert float((got.double() - want).abs().max()) <= 1e-5 * few.vmax
 
 
 @pytest.mark.parametrize("case", [ATTN_CASES[1], ATTN_CASES[4], ATTN_CASES[9], ATTN_CASES[15]])
