@@ -53,13 +53,15 @@ constexpr int STAGES = 3;              // tiles in the ring: what arrives while 
 // Requests with more query rows a KV head go to k_kv4_prompt.cu. Measured, 16
 // requests over 4000 keys, 8 KV heads (256: 4), here and there: 64 values a
 // head, 128 rows 181 and 212 us; 128, 96 rows 259 and 361, 128 rows 339 and
-// 293; 256, 64 rows 221 and 246, 96 rows 325 and 249.
+// 293; 256, 64 rows 221 and 246, 96 rows 325 and 249. With few key tiles (one
+// request: 250 to 500 of them), where more and shorter pieces are what counts,
+// twice as many stay here: 128, 128 rows 41 and 72 us; 256, 128 rows 42 and 77.
 constexpr int few_rows(int D) { return D == 64 ? 128 : D == 128 ? 96 : 64; }
 // Several row tiles a segment share the unpacking, single ones make more and
 // shorter segments: 16 requests over 4000 keys, 8 KV heads x 128, 32 rows, two
 // tiles 101 us, one 118; one request, two 34 us, one 24. So several from this
 // many key tiles on (the most that the tables can hold).
-constexpr long long MANY_TILES = 4096;
+constexpr long long MANY_TILES = 4096, FEW_TILES = 1024;
 constexpr int MIN_TILES = 4;           // a run is at least this long, while tiles are few
 // A row's weights are taken against a held score, 2^11 at it, which moves only
 // when a score passes it by more than 2^4: then no weight passes 2^15, within a
@@ -189,7 +191,7 @@ __device__ __forceinline__ void segment_tiles(const Kv4Args& a, Segment& s, int 
 	s.r = r;
 	s.x = kv4_request(a, r);
 	s.rows = s.x.n_new * a.group;
-	if (s.rows > few_rows(a.D)) s.rows = 0; // the tensor-memory kernel's
+	if (s.rows > a.few_rows) s.rows = 0; // the tensor-memory kernel's
 	s.last = min(s.x.pos0 + s.x.n_new - 1, s.x.keys - 1);
 	s.first = a.window > 0 ? max(0, s.x.pos0 - a.window + 1) : 0;
 	s.tile0 = s.first / TILE;
@@ -865,6 +867,17 @@ int launch_decode4(const Kv4Args& a, void* workspace, cudaStream_t st)
 	return (int)cudaGetLastError();
 }
 
+// The most key tiles that a call can have, by what its tables can hold.
+long long most_tiles(const nncu_kv4_attn* a)
+{
+	const long long span = (long long)a->max_blocks * a->pool.page_size, seen = (long long)a->window + a->max_new;
+	return (a->window > 0 && seen < span ? seen : span) / TILE * a->n_req * a->pool.n_kv;
+}
+int few_rows_of(const nncu_kv4_attn* a)
+{
+	return most_tiles(a) < FEW_TILES ? 2 * few_rows(a->pool.head_dim) : few_rows(a->pool.head_dim);
+}
+
 int refuse(const char* msg) { return set_error(NNCU_ERR_INVALID_ARGUMENT, msg); }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -900,7 +913,7 @@ extern "C" int nncu_kv4_workspace_bytes(const nncu_kv4_attn* a, size_t* bytes)
 	if (!bytes) return refuse("kv4 workspace: NULL argument");
 	*bytes = ws_bytes(a->pool.head_dim);
 	const long long group = a->n_head / a->pool.n_kv;
-	if (group * a->max_new > few_rows(a->pool.head_dim))
+	if (group * a->max_new > few_rows_of(a))
 		*bytes = kv4_prompt_ws_end(a->pool.head_dim, *bytes, a->n_req, group * a->n_tok, a->pool.n_kv);
 	return NNCU_OK;
 }
@@ -948,14 +961,12 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 	while ((1 << shift) < p->pool.page_size) ++shift;
 	const Kv4Args a{static_cast<const uint8_t*>(p->pool.pages), p->pool.n_pages, p->pool.page_size, shift,
 	                p->pool.n_kv, p->pool.head_dim, p->n_req, p->n_tok, p->n_head, p->n_head / p->pool.n_kv,
-	                p->max_new, p->max_blocks, p->window, p->scale, p->softcap, p->block_table, p->table_stride,
+	                p->max_new, p->max_blocks, p->window, few_rows_of(p), p->scale, p->softcap, p->block_table, p->table_stride,
 	                p->seq_len, p->q_start, p->q, p->q_stride, p->out, p->out_stride};
 	const auto st = static_cast<cudaStream_t>(stream);
 	const long long rows = (long long)a.group * p->max_new;
 	// (a call that may have prompts still decodes the requests with few rows here)
-	const long long few = rows < few_rows(a.D) ? rows : few_rows(a.D), tiles8 = (few + 7) / 8;
-	const long long span = (long long)a.max_blocks * a.page, seen = (long long)a.window + a.max_new;
-	const long long tiles = (a.window > 0 && seen < span ? seen : span) / TILE * a.n_req * a.n_kv;
+	const long long few = rows < a.few_rows ? rows : a.few_rows, tiles8 = (few + 7) / 8, tiles = most_tiles(p);
 	int e;
 	if (a.D == 256)
 		e = launch_decode4<256, 1>(a, p->workspace, st);
@@ -968,6 +979,6 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 		    : tiles8 == 2                     ? launch_decode4<64, 2>(a, p->workspace, st)
 		    : tiles8 == 3                     ? launch_decode4<64, 3>(a, p->workspace, st)
 		                                      : launch_decode4<64, 4>(a, p->workspace, st);
-	if (!e && rows > few_rows(a.D)) e = launch_kv4_prompt(a, p->workspace, ws_bytes(a.D), few_rows(a.D), stream);
+	if (!e && rows > a.few_rows) e = launch_kv4_prompt(a, p->workspace, ws_bytes(a.D), a.few_rows, stream);
 	return e ? set_cuda_error(e, "kv4 attention launch") : NNCU_OK;
 }

@@ -44,6 +44,7 @@ struct Kv4Args
 	const uint8_t* pages;
 	int n_pages, page, page_shift, n_kv, D;
 	int n_req, n_tok, n_head, group, max_new, max_blocks, window;
+	int few_rows; // requests with more query rows a KV head are the tensor-memory kernel's
 	float scale, softcap;
 	const int* table;
 	size_t table_stride;

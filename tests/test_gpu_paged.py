@@ -296,9 +296,10 @@ ATTN_CASES = [
     ([(4000, 1)] + [(40 + 3 * i, 1) for i in range(30)], 1, 4, 64, 16, 0, 0.0),
     ([(3, 5), (0, 2), (40, 41)], 2, 2, 128, 64, 0, 0.0),  # more tokens than keys: the first see none
     ([(3, 70), (150, 60)], 2, 2, 128, 64, 0, 0.0),        # the same among many rows
-    ([(200, 24), (200, 25), (90, 1)], 1, 4, 128, 64, 0, 0.0),  # 96 and 100 rows a KV head: one kernel and the other
-    ([(200, 32), (200, 33)], 1, 4, 64, 32, 0, 0.0),
-    ([(200, 16), (200, 17)], 1, 4, 256, 64, 0, 0.0),
+    ([(200, 24), (200, 25), (90, 1)], 1, 4, 128, 64, 0, 0.0),
+    ([(200, 48), (200, 49), (90, 1)], 1, 4, 128, 64, 0, 0.0),  # 192 and 196 rows a KV head: one kernel and the other
+    ([(200, 64), (200, 65)], 1, 4, 64, 32, 0, 0.0),
+    ([(200, 32), (200, 33)], 1, 4, 256, 64, 0, 0.0),
 ]
 # enough key tiles for several row tiles a segment: 8, 16, 24, 32 rows and more
 ATTN_MANY = [([(60 + 7 * (i % 9), n) for i in range(300)], 8, g, d, 64, 0, 0.0)
