@@ -30,7 +30,7 @@
 // What bounds it: issue slots, about 470 instructions per 16 keys of 128
 // values (150 of them unpack), not memory. 64 requests of 512 to 8192 keys,
 // 32/8 heads x 128: 92 us, 2.26 TB/s of the cache; 131072 keys, 8/4 x 256,
-// four tokens: 88 us, 1.7 TB/s; 4096 keys, 32/8 x 128: 15 us (latency).
+// four tokens: 89 us, 1.7 TB/s; 4096 keys, 32/8 x 128: 15 us (latency).
 // Requests with many query rows a KV head (few_rows) are left to the
 // tensor-memory kernel: it takes 128 rows or more at a time for the price of
 // one unpacking, this one 8 to 32.
