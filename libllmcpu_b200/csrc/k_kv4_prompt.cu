@@ -107,13 +107,6 @@ struct PromptWs
 	int max_blocks, max_pieces;
 };
 
-struct Block
-{
-	Kv4Request x;
-	int rows, row0;
-	int lo, hi; // tiles [lo, hi] of all rows
-};
-
 // The tiles of rows [row0, row0 + n) of a request; lo > hi: no keys.
 __device__ __forceinline__ void row_tiles(const Kv4Args& a, const Kv4Request& x, int rows, int row0, int n, int& lo, int& hi)
 {
