@@ -24,7 +24,9 @@ namespace
 // tokens 7.7 us.
 
 constexpr int STEP_THREADS = 512;
-constexpr int SAT = 1 << 30; // running sums of absurd lengths stop here instead of wrapping
+// Running sums of absurd lengths stop here instead of wrapping: the sum of two such ends still fits an int. What goes
+// into a sum is held to it too.
+constexpr int SAT = (1 << 30) - 1;
 
 __device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, SAT); }
 
@@ -95,9 +97,9 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 		c_tok = sat_add(c_tok, t);
 		const bool fits = !ends && past >= 0 && (long long)past + nn <= room && q_end <= s.max_tok;
 		const int need = fits ? max(0, (int)(((long long)past + nn + s.page_size - 1) / s.page_size) - held) : 0;
-		const int l_end = sat_add(c_lack, block_scan(need, warp_sums, t));
+		const int l_end = sat_add(c_lack, block_scan(min(need, SAT), warp_sums, t));
 		c_lack = sat_add(c_lack, t);
-		const int b_end = sat_add(c_back, block_scan(ends ? held : 0, warp_sums, t));
+		const int b_end = sat_add(c_back, block_scan(ends ? min(held, SAT) : 0, warp_sums, t));
 		c_back = sat_add(c_back, t);
 		if (i < n) tok[i + 1] = q_end, lack[i + 1] = l_end, back[i + 1] = b_end;
 	}
