@@ -109,17 +109,18 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 	const int count = max(0, min(s.queue[1], np));
 	const int head = ((s.queue[0] % np) + np) % np;
 	const int taken = lack[last_at_most(lack, n, count)];
-	const auto served = [&](int r, int nn, int past) {
-		const int need = lack[r + 1] - lack[r];
+	// Behind a request that the ring did not suffice for, one that lacks no page is served still. (Whether it lacks one
+	// does not follow from the sum, which may have come to its end.)
+	const auto served = [&](int r, int nn, int past, int held) {
 		return nn >= 0 && past >= 0 && (long long)past + nn <= room && tok[r + 1] <= s.max_tok &&
-		       (need == 0 || lack[r + 1] <= count);
+		       (lack[r + 1] <= count || (long long)held * s.page_size >= (long long)past + nn);
 	};
 	const int step = gridDim.x * STEP_THREADS, me = blockIdx.x * STEP_THREADS + (int)threadIdx.x;
 
 	for (int r = me; r < n; r += step)
 	{
 		const int nn = s.n_new[r], past = s.past[r], held = max(0, min(s.held[r], s.max_blocks));
-		const bool ok = served(r, nn, past);
+		const bool ok = served(r, nn, past, held);
 		s.held_out[r] = nn < 0 ? 0 : held + (ok ? lack[r + 1] - lack[r] : 0);
 		s.seq_len[r] = nn < 0 ? 0 : ok ? past + nn : past;
 		s.q_start[r] = tok[r];
@@ -149,11 +150,11 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 		if (t < tok[n])
 		{
 			req = last_at_most(tok, n - 1, t);
-			const int nn = s.n_new[req], past = s.past[req];
+			const int nn = s.n_new[req], past = s.past[req], held = max(0, min(s.held[req], s.max_blocks));
 			pos = past + t - tok[req];
-			if (served(req, nn, past))
+			if (served(req, nn, past, held))
 			{
-				const int held = max(0, min(s.held[req], s.max_blocks)), b = pos / s.page_size;
+				const int b = pos / s.page_size;
 				const int page = b < held ? s.block_table[(size_t)req * s.table_stride + b]
 				                          : s.ring[(head + lack[req] + b - held) % np];
 				slot = page * s.page_size + pos % s.page_size;

@@ -53,3 +53,37 @@ def test_step_of_lengths_past_any_sum(nncu, torch_cuda, new):
     want = P.step(past, new, held, [3, 9], ring, table, page, n_pages, max_blocks, max_tok)
     Step(torch_cuda, nncu, past, new, held, [3, 9], ring, dev(torch_cuda, table, torch_cuda.int32), page, max_blocks,
          max_tok).check(want)
+
+
+def test_step_of_more_lacking_pages_than_any_sum(nncu, torch_cuda):
+    """1025 requests that lack 2^20 pages each, then one that lacks a single page: the sum has reached its end, but the
+    ring suffices for none of them."""
+    torch = torch_cuda
+    n, page, max_blocks, n_pages = 1026, 16, 1 << 20, 64
+    past, new, held = [(1 << 24) - 1] * (n - 1) + [0], [1] * (n - 1) + [3], [0] * n
+    table = torch.empty(n, max_blocks, dtype=torch.int32, device="cuda")
+    want = P.step(past, new, held, [60, 40], np.arange(n_pages), np.zeros((n, 1)), page, n_pages, max_blocks, n + 8)
+    want["queue"][2] = SUM_END  # (pages that were missing)
+    Step(torch, nncu, past, new, held, [60, 40], np.arange(n_pages), table, page, max_blocks, n + 8).check(want)
+
+
+def test_step_of_lengths_near_the_largest(nncu, torch_cuda):
+    """Pages of one token and tables of 2^31 - 1: needs near 2^31, whose requests are not served, so that no entry of
+    the table is touched."""
+    torch = torch_cuda
+    most, n_pages = (1 << 31) - 1, 64
+    past, new, held = [most - 3, most - 1, 0, 7], [2, 1, 3, 0], [0, 0, 0, 7]
+    table = torch.zeros(4, 8, dtype=torch.int32, device="cuda")
+    want = P.step(past, new, held, [5, 40], np.arange(n_pages), np.zeros((4, 8)), 1, n_pages, most, 20)
+    assert want["seq_len"] == past
+    want["queue"][2] = SUM_END
+    i32, z = torch.int32, lambda k: torch.full((k,), -99, dtype=torch.int32, device="cuda")
+    out = dict(held_out=z(4), queue_out=z(4), seq_len=z(4), q_start=z(5), positions=z(20), slots=z(20), token_req=z(20))
+    nncu.paged_step_dev(nncu.paged_step(n_req=4, page_size=1, n_pages=n_pages, max_blocks=most, max_tok=20,
+                                        table_stride=most, past=dev(torch, past, i32), n_new=dev(torch, new, i32),
+                                        held=dev(torch, held, i32), queue=dev(torch, [5, 40], i32),
+                                        ring=torch.arange(n_pages, dtype=i32, device="cuda"), block_table=table, **out))
+    torch.cuda.synchronize()
+    for name, key in (("held_out", "held"), ("queue_out", "queue"), ("seq_len",) * 2, ("q_start",) * 2, ("slots",) * 2,
+                      ("token_req",) * 2, ("positions",) * 2):
+        np.testing.assert_array_equal(out[name].cpu().numpy(), want[key], err_msg=name)
