@@ -23,7 +23,7 @@ namespace
 // launch and its dependent loads: 256 requests 5.7 us, 60 requests with 65 K
 // tokens 7.7 us.
 
-constexpr int STEP_THREADS = 512;
+constexpr int STEP_THREADS = 512, STEP_WARPS = STEP_THREADS / 32;
 // Running sums of absurd lengths stop here instead of wrapping: the sum of two such ends still fits an int. What goes
 // into a sum is held to it too.
 constexpr int SAT = (1 << 30) - 1;
@@ -45,7 +45,7 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total)
 	__syncthreads();
 	int before = 0, all = 0;
 #pragma unroll
-	for (int w = 0; w < STEP_THREADS / 32; ++w)
+	for (int w = 0; w < STEP_WARPS; ++w)
 	{
 		const int s = warp_sums[w];
 		if (w < warp) before = sat_add(before, s);
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 	int* tok = sm;             // [n + 1] running sum of new tokens
 	int* lack = sm + (n + 1);  // [n + 1] ... of pages to take
 	int* back = lack + n + 1;  // [n + 1] ... of pages given back
-	__shared__ int warp_sums[STEP_THREADS / 32];
+	__shared__ int warp_sums[STEP_WARPS];
 	const long long room = (long long)s.max_blocks * s.page_size;
 
 	if (threadIdx.x == 0) tok[0] = lack[0] = back[0] = 0;
@@ -613,7 +613,7 @@ extern "C" int nncu_paged_step_dev(const nncu_paged_step* s, void* stream)
 	if (s->held_out == s->held || s->queue_out == s->queue)
 		return refuse("paged step: held_out and queue_out must not be the inputs");
 	const size_t smem = 3 * sizeof(int) * ((size_t)s->n_req + 1);
-	if (smem > 48 * 1024)
+	if (smem + STEP_WARPS * sizeof(int) > 48 * 1024) // what a kernel has unasked, its fixed arrays included
 	{
 		const cudaError_t ce = cudaFuncSetAttribute(paged_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
 		                                            3 * (int)sizeof(int) * (NNCU_PAGED_MAX_REQ + 1));

@@ -87,3 +87,36 @@ def test_step_of_lengths_near_the_largest(nncu, torch_cuda):
     for name, key in (("held_out", "held"), ("queue_out", "queue"), ("seq_len",) * 2, ("q_start",) * 2, ("slots",) * 2,
                       ("token_req",) * 2, ("positions",) * 2):
         np.testing.assert_array_equal(out[name].cpu().numpy(), want[key], err_msg=name)
+
+
+def steps_of(counts):
+    import torch
+
+    import libllmcpu_b200 as N
+
+    for n in counts:
+        rng = np.random.default_rng(n)
+        past, new = rng.integers(0, 60, n), rng.integers(0, 3, n)
+        held = -(-past // 16)
+        n_pages, max_tok = int(held.sum()) + 900, int(new.sum()) + 5
+        ids, at = rng.permutation(n_pages), 0
+        table = np.full((n, 5), -7)
+        for r in range(n):
+            table[r, :held[r]] = ids[at:at + held[r]]
+            at += held[r]
+        ring = np.full(n_pages, -9)
+        ring[:n_pages - at] = ids[at:]
+        want = P.step(past, new, held, [0, n_pages - at], ring, table, 16, n_pages, 5, max_tok)
+        Step(torch, N, past, new, held, [0, n_pages - at], ring, dev(torch, table, torch.int32), 16, 5,
+             max_tok).check(want)
+
+
+def test_step_whose_sums_just_fill_48_kb(nncu, torch_cuda):
+    """4090 to 4095 requests: their sums fill the 48 KB that a kernel has unasked, less its other shared words. In a
+    process of its own, where no larger call has asked for more before."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = "import test_gpu_paged_edges as t; t.steps_of([4089, 4090, 4093, 4095, 4096])"
+    path = os.pathsep.join([here, os.path.dirname(here), os.environ.get("PYTHONPATH", "")])
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": path})
+    assert r.returncode == 0, r.stderr[-2000:]
