@@ -399,8 +399,10 @@ int nncu_argmax_rows_dev(const float* x, size_t x_stride, int32_t n_rows, uint32
  * seq_len[n_req] (past + n_new; past where not served; 0 where ended),
  * q_start[n_req + 1], and for every place t of the token buffer positions[t]
  * (0 past the end), slots[t] = page * page_size + position % page_size (-1: no
- * slot) and token_req[t] (-1 past the end). held_out and queue_out must not be
- * held and queue (a caller swaps the two from step to step). */
+ * slot) and token_req[t] (-1 past the end). No two of the arrays may share
+ * entries where one of them is written: held_out and queue_out are not held
+ * and queue (a caller swaps the two from step to step), seq_len is not past (it
+ * is copied there, or the two are swapped). */
 #define NNCU_PAGED_MAX_REQ 8192
 typedef struct nncu_paged_step
 {

@@ -598,6 +598,40 @@ int kv4_check_pool(const nncu_kv4_pool* p, const char* what, bool need_pages)
 
 using namespace nncu;
 
+namespace
+{
+
+// Whether an array that a step writes shares entries with another of its arrays: CTAs read and write them at the same
+// time.
+bool step_arrays_meet(const nncu_paged_step& s)
+{
+	struct Array
+	{
+		const int32_t* p;
+		size_t n;
+	};
+	const size_t n = s.n_req, tok = s.max_tok;
+	const Array all[] = {{s.held_out, n},  {s.queue_out, 4}, {s.seq_len, n},   {s.q_start, n + 1},          {s.positions, tok},
+	                     {s.slots, tok},   {s.token_req, tok}, {s.ring, (size_t)s.n_pages}, // written, the ones below only read
+	                     {s.past, n},      {s.n_new, n},     {s.held, n},      {s.queue, 2}};
+	constexpr int ALL = sizeof all / sizeof all[0], WRITTEN = 8;
+	const auto at = [](const int32_t* p) { return reinterpret_cast<uintptr_t>(p); };
+	const uintptr_t table = at(s.block_table), row = 4 * (uintptr_t)s.table_stride;
+	for (int i = 0; i < ALL; ++i)
+	{
+		const uintptr_t p = at(all[i].p), e = p + 4 * all[i].n;
+		if (p == e) continue;
+		for (int j = 0; j < i && j < WRITTEN; ++j)
+			if (p < at(all[j].p + all[j].n) && at(all[j].p) < e) return true;
+		// the table's rows, without what lies between them
+		if (e <= table || p >= table + (n - 1) * row + 4 * (uintptr_t)s.max_blocks) continue;
+		if (p < table || (p - table) % row < 4 * (uintptr_t)s.max_blocks || (p - table) % row + (e - p) > row) return true;
+	}
+	return false;
+}
+
+} // namespace
+
 extern "C" int nncu_paged_step_dev(const nncu_paged_step* s, void* stream)
 {
 	if (!s) return refuse("paged step: NULL argument");
@@ -612,6 +646,7 @@ extern "C" int nncu_paged_step_dev(const nncu_paged_step* s, void* stream)
 		return refuse("paged step: NULL array");
 	if (s->held_out == s->held || s->queue_out == s->queue)
 		return refuse("paged step: held_out and queue_out must not be the inputs");
+	if (step_arrays_meet(*s)) return refuse("paged step: an array that is written must not meet another one");
 	const size_t smem = 3 * sizeof(int) * ((size_t)s->n_req + 1);
 	if (smem + STEP_WARPS * sizeof(int) > 48 * 1024) // what a kernel has unasked, its fixed arrays included
 	{

@@ -35,12 +35,15 @@ class Step:
                                       block_table=table, **self.out))
         torch.cuda.synchronize()
 
-    def check(self, want):
+    def check_all(self, want, end=(1 << 31) - 1):
         for name, key in (("held_out", "held"), ("queue_out", "queue"), ("seq_len",) * 2, ("q_start",) * 2,
                           ("positions",) * 2, ("slots",) * 2, ("token_req",) * 2):
             np.testing.assert_array_equal(self.out[name].cpu().numpy(),
-                                          np.minimum(np.asarray(want[key], np.int64), SUM_END), err_msg=name)
+                                          np.minimum(np.asarray(want[key], np.int64), end), err_msg=name)
         np.testing.assert_array_equal(self.ring.cpu().numpy(), np.asarray(want["ring"]))
+
+    def check(self, want):
+        self.check_all(want, SUM_END)
 
 
 @pytest.mark.parametrize("new", [[1 << 30, 1 << 30, 3, 2], [3, (1 << 31) - 1, (1 << 31) - 1, 5], [1 << 30] * 40 + [4]])
@@ -68,25 +71,18 @@ def test_step_of_more_lacking_pages_than_any_sum(nncu, torch_cuda):
 
 
 def test_step_of_lengths_near_the_largest(nncu, torch_cuda):
-    """Pages of one token and tables of 2^31 - 1: needs near 2^31, whose requests are not served, so that no entry of
-    the table is touched."""
+    """Pages of one token, a table of 2^31 - 1 a request: a need as large, then a small one; neither is served, and no
+    entry of the table is touched."""
     torch = torch_cuda
     most, n_pages = (1 << 31) - 1, 64
-    past, new, held = [most - 3, most - 1, 0, 7], [2, 1, 3, 0], [0, 0, 0, 7]
-    table = torch.zeros(4, 8, dtype=torch.int32, device="cuda")
-    want = P.step(past, new, held, [5, 40], np.arange(n_pages), np.zeros((4, 8)), 1, n_pages, most, 20)
+    past, new, held = [most - 1, 0], [1, 3], [0, 0]
+    table = torch.empty(2 * most, dtype=torch.int32, device="cuda").view(2, most)
+    want = P.step(past, new, held, [5, 40], np.arange(n_pages), np.zeros((2, 4)), 1, n_pages, most, 20)
     assert want["seq_len"] == past
     want["queue"][2] = SUM_END
-    i32, z = torch.int32, lambda k: torch.full((k,), -99, dtype=torch.int32, device="cuda")
-    out = dict(held_out=z(4), queue_out=z(4), seq_len=z(4), q_start=z(5), positions=z(20), slots=z(20), token_req=z(20))
-    nncu.paged_step_dev(nncu.paged_step(n_req=4, page_size=1, n_pages=n_pages, max_blocks=most, max_tok=20,
-                                        table_stride=most, past=dev(torch, past, i32), n_new=dev(torch, new, i32),
-                                        held=dev(torch, held, i32), queue=dev(torch, [5, 40], i32),
-                                        ring=torch.arange(n_pages, dtype=i32, device="cuda"), block_table=table, **out))
-    torch.cuda.synchronize()
-    for name, key in (("held_out", "held"), ("queue_out", "queue"), ("seq_len",) * 2, ("q_start",) * 2, ("slots",) * 2,
-                      ("token_req",) * 2, ("positions",) * 2):
-        np.testing.assert_array_equal(out[name].cpu().numpy(), want[key], err_msg=name)
+    Step(torch, nncu, past, new, held, [5, 40], np.arange(n_pages), table, 1, most, 20).check_all(want)
+    del table
+    torch.cuda.empty_cache()
 
 
 def steps_of(counts):
