@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "kv4.cuh"
+#include "kv4_plan.h"
 #include "tc.cuh"
 
 namespace nncu
@@ -51,8 +52,6 @@ namespace
 
 constexpr int BN = 64;           // keys a tile
 constexpr int PT = 512;          // threads
-constexpr int SHARES = 2 * 148;  // pieces are about total / SHARES tiles long, and not under MIN_PIECE
-constexpr int MIN_PIECE = 8;
 constexpr float HELD = 11.0f, HELD_TOP = 15.0f; // see k_kv4_attn.cu
 constexpr int PLAN_THREADS = 1024;
 // Each product cuts the accumulator off at 24 bits, always towards zero: over
@@ -127,19 +126,20 @@ __device__ __forceinline__ int prompt_rows(const Kv4Args& a, const Kv4Request& x
 }
 
 // Inclusive running sum over the CTA, and the total.
-__device__ __forceinline__ int plan_scan(int v, int* sums, int& total)
+template <typename T>
+__device__ __forceinline__ T plan_scan(T v, T* sums, T& total)
 {
 	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
 	for (int o = 1; o < 32; o <<= 1)
 	{
-		const int u = __shfl_up_sync(0xffffffffu, v, o);
+		const T u = __shfl_up_sync(0xffffffffu, v, o);
 		if (lane >= o) v += u;
 	}
 	__syncthreads();
 	if (lane == 31) sums[warp] = v;
 	__syncthreads();
-	int before = 0, all = 0;
+	T before = 0, all = 0;
 	for (int w = 0; w < PLAN_THREADS / 32; ++w)
 	{
 		if (w < warp) before += sums[w];
@@ -153,6 +153,7 @@ template <int BR>
 __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const Kv4Args a, const PromptWs ws, int min_rows)
 {
 	__shared__ int sums[PLAN_THREADS / 32];
+	__shared__ long long tile_sums[PLAN_THREADS / 32];
 	const int tid = threadIdx.x;
 	int at = 0, total;
 	for (int r0 = 0; r0 < a.n_req; r0 += PLAN_THREADS)
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const Kv4Args a,
 		return lo;
 	};
 	// the blocks' tiles, and what a piece may have of them
-	int mine = 0;
+	long long mine = 0, tiles;
 	for (int b = tid; b < blocks; b += PLAN_THREADS)
 	{
 		const int r = find(b);
@@ -191,12 +192,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const Kv4Args a,
 		ws.tiles[b] = n;
 		mine += n;
 	}
-	plan_scan(mine, sums, total);
-	const int longest = max(MIN_PIECE, (int)(((long long)total * a.n_kv + SHARES - 1) / SHARES));
+	plan_scan(mine, tile_sums, tiles);
+	const int longest = kv4_longest(tiles, a.n_kv);
 	int pieces = 0, split = 0;
 	for (int b0 = 0; b0 < blocks; b0 += PLAN_THREADS)
 	{
-		const int b = b0 + tid, n = b < blocks ? ws.tiles[b] : 0, np = (n + longest - 1) / longest;
+		const int b = b0 + tid, n = b < blocks ? ws.tiles[b] : 0, np = n / longest + (n % longest > 0);
 		int t1, t2;
 		const int p1 = pieces + plan_scan(np, sums, t1), s1 = split + plan_scan(np > 1 ? np : 0, sums, t2);
 		pieces += t1;
@@ -962,7 +963,7 @@ size_t prompt_ws(unsigned char* base, size_t at, int n_req, long long rows, int 
 {
 	using L = PShape<D>;
 	// every block but a request's last is full; a block cut into n pieces holds more than n - 1 shares
-	const long long blocks = rows / L::BR + n_req, pieces = blocks + SHARES;
+	const long long blocks = rows / L::BR + n_req, pieces = blocks + KV4_SHARES;
 	ws.max_blocks = (int)blocks;
 	ws.max_pieces = (int)pieces;
 	const auto take = [&](size_t bytes) {
@@ -976,7 +977,7 @@ size_t prompt_ws(unsigned char* base, size_t at, int n_req, long long rows, int 
 	ws.tiles = reinterpret_cast<int*>(take(4 * (size_t)blocks));
 	ws.pieces = reinterpret_cast<Piece*>(take(sizeof(Piece) * (size_t)pieces));
 	ws.counters = reinterpret_cast<int*>(take(4 * (size_t)blocks * n_kv));
-	ws.parts = reinterpret_cast<float*>(take((size_t)2 * SHARES * L::PART * 4));
+	ws.parts = reinterpret_cast<float*>(take((size_t)2 * KV4_SHARES * L::PART * 4));
 	ws.sums = reinterpret_cast<float*>(take((size_t)MAX_SMS * L::BR * D * 4));
 	return at;
 }
