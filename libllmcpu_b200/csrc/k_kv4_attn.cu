@@ -480,10 +480,12 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 		for (int t = tile; t < tile + n; ++t, ++it)
 		{
 			const int stage = it % STAGES;
-			if (!*abort_ && !kv4_wait(&full[stage], (it / STAGES) & 1, ws.err, DEVERR_WAIT_FULL)) *abort_ = 1;
+			const bool came = !*abort_ && kv4_wait(&full[stage], (it / STAGES) & 1, ws.err, DEVERR_WAIT_FULL);
+			if (!came) *abort_ = 1;
 			const unsigned char* st = smem + stage * L::STAGE;
 			const int key0 = (s.tile0 + t) * TILE + warp * 16;
-			if (loaded[stage] >> warp & 1)
+			// (one answer for the warp, whose lanes work together below: after a wait that ran out they might see different ones)
+			if (__all_sync(0xffffffffu, came && (loaded[stage] >> warp & 1)))
 			{
 				// ---- scores of 16 keys ----
 				float sc[R][4];

@@ -116,3 +116,86 @@ def test_step_whose_sums_just_fill_48_kb(nncu, torch_cuda):
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                        env={**os.environ, "PYTHONPATH": path})
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+class Cache:
+    """Requests' keys and values in a pool: random pages, written by the append, read back as the values they stand for."""
+
+    def __init__(self, torch, N, lens, n_kv, d, page, seed=0, rise=0.0):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        self.torch, self.N, self.lens, self.n_kv, self.d = torch, N, lens, n_kv, d
+        blocks = [-(-n // page) for n in lens]
+        n_pages = sum(blocks) + 3
+        ids = np.random.default_rng(seed).permutation(n_pages)
+        self.table = np.full((len(lens), max(blocks)), -1)
+        self.kv, at = [], 0
+        self.pages = torch.zeros(N.kv4_bytes(n_pages, page, n_kv, d), dtype=torch.uint8, device="cuda")
+        self.pool = N.kv4_pool(self.pages, n_pages, page, n_kv, d)
+        # keys along `axis` grow with their position: scores of a query that lies along it rise by `rise`
+        self.axis = torch.randn(d, generator=gen, device="cuda")
+        self.axis /= self.axis.norm()
+        for r, n in enumerate(lens):
+            self.table[r, :blocks[r]] = ids[at:at + blocks[r]]
+            at += blocks[r]
+            k, v = (torch.randn(n, n_kv, d, generator=gen, device="cuda") for _ in range(2))
+            k += rise * torch.linspace(0, 1, n, device="cuda")[:, None, None] * self.axis
+            back = [torch.zeros(n, n_kv * d, device="cuda") for _ in range(2)]
+            slots = dev(torch, self.table[r, np.arange(n) // page] * page + np.arange(n) % page, torch.int32)
+            N.kv4_append_dev(N.kv4_rows(self.pool, slots=slots, n_tok=n, k=k, v=v))
+            N.kv4_read_dev(N.kv4_rows(self.pool, slots=slots, n_tok=n, k=back[0], v=back[1]))
+            self.kv.append([x.view(n, n_kv, d).double().cpu().numpy() for x in back])
+        self.vmax = max([float(np.abs(kv[1]).max()) for kv in self.kv if kv[1].size] + [0.0])
+
+    def attn(self, new, group, scale, window=0, softcap=0.0, along=0.0, seed=1):
+        """The call of `new` tokens a request; self.out has its rows, self.q its queries."""
+        torch, N = self.torch, self.N
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        nh, n_tok, i32 = self.n_kv * group, sum(new), torch.int32
+        self.group, self.new, self.args = group, new, (window, scale, softcap)
+        q = torch.randn(n_tok, nh, self.d, generator=gen, device="cuda") + along * self.axis
+        self.q = q.view(n_tok, nh * self.d)
+        self.out = torch.full_like(self.q, 5.0)
+        self.start = np.concatenate([[0], np.cumsum(new)])
+        call = N.kv4_attn(self.pool, n_req=len(new), n_tok=n_tok, n_head=nh, max_new=max(new),
+                          max_blocks=self.table.shape[1], block_table=dev(torch, self.table, i32),
+                          seq_len=dev(torch, self.lens, i32), q_start=dev(torch, self.start, i32), q=self.q,
+                          out=self.out, window=window, scale=scale, softcap=softcap)
+        self.ws = torch.zeros(N.kv4_workspace_bytes(call), dtype=torch.uint8, device="cuda")
+        call.workspace, call.workspace_bytes = self.ws.data_ptr(), self.ws.numel()
+        return call
+
+    def rows(self, r, tokens, heads=None):
+        """(what the call gave, what the definition gives) for tokens of request r, [rows, head_dim]."""
+        window, scale, softcap = self.args
+        got, want = [], []
+        for t in tokens:
+            for h in range(self.n_kv * self.group) if heads is None else heads:
+                at = (int(self.start[r]) + t, slice(h * self.d, (h + 1) * self.d))
+                kv = [x[:, h // self.group] for x in self.kv[r]]
+                got.append(self.out[at].double().cpu().numpy())
+                want.append(P.attention(self.q[at].cpu().numpy(), *kv, self.lens[r] - self.new[r] + t, window, scale,
+                                        softcap))
+        return np.array(got), np.array(want)
+
+
+@pytest.mark.parametrize("new", [1, 90])
+def test_check_reports_and_clears(nncu, torch_cuda, new):
+    """The error word that a wait which ran out leaves (written here by the host): reported once, the workspace is
+    cleared, and the next call is right."""
+    torch = torch_cuda
+    c = Cache(torch, nncu, [2000, 1500], 2, 128, 64)
+    call = c.attn([new] * 2, 4, 128 ** -0.5)
+    nncu.kv4_attention_dev(call)
+    nncu.kv4_check(call)
+    first = c.out.clone()
+    c.ws[:4].view(torch.int32)[0] = 1
+    c.ws[256:4096] = 7  # and counters that a call was left with
+    with pytest.raises(nncu.NnncError) as e:
+        nncu.kv4_check(call)
+    assert e.value.status == nncu.ERR_TIMEOUT and "ran out" in str(e.value)
+    assert int(c.ws.count_nonzero()) == 0
+    nncu.kv4_check(call)
+    c.out.fill_(5.0)
+    nncu.kv4_attention_dev(call)
+    nncu.kv4_check(call)
+    assert torch.equal(c.out, first)
