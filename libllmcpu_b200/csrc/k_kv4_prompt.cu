@@ -773,6 +773,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 							alpha = ex2(HELD - over);
 							held += HELD - over;
 						}
+						tmem_wait_st(); // (stores that are under way need not land in their order)
 						write_p(held);
 					}
 				}

@@ -199,3 +199,67 @@ def test_check_reports_and_clears(nncu, torch_cuda, new):
     nncu.kv4_attention_dev(call)
     nncu.kv4_check(call)
     assert torch.equal(c.out, first)
+
+
+# The relative size (2-norm) of an output's error over long spans. A tensor-memory product cuts its accumulator off
+# towards zero, 2^-24 of it in the mean. O takes 8 products a tile of 64 keys and starts anew every 6 tiles: 48 cuts of a
+# sum that grows from nothing, half of 48 * 2^-24 = 1.4e-6. Scores (up to 7 in base 2, 2 in the mean) take up to 16
+# products: 2 * 16 / 2 * 2^-24 * ln 2 = 0.7e-6. The exponential 2^-22 and the halves of q and of the weights (2^-22
+# each), at random among the keys: 0.5e-6. Together 2.6e-6; without the new starts a piece of 50 tiles or more has 200
+# cuts at half its size and more: 12e-6.
+LONG = 4e-6
+
+
+@pytest.mark.parametrize("d,n_kv,group,keys,new,page", [
+    (64, 8, 4, 16000, 1024, 16), (128, 8, 4, 16000, 1000, 32), (256, 4, 2, 16000, 1001, 16), (128, 8, 4, 15990, 900, 256),
+])
+def test_prompts_in_long_pieces(nncu, torch_cuda, d, n_kv, group, keys, new, page):
+    """Pieces of 50 tiles and more: sums added up many times, tables read in many parts; again the same, bit for bit."""
+    torch = torch_cuda
+    c = Cache(torch, nncu, [keys], n_kv, d, page)
+    call = c.attn([new], group, d ** -0.5)
+    nncu.kv4_attention_dev(call)
+    nncu.kv4_check(call)
+    first = c.out.clone()
+    for t in (0, 131, 514, new - 1):
+        got, want = c.rows(0, [t])
+        assert np.linalg.norm(got - want) <= LONG * np.linalg.norm(want), t
+    for _ in range(3):
+        c.out.fill_(5.0)
+        nncu.kv4_attention_dev(call)
+        assert torch.equal(c.out, first)
+
+
+# With scores that rise to 13 in base 2 each product may cut off 2^-24 of them, always towards zero: D / 16 times
+# 13 * 2^-24 * ln 2, 8.6e-6 for 256 values, beside the above.
+@pytest.mark.parametrize("d,n_kv,group,keys,new,page", [(64, 8, 4, 16000, 1024, 32), (128, 8, 4, 9000, 2000, 16),
+                                                        (256, 4, 2, 16000, 1000, 64)])
+def test_scores_that_rise_along_long_pieces(nncu, torch_cuda, d, n_kv, group, keys, new, page):
+    """The held score moves after sums have been put aside: they follow it."""
+    c = Cache(torch_cuda, nncu, [keys], n_kv, d, page, rise=9.0)
+    call = c.attn([new], group, d ** -0.5, along=d ** 0.5)
+    nncu.kv4_attention_dev(call)
+    nncu.kv4_check(call)
+    for t in (0, new // 2, new - 1):
+        got, want = c.rows(0, [t])
+        assert np.linalg.norm(got - want) <= (LONG + d / 16 * 0.54e-6) * np.linalg.norm(want), t
+
+
+@pytest.mark.parametrize("rise", [0.0, 9.0])
+@pytest.mark.parametrize("d,n_kv,group,lens,new,page", [
+    (128, 8, 4, [16000, 15000, 16000, 9000], 1, 16), (64, 8, 4, [16000] * 4, 8, 16), (128, 8, 4, [16000] * 4, 8, 32),
+    (256, 4, 2, [30000, 16001], 3, 16), (64, 8, 4, [16000, 12345, 16000], 1, 64),
+])
+def test_decode_in_long_runs(nncu, torch_cuda, d, n_kv, group, lens, new, page, rise):
+    """Runs of more tiles than a table read has (8 at 16 keys a page), and segments cut anywhere."""
+    torch = torch_cuda
+    c = Cache(torch, nncu, lens, n_kv, d, page, rise=rise)
+    call = c.attn([new] * len(lens), group, d ** -0.5, along=d ** 0.5 if rise else 0.0)
+    nncu.kv4_attention_dev(call)
+    nncu.kv4_check(call)
+    first = c.out.clone()
+    for r in range(len(lens)):
+        got, want = c.rows(r, [new - 1])
+        assert np.linalg.norm(got - want) <= (LONG + d / 16 * 0.54e-6 * (rise > 0)) * np.linalg.norm(want), r
+    nncu.kv4_attention_dev(call)
+    assert torch.equal(c.out, first)
