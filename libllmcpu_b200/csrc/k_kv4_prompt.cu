@@ -57,8 +57,10 @@ constexpr int PLAN_THREADS = 1024;
 // Each product cuts the accumulator off at 24 bits, always towards zero: over
 // a long run of tiles that adds up (6e-6 of the output after 50 tiles). So O
 // starts anew every FRESH tiles, and the threads add up what it held, rounded
-// to nearest, in the CTA's part of the workspace (one per SM: a CTA fills it).
-constexpr int FRESH = 6, MAX_SMS = 192;
+// to nearest, in a place of the workspace that a CTA takes for itself while it
+// runs. There are at least as many places as SMs, and a CTA fills an SM (its
+// registers, its tensor memory), so one is always free.
+constexpr int FRESH = 6, PLACES = 192, PLACE_TRIES = 1 << 20;
 
 template <int D>
 struct PShape
@@ -102,7 +104,8 @@ struct PromptWs
 	Piece* pieces;
 	int* counters;   // [blocks][n_kv]
 	float* parts;
-	float* sums;     // [MAX_SMS][D / 4][BR] of 4: what O held before it started anew
+	int* taken;      // [PLACES] whether a CTA has the place
+	float* sums;     // [PLACES][D / 4][BR] of 4: what O held before it started anew
 	int max_blocks, max_pieces;
 };
 
@@ -166,6 +169,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv4_plan_kernel(const Kv4Args a,
 		at += total;
 	}
 	if (tid == 0) ws.blk0[0] = 0;
+	if (tid < PLACES) ws.taken[tid] = 0; // (a call that gave up may have left them)
 	__syncthreads();
 	const int blocks = min(at, ws.max_blocks);
 	const auto find = [&](int b) {
@@ -297,12 +301,10 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 	uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
 	volatile int* flags = reinterpret_cast<volatile int*>(bars + 31); // [0] abort, [1] a V scale was no number
 	int* shared_last = reinterpret_cast<int*>(bars + 32);
+	int* place = shared_last + 1; // where O's earlier sums go
 	int* loaded = reinterpret_cast<int*>(bars + 33); // [16] by tile: which 16-key parts of it are in the cache
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-	uint32_t sm;
-	asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
-	sm = min(sm, (uint32_t)MAX_SMS - 1);
 	const Kv4Request x = kv4_request(a, pc.r);
 	const int rows = prompt_rows(a, x, min_rows);
 	// each Q tile's key tiles within the piece; none: lo > hi
@@ -341,10 +343,24 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 		fence_barrier_init();
 	}
 	if (warp == 1) tmem_alloc(tmem_slot, L::COLS);
+	if (threadIdx.x == 64)
+	{
+		// (The SM's number is where it looks first: no other CTA is likely to have that place. A try takes about 1 us. Kept
+		// short: a longer form here, or one among the roles below, made the whole kernel 4 to 6 % slower.)
+		uint32_t at;
+		asm volatile("mov.u32 %0, %%smid;" : "=r"(at));
+		at = at % PLACES;
+		int was;
+#pragma unroll 1
+		for (int i = 0; (was = atomicCAS(ws.taken + at, 0, 1)) != 0 && i < PLACE_TRIES; ++i) at = at + 1 < PLACES ? at + 1 : 0;
+		__threadfence();
+		*place = was ? -1 : (int)at;
+	}
 	tc_fence_before();
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = *tmem_slot;
+	if (*place < 0) flags[0] = 1, atomicCAS(ws.err, 0, DEVERR_PLAN);
 	if (tmem != 0) flags[0] = 1, atomicCAS(ws.err, 0, DEVERR_PLAN); // (cannot be: see the products' warp)
 
 	// registers to the softmax (the launch gives every thread 128: 128 x (72 + 104 + 2 x 168) = 512 x 128)
@@ -663,7 +679,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			// HELD - held score (1e30: no key seen; places without a row: any score, for they never see one)
 			float held = real ? 1e30f : 0.0f, l = 0.0f;
 			// O's earlier parts, relative to sums_held
-			float4* sums = reinterpret_cast<float4*>(ws.sums + (size_t)sm * L::BR * D) + 128 * X + r;
+			float4* sums = reinterpret_cast<float4*>(ws.sums + (size_t)max(*place, 0) * L::BR * D) + 128 * X + r;
 			float sums_held = 0.0f;
 			bool have_sums = false;
 			const auto add_up = [&](float now) {
@@ -949,6 +965,11 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 	}
 	tc_fence_before();
 	__syncthreads();
+	if (threadIdx.x == 64 && *place >= 0)
+	{
+		__threadfence();
+		atomicExch(ws.taken + *place, 0); // (the barrier has gathered every use of it)
+	}
 	if (warp == 1)
 	{
 		tc_fence_after();
@@ -979,7 +1000,8 @@ size_t prompt_ws(unsigned char* base, size_t at, int n_req, long long rows, int 
 	ws.pieces = reinterpret_cast<Piece*>(take(sizeof(Piece) * (size_t)pieces));
 	ws.counters = reinterpret_cast<int*>(take(4 * (size_t)blocks * n_kv));
 	ws.parts = reinterpret_cast<float*>(take((size_t)2 * KV4_SHARES * L::PART * 4));
-	ws.sums = reinterpret_cast<float*>(take((size_t)MAX_SMS * L::BR * D * 4));
+	ws.taken = reinterpret_cast<int*>(take(PLACES * 4));
+	ws.sums = reinterpret_cast<float*>(take((size_t)PLACES * L::BR * D * 4));
 	return at;
 }
 

@@ -263,3 +263,28 @@ def test_decode_in_long_runs(nncu, torch_cuda, d, n_kv, group, lens, new, page, 
         assert np.linalg.norm(got - want) <= (LONG + d / 16 * 0.54e-6 * (rise > 0)) * np.linalg.norm(want), r
     nncu.kv4_attention_dev(call)
     assert torch.equal(c.out, first)
+
+
+def test_long_prompts_side_by_side(nncu, torch_cuda):
+    """Two calls on two streams with workspaces of their own, whose prompt parts were left full of ones: the places that
+    their sums are kept in are each call's own, and found free."""
+    torch = torch_cuda
+    c = [Cache(torch, nncu, [16000], 8, 128, 64, seed=s) for s in (3, 4)]
+    calls = [x.attn([1000], 4, 128 ** -0.5) for x in c]
+    for call in calls:
+        nncu.kv4_attention_dev(call)
+        nncu.kv4_check(call)
+    first = [x.out.clone() for x in c]
+    streams = [torch.cuda.Stream() for _ in c]
+    for x in c:
+        x.ws[-(1 << 25):].fill_(255)
+    for _ in range(3):
+        for x, call, st in zip(c, calls, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                x.out.fill_(5.0)
+                nncu.kv4_attention_dev(call, st)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x.out, f) for x, f in zip(c, first))
+    for call in calls:
+        nncu.kv4_check(call)
