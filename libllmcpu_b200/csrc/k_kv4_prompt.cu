@@ -39,6 +39,7 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -653,7 +654,8 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 				{
 					const float top = tops[i];
 					const int ex = top > 0.0f ? max(-100, min(100, ilogbf(top))) : 0;
-					const float g = __uint_as_float((uint32_t)(127 + 13 - ex) << 23); // the largest to [2^13, 2^14)
+					// the largest to [2^13, 2^14); the scale's sign too, so that mult below has none
+					const float g = copysignf(__uint_as_float((uint32_t)(127 + 13 - ex) << 23), a.scale);
 					const int first = i0 + i * RPI, rr = wq * 32 + first + lane / LPR;
 					const float g2 = __shfl_sync(0xffffffffu, g, (lane - first) * LPR & 31);
 					if (lane >= first && lane < first + RPI) f = g2;
@@ -674,7 +676,8 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			mbar_arrive(q_ready);
 
 			// ---- the softmax, O kept in scale ----
-			const float mult = (a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f) / f;
+			// (never zero: a masked score times mult stays -infinity. The least normal float leaves any score at zero.)
+			const float mult = fmaxf((a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f) / f, FLT_MIN);
 			const float cap2 = a.softcap * 1.4426950408889634f;
 			// HELD - held score (1e30: no key seen; places without a row: any score, for they never see one)
 			float held = real ? 1e30f : 0.0f, l = 0.0f;

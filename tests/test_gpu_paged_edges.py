@@ -288,3 +288,27 @@ def test_long_prompts_side_by_side(nncu, torch_cuda):
         assert all(torch.equal(x.out, f) for x, f in zip(c, first))
     for call in calls:
         nncu.kv4_check(call)
+
+
+# Weights are good to 6e-6 for scores up to 40 in base 2 (their rounding and the products' sums 2^-24 of their size, the
+# exponential 2^-22, the halves of q and of the weights 2^-21), and an output is a mean of values no larger than vmax.
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.1, -0.25, 1e-38, 0.3])
+@pytest.mark.parametrize("d,new", [(64, 3), (64, 150), (128, 130), (256, 150)])
+def test_any_scale(nncu, torch_cuda, d, new, scale, softcap):
+    """A scale of zero weighs all keys alike, a negative one turns the order round: masked keys stay masked."""
+    c = Cache(torch_cuda, nncu, [new + 70], 2, d, 16)
+    nncu.kv4_attention_dev(c.attn([new], 2, scale, softcap=softcap))
+    got, want = c.rows(0, sorted({0, 1, new // 2, new - 1}))
+    assert np.abs(got - want).max() <= 1e-5 * c.vmax
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-4])
+def test_any_scale_of_tiny_queries(nncu, torch_cuda, scale):
+    """Queries near 2^-100, whose scores vanish: a mean of the values."""
+    c = Cache(torch_cuda, nncu, [300], 1, 64, 16)
+    call = c.attn([200], 2, scale)
+    c.q *= 2.0 ** -100
+    nncu.kv4_attention_dev(call)
+    got, want = c.rows(0, [0, 100, 199])
+    assert np.abs(got - want).max() <= 1e-5 * c.vmax
