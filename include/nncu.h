@@ -496,7 +496,7 @@ int nncu_kv4_read_dev(const nncu_kv4_rows* rows, void* stream);
  * q_start[r] .. q_start[r + 1) are the last of its seq_len[r] keys (appended
  * before this call), so token t of n sits at position seq_len - n + t and sees
  * the keys up to itself, `window` at most (0: all). scale, softcap as in
- * nncu_attn_params. Query head h reads KV head h / (n_head / n_kv); rows are
+ * nncu_attn_params, both finite. Query head h reads KV head h / (n_head / n_kv); rows are
  * n_head * head_dim floats, strides in floats. A token that sees no key gets
  * zeros; keys on pages outside the pool are not seen; a seq_len past its
  * table row (max_blocks pages) counts as that row's end. max_new bounds the new

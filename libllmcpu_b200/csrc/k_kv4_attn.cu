@@ -37,6 +37,7 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <cmath>
 #include <cstdio>
 
 #include "kv4.cuh"
@@ -949,7 +950,8 @@ extern "C" int nncu_kv4_attention_dev(const nncu_kv4_attn* p, void* stream)
 	const size_t row = (size_t)p->n_head * p->pool.head_dim;
 	if (p->n_tok > 1 && (p->q_stride < row || p->out_stride < row))
 		return refuse("kv4 attention: strides shorter than a row");
-	if (!(p->softcap >= 0.0f) || !(p->scale == p->scale)) return refuse("kv4 attention: bad scale or softcap");
+	if (!(p->softcap >= 0.0f) || std::isinf(p->softcap) || !std::isfinite(p->scale))
+		return refuse("kv4 attention: bad scale or softcap");
 	size_t need = 0;
 	rc = nncu_kv4_workspace_bytes(p, &need);
 	if (rc != NNCU_OK) return rc;

@@ -56,3 +56,14 @@ def test_step_arrays_must_not_meet(L):
     # rows of 4 entries, 16 apart: in the second row, into the third from before it, before the table
     for p in (16 * 4 + 8, 2 * 16 * 4 - 4, -4):
         meets(L, table_stride=16, held=at["block_table"] + p)
+
+
+POOL = dict(pages=A, n_pages=8, page_size=64, n_kv=2, head_dim=128)
+ATTN = dict(n_req=2, n_tok=2, n_head=8, max_new=1, max_blocks=4, block_table=A, seq_len=A, q_start=A, q=A, out=A,
+            workspace=A, workspace_bytes=1 << 40)
+
+
+@pytest.mark.parametrize("change", [dict(scale=float("inf")), dict(scale=float("-inf")), dict(softcap=float("inf"))])
+def test_attention_wants_finite_scales(L, change):
+    """Their products with a score of zero are NaN."""
+    refused(L.nncu_kv4_attention_dev(N.kv4_attn(N.kv4_pool(**POOL), **{**ATTN, **change}), None), L, "scale or softcap")
