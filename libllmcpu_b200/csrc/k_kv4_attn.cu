@@ -194,7 +194,7 @@ __device__ __forceinline__ void segment_tiles(const Kv4Args& a, Segment& s, int 
 	s.rows = s.x.n_new * a.group;
 	if (s.rows > a.few_rows) s.rows = 0; // the tensor-memory kernel's
 	s.last = min(s.x.pos0 + s.x.n_new - 1, s.x.keys - 1);
-	s.first = a.window > 0 ? max(0, s.x.pos0 - a.window + 1) : 0;
+	s.first = kv4_first_key(a, s.x.pos0);
 	s.tile0 = s.first / TILE;
 	s.tiles = s.rows == 0 ? 0 : s.last < s.first ? 1 : s.last / TILE - s.tile0 + 1;
 }
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 				l[r][e] = 0.0f;
 				if (row2 < s.rows)
 				{
-					all_from = max(all_from, a.window > 0 ? at[r][e] - a.window + 1 : 0);
+					all_from = max(all_from, kv4_first_key(a, at[r][e]));
 					all_to = min(all_to, min(at[r][e], s.x.keys - 1));
 				}
 			}
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 						for (int e = 0; e < 4; ++e)
 						{
 							const int k = kx + (e & 2 ? 8 : 0), pos = at[r][e & 1];
-							if (k > pos || k >= end || (a.window > 0 && k <= pos - a.window)) sc[r][e] = -CUDART_INF_F;
+							if (k > pos || k >= end || (a.window > 0 && pos - k >= a.window)) sc[r][e] = -CUDART_INF_F;
 						}
 				}
 #pragma unroll
@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<D, R>::CTAS)) kv4_decode_kerne
 			{
 				// a row that sees a value that is no number has none in the group
 				const int pos = s.x.pos0 + rr / a.group;
-				const int from = max(a.window > 0 ? max(0, pos - a.window + 1) : 0, (s.tile0 + tile) * TILE);
+				const int from = max(kv4_first_key(a, pos), (s.tile0 + tile) * TILE);
 				const int to = min(min(pos, s.x.keys - 1), (s.tile0 + tile + n) * TILE - 1);
 				for (int k = from; k <= to; ++k)
 				{

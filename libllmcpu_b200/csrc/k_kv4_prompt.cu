@@ -117,7 +117,7 @@ __device__ __forceinline__ void row_tiles(const Kv4Args& a, const Kv4Request& x,
 	hi = 0;
 	if (row0 >= rows) return;
 	const int p0 = x.pos0 + row0 / a.group, p1 = x.pos0 + (min(rows, row0 + n) - 1) / a.group;
-	const int first = a.window > 0 ? max(0, p0 - a.window + 1) : 0, last = min(p1, x.keys - 1);
+	const int first = kv4_first_key(a, p0), last = min(p1, x.keys - 1);
 	if (last < first) return;
 	lo = first / BN;
 	hi = last / BN;
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(PT, 1) kv4_prompt_kernel(const Kv4Args a, cons
 			const int row = pc.row0 + 128 * X + r, tok = row / a.group;
 			const bool real = row < rows;
 			const int qp = x.pos0 + tok;
-			const int kf = a.window > 0 ? max(0, qp - a.window + 1) : 0, kl = real ? min(qp, x.keys - 1) : -1;
+			const int kf = kv4_first_key(a, qp), kl = real ? min(qp, x.keys - 1) : -1;
 
 			// ---- the warp's 32 rows of Q, as two 16-bit halves: whole rows, LPR lanes each ----
 			constexpr int LPR = D / 4 < 32 ? D / 4 : 32, VPL = D / 4 / LPR, RPI = 32 / LPR;

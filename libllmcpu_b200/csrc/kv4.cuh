@@ -81,6 +81,12 @@ __device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, int* er
 	return false;
 }
 
+// The first key that a query at `pos` sees. (Written so that no position, below zero too, and no window overflow.)
+__device__ __forceinline__ int kv4_first_key(const Kv4Args& a, int pos)
+{
+	return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
+}
+
 // One request's place in the packed tokens and its keys.
 struct Kv4Request
 {
@@ -98,7 +104,6 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4Args& a, int r)
 	x.n_new = max(0, min(min(n, a.max_new), a.n_tok - s));
 	return x;
 }
-
 
 // A pool's geometry (and, unless told otherwise, its pages) checked:
 // NNCU_OK or the refusal (k_paged.cu).

@@ -312,3 +312,13 @@ def test_any_scale_of_tiny_queries(nncu, torch_cuda, scale):
     nncu.kv4_attention_dev(call)
     got, want = c.rows(0, [0, 100, 199])
     assert np.abs(got - want).max() <= 1e-5 * c.vmax
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 50, 1000])
+@pytest.mark.parametrize("keys,new", [(1, 5), (3, 40), (70, 300), (900, 4)])
+def test_windows_of_any_size(nncu, torch_cuda, keys, new, window):
+    """More new tokens than keys (the first see none), and a window that all positions fit in."""
+    c = Cache(torch_cuda, nncu, [keys], 2, 128, 16)
+    nncu.kv4_attention_dev(c.attn([new], 2, 128 ** -0.5, window=window))
+    got, want = c.rows(0, sorted({0, max(0, new - keys - 1), max(0, new - keys), new - 1}))
+    assert np.abs(got - want).max() <= 1e-5 * c.vmax
