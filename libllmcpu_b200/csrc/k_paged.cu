@@ -667,6 +667,7 @@ extern "C" int nncu_rope_axes_dev(const nncu_rope_axes* r, void* stream)
 {
 	if (!r) return refuse("rope axes: NULL argument");
 	if (r->n_tok < 0 || (!r->q && !r->k)) return refuse("rope axes: negative n_tok or no rows");
+	if (r->n_tok > INT32_MAX - ROPE_CTAS) return refuse("rope axes: n_tok too large"); // (the CTAs count past it by that many)
 	if (r->head_dim <= 0 || r->head_dim > 512 || r->head_dim % 2) return refuse("rope axes: head_dim must be even, up to 512");
 	if (r->n_rot < 0 || r->n_rot % 2 || r->n_rot > r->head_dim) return refuse("rope axes: n_rot must be even, up to head_dim");
 	if (r->rope_mode != NNCU_ROPE_NEOX && r->rope_mode != NNCU_ROPE_NORM) return refuse("rope axes: unknown rope mode");

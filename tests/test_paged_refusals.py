@@ -67,3 +67,10 @@ ATTN = dict(n_req=2, n_tok=2, n_head=8, max_new=1, max_blocks=4, block_table=A, 
 def test_attention_wants_finite_scales(L, change):
     """Their products with a score of zero are NaN."""
     refused(L.nncu_kv4_attention_dev(N.kv4_attn(N.kv4_pool(**POOL), **{**ATTN, **change}), None), L, "scale or softcap")
+
+
+@pytest.mark.parametrize("n_tok", [2 ** 31 - 1, 2 ** 31 - 592])
+def test_rope_axes_counts_with_32_bits(L, n_tok):
+    """A CTA takes every 592nd token, and stops at the first number past the last one."""
+    rope = N.rope_axes(n_tok=n_tok, n_head=1, n_kv=1, head_dim=2, positions=A, inv_freq=A, q=A, pos_stride=n_tok)
+    refused(L.nncu_rope_axes_dev(rope, None), L, "n_tok")
