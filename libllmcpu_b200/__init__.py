@@ -523,10 +523,35 @@ def argmax_rows_dev(x, n_rows: int, n: int, out, x_stride=None, stream=None) -> 
 
 # ---- serving from a paged cache held in 4 bits ------------------------------------------
 # The descriptions are filled once from device tensors (or raw pointers), which
-# they keep alive, and passed to their call step after step.
+# they keep alive, and passed to their call step after step. What a call could
+# not read as it is (another type, values apart) is refused here.
+
+_INT32 = ("past", "n_new", "held", "queue", "ring", "block_table", "held_out", "queue_out", "seq_len", "q_start",
+          "positions", "slots", "token_req")
+_FLOAT32 = ("inv_freq", "q_gamma", "k_gamma", "q", "k", "v", "q_out", "k_out", "out")
+_TYPES = {**dict.fromkeys(_INT32, "int32"), **dict.fromkeys(_FLOAT32, "float32")}
+_ROWS = ("block_table", "positions", "q", "k", "v", "q_out", "k_out", "out")  # rows may lie apart
+
+
+def _dense(x, dims: int) -> bool:
+    """Whether the last `dims` dimensions of a tensor lie side by side."""
+    n = 1
+    for i in range(1, dims + 1):
+        if x.shape[-i] > 1 and x.stride(-i) != n:
+            return False
+        n *= x.shape[-i]
+    return True
+
 
 def _fill(s, **kw):
+    known = {f[0] for f in s._fields_}
     for name, v in kw.items():
+        if name not in known:
+            raise TypeError(f"{type(s).__name__} has no {name}")
+        if hasattr(v, "dtype") and name in _TYPES and str(v.dtype).rpartition(".")[2] != _TYPES[name]:
+            raise ValueError(f"{name}: values of {_TYPES[name]} are read, not {v.dtype}")
+        if hasattr(v, "data_ptr") and not _dense(v, v.ndim - 1 if name in _ROWS and v.ndim > 1 else v.ndim):
+            raise ValueError(f"{name}: the values of a row lie side by side")
         setattr(s, name, v if isinstance(v, (int, float, C.Structure, C.Array)) else _ptr(v))
     s._keep = kw
     return s
@@ -538,8 +563,6 @@ def _stride(x, given, row: int) -> int:
         return int(given)
     if x is None or isinstance(x, (int, np.ndarray)) or x.ndim < 2:
         return row
-    if x.stride(-1) != 1:
-        raise ValueError("the values of a row lie side by side")
     return int(x.stride(0)) if x.shape[0] > 1 else row
 
 

@@ -74,3 +74,43 @@ def test_rope_axes_counts_with_32_bits(L, n_tok):
     """A CTA takes every 592nd token, and stops at the first number past the last one."""
     rope = N.rope_axes(n_tok=n_tok, n_head=1, n_kv=1, head_dim=2, positions=A, inv_freq=A, q=A, pos_stride=n_tok)
     refused(L.nncu_rope_axes_dev(rope, None), L, "n_tok")
+
+
+def test_tensors_of_other_types_are_refused():
+    torch = pytest.importorskip("torch")
+    z = torch.zeros
+    i32, rows = torch.int32, dict(n_tok=4, n_head=2, n_kv=2, head_dim=64, inv_freq=A)
+    pool = N.kv4_pool(z(8, dtype=torch.uint8), 8, 64, 2, 128)
+    with pytest.raises(ValueError, match="positions.*int32.*int64"):
+        N.rope_axes(**rows, positions=torch.arange(4), q=A)
+    with pytest.raises(ValueError, match="q: .*float32.*bfloat16"):
+        N.rope_axes(**rows, positions=A, q=z(4, 128, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="slots.*int32"):
+        N.kv4_rows(pool, slots=z(4), n_tok=4, k=A, v=A)
+    with pytest.raises(ValueError, match="seq_len.*int32"):
+        N.kv4_attn(pool, **{**ATTN, "seq_len": z(2, dtype=torch.int64)})
+    with pytest.raises(ValueError, match="past.*int32"):
+        step(past=z(4, dtype=torch.int64))
+    with pytest.raises(TypeError, match="no_such"):
+        step(no_such=A)
+    assert step(past=z(4, dtype=i32))[0].past
+
+
+def test_tensors_whose_values_lie_apart_are_refused():
+    torch = pytest.importorskip("torch")
+    z, i32 = torch.zeros, torch.int32
+    rope = dict(n_tok=4, n_head=2, n_kv=2, head_dim=64, inv_freq=A)
+    apart = "lie side by side"
+    with pytest.raises(ValueError, match=apart):  # every other entry of a vector
+        N.rope_axes(**rope, positions=z(8, dtype=i32)[::2], q=A)
+    with pytest.raises(ValueError, match=apart):
+        step(n_new=z(4, 2, dtype=i32)[:, 0])
+    with pytest.raises(ValueError, match=apart):  # heads with a gap behind each, or in another order
+        N.rope_axes(**rope, positions=A, q=z(4, 2, 80)[..., :64])
+    with pytest.raises(ValueError, match=apart):
+        N.rope_axes(**rope, positions=A, q=z(2, 4, 64).transpose(0, 1))
+    # rows apart are served, and what has one entry lies side by side whatever its strides
+    r = N.rope_axes(**rope, positions=z(4, 1, dtype=i32).T, q=z(4, 3, 64)[:, :2], k=z(8, 2, 64)[::2])
+    assert (r.q_stride, r.k_stride) == (3 * 64, 2 * 2 * 64)
+    r = N.rope_axes(**{**rope, "n_tok": 1}, positions=z(1, 3, dtype=i32).T, q=A, sections=[16, 8, 8])
+    assert r.pos_stride == 1
