@@ -25,8 +25,8 @@ namespace
 
 constexpr int STEP_THREADS = 512, STEP_WARPS = STEP_THREADS / 32;
 // Running sums of absurd lengths stop here instead of wrapping: the sum of two such ends still fits an int. What goes
-// into a sum is held to it too.
-constexpr int SAT = (1 << 30) - 1;
+// into a sum is held to it too. The bit above says that the request is served.
+constexpr int SAT = (1 << 30) - 1, SERVED = 1 << 30;
 
 __device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, SAT); }
 
@@ -55,14 +55,15 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total)
 	return sat_add(before, v);
 }
 
-// The last i of [0, n] with a[i] <= x (a rising, a[0] <= x).
+// The last i of [0, n] with a[i] <= x (a rising, a[0] <= x), in the bits of MASK.
+template <int MASK = -1>
 __device__ __forceinline__ int last_at_most(const int* a, int n, int x)
 {
 	int lo = 0, hi = n;
 	while (lo < hi)
 	{
 		const int mid = (lo + hi + 1) >> 1;
-		if (a[mid] <= x)
+		if ((a[mid] & MASK) <= x)
 			lo = mid;
 		else
 			hi = mid - 1;
@@ -76,9 +77,10 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 	const int n = s.n_req;
 	int* tok = sm;             // [n + 1] running sum of new tokens
 	int* lack = sm + (n + 1);  // [n + 1] ... of pages to take
-	int* back = lack + n + 1;  // [n + 1] ... of pages given back
+	int* back = lack + n + 1;  // [n + 1] ... of pages given back, and whether the request before is SERVED
 	__shared__ int warp_sums[STEP_WARPS];
 	const long long room = (long long)s.max_blocks * s.page_size;
+	const int np = s.n_pages, count = max(0, min(s.queue[1], np));
 
 	if (threadIdx.x == 0) tok[0] = lack[0] = back[0] = 0;
 	int c_tok = 0, c_lack = 0, c_back = 0;
@@ -101,26 +103,20 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 		c_lack = sat_add(c_lack, t);
 		const int b_end = sat_add(c_back, block_scan(ends ? min(held, SAT) : 0, warp_sums, t));
 		c_back = sat_add(c_back, t);
-		if (i < n) tok[i + 1] = q_end, lack[i + 1] = l_end, back[i + 1] = b_end;
+		// (Behind a request that the ring did not suffice for, one that lacks no page is served still.)
+		const bool ok = fits && (need == 0 || l_end <= count);
+		if (i < n) tok[i + 1] = q_end, lack[i + 1] = l_end, back[i + 1] = b_end | (ok ? SERVED : 0);
 	}
 	__syncthreads();
 
-	const int np = s.n_pages;
-	const int count = max(0, min(s.queue[1], np));
 	const int head = ((s.queue[0] % np) + np) % np;
-	const int taken = lack[last_at_most(lack, n, count)];
-	// Behind a request that the ring did not suffice for, one that lacks no page is served still. (Whether it lacks one
-	// does not follow from the sum, which may have come to its end.)
-	const auto served = [&](int r, int nn, int past, int held) {
-		return nn >= 0 && past >= 0 && (long long)past + nn <= room && tok[r + 1] <= s.max_tok &&
-		       (lack[r + 1] <= count || (long long)held * s.page_size >= (long long)past + nn);
-	};
+	const int taken = lack[last_at_most(lack, n, count)], given = back[n] & SAT;
 	const int step = gridDim.x * STEP_THREADS, me = blockIdx.x * STEP_THREADS + (int)threadIdx.x;
 
 	for (int r = me; r < n; r += step)
 	{
 		const int nn = s.n_new[r], past = s.past[r], held = max(0, min(s.held[r], s.max_blocks));
-		const bool ok = served(r, nn, past, held);
+		const bool ok = back[r + 1] & SERVED;
 		s.held_out[r] = nn < 0 ? 0 : held + (ok ? lack[r + 1] - lack[r] : 0);
 		s.seq_len[r] = nn < 0 ? 0 : ok ? past + nn : past;
 		s.q_start[r] = tok[r];
@@ -129,7 +125,7 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 	{
 		s.q_start[n] = tok[n];
 		s.queue_out[0] = (head + taken) % np;
-		s.queue_out[1] = count - taken + back[n];
+		s.queue_out[1] = count - taken + given;
 		s.queue_out[2] = lack[n] - taken;
 		s.queue_out[3] = tok[n];
 	}
@@ -139,10 +135,10 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 		const int b = max(0, min(s.held[r], s.max_blocks)) + x - lack[r];
 		s.block_table[(size_t)r * s.table_stride + b] = s.ring[(head + x) % np];
 	}
-	for (int x = me; x < back[n]; x += step) // the returned pages, behind the free ones
+	for (int x = me; x < given; x += step) // the returned pages, behind the free ones
 	{
-		const int r = last_at_most(back, n - 1, x);
-		s.ring[((long long)head + count + x) % np] = s.block_table[(size_t)r * s.table_stride + x - back[r]];
+		const int r = last_at_most<SAT>(back, n - 1, x);
+		s.ring[((long long)head + count + x) % np] = s.block_table[(size_t)r * s.table_stride + x - (back[r] & SAT)];
 	}
 	for (int t = me; t < s.max_tok; t += step)
 	{
@@ -150,9 +146,9 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 		if (t < tok[n])
 		{
 			req = last_at_most(tok, n - 1, t);
-			const int nn = s.n_new[req], past = s.past[req], held = max(0, min(s.held[req], s.max_blocks));
-			pos = past + t - tok[req];
-			if (served(req, nn, past, held))
+			const int held = max(0, min(s.held[req], s.max_blocks));
+			pos = s.past[req] + t - tok[req];
+			if (back[req + 1] & SERVED)
 			{
 				const int b = pos / s.page_size;
 				const int page = b < held ? s.block_table[(size_t)req * s.table_stride + b]
