@@ -495,9 +495,11 @@ int nncu_kv4_read_dev(const nncu_kv4_rows* rows, void* stream);
 /* Causal attention of the packed tokens over the pool: request r's new tokens
  * q_start[r] .. q_start[r + 1) are the last of its seq_len[r] keys (appended
  * before this call), so token t of n sits at position seq_len - n + t and sees
- * the keys up to itself, `window` at most (0: all). scale, softcap as in
- * nncu_attn_params, both finite. Query head h reads KV head h / (n_head / n_kv); rows are
- * n_head * head_dim floats, strides in floats. A token that sees no key gets
+ * the keys up to itself, `window` at most (0: all). scale (of any sign) and
+ * softcap as in nncu_attn_params, both finite. Query head h reads KV head h /
+ * (n_head / n_kv); rows are n_head * head_dim floats, strides in floats. The
+ * kernels are chosen by what a table row can hold (max_blocks), which should
+ * not be far more than the requests' lengths. A token that sees no key gets
  * zeros; keys on pages outside the pool are not seen; a seq_len past its
  * table row (max_blocks pages) counts as that row's end. max_new bounds the new
  * tokens of one request and n_tok their sum: tokens past either are left out

@@ -28,9 +28,10 @@
 // exponents and cuts off the bits that the denormals lack: 3e-6 instead of
 // 1e-6 of the output.)
 // What bounds it: issue slots, about 470 instructions per 16 keys of 128
-// values (150 of them unpack), not memory. 64 requests of 512 to 8192 keys,
-// 32/8 heads x 128: 92 us, 2.26 TB/s of the cache; 131072 keys, 8/4 x 256,
-// four tokens: 89 us, 1.7 TB/s; 4096 keys, 32/8 x 128: 15 us (latency).
+// values (150 of them unpack), and pieces' starts and ends (a third of the
+// cycles), not memory. 64 requests of 512 to 8192 keys, 32/8 heads x 128: 93
+// us, 2.24 TB/s of the cache; 131072 keys, 8/4 x 256, four tokens: 89 us, 1.7
+// TB/s; 4096 keys, 32/8 x 128: 16 us (latency).
 // Requests with many query rows a KV head (few_rows) are left to the
 // tensor-memory kernel: it takes 128 rows or more at a time for the price of
 // one unpacking, this one 8 to 32.
@@ -61,7 +62,9 @@ constexpr int few_rows(int D) { return D == 64 ? 128 : D == 128 ? 96 : 64; }
 // Several row tiles a segment share the unpacking, single ones make more and
 // shorter segments: 16 requests over 4000 keys, 8 KV heads x 128, 32 rows, two
 // tiles 101 us, one 118; one request, two 34 us, one 24. So several from this
-// many key tiles on (the most that the tables can hold).
+// many key tiles on. (The most that the tables can hold, the lengths being on
+// the device: one request over 4000 keys with a table for 131072 takes two row
+// tiles, 34 us, and with 128 rows the other kernel, 66 us instead of 41.)
 constexpr long long MANY_TILES = 4096, FEW_TILES = 1024;
 constexpr int MIN_TILES = 4;           // a run is at least this long, while tiles are few
 // A row's weights are taken against a held score, 2^11 at it, which moves only

@@ -34,8 +34,8 @@
 // What bounds it: the products, which take 120 cycles each beside the
 // unpacking where they take 53 alone, and (head_dim 256, 128 rows a block) the
 // unpacking itself. Six prompts of 200 to 2048 tokens over 777 to 4096 keys,
-// 32/8 heads x 128: 563 us, 214 TFLOP/s (427 of 16-bit products); 1000 tokens
-// over 16000 keys, 8/4 x 256: 615 us, 206 TFLOP/s.
+// 32/8 heads x 128: 571 us, 211 TFLOP/s (422 of 16-bit products); 1000 tokens
+// over 16000 keys, 8/4 x 256: 621 us, 204 TFLOP/s.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 

@@ -20,8 +20,8 @@ namespace
 // forms all three (12 bytes a request from L2, a scan in shared memory)
 // instead of waiting for another one, then handles its share of the tokens,
 // the new pages and the returned pages: one launch, no workspace. Bound by the
-// launch and its dependent loads: 256 requests 5.7 us, 60 requests with 65 K
-// tokens 7.7 us.
+// launch and its dependent loads: 256 requests 5.8 us, 60 requests with 65 K
+// tokens 7.6 us.
 
 constexpr int STEP_THREADS = 512, STEP_WARPS = STEP_THREADS / 32;
 // Running sums of absurd lengths stop here instead of wrapping: the sum of two such ends still fits an int. What goes
@@ -171,8 +171,9 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const nncu_pag
 // lanes, and a lane has the same places of every vector. Its item is the 2 VEC
 // values that turn together (NEOX: VEC at e and VEC at e + n_rot / 2), so no
 // exchange between lanes is needed but the norm's sum. 8192 tokens of 16/4
-// heads x 256: 73 us, 4.6 TB/s (one CTA a token, gains and angles read for
-// every vector: 85 us); 64 tokens of 32/8 x 128: 3.8 us.
+// heads x 256: 74 us, 4.6 TB/s (one CTA a token, gains and angles read for
+// every vector: 85 us); 64 tokens of 32/8 x 128: 4.2 us. What is in flight runs
+// out at a token's end: the next one's first loads follow this one's stores.
 
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_CTAS = 4 * 148; // what fits on the SMs at once: more tokens are taken in turn
@@ -360,12 +361,15 @@ int launch_rope_axes(const RopeArgs& g, cudaStream_t st)
 
 // ---- the 4-bit cache's write -----------------------------------------------------------
 //
-// Memory bound: 4 bytes a value in, 0.5625 out. A lane takes 8 values, which
-// become one 32-bit word, four lanes a group of 32: its largest magnitude (with
-// its sign as the lowest bit, so that the positive one wins a tie) meets in two
-// exchanges, and every lane forms the scale and its reciprocal. blockIdx.y: K
-// or V. 8191 tokens of 4 heads x 256, written and read back: 44 us, 3.5 TB/s
-// (four values a lane and three exchanges of three values: 60 us).
+// 4 bytes a value in, 0.5625 out. A lane takes 8 values, which become one
+// 32-bit word, four lanes a group of 32: its largest magnitude (with its sign as
+// the lowest bit, so that the positive one wins a tie) meets in two exchanges,
+// and every lane forms the scale and its reciprocal. blockIdx.y: K or V. 8191
+// tokens of 4 heads x 256, written and read back: 45 us, 3.4 TB/s (four values a
+// lane and three exchanges of three values: 60 us). 16384 tokens: the write 41
+// us, 3.7 TB/s, bound by loads in flight and issue slots (70 % busy); the read 50
+// us, 3.1 TB/s, bound by the load and store path (L1 87 % busy). Every thread
+// also copies its parameters, which it indexes by K or V, to local memory.
 
 constexpr int ROWS_THREADS = 256;
 constexpr int ROWS_ITEMS = 2;           // pieces (8 values, 32 bytes) in flight a thread
