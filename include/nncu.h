@@ -533,6 +533,104 @@ int nncu_kv4_attention_dev(const nncu_kv4_attn* a, void* stream);
  * workspace is then cleared. */
 int nncu_kv4_check(const nncu_kv4_attn* a, void* stream);
 
+/* ---- a serving batch's projections in 8-bit integers -------------------------
+ * No counterpart in libnnc, whose projections are gemvs (above): a step of
+ * many tokens multiplies on the tensor cores. A row in 8 bits is `cols` codes
+ * (int8) and one float scale, value = scale * code; hidden states have a scale
+ * a token, weights one an output channel. Device pointers, asynchronous on
+ * `stream`, no allocation, nothing kept between calls; the structs are filled
+ * once. Rows of codes start on 16 bytes (base and code_stride); what lies
+ * between two rows is neither read as values nor written. */
+
+/* Rows quantised, with the norm before a projection: z = x * gamma (a float
+ * product; gamma NULL: x), s = max(max |z| / 127, 2^-126), code = z / s rounded
+ * to the nearest integer, ties to even. The row's scale is s, with `norm` s /
+ * sqrt(mean(x^2) + eps): an RMS norm is a factor of the row and leaves its
+ * codes alone (where that mean and eps are both zero: s). A row whose z has a NaN or an infinity gets codes of zero and
+ * the scale NaN. Weights are laid out by the same call, a row a channel. */
+typedef struct nncu_i8_rows
+{
+	int32_t n, cols;
+	int32_t x_type; /* nncu_kv_type: float, bf16 or f16 */
+	int32_t norm;
+	float eps;
+	const void* x;
+	size_t x_stride; /* in values */
+	const float* gamma; /* cols, or NULL */
+	int8_t* codes;
+	size_t code_stride; /* in bytes: a multiple of 16 */
+	float* scales; /* n */
+} nncu_i8_rows;
+int nncu_i8_quantise_dev(const nncu_i8_rows* r, void* stream);
+
+/* Rows read: out[t] = codes[id] * (scales[id] * mult), id = ids[t] (ids NULL:
+ * t). The token embedding of a table that the lm_head shares, `mult` the
+ * model's factor on it. An id outside [0, n_rows) gives zeros. */
+typedef struct nncu_i8_lookup
+{
+	int32_t n, cols, n_rows;
+	float mult;
+	const int32_t* ids;
+	const int8_t* codes;
+	size_t code_stride;
+	const float* scales;
+	float* out;
+	size_t out_stride; /* in floats */
+} nncu_i8_lookup;
+int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream);
+
+/* y[t][o] = x_scales[t] * w_scales[o] * sum_c x[t][c] * w[o][c] + bias[o] +
+ * add[t][o] for n_tok tokens and `rows` channels. The sum is exact (32-bit
+ * integers: cols up to 131071), so nothing of a result goes by the other
+ * tokens of its call. bias and add NULL: none; add may be y (a residual stream in
+ * place), otherwise y meets none of the inputs. */
+typedef struct nncu_i8_linear
+{
+	int32_t n_tok, rows, cols;
+	const int8_t* x;
+	size_t x_stride; /* in bytes: a multiple of 16 */
+	const float* x_scales;
+	const int8_t* w;
+	size_t w_stride; /* in bytes: a multiple of 16 */
+	const float* w_scales;
+	const float* bias;
+	const float* add;
+	size_t add_stride; /* in floats */
+	float* y;
+	size_t y_stride;
+} nncu_i8_linear;
+int nncu_i8_linear_dev(const nncu_i8_linear* l, void* stream);
+/* Wait for `stream` and report whether a product on the current device since
+ * the last check had a bounded wait run out (NNCU_ERR_TIMEOUT: the outputs
+ * since then are void); the word is then cleared. */
+int nncu_i8_check(void* stream);
+
+/* Of n rows of logits (`stride` floats apart), p = softmax(scale * logits):
+ * the natural logarithm of a given token's probability and its rank (how many
+ * tokens come before it), the row's entropy, and the `top` (0 to 32) likeliest
+ * tokens with their log probabilities. Tokens come in the order of their
+ * logits, equal ones by their index, a NaN as -infinity. Logits of -infinity are
+ * masked: probability zero; where fewer than `top` are left, the other ids are
+ * -1 and their log probabilities -infinity. A row that is masked whole has
+ * the entropy 0. A NaN or +infinity makes its row's log probabilities and entropy
+ * NaN. A given token outside the vocabulary (a padded buffer's) gets
+ * logprob 0 and rank -1. Outputs that are NULL are left out (tokens is needed
+ * for logprob and rank). Device pointers, asynchronous on `stream`. */
+typedef struct nncu_logprobs
+{
+	int32_t n, n_vocab, top;
+	float scale; /* above 0: one over the temperature */
+	const float* logits;
+	size_t stride;
+	const int32_t* tokens; /* n */
+	float* logprob;
+	int32_t* rank;
+	float* entropy;
+	int32_t* top_ids; /* [n][top] */
+	float* top_logprobs;
+} nncu_logprobs;
+int nncu_logprobs_dev(const nncu_logprobs* l, void* stream);
+
 /* One layer's decode / verify attention that allocates nothing: the same
  * K1 + K2 kernels as nncu_attention_batch_dev for one job, with every buffer
  * the caller's. No counterpart in the reference, whose CPU path never

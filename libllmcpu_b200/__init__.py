@@ -36,7 +36,9 @@ __all__ = [
     "gemv_bf16w_argmax_dev", "Weight", "AttnWeights", "weight", "W_BF16", "W_Q8_0", "W_Q4_S", "logits_batch_dev",
     "argmax_rows_dev", "PagedStep", "paged_step", "paged_step_dev", "RopeAxes", "rope_axes", "rope_axes_dev",
     "Kv4Pool", "kv4_pool", "kv4_bytes", "Kv4Rows", "kv4_rows", "kv4_append_dev", "kv4_read_dev", "Kv4Attn",
-    "kv4_attn", "kv4_workspace_bytes", "kv4_attention_dev", "kv4_check", "EXPORTS",
+    "kv4_attn", "kv4_workspace_bytes", "kv4_attention_dev", "kv4_check", "I8Rows", "i8_rows", "i8_quantise_dev",
+    "I8Lookup", "i8_lookup", "i8_lookup_dev", "I8Linear", "i8_linear", "i8_linear_dev", "i8_check", "Logprobs",
+    "logprobs", "logprobs_dev", "EXPORTS",
 ]
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -66,7 +68,8 @@ EXPORTS = [
     "nncu_attention_forward_batch_dev",
     "nncu_argmax_rows_dev", "nncu_paged_step_dev", "nncu_rope_axes_dev", "nncu_kv4_bytes", "nncu_kv4_append_dev",
     "nncu_kv4_read_dev", "nncu_kv4_workspace_bytes", "nncu_kv4_attention_dev",
-    "nncu_kv4_check",
+    "nncu_kv4_check", "nncu_i8_quantise_dev", "nncu_i8_lookup_dev", "nncu_i8_linear_dev", "nncu_i8_check",
+    "nncu_logprobs_dev",
 ]
 GROUP_HANDLE_BYTES = 64
 
@@ -178,6 +181,39 @@ class Kv4Attn(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class I8Rows(C.Structure):
+    """nncu_i8_rows (include/nncu.h): rows to quantise to 8 bits, with their norm."""
+
+    _fields_ = [(n, C.c_int32) for n in ("n", "cols", "x_type", "norm")] + \
+               [("eps", C.c_float), ("x", C.c_void_p), ("x_stride", C.c_size_t), ("gamma", C.c_void_p),
+                ("codes", C.c_void_p), ("code_stride", C.c_size_t), ("scales", C.c_void_p)]
+
+
+class I8Lookup(C.Structure):
+    """nncu_i8_lookup (include/nncu.h): 8-bit rows to read as floats."""
+
+    _fields_ = [(n, C.c_int32) for n in ("n", "cols", "n_rows")] + \
+               [("mult", C.c_float), ("ids", C.c_void_p), ("codes", C.c_void_p), ("code_stride", C.c_size_t),
+                ("scales", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_size_t)]
+
+
+class I8Linear(C.Structure):
+    """nncu_i8_linear (include/nncu.h): tokens times weights, both in 8 bits."""
+
+    _fields_ = [(n, C.c_int32) for n in ("n_tok", "rows", "cols")] + \
+               [("x", C.c_void_p), ("x_stride", C.c_size_t), ("x_scales", C.c_void_p), ("w", C.c_void_p),
+                ("w_stride", C.c_size_t), ("w_scales", C.c_void_p), ("bias", C.c_void_p), ("add", C.c_void_p),
+                ("add_stride", C.c_size_t), ("y", C.c_void_p), ("y_stride", C.c_size_t)]
+
+
+class Logprobs(C.Structure):
+    """nncu_logprobs (include/nncu.h): what is reported of rows of logits."""
+
+    _fields_ = [(n, C.c_int32) for n in ("n", "n_vocab", "top")] + \
+               [("scale", C.c_float), ("logits", C.c_void_p), ("stride", C.c_size_t)] + \
+               [(n, C.c_void_p) for n in ("tokens", "logprob", "rank", "entropy", "top_ids", "top_logprobs")]
+
+
 class PerfPhase(C.Structure):
     _fields_ = [("ms", C.c_double), ("calls", C.c_int64), ("bytes", C.c_uint64)]
 
@@ -283,6 +319,11 @@ def lib() -> C.CDLL:
     L.nncu_kv4_workspace_bytes.argtypes = [C.POINTER(Kv4Attn), C.POINTER(sz)]
     L.nncu_kv4_attention_dev.argtypes = [C.POINTER(Kv4Attn), vp]
     L.nncu_kv4_check.argtypes = [C.POINTER(Kv4Attn), vp]
+    L.nncu_i8_quantise_dev.argtypes = [C.POINTER(I8Rows), vp]
+    L.nncu_i8_lookup_dev.argtypes = [C.POINTER(I8Lookup), vp]
+    L.nncu_i8_linear_dev.argtypes = [C.POINTER(I8Linear), vp]
+    L.nncu_i8_check.argtypes = [vp]
+    L.nncu_logprobs_dev.argtypes = [C.POINTER(Logprobs), vp]
     L.nncu_host_register.argtypes = [vp, sz]
     L.nncu_host_unregister.argtypes = [vp]
     L.nncu_sync.argtypes = [vp, vp]
@@ -521,7 +562,7 @@ def argmax_rows_dev(x, n_rows: int, n: int, out, x_stride=None, stream=None) -> 
                                       _ptr(out), _stream(stream)))
 
 
-# ---- serving from a paged cache held in 4 bits ------------------------------------------
+# ---- serving: the descriptions -----------------------------------------------------------
 # The descriptions are filled once from device tensors (or raw pointers), which
 # they keep alive, and passed to their call step after step. What a call could
 # not read as it is (another type, values apart) is refused here.
@@ -530,12 +571,15 @@ _INT32 = ("past", "n_new", "held", "queue", "ring", "block_table", "held_out", "
           "positions", "slots", "token_req")
 _FLOAT32 = ("inv_freq", "q_gamma", "k_gamma", "q", "k", "v", "q_out", "k_out", "out")
 _TYPES = {**dict.fromkeys(_INT32, "int32"), **dict.fromkeys(_FLOAT32, "float32")}
-_ROWS = ("block_table", "positions", "q", "k", "v", "q_out", "k_out", "out")  # rows may lie apart
+_ROWS = ("block_table", "positions", "q", "k", "v", "q_out", "k_out", "out", "codes", "x", "w", "add", "y",
+         "logits")  # rows may lie apart
 
 
 def _dense(x, dims: int) -> bool:
     """Whether the last `dims` dimensions of a tensor lie side by side."""
     n = 1
+    if 0 in x.shape:
+        return True
     for i in range(1, dims + 1):
         if x.shape[-i] > 1 and x.stride(-i) != n:
             return False
@@ -659,6 +703,100 @@ def kv4_attention_dev(a: Kv4Attn, stream=None) -> None:
 def kv4_check(a: Kv4Attn, stream=None) -> None:
     """nncu_kv4_check: wait for `stream`; raise (ERR_TIMEOUT) if a kernel using a's workspace timed out."""
     _check(lib().nncu_kv4_check(C.byref(a), _stream(stream)))
+
+
+# ---- a serving batch's projections in 8-bit integers, and its logits -------------------------
+
+_X_TYPES = {"float32": KV_F32, "bfloat16": KV_BF16, "float16": KV_F16}
+_I8_TYPES = dict(codes="int8", x="int8", w="int8", tokens="int32", rank="int32", top_ids="int32", ids="int32",
+                 **dict.fromkeys(("gamma", "scales", "x_scales", "w_scales", "bias", "add", "y", "out", "logits",
+                                  "logprob", "entropy", "top_logprobs"), "float32"))
+
+
+def _fill_dev(s, shapes, **kw):
+    """_fill for device tensors: their types, shapes (where a tensor says them) and devices agree with the call.
+    `shapes`: the rows and the values of a row (or the values, of a vector) that the call reaches."""
+    device = None
+    for name, v in kw.items():
+        if not hasattr(v, "data_ptr"):
+            continue
+        want = _I8_TYPES[name] if not (name == "x" and isinstance(s, I8Rows)) else None
+        if want and str(v.dtype).rpartition(".")[2] != want:
+            raise ValueError(f"{name}: values of {want} are read, not {v.dtype}")
+        if v.device.type != "cuda" or (device is not None and v.device != device):
+            raise ValueError(f"{name}: on {v.device}; the call's arrays lie on one GPU")
+        device = v.device
+        n, row = shapes[name]
+        one = v.ndim == 2 and name in _ROWS
+        if (one and n > 0 and (v.shape[0] < n or v.shape[1] < row)) or (not one and v.numel() < n * row):
+            raise ValueError(f"{name}: {tuple(v.shape)} is less than {n} x {row}")
+    return _fill(s, **kw)
+
+
+def i8_rows(n: int, cols: int, x, codes, scales, gamma=None, norm: int = 0, eps: float = 1e-6, x_type=None,
+            x_stride=None, code_stride=None) -> I8Rows:
+    """An nncu_i8_rows; x float32, bfloat16 or float16 rows (the type of a tensor is its own)."""
+    if hasattr(x, "dtype") and str(x.dtype).rpartition(".")[2] not in _X_TYPES:
+        raise ValueError(f"x: float32, bfloat16 or float16 rows are read, not {x.dtype}")
+    if x_type is None:
+        x_type = _X_TYPES[str(x.dtype).rpartition(".")[2]] if hasattr(x, "dtype") else KV_F32
+    return _fill_dev(I8Rows(), dict(x=(n, cols), codes=(n, cols), scales=(n, 1), gamma=(1, cols)), n=n, cols=cols,
+                     x_type=x_type, norm=int(norm), eps=eps, x=x, x_stride=_stride(x, x_stride, cols), gamma=gamma,
+                     codes=codes, code_stride=_stride(codes, code_stride, cols), scales=scales)
+
+
+def i8_quantise_dev(r: I8Rows, stream=None) -> None:
+    """nncu_i8_quantise_dev: rows normed and quantised to 8 bits."""
+    _check(lib().nncu_i8_quantise_dev(C.byref(r), _stream(stream)))
+
+
+def i8_lookup(n: int, cols: int, n_rows: int, codes, scales, out, ids=None, mult: float = 1.0, code_stride=None,
+              out_stride=None) -> I8Lookup:
+    """An nncu_i8_lookup: the rows `ids` (or each in turn) of an 8-bit table."""
+    return _fill_dev(I8Lookup(), dict(codes=(n_rows, cols), scales=(n_rows, 1), out=(n, cols), ids=(n, 1)), n=n,
+                     cols=cols, n_rows=n_rows, mult=mult, ids=ids, codes=codes,
+                     code_stride=_stride(codes, code_stride, cols), scales=scales, out=out,
+                     out_stride=_stride(out, out_stride, cols))
+
+
+def i8_lookup_dev(l: I8Lookup, stream=None) -> None:
+    """nncu_i8_lookup_dev: rows of an 8-bit table as floats."""
+    _check(lib().nncu_i8_lookup_dev(C.byref(l), _stream(stream)))
+
+
+def i8_linear(n_tok: int, rows: int, cols: int, x, x_scales, w, w_scales, y, bias=None, add=None, x_stride=None,
+              w_stride=None, add_stride=None, y_stride=None) -> I8Linear:
+    """An nncu_i8_linear: y = x w^T of n_tok tokens and `rows` channels."""
+    return _fill_dev(I8Linear(), dict(x=(n_tok, cols), x_scales=(n_tok, 1), w=(rows, cols), w_scales=(rows, 1),
+                                      bias=(rows, 1), add=(n_tok, rows), y=(n_tok, rows)),
+                     n_tok=n_tok, rows=rows, cols=cols, x=x, x_stride=_stride(x, x_stride, cols), x_scales=x_scales,
+                     w=w, w_stride=_stride(w, w_stride, cols), w_scales=w_scales, bias=bias, add=add,
+                     add_stride=_stride(add, add_stride, rows), y=y, y_stride=_stride(y, y_stride, rows))
+
+
+def i8_linear_dev(l: I8Linear, stream=None) -> None:
+    """nncu_i8_linear_dev: the product of 8-bit tokens and weights."""
+    _check(lib().nncu_i8_linear_dev(C.byref(l), _stream(stream)))
+
+
+def i8_check(stream=None) -> None:
+    """nncu_i8_check: wait for `stream`; raise (ERR_TIMEOUT) if a product on the current device timed out."""
+    _check(lib().nncu_i8_check(_stream(stream)))
+
+
+def logprobs(n: int, n_vocab: int, logits, scale: float = 1.0, tokens=None, logprob=None, rank=None, entropy=None,
+             top: int = 0, top_ids=None, top_logprobs=None, stride=None) -> Logprobs:
+    """An nncu_logprobs: a given token's log probability and rank, the entropy and the `top` likeliest of each row."""
+    return _fill_dev(Logprobs(), dict(logits=(n, n_vocab), top_ids=(n, top), top_logprobs=(n, top),
+                                      **dict.fromkeys(("tokens", "logprob", "rank", "entropy"), (n, 1))),
+                     n=n, n_vocab=n_vocab, top=top, scale=scale, logits=logits,
+                     stride=_stride(logits, stride, n_vocab), tokens=tokens, logprob=logprob, rank=rank,
+                     entropy=entropy, top_ids=top_ids, top_logprobs=top_logprobs)
+
+
+def logprobs_dev(l: Logprobs, stream=None) -> None:
+    """nncu_logprobs_dev: log probabilities, ranks, entropies and likeliest tokens of rows of logits."""
+    _check(lib().nncu_logprobs_dev(C.byref(l), _stream(stream)))
 
 
 def job(layer: int, p: AttnParams, q, k, v, out, seq: int = 0) -> AttnJob:

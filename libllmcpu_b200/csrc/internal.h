@@ -222,6 +222,9 @@ struct JobPointers
 	const void* v_cache;
 };
 int check_alignment(const JobPointers& p, int job, const char* what);
+// NNCU_OK where `p` is memory of the current device; a refusal otherwise (a
+// kernel that reads another device's memory would fault the GPU).
+int check_current_device(const void* p, const char* what);
 // Count kernels launched outside api.cpp (nncu_launch_count).
 void note_launches(int n);
 
