@@ -7,7 +7,7 @@
 #include <cstdio>
 
 #include "common.cuh"
-#include "nncu.h"
+#include "i8.h"
 
 namespace nncu
 {
@@ -84,46 +84,6 @@ __global__ void __launch_bounds__(256) i8_lookup_kernel(const nncu_i8_lookup l)
 	const float s = in ? l.scales[id] * l.mult : 0.0f;
 	const int8_t* c = l.codes + (size_t)(in ? id : 0) * l.code_stride;
 	for (int i = threadIdx.x; i < l.cols; i += 256) l.out[t * l.out_stride + i] = in ? s * (float)c[i] : 0.0f;
-}
-
-// y in tiles of 64 tokens by 64 channels, 64 columns at a time through shared memory.
-__global__ void __launch_bounds__(256) i8_linear_kernel(const nncu_i8_linear l)
-{
-	__shared__ int xs[64][17], ws[64][17];
-	const int o0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
-	const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-	int acc[4][4] = {};
-	for (int k0 = 0; k0 < l.cols; k0 += 64)
-	{
-		for (int i = threadIdx.x; i < 64 * 16; i += 256)
-		{
-			const int row = i / 16, w = i % 16;
-			int a = 0, b = 0;
-			for (int j = 0; j < 4; ++j)
-			{
-				const int k = k0 + 4 * w + j;
-				if (k >= l.cols) continue;
-				if (t0 + row < l.n_tok) a |= (int)(uint8_t)l.x[(size_t)(t0 + row) * l.x_stride + k] << (8 * j);
-				if (o0 + row < l.rows) b |= (int)(uint8_t)l.w[(size_t)(o0 + row) * l.w_stride + k] << (8 * j);
-			}
-			xs[row][w] = a, ws[row][w] = b;
-		}
-		__syncthreads();
-		for (int w = 0; w < 16; ++w)
-			for (int i = 0; i < 4; ++i)
-				for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(xs[ty * 4 + i][w], ws[tx + 16 * j][w], acc[i][j]);
-		__syncthreads();
-	}
-	for (int i = 0; i < 4; ++i)
-		for (int j = 0; j < 4; ++j)
-		{
-			const int t = t0 + ty * 4 + i, o = o0 + tx + 16 * j;
-			if (t >= l.n_tok || o >= l.rows) continue;
-			float v = (float)acc[i][j] * l.x_scales[t] * l.w_scales[o];
-			if (l.bias) v += l.bias[o];
-			if (l.add) v += l.add[(size_t)t * l.add_stride + o];
-			l.y[(size_t)t * l.y_stride + o] = v;
-		}
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -262,15 +222,17 @@ extern "C" int nncu_i8_linear_dev(const nncu_i8_linear* l, void* stream)
 		return refuse("i8 linear: y must not meet an input (add may be y itself)");
 	const int rc = check_current_device(l->y, "i8 linear");
 	if (rc != NNCU_OK) return rc;
-	const dim3 grid((l->rows + 63) / 64, (l->n_tok + 63) / 64);
-	i8_linear_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(*l);
+	const int e = launch_i8_linear(*l, stream);
+	if (e) cudaGetLastError();
 	note_launches(1);
-	const int e = (int)cudaGetLastError();
 	return e ? set_cuda_error(e, "i8 linear launch") : NNCU_OK;
 }
 
 extern "C" int nncu_i8_check(void* stream)
 {
-	const cudaError_t ce = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
-	return ce == cudaSuccess ? NNCU_OK : set_cuda_error((int)ce, "i8 check: stream");
+	int word = 0;
+	cudaError_t ce = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+	if (ce == cudaSuccess) ce = (cudaError_t)i8_error_word(&word);
+	if (ce != cudaSuccess) return set_cuda_error((int)ce, "i8 check");
+	return word ? set_error(NNCU_ERR_TIMEOUT, "an i8 product's bounded wait timed out; the outputs since the last check are void") : NNCU_OK;
 }

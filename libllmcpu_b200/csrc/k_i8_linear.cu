@@ -1,0 +1,587 @@
+// k_i8_linear.cu -- the product of 8-bit tokens and weights
+// (nncu_i8_linear_dev) on the 5th-generation tensor cores.
+//
+// Mathematics. y[t][o] = xs[t] ws[o] sum_c x[t][c] w[o][c]: the codes go to
+// tcgen05.mma kind::i8 as they are and their sums are exact 32-bit integers,
+// so any order of summing, any split over the columns and any tile give the
+// same bits; the scales are an epilogue.
+//
+// Channels are the M dimension (a TMEM lane each), tokens the N dimension (a
+// column each), both operands K-major rows of 128 codes, 128-byte swizzled as
+// TMA writes them. A thread of the epilogue holds one channel, so a warp's
+// store of one token's 32 channels is one 128-byte line.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdio>
+#include <cstdlib>
+
+#include "i8.h"
+#include "tc.cuh"
+
+namespace nncu
+{
+namespace
+{
+
+constexpr int KB = 128;         // columns of a stage: one swizzled row
+constexpr int W_BYTES = 128 * KB; // a stage's 128 channels
+constexpr int MAX_STAGES = 12;
+
+__device__ int g_i8_error; // the first bounded wait that ran out
+
+struct Args
+{
+	int n_tok, rows, bn, n_kb, stages, split;
+	int tiles_o, tiles_t; // of the pair kernel
+	const float* xs;
+	const float* ws;
+	const float* bias;
+	const float* add;
+	float* y;
+	size_t add_stride, y_stride;
+};
+
+// Instruction descriptor of kind::i8: signed 8-bit operands, both K-major, 32-bit integer sums.
+__host__ __device__ constexpr uint32_t i8_idesc(int M, int N)
+{
+	return (2u << 4) | (1u << 7) | (1u << 10) | (((uint32_t)N >> 3) << 17) | (((uint32_t)M >> 4) << 24);
+}
+
+// The products are issued by a whole warp, converged, and executed by its elected lane; conditions on their way are
+// votes or go by the launch's own numbers, so that the operands' descriptors live in the warp's uniform registers
+// (from a branch that one lane takes, a product cost about 200 cycles, whatever its size).
+__device__ __forceinline__ uint32_t elect_one()
+{
+	uint32_t r;
+	asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+	return r;
+}
+// D (+)= A B, both in shared memory: a, b the low words of their descriptors, `high` the word that they share.
+template <int GROUP>
+__device__ __forceinline__ void mma_i8(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t id, uint32_t acc, uint32_t lead)
+{
+	if constexpr (GROUP == 1)
+		asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+		             "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\t"
+		             "@q tcgen05.mma.cta_group::1.kind::i8 [%0], x, y, %4, p;\n\t}" ::"r"(d),
+		             "r"(a), "r"(b), "r"(high), "r"(id), "r"(acc), "r"(lead)
+		             : "memory");
+	else
+		asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+		             "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\t"
+		             "@q tcgen05.mma.cta_group::2.kind::i8 [%0], x, y, %4, p;\n\t}" ::"r"(d),
+		             "r"(a), "r"(b), "r"(high), "r"(id), "r"(acc), "r"(lead)
+		             : "memory");
+}
+// The products so far done: an arrival on the barrier, the pair's on the one at this place of both CTAs.
+template <int GROUP>
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead, uint16_t both = 0)
+{
+	if constexpr (GROUP == 1)
+		asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+		             "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+		             "r"(lead)
+		             : "memory");
+	else
+		asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+		             "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
+		                 smem_u32(bar)),
+		             "r"(lead), "h"(both)
+		             : "memory");
+}
+__device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+{
+	asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+	                 dst),
+	             "l"(map), "r"(x), "r"(y), "r"(bar)
+	             : "memory");
+}
+// ... whose barrier may be the other CTA's of the pair.
+__device__ __forceinline__ void tma2_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+{
+	asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+	             "[%4];" ::"r"(dst),
+	             "l"(map), "r"(x), "r"(y), "r"(bar)
+	             : "memory");
+}
+__device__ __forceinline__ void cluster_sync()
+{
+	asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of `addr` (this CTA's shared memory) in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank)
+{
+	uint32_t r;
+	asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+	return r;
+}
+__device__ __forceinline__ int4 ld_cluster4(uint32_t addr)
+{
+	int4 v;
+	asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+	return v;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar)
+{
+	asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, &g_i8_error, 1); }
+
+__device__ __forceinline__ uint32_t pow2_cols(uint32_t n) { return n <= 32 ? 32 : 1u << (32 - __clz(n - 1)); }
+
+// A channel's sums of C tokens from t on, scaled and out; `n` of them are real.
+template <int C>
+__device__ __forceinline__ void put(const Args& a, int t, int o, const int (&acc)[C], const float* xs, float ws, float bias, int n)
+{
+	float v[C];
+#pragma unroll
+	for (int c = 0; c < C; ++c) v[c] = fmaf(__int2float_rn(acc[c]) * xs[c], ws, bias);
+	if (a.add)
+	{
+		const float* p = a.add + (size_t)t * a.add_stride + o;
+#pragma unroll
+		for (int c = 0; c < C; ++c, p += a.add_stride)
+			if (c < n) v[c] += *p;
+	}
+	float* y = a.y + (size_t)t * a.y_stride + o;
+	if (n >= C)
+	{
+#pragma unroll
+		for (int c = 0; c < C; ++c, y += a.y_stride) *y = v[c];
+	}
+	else
+	{
+#pragma unroll
+		for (int c = 0; c < C; ++c, y += a.y_stride)
+			if (c < n) *y = v[c];
+	}
+}
+
+constexpr int THREADS = 320; // a warp for the loads, one for the products, eight for the epilogue (two to a quarter of TMEM)
+constexpr int EPI = 256;
+
+// The epilogue of a whole tile from TMEM: this warp's lanes (channels) and its half of the columns, out or, as sums
+// only, into `part` ([token][128 channels]).
+__device__ __forceinline__ void tile_out(const Args& a, uint32_t tmem, int ch, int o, int t0, int real, const float* xs, float ws,
+                                         float bias, int* part)
+{
+	const int side = ((int)threadIdx.x - 64) >> 7, quad = (threadIdx.x >> 5) & 3;
+	const bool in = o < a.rows;
+	for (int c0 = 16 * side; c0 < real; c0 += 32)
+	{
+		float f[16];
+		int v[16];
+		tmem_ld16(tmem + ((uint32_t)quad << 21) + c0, f);
+		tmem_wait_ld();
+#pragma unroll
+		for (int c = 0; c < 16; ++c) v[c] = __float_as_int(f[c]);
+		if (part)
+		{
+#pragma unroll
+			for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + ch] = v[c];
+		}
+		else if (in)
+			put<16>(a, t0 + c0, o, v, xs + c0, ws, bias, real - c0);
+	}
+}
+
+// The tokens first, first + step, ... of a tile from the sums of `n` CTAs of the cluster (CTA i's at rank0 + i * rank_step),
+// four channels a lane, a warp a token.
+__device__ __forceinline__ void join_out(const Args& a, const int* part, int rank0, int rank_step, int n, int first, int step, int o0,
+                                         int t0, int real, const float* xs)
+{
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, o = o0 + 4 * lane, left = a.rows - o;
+	float ws[4], bias[4];
+#pragma unroll
+	for (int j = 0; j < 4; ++j) ws[j] = j < left ? a.ws[o + j] : 0.0f, bias[j] = j < left && a.bias ? a.bias[o + j] : 0.0f;
+	uint32_t from[8];
+#pragma unroll
+	for (int i = 0; i < 8; ++i) from[i] = mapa(smem_u32(part) + 16 * lane, i < n ? rank0 + i * rank_step : rank0);
+	const bool wide = left >= 4 && a.y_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+	for (int c = first + step * warp; c < real; c += step * (THREADS / 32))
+	{
+		int4 q[8];
+#pragma unroll
+		for (int i = 0; i < 8; ++i) q[i] = i < n ? ld_cluster4(from[i] + c * 512) : make_int4(0, 0, 0, 0);
+		int4 sum = q[0];
+#pragma unroll
+		for (int i = 1; i < 8; ++i) sum.x += q[i].x, sum.y += q[i].y, sum.z += q[i].z, sum.w += q[i].w;
+		const int acc[4] = {sum.x, sum.y, sum.z, sum.w};
+		const int t = t0 + c;
+		float v[4];
+#pragma unroll
+		for (int j = 0; j < 4; ++j)
+		{
+			v[j] = fmaf(__int2float_rn(acc[j]) * xs[c], ws[j], bias[j]);
+			if (a.add && j < left) v[j] += a.add[(size_t)t * a.add_stride + o + j];
+		}
+		float* y = a.y + (size_t)t * a.y_stride + o;
+		if (wide)
+			*reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+		else
+#pragma unroll
+			for (int j = 0; j < 4; ++j)
+				if (j < left) y[j] = v[j];
+	}
+}
+
+// ---- few tokens ------------------------------------------------------------------------
+//
+// A cluster of `split` CTAs per tile of 128 channels x bn tokens, each with its
+// share of the columns; their sums meet in shared memory, every CTA adding up
+// the tokens t % split = its rank out of the others' (integers: no order).
+
+__global__ void __launch_bounds__(THREADS, 2)
+	i8_split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Args a)
+{
+	extern __shared__ uint8_t raw[];
+	__shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], done;
+	__shared__ uint32_t tmem_slot;
+	__shared__ float xs_s[256];
+	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	const int split = a.split, rank = (int)blockIdx.x % split; // (clusters lie along x)
+	const int o0 = (int)(blockIdx.x / split) * 128, t0 = (int)blockIdx.y * a.bn;
+	const int k0 = (int)((long long)a.n_kb * rank / split), n = (int)((long long)a.n_kb * (rank + 1) / split) - k0;
+	const uint32_t stage = W_BYTES + a.bn * KB, cols = pow2_cols(a.bn);
+	const int real = min(a.bn, a.n_tok - t0);
+
+	if (threadIdx.x == 0)
+	{
+		for (int s = 0; s < a.stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+		mbar_init(&done, 1);
+		fence_barrier_init();
+	}
+	if (warp == 1) tmem_alloc(&tmem_slot, cols);
+	tc_fence_before();
+	__syncthreads();
+	tc_fence_after();
+	const uint32_t tmem = tmem_slot;
+
+	if (warp == 0)
+	{
+		if (lane == 0)
+		{
+			int i = 0;
+			for (; i < n; ++i)
+			{
+				const int s = i % a.stages;
+				if (i >= a.stages && !wait(&empty[s], (uint32_t)(i / a.stages - 1) & 1)) break;
+				mbar_arrive_expect_tx(&full[s], stage);
+				const uint32_t dst = smem_u32(smem) + s * stage, bar = smem_u32(&full[s]);
+				tma2(dst, &wmap, (k0 + i) * KB, o0, bar);
+				tma2(dst + W_BYTES, &xmap, (k0 + i) * KB, t0, bar);
+			}
+			// a wait that ran out: what is in flight lands before the CTA ends
+			if (i < n)
+				for (int j = max(0, i - a.stages); j < i; ++j) wait(&full[j % a.stages], (uint32_t)(j / a.stages) & 1);
+		}
+		__syncwarp();
+	}
+	else if (warp == 1)
+	{
+		const uint32_t lead = elect_one(), id = i8_idesc(128, a.bn), high = (uint32_t)(sdesc(0, 16, 1024) >> 32);
+		for (int i = 0; i < n; ++i)
+		{
+			const int s = i % a.stages;
+			if (!__all_sync(0xffffffffu, wait(&full[s], (uint32_t)(i / a.stages) & 1))) break;
+			tc_fence_after();
+			const uint32_t at = smem_u32(smem) + s * stage;
+			const uint32_t da = (uint32_t)sdesc(at, 16, 1024), db = (uint32_t)sdesc(at + W_BYTES, 16, 1024);
+#pragma unroll
+			for (int k = 0; k < KB / 32; ++k) mma_i8<1>(tmem, da + 2 * k, db + 2 * k, high, id, i > 0 || k > 0, lead);
+			commit<1>(&empty[s], lead);
+			if (i == n - 1) commit<1>(&done, lead);
+		}
+	}
+	else
+	{
+		const int ch = (warp & 3) * 32 + lane, o = o0 + ch;
+		const bool in = o < a.rows && split == 1;
+		const float ws = in ? a.ws[o] : 0.0f, bias = in && a.bias ? a.bias[o] : 0.0f;
+		for (int c = (int)threadIdx.x - 64; c < a.bn; c += EPI) xs_s[c] = c < real ? a.xs[t0 + c] : 0.0f;
+		named_sync(1, EPI);
+		const bool ok = wait(&done, 0);
+		tc_fence_after();
+		if (__all_sync(0xffffffffu, ok)) tile_out(a, tmem, ch, o, t0, real, xs_s, ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
+		tc_fence_before();
+	}
+	__syncthreads();
+	if (split > 1)
+	{
+		cluster_sync();
+		join_out(a, reinterpret_cast<const int*>(smem), 0, 1, split, rank, split, o0, t0, real, xs_s);
+		cluster_sync(); // nobody reads this CTA's sums any more
+	}
+	if (warp == 1)
+	{
+		tc_fence_after();
+		tmem_dealloc(tmem, cols);
+	}
+}
+
+// ---- many tokens ------------------------------------------------------------------------
+//
+// One pair of CTAs per two SMs, walking tiles of 256 channels x bn tokens: each
+// CTA brings 128 of the channels and half of the tokens, and one product
+// (cta_group::2) of both SMs' tensor cores reads both. Two accumulators in TMEM:
+// the epilogue of a tile runs beside the next one's products.
+
+constexpr int P_GROUP = 8; // channel tiles that are walked together, so that their weights stay in L2
+
+__device__ __forceinline__ void pair_tile(const Args& a, int id, int& o0, int& t0)
+{
+	const int per = P_GROUP * a.tiles_t, g = id / per, in = id % per;
+	const int size = min(P_GROUP, a.tiles_o - g * P_GROUP);
+	o0 = (g * P_GROUP + in % size) * 256;
+	t0 = in / size * a.bn;
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+	i8_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Args a)
+{
+	extern __shared__ uint8_t raw[];
+	__shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
+	__shared__ uint32_t tmem_slot;
+	__shared__ float xs_s[2][256];
+	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	const int split = a.split, in_cluster = (int)blockIdx.x % (2 * split), rank = in_cluster & 1, first = in_cluster - rank, part = in_cluster >> 1;
+	const int pair = (int)blockIdx.x / (2 * split), pairs = (int)gridDim.x / (2 * split); // (clusters, where they are of more)
+	const int k0 = (int)((long long)a.n_kb * part / split), n_kb = (int)((long long)a.n_kb * (part + 1) / split) - k0;
+	const int tiles = a.tiles_o * a.tiles_t, half = a.bn / 2;
+	const uint32_t stage = W_BYTES + half * KB;
+
+	if (threadIdx.x == 0)
+	{
+		for (int s = 0; s < a.stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+		for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1), mbar_init(&acc_empty[b], 2 * EPI / 32);
+		fence_barrier_init();
+	}
+	if (warp == 1)
+	{
+		asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u)
+		             : "memory");
+		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+	}
+	tc_fence_before();
+	__syncthreads();
+	cluster_sync(); // both CTAs' barriers are there
+	tc_fence_after();
+	constexpr uint32_t tmem = 0; // (512 columns are all there are: the allocation starts at the first)
+
+	if (warp == 0)
+	{
+		if (lane == 0)
+		{
+			int i = 0; // stages so far
+			bool ok = true;
+			for (int id = pair; id < tiles && ok; id += pairs)
+			{
+				int o0, t0;
+				pair_tile(a, id, o0, t0);
+				for (int k = 0; k < n_kb; ++k, ++i)
+				{
+					const int s = i % a.stages;
+					if (i >= a.stages && !(ok = wait(&empty[s], (uint32_t)(i / a.stages - 1) & 1))) break;
+					if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * stage); // both CTAs' bytes land on the first one's barrier
+					const uint32_t dst = smem_u32(smem) + s * stage, bar = mapa(smem_u32(&full[s]), first);
+					tma2_pair(dst, &wmap, (k0 + k) * KB, o0 + rank * 128, bar);
+					tma2_pair(dst + W_BYTES, &xmap, (k0 + k) * KB, t0 + rank * half, bar);
+				}
+			}
+			if (!ok && rank == 0)
+				for (int j = max(0, i - a.stages); j < i; ++j) wait(&full[j % a.stages], (uint32_t)(j / a.stages) & 1);
+		}
+		__syncwarp();
+	}
+	else if (warp == 1)
+	{
+		if (rank == 0)
+		{
+			const uint32_t lead = elect_one(), idesc = i8_idesc(256, a.bn), high = (uint32_t)(sdesc(0, 16, 1024) >> 32);
+			const uint16_t both = (uint16_t)(3u << first);
+			int i = 0, n = 0;
+			bool ok = true;
+			for (int id = pair; id < tiles && ok; id += pairs, ++n)
+			{
+				const int b = n & 1;
+				if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait(&acc_empty[b], (uint32_t)(n / 2 - 1) & 1)))) break;
+				tc_fence_after();
+				for (int k = 0; k < n_kb; ++k, ++i)
+				{
+					const int s = i % a.stages;
+					if (!(ok = __all_sync(0xffffffffu, wait(&full[s], (uint32_t)(i / a.stages) & 1)))) break;
+					tc_fence_after();
+					const uint32_t at = smem_u32(smem) + s * stage;
+					const uint32_t da = (uint32_t)sdesc(at, 16, 1024), db = (uint32_t)sdesc(at + W_BYTES, 16, 1024);
+#pragma unroll
+					for (int q = 0; q < KB / 32; ++q) mma_i8<2>(tmem + b * 256, da + 2 * q, db + 2 * q, high, idesc, k > 0 || q > 0, lead);
+					commit<2>(&empty[s], lead, both);
+					if (k == n_kb - 1) commit<2>(&acc_full[b], lead, both);
+				}
+			}
+		}
+	}
+	else
+	{
+		const int ch = (warp & 3) * 32 + lane;
+		int n = 0;
+		bool ok = true; // (after a wait that ran out the warp goes on through the barriers, without work)
+		for (int id = pair; id < tiles; id += pairs, ++n)
+		{
+			const int b = n & 1;
+			int o0, t0;
+			pair_tile(a, id, o0, t0);
+			const int o = o0 + rank * 128 + ch, real = min(a.bn, a.n_tok - t0);
+			const bool in = o < a.rows && split == 1;
+			const float ws = in ? a.ws[o] : 0.0f, bias = in && a.bias ? a.bias[o] : 0.0f;
+			// (a warp is at most one tile behind another: the barrier below lets none two ahead)
+			for (int c = (int)threadIdx.x - 64; c < a.bn; c += EPI) xs_s[b][c] = c < real ? a.xs[t0 + c] : 0.0f;
+			named_sync(1, EPI);
+			ok = __all_sync(0xffffffffu, ok && wait(&acc_full[b], (uint32_t)(n / 2) & 1));
+			if (!ok) continue;
+			tc_fence_after();
+			tile_out(a, tmem + b * 256, ch, o, t0, real, xs_s[b], ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
+			tc_fence_before();
+			__syncwarp();
+			if (lane == 0) arrive_cluster(mapa(smem_u32(&acc_empty[b]), first));
+		}
+	}
+	__syncthreads();
+	cluster_sync(); // the other CTA's products read this one's memory, its epilogue arrives here
+	if (split > 1) // (one tile a cluster)
+	{
+		int o0, t0;
+		pair_tile(a, pair, o0, t0);
+		join_out(a, reinterpret_cast<const int*>(smem), rank, 2, split, part, split, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), xs_s[0]);
+		cluster_sync(); // nobody reads this CTA's sums any more
+	}
+	if (warp == 1)
+	{
+		tc_fence_after();
+		asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+	}
+}
+
+// ---- host ----------------------------------------------------------------------------------
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's tensor-map encoder, looked up through the runtime (the library loads without the driver).
+Encode encoder()
+{
+	static const Encode e = [] {
+		void* fn = nullptr;
+		cudaDriverEntryPointQueryResult q;
+		if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+		    q != cudaDriverEntryPointSuccess)
+			fn = nullptr;
+		return reinterpret_cast<Encode>(fn);
+	}();
+	return e;
+}
+
+// A map over n rows of `cols` codes, boxes of 128 codes x box rows, swizzled; past the edges it reads zeros.
+bool code_map(CUtensorMap* map, const int8_t* p, int n, int cols, size_t stride, int box)
+{
+	const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)n};
+	const cuuint64_t strides[1] = {n > 1 ? (cuuint64_t)stride : ((cuuint64_t)cols + 15) / 16 * 16};
+	const cuuint32_t boxes[2] = {KB, (cuuint32_t)box}, estr[2] = {1, 1};
+	const Encode e = encoder();
+	return e && e(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dims, strides, boxes, estr,
+	              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+	              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int SMEM_MOST = 216 * 1024;
+
+int configure()
+{
+	static bool configured[64] = {};
+	int dev = 0;
+	cudaError_t ce = cudaGetDevice(&dev);
+	if (ce != cudaSuccess) return (int)ce;
+	if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+	if (configured[dev]) return 0;
+	ce = cudaFuncSetAttribute(i8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
+	if (ce == cudaSuccess) ce = cudaFuncSetAttribute(i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
+	if (ce != cudaSuccess) return (int)ce;
+	configured[dev] = true;
+	return 0;
+}
+
+int up(int x, int m) { return (x + m - 1) / m * m; }
+
+} // namespace
+
+int launch_i8_linear(const nncu_i8_linear& l, void* stream)
+{
+	int e = configure();
+	if (e) return e;
+	constexpr int SMS = 148;
+	Args a{};
+	a.n_tok = l.n_tok, a.rows = l.rows, a.n_kb = (l.cols + KB - 1) / KB;
+	a.xs = l.x_scales, a.ws = l.w_scales, a.bias = l.bias, a.add = l.add, a.y = l.y;
+	a.add_stride = l.add_stride, a.y_stride = l.y_stride;
+	const char* f = getenv("I8_FORCE"); // kernel,bn,split,stages
+	int fk = -1, fb = 0, fs = 0, fst = 0;
+	if (f) sscanf(f, "%d,%d,%d,%d", &fk, &fb, &fs, &fst);
+	const bool pair = fk >= 0 ? fk : l.n_tok >= 256 && l.rows >= 256;
+	CUtensorMap xm, wm;
+	cudaLaunchConfig_t cfg{};
+	cfg.stream = static_cast<cudaStream_t>(stream);
+	if (pair)
+	{
+		a.bn = fb ? fb : 256;
+		a.tiles_o = (l.rows + 255) / 256, a.tiles_t = (l.n_tok + a.bn - 1) / a.bn;
+		const int stage = W_BYTES + a.bn / 2 * KB;
+		a.stages = fst ? fst : min(MAX_STAGES, (SMEM_MOST - 1024) / stage);
+		a.split = fs ? min(fs, a.n_kb) : 1;
+		if (!code_map(&xm, l.x, l.n_tok, l.cols, l.x_stride, a.bn / 2) || !code_map(&wm, l.w, l.rows, l.cols, l.w_stride, 128))
+			return (int)cudaErrorInvalidValue;
+		cudaLaunchAttribute at{};
+		at.id = cudaLaunchAttributeClusterDimension;
+		at.val.clusterDim.x = 2 * a.split, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+		cfg.attrs = &at;
+		cfg.numAttrs = 1;
+		const int tiles = a.tiles_o * a.tiles_t;
+		cfg.gridDim = dim3(2 * (a.split > 1 ? tiles * a.split : min(SMS / 2, tiles)));
+		cfg.blockDim = dim3(THREADS);
+		cfg.dynamicSmemBytes = max(a.stages * stage, a.split > 1 ? a.bn * 512 : 0) + 1024;
+		return (int)cudaLaunchKernelEx(&cfg, i8_pair_kernel, xm, wm, a);
+	}
+	const int tiles_o = (l.rows + 127) / 128;
+	const int parts = (l.n_tok + 255) / 256;
+	a.bn = fb ? fb : up((l.n_tok + parts - 1) / parts, 16);
+	const int tiles_t = (l.n_tok + a.bn - 1) / a.bn;
+	a.split = 1;
+	while (a.split < 8 && 2 * a.split <= a.n_kb && (long long)tiles_o * tiles_t * a.split * 2 <= SMS) a.split *= 2;
+	if (fs) a.split = min(fs, a.n_kb);
+	const int stage = W_BYTES + a.bn * KB;
+	a.stages = fst ? fst : min(MAX_STAGES, (a.bn <= 96 ? 106 * 1024 : SMEM_MOST - 1024) / stage);
+	if (!code_map(&xm, l.x, l.n_tok, l.cols, l.x_stride, a.bn) || !code_map(&wm, l.w, l.rows, l.cols, l.w_stride, 128))
+		return (int)cudaErrorInvalidValue;
+	cudaLaunchAttribute at{};
+	at.id = cudaLaunchAttributeClusterDimension;
+	at.val.clusterDim.x = a.split, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+	cfg.attrs = &at;
+	cfg.numAttrs = a.split > 1;
+	cfg.gridDim = dim3((unsigned)(tiles_o * a.split), (unsigned)tiles_t);
+	cfg.blockDim = dim3(THREADS);
+	cfg.dynamicSmemBytes = max(a.stages * stage, a.split > 1 ? a.bn * 512 : 0) + 1024;
+	return (int)cudaLaunchKernelEx(&cfg, i8_split_kernel, xm, wm, a);
+}
+
+int i8_error_word(int* word)
+{
+	cudaError_t ce = cudaMemcpyFromSymbol(word, g_i8_error, sizeof *word);
+	const int zero = 0;
+	if (ce == cudaSuccess && *word) ce = cudaMemcpyToSymbol(g_i8_error, &zero, sizeof zero);
+	return (int)ce;
+}
+
+} // namespace nncu
