@@ -539,8 +539,9 @@ int nncu_kv4_check(const nncu_kv4_attn* a, void* stream);
  * (int8) and one float scale, value = scale * code; hidden states have a scale
  * a token, weights one an output channel. Device pointers, asynchronous on
  * `stream`, no allocation, nothing kept between calls; the structs are filled
- * once. Rows of codes start on 16 bytes (base and code_stride); what lies
- * between two rows is neither read as values nor written. */
+ * once. Rows have up to 2^24 values; rows of codes start on 16 bytes (base and
+ * code_stride); what lies between two rows is neither read as values nor
+ * written. */
 
 /* Rows quantised, with the norm before a projection: z = x * gamma (a float
  * product; gamma NULL: x), s = max(max |z| / 127, 2^-126), code = z / s rounded
@@ -618,7 +619,7 @@ int nncu_i8_check(void* stream);
  * for logprob and rank). Device pointers, asynchronous on `stream`. */
 typedef struct nncu_logprobs
 {
-	int32_t n, n_vocab, top;
+	int32_t n, n_vocab, top; /* n_vocab: up to 2^30 */
 	float scale; /* above 0: one over the temperature */
 	const float* logits;
 	size_t stride;

@@ -16,74 +16,238 @@ namespace
 
 int refuse(const char* msg) { return set_error(NNCU_ERR_INVALID_ARGUMENT, msg); }
 
+constexpr int I8_COLS = 1 << 24; // the longest rows: their places stay far from 32 bits
 constexpr float I8_TINY = 1.17549435e-38f; // 2^-126: the least step of a row's codes
 
-template <typename T>
-__device__ __forceinline__ float block_reduce(float v, float* sm, T op)
+// ---- quantise -------------------------------------------------------------------------
+//
+// Reads each value once and writes a byte: bound by memory. A row stays in
+// the registers of `per_row` threads (16 values each, 16-byte loads) between
+// its maximum and its codes; longer rows than a CTA holds are read twice. The
+// squares of the norm are summed in 64 bits: float inputs' never overflow, and
+// the scale is rounded once.
+
+constexpr int Q_VALUES = 16; // a thread's values of a row (of a piece of it)
+
+// VEC values at i, zeros past the row's end; at once where the rows lie on 16 bytes.
+template <typename T, int VEC, bool ALIGNED>
+__device__ __forceinline__ void load_values(const T* x, int i, int cols, float* v)
 {
-	__syncthreads();
-	sm[threadIdx.x] = v;
-	__syncthreads();
-	for (int o = blockDim.x / 2; o > 0; o >>= 1)
+	if (ALIGNED && i + VEC <= cols)
 	{
-		if ((int)threadIdx.x < o) sm[threadIdx.x] = op(sm[threadIdx.x], sm[threadIdx.x + o]);
-		__syncthreads();
+		const uint4 q = *reinterpret_cast<const uint4*>(x + i);
+		if constexpr (sizeof(T) == 4)
+			v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
+		else
+		{
+			const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+			for (int j = 0; j < 4; ++j)
+			{
+				const float2 f = widen2(w[j], static_cast<const T*>(nullptr));
+				v[2 * j] = f.x, v[2 * j + 1] = f.y;
+			}
+		}
 	}
-	return sm[0];
+	else
+	{
+#pragma unroll
+		for (int j = 0; j < VEC; ++j) v[j] = i + j < cols ? load_elem(x + i + j) : 0.0f;
+	}
 }
 
-// x / s rounded to the nearest integer, ties to even, exactly. The product with the reciprocal is at most one off next
-// to a border; what is left of x then says which side it lies on (a fused multiply-add, exact here).
-__device__ __forceinline__ float i8_code(float x, float s)
+// x / s rounded to the nearest integer, ties to even, in the low byte: the product with the reciprocal is less than
+// 2^-15 off, so only next to a border does what is left of x, an exact fused multiply-add, decide.
+__device__ __forceinline__ uint32_t i8_code(float x, float s, float inv)
 {
-	float n = rintf(__fdiv_rn(x, s));
-	const float d = fmaf(-n, s, x), h = 0.5f * s;
-	if (d > h || (d == h && ((int)n & 1))) n += 1.0f;
-	if (d < -h || (d == -h && ((int)n & 1))) n -= 1.0f;
-	return n;
+	constexpr float MAGIC = 12582912.0f; // 1.5 * 2^23: the sum's low bits are the rounded integer
+	const float q = x * inv, t = q + MAGIC;
+	uint32_t c = __float_as_uint(t);
+	const float n = t - MAGIC;
+	if (fabsf(q - n) > 0.4999f)
+	{
+		const float d = fmaf(-n, s, x), h = 0.5f * s;
+		if (d > h || (d == h && (c & 1))) ++c;
+		if (d < -h || (d == -h && (c & 1))) --c;
+	}
+	return c;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) i8_quantise_kernel(const nncu_i8_rows r)
+// per_row threads of the CTA (x) take a row, blockDim.y rows a CTA; LOOP: rows longer than their threads hold.
+template <typename T, bool ALIGNED, bool LOOP>
+__global__ void __launch_bounds__(1024) i8_quantise_kernel(const nncu_i8_rows r)
 {
-	__shared__ float sm[256];
-	__shared__ double sum;
-	const size_t t = blockIdx.x;
-	const T* x = static_cast<const T*>(r.x) + t * r.x_stride;
+	constexpr int VEC = 16 / (int)sizeof(T), NV = Q_VALUES / VEC;
+	__shared__ float most_s[32];
+	__shared__ double sum_s[32];
+	const int tid = (int)threadIdx.x, per_row = (int)blockDim.x, warps = per_row / 32;
+	const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+	const bool live = row < r.n;
+	const T* x = static_cast<const T*>(r.x) + (size_t)(live ? row : 0) * r.x_stride;
+	const int piece = per_row * Q_VALUES, cols = live ? r.cols : 0;
+	float v[Q_VALUES];
 	float most = 0.0f;
-	double ss = 0.0;
+	double sum = 0.0;
 	bool bad = false;
-	for (int i = threadIdx.x; i < r.cols; i += 256)
+	const auto load = [&](int p0) {
+#pragma unroll
+		for (int k = 0; k < NV; ++k) load_values<T, VEC, ALIGNED>(x, p0 + (k * per_row + tid) * VEC, cols, v + k * VEC);
+	};
+	const auto gain = [&](int p0) {
+		if (!r.gamma) return;
+#pragma unroll
+		for (int k = 0; k < NV; ++k)
+#pragma unroll
+			for (int j = 0; j < VEC; j += 4)
+			{
+				float g[4];
+				load_values<float, 4, ALIGNED>(r.gamma, p0 + (k * per_row + tid) * VEC + j, cols, g);
+#pragma unroll
+				for (int i = 0; i < 4; ++i) v[k * VEC + j + i] *= g[i];
+			}
+	};
+	for (int p0 = 0; p0 < (LOOP ? cols : 1); p0 += piece)
 	{
-		const float v = load_elem(x + i), z = r.gamma ? v * r.gamma[i] : v;
-		most = fmaxf(most, fabsf(z));
-		bad |= !(fabsf(z) < INFINITY);
-		ss += (double)v * v;
+		load(p0);
+		if (r.norm)
+#pragma unroll
+			for (int j = 0; j < Q_VALUES; ++j) sum += (double)v[j] * v[j];
+		gain(p0);
+#pragma unroll
+		for (int j = 0; j < Q_VALUES; ++j)
+		{
+			most = fmaxf(most, fabsf(v[j]));
+			bad |= !(fabsf(v[j]) < INFINITY);
+		}
 	}
-	if (threadIdx.x == 0) sum = 0.0;
-	bad = __syncthreads_or(bad);
-	atomicAdd(&sum, ss);
-	most = block_reduce(most, sm, [](float a, float b) { return fmaxf(a, b); });
-	const float s = fmaxf(__fdiv_rn(most, 127.0f), I8_TINY);
-	const double mean = sum / r.cols + (double)r.eps;
-	if (threadIdx.x == 0)
-		r.scales[t] = bad ? NAN : r.norm && mean > 0.0 ? (float)((double)s / sqrt(mean)) : s;
-	int8_t* c = r.codes + t * r.code_stride;
-	for (int i = threadIdx.x; i < r.cols; i += 256)
+	if (bad) most = INFINITY; // (a maximum passes over NaN)
+	most = warp_max(most);
+	if (r.norm)
+#pragma unroll
+		for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+	if (warps > 1)
 	{
-		const float v = load_elem(x + i), z = r.gamma ? v * r.gamma[i] : v;
-		c[i] = bad ? 0 : (int8_t)(int)i8_code(z, s);
+		const int at = (int)threadIdx.y * warps; // (32 warps a CTA at most)
+		if (tid % 32 == 0) most_s[at + tid / 32] = most, sum_s[at + tid / 32] = sum;
+		__syncthreads();
+		sum = 0.0;
+		for (int w = 0; w < warps; ++w) most = fmaxf(most, most_s[at + w]);
+		if (tid == 0 && r.norm)
+			for (int w = 0; w < warps; ++w) sum += sum_s[at + w];
+	}
+	bad = !(most < INFINITY);
+	const float s = bad ? 1.0f : fmaxf(__fdiv_rn(most, 127.0f), I8_TINY), inv = bad ? 0.0f : __fdiv_rn(1.0f, s);
+	if (tid == 0 && live)
+	{
+		const double mean = sum / r.cols + (double)r.eps;
+		r.scales[row] = bad ? NAN : r.norm && mean > 0.0 ? (float)((double)s / sqrt(mean)) : s;
+	}
+	int8_t* c = r.codes + (size_t)(live ? row : 0) * r.code_stride;
+	for (int p0 = 0; p0 < (LOOP ? cols : 1); p0 += piece)
+	{
+		if (LOOP)
+		{
+			load(p0);
+			gain(p0);
+		}
+#pragma unroll
+		for (int k = 0; k < NV; ++k)
+		{
+			const int i = p0 + (k * per_row + tid) * VEC;
+			if (i >= cols) continue;
+			uint32_t w[VEC / 4];
+#pragma unroll
+			for (int q = 0; q < VEC / 4; ++q)
+			{
+				uint32_t b[4];
+#pragma unroll
+				for (int j = 0; j < 4; ++j) b[j] = bad ? 0u : i8_code(v[k * VEC + 4 * q + j], s, inv);
+				w[q] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+			}
+			if (i + VEC <= cols)
+			{
+				if constexpr (VEC == 4)
+					*reinterpret_cast<uint32_t*>(c + i) = w[0];
+				else
+					*reinterpret_cast<uint2*>(c + i) = make_uint2(w[0], w[1]);
+			}
+			else
+#pragma unroll
+				for (int j = 0; j < VEC; ++j)
+					if (i + j < cols) c[i + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
+		}
 	}
 }
 
-__global__ void __launch_bounds__(256) i8_lookup_kernel(const nncu_i8_lookup l)
+template <typename T>
+void launch_quantise(const nncu_i8_rows& r, cudaStream_t st)
 {
-	const size_t t = blockIdx.x;
-	const int id = l.ids ? l.ids[t] : (int)t;
+	const bool on16 = (reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.gamma)) % 16 == 0 &&
+	                  (r.n == 1 || r.x_stride * sizeof(T) % 16 == 0);
+	const int need = (r.cols + Q_VALUES - 1) / Q_VALUES, per_row = need > 1024 ? 1024 : (need + 31) / 32 * 32;
+	const int rows = per_row >= 128 ? 1 : 128 / per_row; // short rows: several to a CTA
+	const dim3 block(per_row, rows), grid((unsigned)(((long long)r.n + rows - 1) / rows));
+	if (need > 1024)
+	{
+		if (on16)
+			i8_quantise_kernel<T, true, true><<<grid, block, 0, st>>>(r);
+		else
+			i8_quantise_kernel<T, false, true><<<grid, block, 0, st>>>(r);
+	}
+	else if (on16)
+		i8_quantise_kernel<T, true, false><<<grid, block, 0, st>>>(r);
+	else
+		i8_quantise_kernel<T, false, false><<<grid, block, 0, st>>>(r);
+}
+
+// ---- look up ----------------------------------------------------------------------------
+//
+// Four bytes written for each one read: bound by the stores. A lane turns four
+// codes into one 16-byte store, so that a warp's is 512 bytes in a row; four
+// such loads are in flight a lane. A code becomes a float by putting it, as
+// code + 128, below the bits of 2^23 and taking 2^23 + 128 off again.
+
+constexpr int L_THREADS = 128, L_ITEMS = 4;
+
+template <bool ALIGNED>
+__global__ void __launch_bounds__(L_THREADS) i8_lookup_kernel(const nncu_i8_lookup l)
+{
+	const int t = (int)blockIdx.x;
+	const int id = l.ids ? l.ids[t] : t;
 	const bool in = id >= 0 && id < l.n_rows;
 	const float s = in ? l.scales[id] * l.mult : 0.0f;
 	const int8_t* c = l.codes + (size_t)(in ? id : 0) * l.code_stride;
-	for (int i = threadIdx.x; i < l.cols; i += 256) l.out[t * l.out_stride + i] = in ? s * (float)c[i] : 0.0f;
+	float* out = l.out + (size_t)t * l.out_stride;
+	const int i0 = ((int)blockIdx.y * L_ITEMS * L_THREADS + (int)threadIdx.x) * 4;
+	uint32_t w[L_ITEMS];
+#pragma unroll
+	for (int k = 0; k < L_ITEMS; ++k)
+	{
+		const int i = i0 + k * L_THREADS * 4;
+		w[k] = 0;
+		if (!in) continue;
+		if (i + 4 <= l.cols)
+			w[k] = *reinterpret_cast<const uint32_t*>(c + i);
+		else
+#pragma unroll
+			for (int j = 0; j < 4; ++j)
+				if (i + j < l.cols) w[k] |= (uint32_t)(uint8_t)c[i + j] << (8 * j);
+	}
+#pragma unroll
+	for (int k = 0; k < L_ITEMS; ++k)
+	{
+		const int i = i0 + k * L_THREADS * 4;
+		float v[4];
+#pragma unroll
+		for (int j = 0; j < 4; ++j)
+			v[j] = in ? s * (__uint_as_float(__byte_perm(w[k] ^ 0x80808080u, 0x4B000000u, 0x7540 + j)) - 8388736.0f) : 0.0f;
+		if (ALIGNED && i + 4 <= l.cols)
+			*reinterpret_cast<float4*>(out + i) = make_float4(v[0], v[1], v[2], v[3]);
+		else
+#pragma unroll
+			for (int j = 0; j < 4; ++j)
+				if (i + j < l.cols) out[i + j] = v[j];
+	}
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -138,7 +302,7 @@ using namespace nncu;
 extern "C" int nncu_i8_quantise_dev(const nncu_i8_rows* r, void* stream)
 {
 	if (!r) return refuse("i8 quantise: NULL argument");
-	if (r->n < 0 || r->cols <= 0) return refuse("i8 quantise: bad n or cols");
+	if (r->n < 0 || r->cols <= 0 || r->cols > I8_COLS) return refuse("i8 quantise: bad n or cols (up to 2^24)");
 	if (r->x_type != NNCU_KV_F32 && r->x_type != NNCU_KV_BF16 && r->x_type != NNCU_KV_F16)
 		return refuse("i8 quantise: unknown x_type");
 	if (r->norm && !(r->eps >= 0.0f && r->eps < INFINITY)) return refuse("i8 quantise: eps must be finite and not negative");
@@ -160,11 +324,11 @@ extern "C" int nncu_i8_quantise_dev(const nncu_i8_rows* r, void* stream)
 	if (rc != NNCU_OK) return rc;
 	const auto st = static_cast<cudaStream_t>(stream);
 	if (r->x_type == NNCU_KV_F32)
-		i8_quantise_kernel<float><<<r->n, 256, 0, st>>>(*r);
+		launch_quantise<float>(*r, st);
 	else if (r->x_type == NNCU_KV_BF16)
-		i8_quantise_kernel<__nv_bfloat16><<<r->n, 256, 0, st>>>(*r);
+		launch_quantise<__nv_bfloat16>(*r, st);
 	else
-		i8_quantise_kernel<__half><<<r->n, 256, 0, st>>>(*r);
+		launch_quantise<__half>(*r, st);
 	note_launches(1);
 	const int e = (int)cudaGetLastError();
 	return e ? set_cuda_error(e, "i8 quantise launch") : NNCU_OK;
@@ -173,7 +337,8 @@ extern "C" int nncu_i8_quantise_dev(const nncu_i8_rows* r, void* stream)
 extern "C" int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream)
 {
 	if (!l) return refuse("i8 lookup: NULL argument");
-	if (l->n < 0 || l->cols <= 0 || l->n_rows <= 0) return refuse("i8 lookup: bad n, cols or n_rows");
+	if (l->n < 0 || l->cols <= 0 || l->cols > I8_COLS || l->n_rows <= 0)
+		return refuse("i8 lookup: bad n, cols (up to 2^24) or n_rows");
 	if (!l->ids && l->n > l->n_rows) return refuse("i8 lookup: more rows than the table has, without ids");
 	if (!std::isfinite(l->mult)) return refuse("i8 lookup: mult must be finite");
 	if (l->n == 0) return NNCU_OK;
@@ -191,7 +356,12 @@ extern "C" int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream)
 		return refuse("i8 lookup: out must not meet another array");
 	const int rc = check_current_device(l->out, "i8 lookup");
 	if (rc != NNCU_OK) return rc;
-	i8_lookup_kernel<<<l->n, 256, 0, static_cast<cudaStream_t>(stream)>>>(*l);
+	const dim3 grid((unsigned)l->n, (unsigned)((l->cols + 4 * L_ITEMS * L_THREADS - 1) / (4 * L_ITEMS * L_THREADS)));
+	const auto st = static_cast<cudaStream_t>(stream);
+	if (aligned16(l->out) && (l->n == 1 || l->out_stride % 4 == 0))
+		i8_lookup_kernel<true><<<grid, L_THREADS, 0, st>>>(*l);
+	else
+		i8_lookup_kernel<false><<<grid, L_THREADS, 0, st>>>(*l);
 	note_launches(1);
 	const int e = (int)cudaGetLastError();
 	return e ? set_cuda_error(e, "i8 lookup launch") : NNCU_OK;

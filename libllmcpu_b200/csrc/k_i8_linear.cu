@@ -13,9 +13,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <cstdio>
-#include <cstdlib>
-
 #include "i8.h"
 #include "tc.cuh"
 
@@ -33,7 +30,7 @@ __device__ int g_i8_error; // the first bounded wait that ran out
 struct Args
 {
 	int n_tok, rows, bn, n_kb, stages, split;
-	int tiles_o, tiles_t; // of the pair kernel
+	int tiles_o, tiles_t;
 	const float* xs;
 	const float* ws;
 	const float* bias;
@@ -125,6 +122,10 @@ __device__ __forceinline__ int4 ld_cluster4(uint32_t addr)
 __device__ __forceinline__ void arrive_cluster(uint32_t bar)
 {
 	asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
+{
+	asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, &g_i8_error, 1); }
 
@@ -242,13 +243,15 @@ __global__ void __launch_bounds__(THREADS, 2)
 	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	const int split = a.split, rank = (int)blockIdx.x % split; // (clusters lie along x)
-	const int o0 = (int)(blockIdx.x / split) * 128, t0 = (int)blockIdx.y * a.bn;
+	const int tile = (int)(blockIdx.x / split), o0 = tile % a.tiles_o * 128, t0 = tile / a.tiles_o * a.bn;
 	const int k0 = (int)((long long)a.n_kb * rank / split), n = (int)((long long)a.n_kb * (rank + 1) / split) - k0;
 	const uint32_t stage = W_BYTES + a.bn * KB, cols = pow2_cols(a.bn);
 	const int real = min(a.bn, a.n_tok - t0);
 
 	if (threadIdx.x == 0)
 	{
+		prefetch_map(&wmap);
+		prefetch_map(&xmap);
 		for (int s = 0; s < a.stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
 		mbar_init(&done, 1);
 		fence_barrier_init();
@@ -258,6 +261,8 @@ __global__ void __launch_bounds__(THREADS, 2)
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = tmem_slot;
+	griddep_launch_dependents();
+	griddep_wait(); // what came before on the stream is done: up to here nothing was read that it may write
 
 	if (warp == 0)
 	{
@@ -355,6 +360,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 	if (threadIdx.x == 0)
 	{
+		prefetch_map(&wmap);
+		prefetch_map(&xmap);
 		for (int s = 0; s < a.stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
 		for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1), mbar_init(&acc_empty[b], 2 * EPI / 32);
 		fence_barrier_init();
@@ -370,6 +377,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 	cluster_sync(); // both CTAs' barriers are there
 	tc_fence_after();
 	constexpr uint32_t tmem = 0; // (512 columns are all there are: the allocation starts at the first)
+	griddep_launch_dependents();
+	griddep_wait();
 
 	if (warp == 0)
 	{
@@ -516,63 +525,66 @@ int configure()
 
 int up(int x, int m) { return (x + m - 1) / m * m; }
 
+constexpr int SMS = 148;
+
+struct Plan
+{
+	bool pair;
+	int bn, split, tiles_o, tiles_t;
+	int smem; // for the stages
+};
+
+Plan make_plan(int n_tok, int rows, int n_kb)
+{
+	Plan p{};
+	p.pair = n_tok >= 256 && rows >= 256;
+	const int parts = (n_tok + 255) / 256;
+	p.bn = p.pair ? 256 : up((n_tok + parts - 1) / parts, 16);
+	p.tiles_o = (rows + (p.pair ? 255 : 127)) / (p.pair ? 256 : 128);
+	p.tiles_t = (n_tok + p.bn - 1) / p.bn;
+	p.split = 1;
+	while (!p.pair && p.split < 8 && 2 * p.split <= n_kb && (long long)p.tiles_o * p.tiles_t * p.split * 2 <= SMS) p.split *= 2;
+	p.smem = p.pair || p.bn > 96 ? SMEM_MOST : 107 * 1024;
+	return p;
+}
+
 } // namespace
 
 int launch_i8_linear(const nncu_i8_linear& l, void* stream)
 {
 	int e = configure();
 	if (e) return e;
-	constexpr int SMS = 148;
 	Args a{};
 	a.n_tok = l.n_tok, a.rows = l.rows, a.n_kb = (l.cols + KB - 1) / KB;
 	a.xs = l.x_scales, a.ws = l.w_scales, a.bias = l.bias, a.add = l.add, a.y = l.y;
 	a.add_stride = l.add_stride, a.y_stride = l.y_stride;
-	const char* f = getenv("I8_FORCE"); // kernel,bn,split,stages
-	int fk = -1, fb = 0, fs = 0, fst = 0;
-	if (f) sscanf(f, "%d,%d,%d,%d", &fk, &fb, &fs, &fst);
-	const bool pair = fk >= 0 ? fk : l.n_tok >= 256 && l.rows >= 256;
+	const Plan p = make_plan(l.n_tok, l.rows, a.n_kb);
+	a.bn = p.bn, a.split = p.split;
+	const int stage = W_BYTES + (p.pair ? p.bn / 2 : p.bn) * KB;
+	a.stages = min(MAX_STAGES, (p.smem - 1024) / stage);
 	CUtensorMap xm, wm;
+	if (!code_map(&xm, l.x, l.n_tok, l.cols, l.x_stride, p.pair ? p.bn / 2 : p.bn) ||
+	    !code_map(&wm, l.w, l.rows, l.cols, l.w_stride, 128))
+		return (int)cudaErrorInvalidValue;
+	a.tiles_o = p.tiles_o, a.tiles_t = p.tiles_t;
+	cudaLaunchAttribute at[2]{};
+	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	at[0].val.programmaticStreamSerializationAllowed = 1;
+	at[1].id = cudaLaunchAttributeClusterDimension;
+	at[1].val.clusterDim.x = (p.pair ? 2 : 1) * p.split, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
 	cudaLaunchConfig_t cfg{};
 	cfg.stream = static_cast<cudaStream_t>(stream);
-	if (pair)
+	cfg.attrs = at;
+	cfg.numAttrs = at[1].val.clusterDim.x > 1 ? 2 : 1;
+	cfg.blockDim = dim3(THREADS);
+	cfg.dynamicSmemBytes = max(a.stages * stage, p.split > 1 ? p.bn * 512 : 0) + 1024;
+	const long long tiles = (long long)p.tiles_o * p.tiles_t;
+	if (p.pair)
 	{
-		a.bn = fb ? fb : 256;
-		a.tiles_o = (l.rows + 255) / 256, a.tiles_t = (l.n_tok + a.bn - 1) / a.bn;
-		const int stage = W_BYTES + a.bn / 2 * KB;
-		a.stages = fst ? fst : min(MAX_STAGES, (SMEM_MOST - 1024) / stage);
-		a.split = fs ? min(fs, a.n_kb) : 1;
-		if (!code_map(&xm, l.x, l.n_tok, l.cols, l.x_stride, a.bn / 2) || !code_map(&wm, l.w, l.rows, l.cols, l.w_stride, 128))
-			return (int)cudaErrorInvalidValue;
-		cudaLaunchAttribute at{};
-		at.id = cudaLaunchAttributeClusterDimension;
-		at.val.clusterDim.x = 2 * a.split, at.val.clusterDim.y = at.val.clusterDim.z = 1;
-		cfg.attrs = &at;
-		cfg.numAttrs = 1;
-		const int tiles = a.tiles_o * a.tiles_t;
-		cfg.gridDim = dim3(2 * (a.split > 1 ? tiles * a.split : min(SMS / 2, tiles)));
-		cfg.blockDim = dim3(THREADS);
-		cfg.dynamicSmemBytes = max(a.stages * stage, a.split > 1 ? a.bn * 512 : 0) + 1024;
+		cfg.gridDim = dim3(2 * (unsigned)(p.split > 1 ? tiles * p.split : min(tiles, (long long)SMS / 2)));
 		return (int)cudaLaunchKernelEx(&cfg, i8_pair_kernel, xm, wm, a);
 	}
-	const int tiles_o = (l.rows + 127) / 128;
-	const int parts = (l.n_tok + 255) / 256;
-	a.bn = fb ? fb : up((l.n_tok + parts - 1) / parts, 16);
-	const int tiles_t = (l.n_tok + a.bn - 1) / a.bn;
-	a.split = 1;
-	while (a.split < 8 && 2 * a.split <= a.n_kb && (long long)tiles_o * tiles_t * a.split * 2 <= SMS) a.split *= 2;
-	if (fs) a.split = min(fs, a.n_kb);
-	const int stage = W_BYTES + a.bn * KB;
-	a.stages = fst ? fst : min(MAX_STAGES, (a.bn <= 96 ? 106 * 1024 : SMEM_MOST - 1024) / stage);
-	if (!code_map(&xm, l.x, l.n_tok, l.cols, l.x_stride, a.bn) || !code_map(&wm, l.w, l.rows, l.cols, l.w_stride, 128))
-		return (int)cudaErrorInvalidValue;
-	cudaLaunchAttribute at{};
-	at.id = cudaLaunchAttributeClusterDimension;
-	at.val.clusterDim.x = a.split, at.val.clusterDim.y = at.val.clusterDim.z = 1;
-	cfg.attrs = &at;
-	cfg.numAttrs = a.split > 1;
-	cfg.gridDim = dim3((unsigned)(tiles_o * a.split), (unsigned)tiles_t);
-	cfg.blockDim = dim3(THREADS);
-	cfg.dynamicSmemBytes = max(a.stages * stage, a.split > 1 ? a.bn * 512 : 0) + 1024;
+	cfg.gridDim = dim3((unsigned)(tiles * p.split));
 	return (int)cudaLaunchKernelEx(&cfg, i8_split_kernel, xm, wm, a);
 }
 

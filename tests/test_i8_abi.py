@@ -35,7 +35,7 @@ def refused(rc, L, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(n=-1), "n or cols"), (dict(cols=0), "n or cols"), (dict(x_type=3), "x_type"), (dict(eps=-1.0), "eps"),
+    (dict(n=-1), "n or cols"), (dict(cols=0), "n or cols"), (dict(cols=(1 << 24) + 1), "cols"), (dict(x_type=3), "x_type"), (dict(eps=-1.0), "eps"),
     (dict(eps=float("nan")), "eps"), (dict(x=None), "NULL"), (dict(codes=None), "NULL"), (dict(scales=None), "NULL"),
     (dict(x=at(0) + 2), "aligned"), (dict(x=at(0) + 1, x_type=N.KV_BF16), "aligned"), (dict(gamma=at(3) + 2), "aligned"),
     (dict(codes=at(1) + 8), "16-byte"), (dict(code_stride=104), "16-byte"), (dict(code_stride=96), "strides"),
@@ -47,7 +47,7 @@ def test_quantise_refuses(L, change, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(n=-1), "bad n"), (dict(cols=0), "cols"), (dict(n_rows=0), "n_rows"), (dict(mult=float("inf")), "mult"),
+    (dict(n=-1), "bad n"), (dict(cols=0), "cols"), (dict(cols=(1 << 24) + 1), "cols"), (dict(n_rows=0), "n_rows"), (dict(mult=float("inf")), "mult"),
     (dict(codes=None), "NULL"), (dict(scales=None), "NULL"), (dict(out=None), "NULL"), (dict(ids=at(3) + 1), "aligned"),
     (dict(out=at(2) + 2), "aligned"), (dict(codes=at(0) + 4), "16-byte"), (dict(code_stride=100), "16-byte"),
     (dict(code_stride=96), "strides"), (dict(out_stride=99), "strides"), (dict(out_stride=1 << 61), "strides"),
@@ -73,7 +73,7 @@ def test_linear_refuses(L, change, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(n=-1), "bad n"), (dict(n_vocab=0), "n_vocab"), (dict(top=33), "top"), (dict(top=-1), "top"),
+    (dict(n=-1), "bad n"), (dict(n_vocab=0), "n_vocab"), (dict(n_vocab=(1 << 30) + 1), "n_vocab"), (dict(top=33), "top"), (dict(top=-1), "top"),
     (dict(top=5, n_vocab=4), "top"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(logits=None), "logits"),
     (dict(tokens=None), "tokens"), (dict(tokens=None, logprob=None), "tokens"),
