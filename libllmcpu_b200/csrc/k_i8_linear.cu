@@ -13,6 +13,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
+
 #include "i8.h"
 #include "tc.cuh"
 
@@ -21,15 +23,16 @@ namespace nncu
 namespace
 {
 
-constexpr int KB = 128;         // columns of a stage: one swizzled row
-constexpr int W_BYTES = 128 * KB; // a stage's 128 channels
+constexpr int KB = 128;           // columns of a panel: one swizzled row
+constexpr int W_BYTES = 128 * KB; // a panel's 128 channels
 constexpr int MAX_STAGES = 12;
 
 __device__ int g_i8_error; // the first bounded wait that ran out
 
 struct Args
 {
-	int n_tok, rows, bn, n_kb, stages, split;
+	int n_tok, rows, bn, n_kb, stages, split; // n_kb: stages of the columns
+	int panels; // of a stage: one or two
 	int tiles_o, tiles_t;
 	const float* xs;
 	const float* ws;
@@ -87,19 +90,28 @@ __device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead, uint16_t bo
 		             "r"(lead), "h"(both)
 		             : "memory");
 }
-__device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+// The copies are issued the same way. One box of a map into shared memory; in a pair (GROUP 2) the barrier may be the
+// other CTA's.
+template <int GROUP>
+__device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint32_t lead)
 {
-	asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-	                 dst),
-	             "l"(map), "r"(x), "r"(y), "r"(bar)
-	             : "memory");
+	if constexpr (GROUP == 1)
+		asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+		             "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+		             "l"(map), "r"(x), "r"(y), "r"(bar), "r"(lead)
+		             : "memory");
+	else
+		asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+		             "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(
+		                 dst),
+		             "l"(map), "r"(x), "r"(y), "r"(bar), "r"(lead)
+		             : "memory");
 }
-// ... whose barrier may be the other CTA's of the pair.
-__device__ __forceinline__ void tma2_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+__device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes, uint32_t lead)
 {
-	asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-	             "[%4];" ::"r"(dst),
-	             "l"(map), "r"(x), "r"(y), "r"(bar)
+	asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+	             "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+	             "r"(bytes), "r"(lead)
 	             : "memory");
 }
 __device__ __forceinline__ void cluster_sync()
@@ -128,6 +140,24 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
 	asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, &g_i8_error, 1); }
+
+// A place of the ring of stages and the round that it is in (a division by the number of stages costs as much as a stage).
+struct Ring
+{
+	int s = 0;
+	uint32_t round = 0;
+	__device__ __forceinline__ void next(int stages)
+	{
+		if (++s == stages) s = 0, ++round;
+	}
+};
+
+// After a wait that ran out: what is in flight lands before the CTA ends (the places behind `at`, a round of them).
+__device__ __forceinline__ void land(uint64_t* full, Ring at, int stages)
+{
+	for (int s = 0; s < stages; ++s)
+		if (s < at.s || at.round > 0) wait(&full[s], (s < at.s ? at.round : at.round - 1) & 1);
+}
 
 __device__ __forceinline__ uint32_t pow2_cols(uint32_t n) { return n <= 32 ? 32 : 1u << (32 - __clz(n - 1)); }
 
@@ -245,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 	const int split = a.split, rank = (int)blockIdx.x % split; // (clusters lie along x)
 	const int tile = (int)(blockIdx.x / split), o0 = tile % a.tiles_o * 128, t0 = tile / a.tiles_o * a.bn;
 	const int k0 = (int)((long long)a.n_kb * rank / split), n = (int)((long long)a.n_kb * (rank + 1) / split) - k0;
-	const uint32_t stage = W_BYTES + a.bn * KB, cols = pow2_cols(a.bn);
+	const uint32_t x_at = W_BYTES * a.panels, stage = x_at + a.bn * KB * a.panels, cols = pow2_cols(a.bn);
 	const int real = min(a.bn, a.n_tok - t0);
 
 	if (threadIdx.x == 0)
@@ -266,37 +296,43 @@ __global__ void __launch_bounds__(THREADS, 2)
 
 	if (warp == 0)
 	{
-		if (lane == 0)
+		const uint32_t lead = elect_one(), base = smem_u32(smem);
+		Ring at;
+		bool ok = true;
+		for (int i = 0; i < n; ++i, at.next(a.stages))
 		{
-			int i = 0;
-			for (; i < n; ++i)
+			if (at.round > 0 && !(ok = __all_sync(0xffffffffu, wait(&empty[at.s], (at.round - 1) & 1)))) break;
+			expect(&full[at.s], stage, lead);
+			const uint32_t dst = base + at.s * stage, bar = smem_u32(&full[at.s]);
+			const int k = (k0 + i) * KB * a.panels;
+			tma2<1>(dst, &wmap, k, o0, bar, lead);
+			tma2<1>(dst + x_at, &xmap, k, t0, bar, lead);
+			if (a.panels > 1) // (past the last column: zeros)
 			{
-				const int s = i % a.stages;
-				if (i >= a.stages && !wait(&empty[s], (uint32_t)(i / a.stages - 1) & 1)) break;
-				mbar_arrive_expect_tx(&full[s], stage);
-				const uint32_t dst = smem_u32(smem) + s * stage, bar = smem_u32(&full[s]);
-				tma2(dst, &wmap, (k0 + i) * KB, o0, bar);
-				tma2(dst + W_BYTES, &xmap, (k0 + i) * KB, t0, bar);
+				tma2<1>(dst + W_BYTES, &wmap, k + KB, o0, bar, lead);
+				tma2<1>(dst + x_at + a.bn * KB, &xmap, k + KB, t0, bar, lead);
 			}
-			// a wait that ran out: what is in flight lands before the CTA ends
-			if (i < n)
-				for (int j = max(0, i - a.stages); j < i; ++j) wait(&full[j % a.stages], (uint32_t)(j / a.stages) & 1);
 		}
+		if (!ok) land(full, at, a.stages);
 		__syncwarp();
 	}
 	else if (warp == 1)
 	{
 		const uint32_t lead = elect_one(), id = i8_idesc(128, a.bn), high = (uint32_t)(sdesc(0, 16, 1024) >> 32);
-		for (int i = 0; i < n; ++i)
+		const uint32_t base = (uint32_t)sdesc(smem_u32(smem), 16, 1024); // (the stages' addresses stay within its field)
+		Ring at;
+		for (int i = 0; i < n; ++i, at.next(a.stages))
 		{
-			const int s = i % a.stages;
-			if (!__all_sync(0xffffffffu, wait(&full[s], (uint32_t)(i / a.stages) & 1))) break;
+			if (!__all_sync(0xffffffffu, wait(&full[at.s], at.round & 1))) break;
 			tc_fence_after();
-			const uint32_t at = smem_u32(smem) + s * stage;
-			const uint32_t da = (uint32_t)sdesc(at, 16, 1024), db = (uint32_t)sdesc(at + W_BYTES, 16, 1024);
+			const uint32_t da = base + at.s * (stage >> 4), db = da + (x_at >> 4);
 #pragma unroll
 			for (int k = 0; k < KB / 32; ++k) mma_i8<1>(tmem, da + 2 * k, db + 2 * k, high, id, i > 0 || k > 0, lead);
-			commit<1>(&empty[s], lead);
+			if (a.panels > 1)
+#pragma unroll
+				for (int k = 0; k < KB / 32; ++k)
+					mma_i8<1>(tmem, da + (W_BYTES >> 4) + 2 * k, db + a.bn * (KB >> 4) + 2 * k, high, id, 1, lead);
+			commit<1>(&empty[at.s], lead);
 			if (i == n - 1) commit<1>(&done, lead);
 		}
 	}
@@ -356,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 	const int pair = (int)blockIdx.x / (2 * split), pairs = (int)gridDim.x / (2 * split); // (clusters, where they are of more)
 	const int k0 = (int)((long long)a.n_kb * part / split), n_kb = (int)((long long)a.n_kb * (part + 1) / split) - k0;
 	const int tiles = a.tiles_o * a.tiles_t, half = a.bn / 2;
-	const uint32_t stage = W_BYTES + half * KB;
+	const uint32_t x_at = W_BYTES * a.panels, stage = x_at + half * KB * a.panels;
 
 	if (threadIdx.x == 0)
 	{
@@ -382,27 +418,29 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 	if (warp == 0)
 	{
-		if (lane == 0)
+		const uint32_t lead = elect_one(), base = smem_u32(smem);
+		Ring at;
+		bool ok = true;
+		for (int id = pair; id < tiles && ok; id += pairs)
 		{
-			int i = 0; // stages so far
-			bool ok = true;
-			for (int id = pair; id < tiles && ok; id += pairs)
+			int o0, t0;
+			pair_tile(a, id, o0, t0);
+			for (int k = 0; k < n_kb; ++k, at.next(a.stages))
 			{
-				int o0, t0;
-				pair_tile(a, id, o0, t0);
-				for (int k = 0; k < n_kb; ++k, ++i)
+				if (at.round > 0 && !(ok = __all_sync(0xffffffffu, wait(&empty[at.s], (at.round - 1) & 1)))) break;
+				if (rank == 0) expect(&full[at.s], 2 * stage, lead); // both CTAs' bytes land on the first one's barrier
+				const uint32_t dst = base + at.s * stage, bar = mapa(smem_u32(&full[at.s]), first);
+				const int c = (k0 + k) * KB * a.panels;
+				tma2<2>(dst, &wmap, c, o0 + rank * 128, bar, lead);
+				tma2<2>(dst + x_at, &xmap, c, t0 + rank * half, bar, lead);
+				if (a.panels > 1)
 				{
-					const int s = i % a.stages;
-					if (i >= a.stages && !(ok = wait(&empty[s], (uint32_t)(i / a.stages - 1) & 1))) break;
-					if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * stage); // both CTAs' bytes land on the first one's barrier
-					const uint32_t dst = smem_u32(smem) + s * stage, bar = mapa(smem_u32(&full[s]), first);
-					tma2_pair(dst, &wmap, (k0 + k) * KB, o0 + rank * 128, bar);
-					tma2_pair(dst + W_BYTES, &xmap, (k0 + k) * KB, t0 + rank * half, bar);
+					tma2<2>(dst + W_BYTES, &wmap, c + KB, o0 + rank * 128, bar, lead);
+					tma2<2>(dst + x_at + half * KB, &xmap, c + KB, t0 + rank * half, bar, lead);
 				}
 			}
-			if (!ok && rank == 0)
-				for (int j = max(0, i - a.stages); j < i; ++j) wait(&full[j % a.stages], (uint32_t)(j / a.stages) & 1);
 		}
+		if (!ok && rank == 0) land(full, at, a.stages);
 		__syncwarp();
 	}
 	else if (warp == 1)
@@ -411,23 +449,27 @@ __global__ void __launch_bounds__(THREADS, 1)
 		{
 			const uint32_t lead = elect_one(), idesc = i8_idesc(256, a.bn), high = (uint32_t)(sdesc(0, 16, 1024) >> 32);
 			const uint16_t both = (uint16_t)(3u << first);
-			int i = 0, n = 0;
+			const uint32_t base = (uint32_t)sdesc(smem_u32(smem), 16, 1024); // (the stages' addresses stay within its field)
+			Ring at;
+			int n = 0;
 			bool ok = true;
 			for (int id = pair; id < tiles && ok; id += pairs, ++n)
 			{
 				const int b = n & 1;
 				if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait(&acc_empty[b], (uint32_t)(n / 2 - 1) & 1)))) break;
 				tc_fence_after();
-				for (int k = 0; k < n_kb; ++k, ++i)
+				for (int k = 0; k < n_kb; ++k, at.next(a.stages))
 				{
-					const int s = i % a.stages;
-					if (!(ok = __all_sync(0xffffffffu, wait(&full[s], (uint32_t)(i / a.stages) & 1)))) break;
+					if (!(ok = __all_sync(0xffffffffu, wait(&full[at.s], at.round & 1)))) break;
 					tc_fence_after();
-					const uint32_t at = smem_u32(smem) + s * stage;
-					const uint32_t da = (uint32_t)sdesc(at, 16, 1024), db = (uint32_t)sdesc(at + W_BYTES, 16, 1024);
+					const uint32_t da = base + at.s * (stage >> 4), db = da + (x_at >> 4);
 #pragma unroll
 					for (int q = 0; q < KB / 32; ++q) mma_i8<2>(tmem + b * 256, da + 2 * q, db + 2 * q, high, idesc, k > 0 || q > 0, lead);
-					commit<2>(&empty[s], lead, both);
+					if (a.panels > 1)
+#pragma unroll
+						for (int q = 0; q < KB / 32; ++q)
+							mma_i8<2>(tmem + b * 256, da + (W_BYTES >> 4) + 2 * q, db + half * (KB >> 4) + 2 * q, high, idesc, 1, lead);
+					commit<2>(&empty[at.s], lead, both);
 					if (k == n_kb - 1) commit<2>(&acc_full[b], lead, both);
 				}
 			}
@@ -523,29 +565,65 @@ int configure()
 	return 0;
 }
 
-int up(int x, int m) { return (x + m - 1) / m * m; }
-
 constexpr int SMS = 148;
 
 struct Plan
 {
 	bool pair;
-	int bn, split, tiles_o, tiles_t;
+	int bn, split, panels, tiles_o, tiles_t;
 	int smem; // for the stages
 };
 
+// Which kernel, how many tokens a tile, over how many CTAs (pairs) a tile's columns are split, one or two panels a
+// stage, one CTA per SM or two (of half the memory): the least of an estimate in SM cycles. Its constants were
+// fitted to 6700 timings of 140 shapes (1 to 4096 tokens, 128 to 262144 channels, 300 to 16384 columns, weights from
+// HBM); the choices it makes there are 3 % slower than the best of all in the mean, 19 % at worst. What they stand for:
+//  - a stage costs the issue of its copies and products (one panel 500, two together 110 a panel: the second panel's
+//    go along), its products (a pair's 210 + 1.5 a token, a single CTA's the fourth of which is 57 or 44 + 0.36 a
+//    token), its bytes into an SM (62 a cycle) or, over all SMs, out of L2 (8000 a cycle);
+//  - clusters of 4 and more do not fill every SM;
+//  - a launch's start and end, the epilogue by token, and the joining of a split tile through shared memory.
+// Both sides, microseconds: 1 token, 6144 channels, 4096 columns: whole columns, two panels 7.5, one panel 8.8, split
+// over four 8.3; 1 x 2560 x 10240: split over eight 8.1, whole 12.0; 777 x 2560 x 2048: single CTAs 7.7, pairs 8.6;
+// 1024 x 6144 x 4096: pairs 22.9, single CTAs 30.4.
 Plan make_plan(int n_tok, int rows, int n_kb)
 {
-	Plan p{};
-	p.pair = n_tok >= 256 && rows >= 256;
-	const int parts = (n_tok + 255) / 256;
-	p.bn = p.pair ? 256 : up((n_tok + parts - 1) / parts, 16);
-	p.tiles_o = (rows + (p.pair ? 255 : 127)) / (p.pair ? 256 : 128);
-	p.tiles_t = (n_tok + p.bn - 1) / p.bn;
-	p.split = 1;
-	while (!p.pair && p.split < 8 && 2 * p.split <= n_kb && (long long)p.tiles_o * p.tiles_t * p.split * 2 <= SMS) p.split *= 2;
-	p.smem = p.pair || p.bn > 96 ? SMEM_MOST : 107 * 1024;
-	return p;
+	// how many clusters run at once with one CTA per SM and with two, by CTAs of a cluster
+	static const int alone[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15}, both[9] = {0, 296, 148, 93, 71, 56, 45, 37, 33};
+	Plan best{};
+	double least = 0;
+	const auto consider = [&](bool pair, int bn, int split, int panels, bool two) {
+		const int stage = (W_BYTES + (pair ? bn / 2 : bn) * KB) * panels, smem = two ? 107 * 1024 : SMEM_MOST;
+		const int ctas = (pair ? 2 : 1) * split;
+		if (split * panels > n_kb || (smem - 1024) / stage < 2 || (panels > 1 && (smem - 1024) / stage < 3)) return;
+		const long long tiles_o = (rows + (pair ? 255 : 127)) / (pair ? 256 : 128), tiles_t = (n_tok + bn - 1) / bn, tiles = tiles_o * tiles_t;
+		const long long slots = two ? both[ctas] : alone[ctas];
+		if ((two || split > 1) && tiles > 2 * slots && split > 1) return;
+		const double waves = (double)((tiles + slots - 1) / slots), active = (double)((tiles < slots ? tiles : slots) * ctas);
+		const double per_sm = two && tiles > alone[ctas] ? 2 : 1;
+		const double bytes = (128 + (pair ? bn / 2 : bn)) * 128.0;
+		const double issue = panels > 1 ? 110 : 500;
+		const double products = pair ? 210 + 1.5 * bn : 4 * fmax(57.0, 44 + 0.36 * bn) * per_sm;
+		const double load = fmax(bytes * per_sm / 62, active * bytes / 8000);
+		const double columns = (double)((n_kb + split - 1) / split) * fmax(fmax(issue, products), load);
+		double t = fmax(waves * columns, (double)rows * n_kb * KB / 3300) + (pair ? 6300 : 5400) + 12.0 * bn * waves * (split > 1 ? 0.5 : 1);
+		if (split > 1) t += 3600 + 77 * bn;
+		if (best.bn == 0 || t < least)
+		{
+			least = t;
+			best = {pair, bn, split, panels, (int)tiles_o, (int)tiles_t, smem};
+		}
+	};
+	const int most = n_tok < 256 ? (n_tok + 15) / 16 * 16 : 256;
+	for (int bn = 16; bn <= most; bn += 16)
+		for (int split = 1; split <= 8; split *= 2)
+			for (int panels = 1; panels <= 2; ++panels)
+				for (int two = 0; two < 2; ++two) consider(false, bn, split, panels, two);
+	if (n_tok > 32 && rows > 128)
+		for (int bn = 64; bn <= (most + 31) / 32 * 32; bn += 32)
+			for (int split = 1; split <= 4; ++split)
+				for (int panels = 1; panels <= 2; ++panels) consider(true, bn, split, panels, false);
+	return best;
 }
 
 } // namespace
@@ -555,12 +633,12 @@ int launch_i8_linear(const nncu_i8_linear& l, void* stream)
 	int e = configure();
 	if (e) return e;
 	Args a{};
-	a.n_tok = l.n_tok, a.rows = l.rows, a.n_kb = (l.cols + KB - 1) / KB;
+	a.n_tok = l.n_tok, a.rows = l.rows;
 	a.xs = l.x_scales, a.ws = l.w_scales, a.bias = l.bias, a.add = l.add, a.y = l.y;
 	a.add_stride = l.add_stride, a.y_stride = l.y_stride;
-	const Plan p = make_plan(l.n_tok, l.rows, a.n_kb);
-	a.bn = p.bn, a.split = p.split;
-	const int stage = W_BYTES + (p.pair ? p.bn / 2 : p.bn) * KB;
+	const Plan p = make_plan(l.n_tok, l.rows, (l.cols + KB - 1) / KB);
+	a.bn = p.bn, a.split = p.split, a.panels = p.panels, a.n_kb = (l.cols + KB * p.panels - 1) / (KB * p.panels);
+	const int stage = (W_BYTES + (p.pair ? p.bn / 2 : p.bn) * KB) * p.panels;
 	a.stages = min(MAX_STAGES, (p.smem - 1024) / stage);
 	CUtensorMap xm, wm;
 	if (!code_map(&xm, l.x, l.n_tok, l.cols, l.x_stride, p.pair ? p.bn / 2 : p.bn) ||
