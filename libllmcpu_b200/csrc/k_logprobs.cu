@@ -21,6 +21,7 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "nncu.h"
@@ -35,20 +36,21 @@ __device__ __forceinline__ void cluster_sync()
 	asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The generic address of `p` (this CTA's shared memory) in the cluster's CTA `rank`.
-__device__ __forceinline__ const void* cluster_map(const void* p, int rank)
+__device__ __forceinline__ void* cluster_map(const void* p, int rank)
 {
 	uint64_t r;
 	asm volatile("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
-	return reinterpret_cast<const void*>(r);
+	return reinterpret_cast<void*>(r);
 }
 
 int refuse(const char* msg) { return set_error(NNCU_ERR_INVALID_ARGUMENT, msg); }
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32, LP_TOP = 32;
-constexpr int LP_ITEMS = 4;                      // 16-byte loads a thread has in flight
-constexpr int LP_GROUP = LP_THREADS * LP_ITEMS;  // vectors (of four logits) that the CTA takes at a time
-constexpr int LP_CLUSTER = 8;                    // the most CTAs that share a row
-constexpr int LP_FOUND = LP_TOP * 4 * LP_ITEMS + LP_WARPS * LP_TOP;
+constexpr int LP_TOP = 32;
+constexpr int LP_ITEMS = 4;   // 16-byte loads a thread has in flight
+constexpr int LP_CLUSTER = 8; // the most CTAs that share a row
+constexpr int LP_FIRST = 4;   // of each warp's candidates, those that bound the others
+constexpr int LP_WIDE = 512, LP_NARROW = 256;      // threads of a CTA: where rows are few, and where they are many
+constexpr int LP_WIDE_CTAS = 2, LP_NARROW_CTAS = 5; // per SM
 
 using Key = unsigned long long;
 
@@ -116,10 +118,10 @@ struct LpArgs
 {
 	nncu_logprobs l;
 	float k; // scale / ln 2
-	int parts;
+	int parts; // CTAs that share a row
 };
 
-// What a CTA hands to the one that finishes its row.
+// What a CTA knows of its part of a row.
 struct Part
 {
 	Key top[LP_TOP];
@@ -127,77 +129,260 @@ struct Part
 	int before;
 };
 
-template <bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const LpArgs a)
+// Two floats' sum, and product and sum, in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
 {
-	__shared__ Part mine;
-	__shared__ Stat warp_stat[LP_WARPS];
-	__shared__ int warp_before[LP_WARPS];
-	__shared__ Key lists[TOP ? LP_WARPS : 1][LP_TOP], found[TOP ? LP_FOUND : 1];
-	__shared__ int n_found, n_again;
-	__shared__ short again[TOP ? LP_TOP : 1];
-	const nncu_logprobs& l = a.l;
-	const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	const int part = (int)(blockIdx.x % a.parts);
-	const size_t r = blockIdx.x / a.parts;
-	const int n = l.n_vocab;
-	const float* x = l.logits + r * l.stride;
-	// Vectors of four logits lie on 16 bytes: the row's first and last one may be cut.
-	const int cut = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
-	const float* base = x - cut;
-	const int nvec = (n + cut + 3) / 4, each = (nvec + a.parts - 1) / a.parts;
-	const int v0 = min(nvec, part * each), v1 = min(nvec, v0 + each);
-	const float k = a.k;
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+	return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+	    "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+	return r;
+}
 
-	const int tok = l.tokens ? l.tokens[r] : -1;
-	const bool in = tok >= 0 && tok < n;
-	const float xt = in ? x[tok] : 0.0f;
-	const bool hidden = in && !(xt > -INFINITY);      // (a NaN comes as -infinity)
-	const float below = nextafterf(xt, -INFINITY);    // x >= xt is x > below
-	const int tok_vec = in ? (tok + cut) / 4 : -1;
-
-	const auto load = [&](int j) {
-		if (j > 0 && j < nvec - 1) return __ldg(reinterpret_cast<const float4*>(base) + j);
+// A row's share of one CTA, in vectors of four logits that lie on 16 bytes: the row's first and last one may be cut.
+struct Share
+{
+	const float* x;
+	int n, cut, nvec, v0, v1;
+	__device__ __forceinline__ Share(const nncu_logprobs& l, size_t r, int part, int parts) : x(l.logits + r * l.stride), n(l.n_vocab)
+	{
+		cut = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
+		nvec = (n + cut + 3) / 4;
+		const int each = (nvec + parts - 1) / parts;
+		v0 = min(nvec, part * each), v1 = min(nvec, v0 + each);
+	}
+	__device__ __forceinline__ const float4* at(int j) const { return reinterpret_cast<const float4*>(x - cut) + j; }
+	__device__ __forceinline__ bool whole(int j) const { return j > 0 && j < nvec - 1 && j < v1; }
+	__device__ __forceinline__ int index(int j, int c) const { return 4 * j + c - cut; }
+	// what is not the share's reads as masked
+	__device__ __forceinline__ float4 load(int j) const
+	{
+		if (whole(j)) return __ldg(at(j));
 		float v[4];
 #pragma unroll
 		for (int c = 0; c < 4; ++c)
 		{
-			const int i = 4 * j + c - cut;
-			v[c] = i >= 0 && i < n ? __ldg(x + i) : -INFINITY;
+			const int i = index(j, c);
+			v[c] = j < v1 && i >= 0 && i < n ? __ldg(x + i) : -INFINITY;
 		}
 		return make_float4(v[0], v[1], v[2], v[3]);
-	};
+	}
+};
 
-	Stat s{-FLT_MAX, 0.0f, 0.0f};
-	int before = 0;
-	float best = -INFINITY, second = -INFINITY; // the largest of the thread's groups, and of the others
-	int best_at = v0;
-	for (int g = v0; g < v1; g += LP_GROUP)
-	{
-		float4 q[LP_ITEMS];
-		if (g > 0 && g + LP_GROUP <= v1 && g + LP_GROUP < nvec)
-		{
+// A thread's largest logits of its share: what the selection goes by.
+struct Best
+{
+	float value, second; // of all groups; of the groups but the one that reached the largest first
+	int group;
+};
+
+template <int T>
+struct Found
+{
+	static constexpr int WARPS = T / 32, MOST = LP_TOP * 4 * LP_ITEMS + WARPS * LP_TOP;
+	Key keys[MOST], bound[WARPS * LP_FIRST], lists[WARPS][LP_TOP], least;
+	int n, n_again;
+	short again[T];
+};
+
+// The likeliest tokens of the CTA's share into top[LP_TOP], falling (0: none).
+template <int T>
+__device__ __forceinline__ void lp_select(const Share& sh, const Best& b, int top, Found<T>& f, Key* out)
+{
+	constexpr int WARPS = Found<T>::WARPS, MOST = Found<T>::MOST;
+	const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	// The thread's first candidate: the first of its largest logits, in the group that reached them first.
+	float v[4 * LP_ITEMS];
 #pragma unroll
-			for (int u = 0; u < LP_ITEMS; ++u) q[u] = __ldg(reinterpret_cast<const float4*>(base) + g + u * LP_THREADS + tid);
-		}
+	for (int u = 0; u < LP_ITEMS; ++u)
+	{
+		const float4 q = b.value > -INFINITY ? sh.load(b.group + u * T + tid) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+		v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
+	}
+	const auto index = [&](int i) { return sh.index(b.group + (i / 4) * T + tid, i % 4); };
+	Key first = 0;
+#pragma unroll
+	for (int i = 4 * LP_ITEMS - 1; i >= 0; --i)
+		if (v[i] == b.value) first = lp_key(b.value, index(i));
+	// The warp's first few of those, one after another.
+	Key left = first;
+#pragma unroll
+	for (int i = 0; i < LP_FIRST; ++i)
+	{
+		const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32));
+		const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32) == hi ? (uint32_t)left : 0u);
+		const Key k = (Key)hi << 32 | lo;
+		if (left == k) left = 0;
+		if (lane == 0) f.bound[warp * LP_FIRST + i] = k;
+	}
+	if (tid == 0) f.n = f.n_again = 0, f.least = 0;
+	if (tid < LP_TOP) out[tid] = 0;
+	__syncthreads();
+	// The top-th of them is a bound: that many tokens are not after it.
+	if (tid < WARPS * LP_FIRST)
+	{
+		const Key k = f.bound[tid];
+		int above = 0;
+#pragma unroll 8
+		for (int j = 0; j < WARPS * LP_FIRST; ++j) above += f.bound[j] > k;
+		if (k != 0 && above == top - 1) f.least = k;
+	}
+	__syncthreads();
+	// What is not after it lies with the threads whose first is not, nearly always in that one's group.
+	Key least = f.least;
+	const auto push = [&](Key k) {
+		const int i = atomicAdd(&f.n, 1);
+		if (i < MOST) f.keys[i] = k;
+	};
+	const auto owners = [&]() {
+		if (first == 0 || first < least) return;
+		if (least == 0 ? b.second > -INFINITY : b.second >= lp_value(least)) // more may lie in the thread's other groups
+			f.again[atomicAdd(&f.n_again, 1)] = (short)tid;
 		else
+		{
+			push(first);
+			const float low = lp_value(least);
+			int more = 0;
+#pragma unroll
+			for (int i = 0; i < 4 * LP_ITEMS; ++i) more += least == 0 ? v[i] > -INFINITY : v[i] >= low;
+			if (more > 1)
+#pragma unroll
+				for (int i = 0; i < 4 * LP_ITEMS; ++i)
+				{
+					const Key k = lp_key(v[i], index(i));
+					if (k != 0 && k != first && k >= least) push(k);
+				}
+		}
+	};
+	owners();
+	__syncthreads();
+	for (int w = warp; w < f.n_again; w += WARPS) // those threads' vectors once more, a warp a thread
+		for (int j = sh.v0 + f.again[w] + lane * T; j < sh.v1; j += 32 * T)
+		{
+			const float4 q = sh.load(j);
+			const float e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+			for (int c = 0; c < 4; ++c)
+			{
+				const Key k = lp_key(e[c], sh.index(j, c));
+				if (k != 0 && k >= least) push(k);
+			}
+		}
+	__syncthreads();
+	if (f.n > MOST)
+	{
+		// Too many: few warps hold the largest, or most of the row is equal. The top-th of all threads' firsts bounds the
+		// owners to `top` of them, and a warp's list what it takes of each.
+		Key list = lp_sort(first, lane);
+		f.lists[warp][lane] = list;
+		__syncthreads();
+		for (int d = WARPS / 2; d > 0; d /= 2)
+		{
+			if (warp < d) f.lists[warp][lane] = list = lp_merge(list, f.lists[warp + d][lane], lane);
+			__syncthreads();
+		}
+		least = f.lists[0][top - 1];
+		if (tid == 0) f.n = f.n_again = 0;
+		__syncthreads();
+		owners();
+		__syncthreads();
+		list = 0;
+		for (int w = warp; w < f.n_again; w += WARPS)
+			for (int j0 = sh.v0 + f.again[w]; j0 < sh.v1; j0 += 32 * T)
+			{
+				const float4 q = sh.load(j0 + lane * T);
+				const float e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+				for (int c = 0; c < 4; ++c)
+				{
+					Key k = lp_key(e[c], sh.index(j0 + lane * T, c));
+					if (k < least) k = 0;
+					if (__any_sync(0xffffffffu, k != 0)) list = lp_merge(list, lp_sort(k, lane), lane);
+				}
+			}
+		if (list != 0) push(list);
+		__syncthreads();
+	}
+	const int n = f.n;
+	for (int i = tid; i < n; i += T)
+	{
+		const Key k = f.keys[i];
+		int above = 0;
+#pragma unroll 4
+		for (int j = 0; j < n; ++j) above += f.keys[j] > k;
+		if (above < LP_TOP) out[above] = k;
+	}
+}
+
+template <bool TOP, int T>
+__global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTAS) logprobs_kernel(const LpArgs a)
+{
+	constexpr int WARPS = T / 32, GROUP = T * LP_ITEMS; // vectors (of four logits) that the CTA takes at a time
+	__shared__ Part parts[LP_CLUSTER]; // this CTA's own at its number; the first CTA of a cluster gets the others'
+	__shared__ Stat warp_stat[WARPS];
+	__shared__ int warp_before[WARPS];
+	__shared__ std::conditional_t<TOP, Found<T>, int> found;
+	const nncu_logprobs& l = a.l;
+	const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	const int part = (int)(blockIdx.x % a.parts);
+	const size_t r = blockIdx.x / a.parts;
+	const float k = a.k;
+	griddep_launch_dependents();
+	if (a.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); // (its end is waited for below: all have begun)
+	griddep_wait();
+
+	const Share sh(l, r, part, a.parts);
+	float v[4 * LP_ITEMS];
+	const auto read = [&](int g) {
+		if (g > 0 && g + GROUP < sh.nvec && g + GROUP <= sh.v1)
 		{
 #pragma unroll
 			for (int u = 0; u < LP_ITEMS; ++u)
 			{
-				const int j = g + u * LP_THREADS + tid;
-				q[u] = j < v1 ? load(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+				const float4 q = __ldg(sh.at(g + u * T + tid));
+				v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
 			}
 		}
+		else
+#pragma unroll
+			for (int u = 0; u < LP_ITEMS; ++u)
+			{
+				const float4 q = sh.load(g + u * T + tid);
+				v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
+			}
+	};
+	read(sh.v0); // (before the token's own logit, which waits for two loads in a row)
+	const int n = l.n_vocab, tok = l.tokens ? l.tokens[r] : -1;
+	const bool in = tok >= 0 && tok < n;
+	const float xt = in ? sh.x[tok] : 0.0f;
+	const bool hidden = in && !(xt > -INFINITY);   // (a NaN comes as -infinity)
+	// What a logit before the token has to pass to come before it (x >= xt is x > the value below xt), and one after it. Of
+	// a masked token all that are before it come first: they are counted at the end.
+	const float pass = hidden ? INFINITY : nextafterf(xt, -INFINITY), pass_after = hidden ? -INFINITY : xt;
+	const int tok_vec = in ? (tok + sh.cut) / 4 : -1;
+	Stat s{-FLT_MAX, 0.0f, 0.0f};
+	int before = 0;
+	Best best{-INFINITY, -INFINITY, sh.v0};
+	for (int g = sh.v0; g < sh.v1;)
+	{
 		float top = -INFINITY;
 #pragma unroll
-		for (int u = 0; u < LP_ITEMS; ++u) top = fmaxf(top, fmaxf(fmaxf(q[u].x, q[u].y), fmaxf(q[u].z, q[u].w)));
+		for (int i = 0; i < 4 * LP_ITEMS; ++i) top = fmaxf(top, v[i]);
 		if (TOP)
 		{
-			if (top > best)
-				second = best, best = top, best_at = g;
+			if (top > best.value)
+				best.second = best.value, best.value = top, best.group = g;
 			else
-				second = fmaxf(second, top);
+				best.second = fmaxf(best.second, top);
 		}
 		if (top > s.m)
 		{
@@ -206,178 +391,114 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const LpArgs a)
 			s.z *= c;
 			s.m = top;
 		}
-		float z = 0.0f, h = 0.0f;
+		float2 z = make_float2(0.0f, 0.0f), h = z;
 #pragma unroll
 		for (int u = 0; u < LP_ITEMS; ++u)
 		{
-			const float v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-			const int j = g + u * LP_THREADS + tid;
-			const float over = j < tok_vec ? below : xt;
+			const float over = g + u * T + tid < tok_vec ? pass : pass_after;
 #pragma unroll
-			for (int c = 0; c < 4; ++c)
+			for (int c = 0; c < 4; c += 2)
 			{
-				const float t = (v[c] - s.m) * k, e = ex2(t);
-				z += e;
-				h = fmaf(e, fmaxf(t, -200.0f), h); // (2^-200 is 0: what is masked adds no 0 * infinity)
-				before += v[c] > over;
+				const float2 x = make_float2(v[4 * u + c], v[4 * u + c + 1]);
+				float2 t = add2(x, make_float2(-s.m, -s.m));
+				t = make_float2(t.x * k, t.y * k);
+				const float2 e = make_float2(ex2(t.x), ex2(t.y));
+				z = add2(z, e);
+				h = fma2(e, make_float2(fmaxf(t.x, -200.0f), fmaxf(t.y, -200.0f)), h); // (2^-200 is 0: what is masked adds no 0 * infinity)
+				before += x.x > over;
+				before += x.y > over;
 			}
 		}
-		s.z += z;
-		s.h += h;
-		if (hidden) // every token that is not masked comes before a masked one, and the masked ones before it
-		{
-#pragma unroll
-			for (int u = 0; u < LP_ITEMS; ++u)
-			{
-				const float v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-				const int j = g + u * LP_THREADS + tid;
-#pragma unroll
-				for (int c = 0; c < 4; ++c)
-				{
-					const int i = 4 * j + c - cut;
-					before -= v[c] > (j < tok_vec ? below : xt);
-					before += j < v1 && i >= 0 && i < n && (v[c] > -INFINITY || i < tok);
-				}
-			}
-		}
+		s.z += z.x + z.y;
+		s.h += h.x + h.y;
+		g += GROUP;
+		if (g < sh.v1) read(g);
 	}
-	// equal ones before the token in its own vector
-	if (in && !hidden && tid == 0 && tok_vec >= v0 && tok_vec < v1)
-		for (int i = max(0, 4 * tok_vec - cut); i < tok; ++i) before += x[i] == xt;
+	if (in && tid == 0)
+	{
+		const int v_first = max(0, 4 * tok_vec - sh.cut); // the first of the token's own vector
+		if (tok_vec >= sh.v0 && tok_vec < sh.v1) // those before it there: equal, or masked as it is
+			for (int i = v_first; i < tok; ++i) before += hidden ? !(sh.x[i] > -INFINITY) : sh.x[i] == xt;
+		if (hidden) before += max(0, min(v_first, 4 * sh.v1 - sh.cut) - max(0, 4 * sh.v0 - sh.cut));
+	}
 
 #pragma unroll
 	for (int d = 16; d > 0; d >>= 1) s = lp_join(s, lp_shfl(s, d), k);
 	before = __reduce_add_sync(0xffffffffu, before);
 	if (lane == 0) warp_stat[warp] = s, warp_before[warp] = before;
-	if (tid == 0) n_found = n_again = 0;
-
-	if (TOP)
+	Part& mine = parts[part];
+	if constexpr (TOP) lp_select(sh, best, l.top, found, mine.top);
+	__syncthreads();
+	if (warp == 0)
 	{
-		// The thread's first candidate: the first of its largest logits, in the group that reached them first.
-		float4 q[LP_ITEMS];
+		s = lane < WARPS ? warp_stat[lane] : Stat{-FLT_MAX, 0.0f, 0.0f};
+		before = __reduce_add_sync(0xffffffffu, lane < WARPS ? warp_before[lane] : 0);
 #pragma unroll
-		for (int u = 0; u < LP_ITEMS; ++u)
-		{
-			const int j = best_at + u * LP_THREADS + tid;
-			q[u] = best > -INFINITY && j < v1 ? load(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-		}
-		Key first = 0;
-#pragma unroll
-		for (int u = LP_ITEMS - 1; u >= 0; --u)
-		{
-			const float v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-			for (int c = 3; c >= 0; --c)
-				if (v[c] == best) first = lp_key(best, 4 * (best_at + u * LP_THREADS + tid) + c - cut);
-		}
-		// The CTA's top tokens are not before the top-th of the threads' firsts, and lie with the threads whose own
-		// first is not after that one: `top` threads at most.
-		Key list = lp_sort(first, lane);
-		lists[warp][lane] = list;
-		__syncthreads();
-#pragma unroll
-		for (int d = LP_WARPS / 2; d > 0; d /= 2)
-		{
-			if (warp < d) lists[warp][lane] = list = lp_merge(list, lists[warp + d][lane], lane);
-			__syncthreads();
-		}
-		const Key least = lists[0][l.top - 1];
-		if (first != 0 && first >= least)
-		{
-			if (least == 0 ? second > -INFINITY : second >= lp_value(least)) // more of them may lie in the thread's other groups
-				again[atomicAdd(&n_again, 1)] = (short)tid;
-			else
-#pragma unroll
-				for (int u = 0; u < LP_ITEMS; ++u)
-				{
-					const float v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-					for (int c = 0; c < 4; ++c)
-					{
-						const Key key = lp_key(v[c], 4 * (best_at + u * LP_THREADS + tid) + c - cut);
-						if (key != 0 && key >= least) found[atomicAdd(&n_found, 1)] = key;
-					}
-				}
-		}
-		__syncthreads();
-		// Those threads' groups once more, a warp a thread.
-		list = 0;
-		for (int w = warp; w < n_again; w += LP_WARPS)
-			for (int j0 = v0 + again[w]; j0 < v1; j0 += 32 * LP_THREADS)
-			{
-				const int j = j0 + lane * LP_THREADS;
-				const float4 v4 = j < v1 ? load(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-				const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-#pragma unroll
-				for (int c = 0; c < 4; ++c)
-				{
-					Key key = lp_key(v[c], 4 * j + c - cut);
-					if (key < least) key = 0;
-					if (__any_sync(0xffffffffu, key != 0)) list = lp_merge(list, lp_sort(key, lane), lane);
-				}
-			}
-		if (list != 0) found[atomicAdd(&n_found, 1)] = list;
-		__syncthreads();
+		for (int d = WARPS / 2; d > 0; d >>= 1) s = lp_join(s, lp_shfl(s, d), k);
+	}
+	if (a.parts > 1)
+	{
+		// to the cluster's first CTA, which finishes the row
+		asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 		if (warp == 0)
 		{
-			list = 0;
-			for (int i = 0; i < n_found; i += 32) list = lp_merge(list, lp_sort(i + lane < n_found ? found[i + lane] : 0, lane), lane);
-			mine.top[lane] = list;
+			Part* to = static_cast<Part*>(cluster_map(&mine, 0));
+			if (TOP) to->top[lane] = mine.top[lane];
+			if (lane == 0) to->stat = s, to->before = before;
+		}
+		__syncthreads();
+		cluster_sync();
+		if (part != 0) return;
+		if (TOP) // the parts' runs into one
+#pragma unroll
+			for (int d = LP_CLUSTER / 2; d > 0; d >>= 1)
+			{
+				if (warp < d && warp + d < a.parts)
+					parts[warp].top[lane] = lp_merge(parts[warp].top[lane], parts[warp + d].top[lane], lane);
+				__syncthreads();
+			}
+		if (warp == 0)
+		{
+			s = lane < a.parts ? parts[lane].stat : Stat{-FLT_MAX, 0.0f, 0.0f};
+			before = __reduce_add_sync(0xffffffffu, lane < a.parts ? parts[lane].before : 0);
+#pragma unroll
+			for (int d = LP_CLUSTER / 2; d > 0; d >>= 1) s = lp_join(s, lp_shfl(s, d), k);
 		}
 	}
-	__syncthreads();
-	if (tid == 0)
+	if (warp != 0) return;
+	s.m = __shfl_sync(0xffffffffu, s.m, 0), s.z = __shfl_sync(0xffffffffu, s.z, 0), s.h = __shfl_sync(0xffffffffu, s.h, 0);
+	const double lz = log((double)s.z), scale = (double)l.scale;
+	if (lane == 0)
 	{
-		s = warp_stat[0];
-		before = warp_before[0];
-		for (int w = 1; w < LP_WARPS; ++w) s = lp_join(s, warp_stat[w], k), before += warp_before[w];
-		mine.stat = s;
-		mine.before = before;
+		if (l.logprob) l.logprob[r] = !in ? 0.0f : s.z == 0.0f ? -INFINITY : (float)(((double)xt - (double)s.m) * scale - lz);
+		if (l.rank) l.rank[r] = in ? before : -1;
+		if (l.entropy) l.entropy[r] = s.z == 0.0f ? 0.0f : (float)(lz - (double)s.h * 0.69314718055994530942 / (double)s.z);
 	}
-	__syncthreads();
-	if (a.parts > 1) cluster_sync();
-	if (part == 0 && warp == 0)
+	if (TOP && lane < l.top)
 	{
-		Key list = TOP ? mine.top[lane] : 0;
-		s = mine.stat;
-		before = mine.before;
-		for (int p = 1; p < a.parts; ++p)
-		{
-			const Part* other = reinterpret_cast<const Part*>(cluster_map(&mine, p));
-			if (TOP) list = lp_merge(list, other->top[lane], lane);
-			s = lp_join(s, other->stat, k);
-			before += other->before;
-		}
-		const double lz = log((double)s.z), scale = (double)l.scale;
-		if (lane == 0)
-		{
-			if (l.logprob)
-				l.logprob[r] = !in ? 0.0f : s.z == 0.0f ? -INFINITY : (float)(((double)xt - (double)s.m) * scale - lz);
-			if (l.rank) l.rank[r] = in ? before : -1;
-			if (l.entropy) l.entropy[r] = s.z == 0.0f ? 0.0f : (float)(lz - (double)s.h * 0.69314718055994530942 / (double)s.z);
-		}
-		if (TOP && lane < l.top)
-		{
-			if (l.top_ids) l.top_ids[r * l.top + lane] = list ? lp_index(list) : -1;
-			if (l.top_logprobs)
-				l.top_logprobs[r * l.top + lane] = list ? (float)(((double)lp_value(list) - (double)s.m) * scale - lz) : -INFINITY;
-		}
+		const Key key = parts[0].top[lane];
+		if (l.top_ids) l.top_ids[r * l.top + lane] = key ? lp_index(key) : -1;
+		if (l.top_logprobs)
+			l.top_logprobs[r * l.top + lane] = key ? (float)(((double)lp_value(key) - (double)s.m) * scale - lz) : -INFINITY;
 	}
-	__syncwarp();
-	if (a.parts > 1) cluster_sync(); // nobody reads this CTA's part any more
 }
 
-// The CTAs that share a row: the least of the waves that n * parts CTAs make of what the GPU holds at once (two a SM;
-// clusters do not fill every SM) times a CTA's time, a row's share and about 4096 logits' worth of start and end.
-int lp_parts(long long n, int n_vocab)
+struct LpPlan
 {
+	bool wide;
+	int parts;
+};
+
+LpPlan lp_plan(long long n, int n_vocab, bool top)
+{
+	(void)top;
 	static const int slots[] = {296, 296, 284, 264};
-	int best = 1;
+	LpPlan best{true, 1};
 	double least = 0;
 	for (int i = 0, parts = 1; parts <= LP_CLUSTER; ++i, parts *= 2)
 	{
 		const double t = (double)((n * parts + slots[i] - 1) / slots[i]) * ((double)n_vocab / parts + 4096.0 * (1 + (parts > 1)));
-		if (parts == 1 || t < least) least = t, best = parts;
+		if (parts == 1 || t < least) least = t, best.parts = parts;
 	}
 	return best;
 }
@@ -419,23 +540,29 @@ extern "C" int nncu_logprobs_dev(const nncu_logprobs* l, void* stream)
 	}
 	const int rc = check_current_device(l->logits, "logprobs");
 	if (rc != NNCU_OK) return rc;
-	LpArgs a{*l, (float)fmin((double)l->scale * 1.44269504088896340736, (double)FLT_MAX), lp_parts(l->n, l->n_vocab)};
-	cudaLaunchConfig_t cfg{};
-	cudaLaunchAttribute at{};
-	at.id = cudaLaunchAttributeClusterDimension;
-	at.val.clusterDim.x = a.parts, at.val.clusterDim.y = at.val.clusterDim.z = 1;
-	cfg.attrs = &at;
-	cfg.numAttrs = a.parts > 1;
-	cfg.blockDim = dim3(LP_THREADS);
-	cfg.stream = static_cast<cudaStream_t>(stream);
+	LpArgs a{*l, (float)fmin((double)l->scale * 1.44269504088896340736, (double)FLT_MAX), 1};
 	const bool tops = l->top > 0 && (l->top_ids || l->top_logprobs);
+	const LpPlan plan = lp_plan(l->n, l->n_vocab, tops);
+	a.parts = plan.parts;
+	cudaLaunchAttribute at[2]{};
+	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	at[0].val.programmaticStreamSerializationAllowed = 1;
+	at[1].id = cudaLaunchAttributeClusterDimension;
+	at[1].val.clusterDim.x = a.parts, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+	cudaLaunchConfig_t cfg{};
+	cfg.attrs = at;
+	cfg.numAttrs = a.parts > 1 ? 2 : 1;
+	cfg.blockDim = dim3(plan.wide ? LP_WIDE : LP_NARROW);
+	cfg.stream = static_cast<cudaStream_t>(stream);
+	const long long most = INT32_MAX / LP_CLUSTER; // rows of a launch
 	int e = 0;
-	const int most = INT32_MAX / LP_CLUSTER; // rows of a launch
-	for (long long r0 = 0; r0 < l->n && !e; r0 += most)
+	for (long long left = l->n; left > 0 && !e; left -= most)
 	{
-		const int rows = (int)(l->n - r0 < most ? l->n - r0 : most);
-		cfg.gridDim = dim3((unsigned)rows * a.parts);
-		e = (int)(tops ? cudaLaunchKernelEx(&cfg, logprobs_kernel<true>, a) : cudaLaunchKernelEx(&cfg, logprobs_kernel<false>, a));
+		const long long rows = left < most ? left : most;
+		cfg.gridDim = dim3((unsigned)(rows * a.parts));
+		const auto kernel = plan.wide ? (tops ? logprobs_kernel<true, LP_WIDE> : logprobs_kernel<false, LP_WIDE>)
+		                              : (tops ? logprobs_kernel<true, LP_NARROW> : logprobs_kernel<false, LP_NARROW>);
+		e = (int)cudaLaunchKernelEx(&cfg, kernel, a);
 		note_launches(1);
 		a.l.logits += (size_t)rows * a.l.stride;
 		if (a.l.tokens) a.l.tokens += rows;
