@@ -28,6 +28,7 @@ constexpr float I8_TINY = 1.17549435e-38f; // 2^-126: the least step of a row's 
 // the scale is rounded once.
 
 constexpr int Q_VALUES = 16; // a thread's values of a row (of a piece of it)
+constexpr int Q_MOST = 512;  // threads of a row, and of a CTA
 
 // VEC values at i, zeros past the row's end; at once where the rows lie on 16 bytes.
 template <typename T, int VEC, bool ALIGNED>
@@ -56,39 +57,44 @@ __device__ __forceinline__ void load_values(const T* x, int i, int cols, float* 
 	}
 }
 
-// x / s rounded to the nearest integer, ties to even, in the low byte: the product with the reciprocal is less than
-// 2^-15 off, so only next to a border does what is left of x, an exact fused multiply-add, decide.
-__device__ __forceinline__ uint32_t i8_code(float x, float s, float inv)
+constexpr float MAGIC = 12582912.0f; // 1.5 * 2^23: a sum's low bits are the rounded integer
+
+// x / s rounded to the nearest integer, ties to even, in the low byte, by the product with the reciprocal, which is less
+// than 2^-15 off; `close` where that is too little to go by.
+__device__ __forceinline__ uint32_t i8_code(float x, float inv, bool& close)
 {
-	constexpr float MAGIC = 12582912.0f; // 1.5 * 2^23: the sum's low bits are the rounded integer
 	const float q = x * inv, t = q + MAGIC;
+	close |= fabsf(q - (t - MAGIC)) > 0.49996f;
+	return __float_as_uint(t);
+}
+// The same where a border is close: what is left of x, an exact fused multiply-add, decides.
+__device__ __forceinline__ uint32_t i8_code_exact(float x, float s, float inv)
+{
+	const float t = x * inv + MAGIC;
 	uint32_t c = __float_as_uint(t);
-	const float n = t - MAGIC;
-	if (fabsf(q - n) > 0.4999f)
-	{
-		const float d = fmaf(-n, s, x), h = 0.5f * s;
-		if (d > h || (d == h && (c & 1))) ++c;
-		if (d < -h || (d == -h && (c & 1))) --c;
-	}
+	const float d = fmaf(-(t - MAGIC), s, x), h = 0.5f * s;
+	if (d > h || (d == h && (c & 1))) ++c;
+	if (d < -h || (d == -h && (c & 1))) --c;
 	return c;
 }
 
 // per_row threads of the CTA (x) take a row, blockDim.y rows a CTA; LOOP: rows longer than their threads hold.
 template <typename T, bool ALIGNED, bool LOOP>
-__global__ void __launch_bounds__(1024) i8_quantise_kernel(const nncu_i8_rows r)
+__global__ void __launch_bounds__(Q_MOST) i8_quantise_kernel(const nncu_i8_rows r)
 {
 	constexpr int VEC = 16 / (int)sizeof(T), NV = Q_VALUES / VEC;
-	__shared__ float most_s[32];
-	__shared__ double sum_s[32];
+	__shared__ uint32_t most_s[Q_MOST / 32];
+	__shared__ double sum_s[Q_MOST / 32];
 	const int tid = (int)threadIdx.x, per_row = (int)blockDim.x, warps = per_row / 32;
 	const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
 	const bool live = row < r.n;
 	const T* x = static_cast<const T*>(r.x) + (size_t)(live ? row : 0) * r.x_stride;
 	const int piece = per_row * Q_VALUES, cols = live ? r.cols : 0;
+	griddep_launch_dependents();
+	griddep_wait();
 	float v[Q_VALUES];
-	float most = 0.0f;
+	uint32_t most = 0; // of the magnitudes' bits, which rise with them; infinities and NaN are above all others
 	double sum = 0.0;
-	bool bad = false;
 	const auto load = [&](int p0) {
 #pragma unroll
 		for (int k = 0; k < NV; ++k) load_values<T, VEC, ALIGNED>(x, p0 + (k * per_row + tid) * VEC, cols, v + k * VEC);
@@ -114,34 +120,21 @@ __global__ void __launch_bounds__(1024) i8_quantise_kernel(const nncu_i8_rows r)
 			for (int j = 0; j < Q_VALUES; ++j) sum += (double)v[j] * v[j];
 		gain(p0);
 #pragma unroll
-		for (int j = 0; j < Q_VALUES; ++j)
-		{
-			most = fmaxf(most, fabsf(v[j]));
-			bad |= !(fabsf(v[j]) < INFINITY);
-		}
+		for (int j = 0; j < Q_VALUES; ++j) most = max(most, __float_as_uint(v[j]) & 0x7FFFFFFFu);
 	}
-	if (bad) most = INFINITY; // (a maximum passes over NaN)
-	most = warp_max(most);
+	most = __reduce_max_sync(0xffffffffu, most);
 	if (r.norm)
 #pragma unroll
 		for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+	const int at = (int)threadIdx.y * warps;
 	if (warps > 1)
 	{
-		const int at = (int)threadIdx.y * warps; // (32 warps a CTA at most)
 		if (tid % 32 == 0) most_s[at + tid / 32] = most, sum_s[at + tid / 32] = sum;
 		__syncthreads();
-		sum = 0.0;
-		for (int w = 0; w < warps; ++w) most = fmaxf(most, most_s[at + w]);
-		if (tid == 0 && r.norm)
-			for (int w = 0; w < warps; ++w) sum += sum_s[at + w];
+		for (int w = 0; w < warps; ++w) most = max(most, most_s[at + w]);
 	}
-	bad = !(most < INFINITY);
-	const float s = bad ? 1.0f : fmaxf(__fdiv_rn(most, 127.0f), I8_TINY), inv = bad ? 0.0f : __fdiv_rn(1.0f, s);
-	if (tid == 0 && live)
-	{
-		const double mean = sum / r.cols + (double)r.eps;
-		r.scales[row] = bad ? NAN : r.norm && mean > 0.0 ? (float)((double)s / sqrt(mean)) : s;
-	}
+	const bool bad = most >= 0x7F800000u;
+	const float s = bad ? 1.0f : fmaxf(__fdiv_rn(__uint_as_float(most), 127.0f), I8_TINY), inv = __fdiv_rn(1.0f, s);
 	int8_t* c = r.codes + (size_t)(live ? row : 0) * r.code_stride;
 	for (int p0 = 0; p0 < (LOOP ? cols : 1); p0 += piece)
 	{
@@ -150,6 +143,16 @@ __global__ void __launch_bounds__(1024) i8_quantise_kernel(const nncu_i8_rows r)
 			load(p0);
 			gain(p0);
 		}
+		uint32_t b[Q_VALUES];
+		bool close = false;
+#pragma unroll
+		for (int j = 0; j < Q_VALUES; ++j) b[j] = i8_code(v[j], inv, close);
+		if (close)
+#pragma unroll
+			for (int j = 0; j < Q_VALUES; ++j) b[j] = i8_code_exact(v[j], s, inv);
+		if (bad)
+#pragma unroll
+			for (int j = 0; j < Q_VALUES; ++j) b[j] = 0;
 #pragma unroll
 		for (int k = 0; k < NV; ++k)
 		{
@@ -159,10 +162,8 @@ __global__ void __launch_bounds__(1024) i8_quantise_kernel(const nncu_i8_rows r)
 #pragma unroll
 			for (int q = 0; q < VEC / 4; ++q)
 			{
-				uint32_t b[4];
-#pragma unroll
-				for (int j = 0; j < 4; ++j) b[j] = bad ? 0u : i8_code(v[k * VEC + 4 * q + j], s, inv);
-				w[q] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+				const uint32_t* p = b + k * VEC + 4 * q;
+				w[q] = __byte_perm(__byte_perm(p[0], p[1], 0x0040), __byte_perm(p[2], p[3], 0x0040), 0x5410);
 			}
 			if (i + VEC <= cols)
 			{
@@ -177,27 +178,43 @@ __global__ void __launch_bounds__(1024) i8_quantise_kernel(const nncu_i8_rows r)
 					if (i + j < cols) c[i + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
 		}
 	}
+	if (tid == 0 && live) // (after the codes: nobody waits for it)
+	{
+		if (r.norm && warps > 1)
+		{
+			sum = 0.0;
+			for (int w = 0; w < warps; ++w) sum += sum_s[at + w];
+		}
+		const double mean = sum / r.cols + (double)r.eps;
+		r.scales[row] = bad ? NAN : r.norm && mean > 0.0 ? (float)((double)s / sqrt(mean)) : s;
+	}
+}
+
+// A launch that may begin while the one before it on the stream ends (its kernels wait for that end before they read).
+template <typename... P, typename... A>
+int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, const A&... args)
+{
+	cudaLaunchAttribute at{};
+	at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	at.val.programmaticStreamSerializationAllowed = 1;
+	cudaLaunchConfig_t cfg{};
+	cfg.gridDim = grid, cfg.blockDim = block, cfg.stream = st;
+	cfg.attrs = &at;
+	cfg.numAttrs = 1;
+	return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T>
-void launch_quantise(const nncu_i8_rows& r, cudaStream_t st)
+int launch_quantise(const nncu_i8_rows& r, cudaStream_t st)
 {
 	const bool on16 = (reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.gamma)) % 16 == 0 &&
 	                  (r.n == 1 || r.x_stride * sizeof(T) % 16 == 0);
-	const int need = (r.cols + Q_VALUES - 1) / Q_VALUES, per_row = need > 1024 ? 1024 : (need + 31) / 32 * 32;
+	const int need = (r.cols + Q_VALUES - 1) / Q_VALUES, per_row = need > Q_MOST ? Q_MOST : (need + 31) / 32 * 32;
 	const int rows = per_row >= 128 ? 1 : 128 / per_row; // short rows: several to a CTA
 	const dim3 block(per_row, rows), grid((unsigned)(((long long)r.n + rows - 1) / rows));
-	if (need > 1024)
-	{
-		if (on16)
-			i8_quantise_kernel<T, true, true><<<grid, block, 0, st>>>(r);
-		else
-			i8_quantise_kernel<T, false, true><<<grid, block, 0, st>>>(r);
-	}
-	else if (on16)
-		i8_quantise_kernel<T, true, false><<<grid, block, 0, st>>>(r);
-	else
-		i8_quantise_kernel<T, false, false><<<grid, block, 0, st>>>(r);
+	if (need > Q_MOST)
+		return launch_dependent(on16 ? i8_quantise_kernel<T, true, true> : i8_quantise_kernel<T, false, true>, grid, block, st, r);
+	return launch_dependent(on16 ? i8_quantise_kernel<T, true, false> : i8_quantise_kernel<T, false, false>, grid, block, st, r);
 }
 
 // ---- look up ----------------------------------------------------------------------------
@@ -207,23 +224,27 @@ void launch_quantise(const nncu_i8_rows& r, cudaStream_t st)
 // such loads are in flight a lane. A code becomes a float by putting it, as
 // code + 128, below the bits of 2^23 and taking 2^23 + 128 off again.
 
-constexpr int L_THREADS = 128, L_ITEMS = 4;
+constexpr int L_ITEMS = 4, L_MOST = 256;
 
+// per_row threads of the CTA (x) take 16 values each of a row, blockDim.y rows a CTA; a row's next pieces along the grid's y.
 template <bool ALIGNED>
-__global__ void __launch_bounds__(L_THREADS) i8_lookup_kernel(const nncu_i8_lookup l)
+__global__ void __launch_bounds__(L_MOST) i8_lookup_kernel(const nncu_i8_lookup l)
 {
-	const int t = (int)blockIdx.x;
-	const int id = l.ids ? l.ids[t] : t;
+	const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+	griddep_launch_dependents();
+	griddep_wait();
+	if (t >= l.n) return;
+	const int per_row = (int)blockDim.x, id = l.ids ? l.ids[t] : (int)t;
 	const bool in = id >= 0 && id < l.n_rows;
 	const float s = in ? l.scales[id] * l.mult : 0.0f;
 	const int8_t* c = l.codes + (size_t)(in ? id : 0) * l.code_stride;
 	float* out = l.out + (size_t)t * l.out_stride;
-	const int i0 = ((int)blockIdx.y * L_ITEMS * L_THREADS + (int)threadIdx.x) * 4;
+	const int i0 = ((int)blockIdx.y * L_ITEMS * per_row + (int)threadIdx.x) * 4;
 	uint32_t w[L_ITEMS];
 #pragma unroll
 	for (int k = 0; k < L_ITEMS; ++k)
 	{
-		const int i = i0 + k * L_THREADS * 4;
+		const int i = i0 + k * per_row * 4;
 		w[k] = 0;
 		if (!in) continue;
 		if (i + 4 <= l.cols)
@@ -236,7 +257,7 @@ __global__ void __launch_bounds__(L_THREADS) i8_lookup_kernel(const nncu_i8_look
 #pragma unroll
 	for (int k = 0; k < L_ITEMS; ++k)
 	{
-		const int i = i0 + k * L_THREADS * 4;
+		const int i = i0 + k * per_row * 4;
 		float v[4];
 #pragma unroll
 		for (int j = 0; j < 4; ++j)
@@ -248,6 +269,16 @@ __global__ void __launch_bounds__(L_THREADS) i8_lookup_kernel(const nncu_i8_look
 			for (int j = 0; j < 4; ++j)
 				if (i + j < l.cols) out[i + j] = v[j];
 	}
+}
+
+int launch_lookup(const nncu_i8_lookup& l, cudaStream_t st)
+{
+	const bool on16 = reinterpret_cast<uintptr_t>(l.out) % 16 == 0 && (l.n == 1 || l.out_stride % 4 == 0);
+	const int need = (l.cols + 4 * L_ITEMS - 1) / (4 * L_ITEMS), pieces = (need + L_MOST - 1) / L_MOST;
+	const int per_row = ((need + pieces - 1) / pieces + 31) / 32 * 32; // the pieces alike: few idle threads
+	const int rows = per_row >= 128 ? 1 : 128 / per_row;
+	const dim3 grid((unsigned)(((long long)l.n + rows - 1) / rows), (unsigned)pieces), block(per_row, rows);
+	return launch_dependent(on16 ? i8_lookup_kernel<true> : i8_lookup_kernel<false>, grid, block, st, l);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -323,14 +354,11 @@ extern "C" int nncu_i8_quantise_dev(const nncu_i8_rows* r, void* stream)
 	const int rc = check_current_device(r->codes, "i8 quantise");
 	if (rc != NNCU_OK) return rc;
 	const auto st = static_cast<cudaStream_t>(stream);
-	if (r->x_type == NNCU_KV_F32)
-		launch_quantise<float>(*r, st);
-	else if (r->x_type == NNCU_KV_BF16)
-		launch_quantise<__nv_bfloat16>(*r, st);
-	else
-		launch_quantise<__half>(*r, st);
+	const int e = r->x_type == NNCU_KV_F32 ? launch_quantise<float>(*r, st)
+	              : r->x_type == NNCU_KV_BF16 ? launch_quantise<__nv_bfloat16>(*r, st)
+	                                          : launch_quantise<__half>(*r, st);
 	note_launches(1);
-	const int e = (int)cudaGetLastError();
+	if (e) cudaGetLastError();
 	return e ? set_cuda_error(e, "i8 quantise launch") : NNCU_OK;
 }
 
@@ -356,14 +384,9 @@ extern "C" int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream)
 		return refuse("i8 lookup: out must not meet another array");
 	const int rc = check_current_device(l->out, "i8 lookup");
 	if (rc != NNCU_OK) return rc;
-	const dim3 grid((unsigned)l->n, (unsigned)((l->cols + 4 * L_ITEMS * L_THREADS - 1) / (4 * L_ITEMS * L_THREADS)));
-	const auto st = static_cast<cudaStream_t>(stream);
-	if (aligned16(l->out) && (l->n == 1 || l->out_stride % 4 == 0))
-		i8_lookup_kernel<true><<<grid, L_THREADS, 0, st>>>(*l);
-	else
-		i8_lookup_kernel<false><<<grid, L_THREADS, 0, st>>>(*l);
+	const int e = launch_lookup(*l, static_cast<cudaStream_t>(stream));
 	note_launches(1);
-	const int e = (int)cudaGetLastError();
+	if (e) cudaGetLastError();
 	return e ? set_cuda_error(e, "i8 lookup launch") : NNCU_OK;
 }
 

@@ -486,20 +486,32 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 struct LpPlan
 {
 	bool wide;
-	int parts;
+	int parts; // CTAs that share a row
 };
 
+// The least of an estimate, in SM cycles: the waves that the CTAs make of what the GPU holds at once (clusters do not
+// fill every SM) times a CTA's start and end and its share, at a pace of its own or, with others on its SM, at a share
+// of the SM's. Its constants were fitted to 1900 timings (1 to 2000 rows of 5000 to 262144 logits, from HBM); its
+// choices are 1.7 % slower there than the best of all in the mean, 20 % at worst. Both sides, microseconds: 64 rows of
+// 151936: wide CTAs, four a row 14.0, narrow ones 17.0; 2000 rows: narrow ones 187, wide ones 194; 1 x 262144: eight
+// wide CTAs 5.3, one 20.6.
 LpPlan lp_plan(long long n, int n_vocab, bool top)
 {
-	(void)top;
-	static const int slots[] = {296, 296, 284, 264};
-	LpPlan best{true, 1};
+	static const int filled[] = {148, 148, 142, 132}; // SMs that clusters of 1, 2, 4, 8 fill
+	LpPlan best{};
 	double least = 0;
-	for (int i = 0, parts = 1; parts <= LP_CLUSTER; ++i, parts *= 2)
-	{
-		const double t = (double)((n * parts + slots[i] - 1) / slots[i]) * ((double)n_vocab / parts + 4096.0 * (1 + (parts > 1)));
-		if (parts == 1 || t < least) least = t, best.parts = parts;
-	}
+	for (int wide = 1; wide >= 0; --wide)
+		for (int i = 0, parts = 1; parts <= LP_CLUSTER; ++i, parts *= 2)
+		{
+			const double slots = filled[i] * (wide ? LP_WIDE_CTAS : LP_NARROW_CTAS), ctas = (double)n * parts;
+			const double beside = fmax(1.0, fmin(ctas, slots) / 148);
+			double ends = wide ? 4000 : 4600;
+			if (top) ends += wide ? 3800 : 2600;
+			if (parts > 1) ends += top ? 1800 : 350;
+			const double pace = fmax(wide ? 0.075 : 0.228, 0.043 * beside); // cycles a logit
+			const double t = ceil(ctas / slots) * (ends * fmax(1.0, 0.13 * beside) + pace * n_vocab / parts);
+			if (best.parts == 0 || t < least) least = t, best = {wide != 0, parts};
+		}
 	return best;
 }
 
