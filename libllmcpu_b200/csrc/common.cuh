@@ -371,6 +371,33 @@ __device__ __forceinline__ float ex2(float x)
 	return y;
 }
 
+// Two floats' sum, product, product and sum in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+	return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+	return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+	float2 r;
+	asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+	    "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+	    : "=f"(r.x), "=f"(r.y)
+	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+	return r;
+}
+
 // Qwen3.5's output gate (model.cpp:1759-1760, nnc_mul_sigmoid_f32): an
 // attention output element times sigmoid(g), as y / (1 + exp(-g)).
 __device__ __forceinline__ float gated(float y, const float* gate, size_t i)

@@ -21,22 +21,27 @@ constexpr float I8_TINY = 1.17549435e-38f; // 2^-126: the least step of a row's 
 
 // ---- quantise -------------------------------------------------------------------------
 //
-// Reads each value once and writes a byte: bound by memory. A row stays in
-// the registers of `per_row` threads (16 values each, 16-byte loads) between
-// its maximum and its codes; longer rows than a CTA holds are read twice. The
+// Reads each value once and writes a byte: bound by memory, and by issue slots
+// as soon as a value costs more than a dozen instructions, so that values go
+// in pairs (one instruction for two), borders are settled for all of a thread's
+// values at once, and the edges of a row are looked for once a thread. A row
+// stays in the registers of `per_row` threads (16-byte loads) between its
+// maximum and its codes; longer rows than a CTA holds are read twice. The
 // squares of the norm are summed in 64 bits: float inputs' never overflow, and
 // the scale is rounded once.
 
+constexpr int Q_MOST = 256, Q_CTAS = 5; // threads of a row, and of a CTA; CTAs per SM
 constexpr int Q_VALUES = 16; // a thread's values of a row (of a piece of it)
-constexpr int Q_MOST = 512;  // threads of a row, and of a CTA
 
-// VEC values at i, zeros past the row's end; at once where the rows lie on 16 bytes.
-template <typename T, int VEC, bool ALIGNED>
+// VEC values at i, zeros past the row's end. FAST: rows on 16 bytes, a multiple of VEC long, so that all of them are there
+// or none (code for odd ends beside it would be issued, without effect, for every value).
+template <typename T, int VEC, bool FAST>
 __device__ __forceinline__ void load_values(const T* x, int i, int cols, float* v)
 {
-	if (ALIGNED && i + VEC <= cols)
+	if constexpr (FAST)
 	{
-		const uint4 q = *reinterpret_cast<const uint4*>(x + i);
+		uint4 q = make_uint4(0, 0, 0, 0);
+		if (i < cols) q = *reinterpret_cast<const uint4*>(x + i);
 		if constexpr (sizeof(T) == 4)
 			v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
 		else
@@ -56,48 +61,173 @@ __device__ __forceinline__ void load_values(const T* x, int i, int cols, float* 
 		for (int j = 0; j < VEC; ++j) v[j] = i + j < cols ? load_elem(x + i + j) : 0.0f;
 	}
 }
+// Their codes, out.
+template <int VEC, bool FAST>
+__device__ __forceinline__ void store_codes(int8_t* c, int i, int cols, const uint32_t* w)
+{
+	if constexpr (FAST)
+	{
+		if (i >= cols) return;
+		if constexpr (VEC == 4)
+			*reinterpret_cast<uint32_t*>(c + i) = w[0];
+		else
+			*reinterpret_cast<uint2*>(c + i) = make_uint2(w[0], w[1]);
+	}
+	else
+#pragma unroll
+		for (int j = 0; j < VEC; ++j)
+			if (i + j < cols) c[i + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
+}
+
+// The largest magnitude of a thread's values joins `most`, an infinity or a NaN makes `odd` a NaN (a maximum passes over NaN).
+__device__ __forceinline__ void magnitudes(const float (&v)[Q_VALUES], float& most, float2& odd)
+{
+#pragma unroll
+	for (int j = 0; j < Q_VALUES; j += 2)
+	{
+		most = fmaxf(most, fmaxf(fabsf(v[j]), fabsf(v[j + 1])));
+		odd = fma2(make_float2(v[j], v[j + 1]), make_float2(0.0f, 0.0f), odd);
+	}
+}
+// Its bits, which rise with it; above all numbers' where there was no number.
+__device__ __forceinline__ uint32_t most_bits(float most, float2 odd)
+{
+	return odd.x + odd.y == 0.0f ? __float_as_uint(most) : 0x7F800000u;
+}
+__device__ __forceinline__ double squares(const float (&v)[Q_VALUES])
+{
+	double a = 0.0, b = 0.0;
+#pragma unroll
+	for (int j = 0; j < Q_VALUES; j += 2) a += (double)v[j] * v[j], b += (double)v[j + 1] * v[j + 1];
+	return a + b;
+}
+
+__device__ __forceinline__ void times_gain(float* v, const float* g)
+{
+#pragma unroll
+	for (int i = 0; i < 4; i += 2)
+	{
+		const float2 z = mul2(make_float2(v[i], v[i + 1]), make_float2(g[i], g[i + 1]));
+		v[i] = z.x, v[i + 1] = z.y;
+	}
+}
 
 constexpr float MAGIC = 12582912.0f; // 1.5 * 2^23: a sum's low bits are the rounded integer
 
-// x / s rounded to the nearest integer, ties to even, in the low byte, by the product with the reciprocal, which is less
-// than 2^-15 off; `close` where that is too little to go by.
-__device__ __forceinline__ uint32_t i8_code(float x, float inv, bool& close)
+// A thread's codes, x / s rounded to the nearest integer n, ties to even, four to a word. The quotient is corrected once, so
+// that half integers come out as such and round to even. What is left of x, d = x - n s (exact: about s / 2 at most, in units
+// of s's or x's last bit), then says whether n is right: where |d| passes s / 2, x lies closer to a border than a float
+// quotient tells, and n is one off. Of 32-bit inputs one in a million does: the largest |d| is returned, and i8_codes_exact
+// writes such a thread's codes once more. Of 16-bit inputs one in two thousand does (their scale is a rounded one too):
+// they are put right here.
+template <bool NARROW>
+__device__ __forceinline__ float i8_codes(const float (&v)[Q_VALUES], float s, float inv, bool bad, uint32_t (&w)[Q_VALUES / 4])
 {
-	const float q = x * inv, t = q + MAGIC;
-	close |= fabsf(q - (t - MAGIC)) > 0.49996f;
-	return __float_as_uint(t);
-}
-// The same where a border is close: what is left of x, an exact fused multiply-add, decides.
-__device__ __forceinline__ uint32_t i8_code_exact(float x, float s, float inv)
-{
-	const float t = x * inv + MAGIC;
-	uint32_t c = __float_as_uint(t);
-	const float d = fmaf(-(t - MAGIC), s, x), h = 0.5f * s;
-	if (d > h || (d == h && (c & 1))) ++c;
-	if (d < -h || (d == -h && (c & 1))) --c;
-	return c;
+	uint32_t b[Q_VALUES];
+	const float2 inv2 = make_float2(inv, inv), s2 = make_float2(-s, -s);
+	float left = 0.0f;
+#pragma unroll
+	for (int j = 0; j < Q_VALUES; j += 2)
+	{
+		const float2 x = make_float2(v[j], v[j + 1]);
+		float2 q = mul2(x, inv2);
+		q = fma2(fma2(q, s2, x), inv2, q);
+		const float2 t = add2(q, make_float2(MAGIC, MAGIC)), n = add2(t, make_float2(-MAGIC, -MAGIC)), d = fma2(n, s2, x);
+		b[j] = __float_as_uint(t.x), b[j + 1] = __float_as_uint(t.y);
+		left = fmaxf(left, fmaxf(fabsf(d.x), fabsf(d.y)));
+	}
+	if (NARROW)
+	{
+		const float h = 0.5f * s;
+		if (__any_sync(0xffffffffu, left > h))
+#pragma unroll
+			for (int j = 0; j < Q_VALUES; ++j)
+			{
+				const float d = fmaf(-(__uint_as_float(b[j]) - MAGIC), s, v[j]);
+				b[j] += (d > h) - (d < -h);
+			}
+	}
+#pragma unroll
+	for (int q = 0; q < Q_VALUES / 4; ++q) // (the low bytes)
+		w[q] = bad ? 0u : __byte_perm(__byte_perm(b[4 * q], b[4 * q + 1], 0x0040), __byte_perm(b[4 * q + 2], b[4 * q + 3], 0x0040), 0x5410);
+	return NARROW || bad ? 0.0f : left;
 }
 
-// per_row threads of the CTA (x) take a row, blockDim.y rows a CTA; LOOP: rows longer than their threads hold.
-template <typename T, bool ALIGNED, bool LOOP>
-__global__ void __launch_bounds__(Q_MOST) i8_quantise_kernel(const nncu_i8_rows r)
+// A thread's codes of the piece of a row from p0 on, by what is left of each. (A call that reads its values anew, so that
+// the common way holds nothing for it, and that takes them apart from the launch's struct, of which every thread would
+// otherwise make a copy.)
+template <typename T, bool FAST>
+__device__ __noinline__ void i8_codes_exact(const T* x, const float* gamma, int8_t* codes, int cols, int p0, float s, float inv)
 {
 	constexpr int VEC = 16 / (int)sizeof(T), NV = Q_VALUES / VEC;
+	float v[Q_VALUES];
+	const auto place = [&](int k) { return p0 + (k * (int)blockDim.x + (int)threadIdx.x) * VEC; };
+#pragma unroll
+	for (int k = 0; k < NV; ++k) load_values<T, VEC, FAST>(x, place(k), cols, v + k * VEC);
+	if (gamma)
+#pragma unroll
+		for (int j = 0; j < Q_VALUES; j += 4)
+		{
+			float g[4];
+			load_values<float, 4, FAST>(gamma, place(j / VEC) + j % VEC, cols, g);
+			times_gain(v + j, g);
+		}
+#pragma unroll
+	for (int k = 0; k < NV; ++k)
+	{
+		uint32_t w[VEC / 4] = {};
+#pragma unroll
+		for (int j = 0; j < VEC; ++j)
+		{
+			const float z = v[k * VEC + j], t = z * inv + MAGIC, d = fmaf(-(t - MAGIC), s, z), h = 0.5f * s;
+			uint32_t c = __float_as_uint(t);
+			if (d > h || (d == h && (c & 1))) ++c;
+			if (d < -h || (d == -h && (c & 1))) --c;
+			w[j / 4] |= (c & 0xFFu) << (8 * (j % 4));
+		}
+		store_codes<VEC, FAST>(codes, place(k), cols, w);
+	}
+}
+
+// The sum of n numbers in shared memory, on a warp.
+__device__ __forceinline__ double sum_all(const double* p, int n)
+{
+	double s = 0.0;
+	for (int i = (int)threadIdx.x % 32; i < n; i += 32) s += p[i];
+#pragma unroll
+	for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+	return s;
+}
+
+// The row's scale, rounded once; 1 / cols in 64 bits.
+__device__ __forceinline__ float i8_scale(const nncu_i8_rows& r, double per_col, float s, bool bad, double sum)
+{
+	if (bad) return NAN;
+	if (!r.norm) return s;
+	const double mean = fma(sum, per_col, (double)r.eps);
+	return mean > 0.0 ? (float)((double)s * rsqrt(mean)) : s;
+}
+
+// per_row threads of the CTA (x) take a row, blockDim.y rows a CTA; LOOP: rows longer than that.
+template <typename T, bool FAST, bool LOOP>
+__global__ void __launch_bounds__(Q_MOST, Q_CTAS) i8_quantise_kernel(const nncu_i8_rows r, double per_col)
+{
+	constexpr int V = Q_VALUES, VEC = 16 / (int)sizeof(T), NV = V / VEC;
 	__shared__ uint32_t most_s[Q_MOST / 32];
-	__shared__ double sum_s[Q_MOST / 32];
+	__shared__ double sum_s[Q_MOST];
 	const int tid = (int)threadIdx.x, per_row = (int)blockDim.x, warps = per_row / 32;
 	const long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y;
 	const bool live = row < r.n;
 	const T* x = static_cast<const T*>(r.x) + (size_t)(live ? row : 0) * r.x_stride;
-	const int piece = per_row * Q_VALUES, cols = live ? r.cols : 0;
+	const int piece = per_row * V, cols = live ? r.cols : 0;
 	griddep_launch_dependents();
 	griddep_wait();
-	float v[Q_VALUES];
-	uint32_t most = 0; // of the magnitudes' bits, which rise with them; infinities and NaN are above all others
+	float v[V], most = 0.0f;
+	float2 odd = make_float2(0.0f, 0.0f);
 	double sum = 0.0;
 	const auto load = [&](int p0) {
 #pragma unroll
-		for (int k = 0; k < NV; ++k) load_values<T, VEC, ALIGNED>(x, p0 + (k * per_row + tid) * VEC, cols, v + k * VEC);
+		for (int k = 0; k < NV; ++k) load_values<T, VEC, FAST>(x, p0 + (k * per_row + tid) * VEC, cols, v + k * VEC);
 	};
 	const auto gain = [&](int p0) {
 		if (!r.gamma) return;
@@ -107,34 +237,30 @@ __global__ void __launch_bounds__(Q_MOST) i8_quantise_kernel(const nncu_i8_rows 
 			for (int j = 0; j < VEC; j += 4)
 			{
 				float g[4];
-				load_values<float, 4, ALIGNED>(r.gamma, p0 + (k * per_row + tid) * VEC + j, cols, g);
-#pragma unroll
-				for (int i = 0; i < 4; ++i) v[k * VEC + j + i] *= g[i];
+				load_values<float, 4, FAST>(r.gamma, p0 + (k * per_row + tid) * VEC + j, cols, g);
+				times_gain(v + k * VEC + j, g);
 			}
 	};
 	for (int p0 = 0; p0 < (LOOP ? cols : 1); p0 += piece)
 	{
 		load(p0);
-		if (r.norm)
-#pragma unroll
-			for (int j = 0; j < Q_VALUES; ++j) sum += (double)v[j] * v[j];
+		if (r.norm) sum += squares(v);
 		gain(p0);
-#pragma unroll
-		for (int j = 0; j < Q_VALUES; ++j) most = max(most, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+		magnitudes(v, most, odd);
 	}
-	most = __reduce_max_sync(0xffffffffu, most);
-	if (r.norm)
-#pragma unroll
-		for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+	uint32_t bits = __reduce_max_sync(0xffffffffu, most_bits(most, odd));
 	const int at = (int)threadIdx.y * warps;
+	if (r.norm) sum_s[(int)threadIdx.y * per_row + tid] = sum;
 	if (warps > 1)
 	{
-		if (tid % 32 == 0) most_s[at + tid / 32] = most, sum_s[at + tid / 32] = sum;
+		if (tid % 32 == 0) most_s[at + tid / 32] = bits;
 		__syncthreads();
-		for (int w = 0; w < warps; ++w) most = max(most, most_s[at + w]);
+		bits = __reduce_max_sync(0xffffffffu, tid % 32 < warps ? most_s[at + tid % 32] : 0u);
 	}
-	const bool bad = most >= 0x7F800000u;
-	const float s = bad ? 1.0f : fmaxf(__fdiv_rn(__uint_as_float(most), 127.0f), I8_TINY), inv = __fdiv_rn(1.0f, s);
+	else
+		__syncwarp();
+	const bool bad = bits >= 0x7F800000u;
+	const float s = bad ? 1.0f : fmaxf(__fdiv_rn(__uint_as_float(bits), 127.0f), I8_TINY), inv = __frcp_rn(s);
 	int8_t* c = r.codes + (size_t)(live ? row : 0) * r.code_stride;
 	for (int p0 = 0; p0 < (LOOP ? cols : 1); p0 += piece)
 	{
@@ -143,62 +269,28 @@ __global__ void __launch_bounds__(Q_MOST) i8_quantise_kernel(const nncu_i8_rows 
 			load(p0);
 			gain(p0);
 		}
-		uint32_t b[Q_VALUES];
-		bool close = false;
+		uint32_t w[V / 4];
+		const float left = i8_codes<sizeof(T) == 2>(v, s, inv, bad, w);
 #pragma unroll
-		for (int j = 0; j < Q_VALUES; ++j) b[j] = i8_code(v[j], inv, close);
-		if (close)
-#pragma unroll
-			for (int j = 0; j < Q_VALUES; ++j) b[j] = i8_code_exact(v[j], s, inv);
-		if (bad)
-#pragma unroll
-			for (int j = 0; j < Q_VALUES; ++j) b[j] = 0;
-#pragma unroll
-		for (int k = 0; k < NV; ++k)
-		{
-			const int i = p0 + (k * per_row + tid) * VEC;
-			if (i >= cols) continue;
-			uint32_t w[VEC / 4];
-#pragma unroll
-			for (int q = 0; q < VEC / 4; ++q)
-			{
-				const uint32_t* p = b + k * VEC + 4 * q;
-				w[q] = __byte_perm(__byte_perm(p[0], p[1], 0x0040), __byte_perm(p[2], p[3], 0x0040), 0x5410);
-			}
-			if (i + VEC <= cols)
-			{
-				if constexpr (VEC == 4)
-					*reinterpret_cast<uint32_t*>(c + i) = w[0];
-				else
-					*reinterpret_cast<uint2*>(c + i) = make_uint2(w[0], w[1]);
-			}
-			else
-#pragma unroll
-				for (int j = 0; j < VEC; ++j)
-					if (i + j < cols) c[i + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
-		}
+		for (int k = 0; k < NV; ++k) store_codes<VEC, FAST>(c, p0 + (k * per_row + tid) * VEC, cols, w + k * (VEC / 4));
+		if (sizeof(T) == 4 && live && left > 0.5f * s) i8_codes_exact<T, FAST>(x, r.gamma, c, cols, p0, s, inv);
 	}
-	if (tid == 0 && live) // (after the codes: nobody waits for it)
+	if (tid < 32) // (one warp, after its codes: nobody waits for it)
 	{
-		if (r.norm && warps > 1)
-		{
-			sum = 0.0;
-			for (int w = 0; w < warps; ++w) sum += sum_s[at + w];
-		}
-		const double mean = sum / r.cols + (double)r.eps;
-		r.scales[row] = bad ? NAN : r.norm && mean > 0.0 ? (float)((double)s / sqrt(mean)) : s;
+		if (r.norm) sum = sum_all(sum_s + (int)threadIdx.y * per_row, per_row);
+		if (tid == 0 && live) r.scales[row] = i8_scale(r, per_col, s, bad, sum);
 	}
 }
 
 // A launch that may begin while the one before it on the stream ends (its kernels wait for that end before they read).
 template <typename... P, typename... A>
-int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t st, const A&... args)
+int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args)
 {
 	cudaLaunchAttribute at{};
 	at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
 	at.val.programmaticStreamSerializationAllowed = 1;
 	cudaLaunchConfig_t cfg{};
-	cfg.gridDim = grid, cfg.blockDim = block, cfg.stream = st;
+	cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = st;
 	cfg.attrs = &at;
 	cfg.numAttrs = 1;
 	return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
@@ -207,14 +299,15 @@ int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t s
 template <typename T>
 int launch_quantise(const nncu_i8_rows& r, cudaStream_t st)
 {
-	const bool on16 = (reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.gamma)) % 16 == 0 &&
-	                  (r.n == 1 || r.x_stride * sizeof(T) % 16 == 0);
+	const bool fast = (reinterpret_cast<uintptr_t>(r.x) | reinterpret_cast<uintptr_t>(r.gamma)) % 16 == 0 &&
+	                  (r.n == 1 || r.x_stride * sizeof(T) % 16 == 0) && r.cols * sizeof(T) % 16 == 0;
 	const int need = (r.cols + Q_VALUES - 1) / Q_VALUES, per_row = need > Q_MOST ? Q_MOST : (need + 31) / 32 * 32;
 	const int rows = per_row >= 128 ? 1 : 128 / per_row; // short rows: several to a CTA
-	const dim3 block(per_row, rows), grid((unsigned)(((long long)r.n + rows - 1) / rows));
+	const long long ctas = ((long long)r.n + rows - 1) / rows;
+	const dim3 block(per_row, rows);
 	if (need > Q_MOST)
-		return launch_dependent(on16 ? i8_quantise_kernel<T, true, true> : i8_quantise_kernel<T, false, true>, grid, block, st, r);
-	return launch_dependent(on16 ? i8_quantise_kernel<T, true, false> : i8_quantise_kernel<T, false, false>, grid, block, st, r);
+		return launch_dependent(fast ? i8_quantise_kernel<T, true, true> : i8_quantise_kernel<T, false, true>, dim3((unsigned)ctas), block, 0, st, r, 1.0 / r.cols);
+	return launch_dependent(fast ? i8_quantise_kernel<T, true, false> : i8_quantise_kernel<T, false, false>, dim3((unsigned)ctas), block, 0, st, r, 1.0 / r.cols);
 }
 
 // ---- look up ----------------------------------------------------------------------------
@@ -278,7 +371,7 @@ int launch_lookup(const nncu_i8_lookup& l, cudaStream_t st)
 	const int per_row = ((need + pieces - 1) / pieces + 31) / 32 * 32; // the pieces alike: few idle threads
 	const int rows = per_row >= 128 ? 1 : 128 / per_row;
 	const dim3 grid((unsigned)(((long long)l.n + rows - 1) / rows), (unsigned)pieces), block(per_row, rows);
-	return launch_dependent(on16 ? i8_lookup_kernel<true> : i8_lookup_kernel<false>, grid, block, st, l);
+	return launch_dependent(on16 ? i8_lookup_kernel<true> : i8_lookup_kernel<false>, grid, block, 0, st, l);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -354,7 +447,7 @@ extern "C" int nncu_i8_quantise_dev(const nncu_i8_rows* r, void* stream)
 	const int rc = check_current_device(r->codes, "i8 quantise");
 	if (rc != NNCU_OK) return rc;
 	const auto st = static_cast<cudaStream_t>(stream);
-	const int e = r->x_type == NNCU_KV_F32 ? launch_quantise<float>(*r, st)
+	const int e = r->x_type == NNCU_KV_F32    ? launch_quantise<float>(*r, st)
 	              : r->x_type == NNCU_KV_BF16 ? launch_quantise<__nv_bfloat16>(*r, st)
 	                                          : launch_quantise<__half>(*r, st);
 	note_launches(1);

@@ -129,25 +129,6 @@ struct Part
 	int before;
 };
 
-// Two floats' sum, and product and sum, in one instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-	float2 r;
-	asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-	    : "=f"(r.x), "=f"(r.y)
-	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-	return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-	float2 r;
-	asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-	    "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-	    : "=f"(r.x), "=f"(r.y)
-	    : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-	return r;
-}
-
 // A row's share of one CTA, in vectors of four logits that lie on 16 bytes: the row's first and last one may be cut.
 struct Share
 {

@@ -39,6 +39,10 @@ QUANTISE = [  # rows, cols, type, gain, norm, values between rows
     (64, 2048, "float32", 1, 1, 0), (9, 2560, "bfloat16", 0, 0, 8), (33, 4096, "float32", 0, 1, 4),
     (7, 4095, "float32", 1, 0, 0), (2, 5000, "float16", 1, 1, 0), (3, 16384, "float32", 1, 1, 0),
     (2, 33000, "bfloat16", 1, 1, 1), (1, 131071, "float32", 1, 1, 0), (700, 1030, "float32", 1, 1, 2),
+    # many rows
+    (2500, 1030, "float32", 1, 1, 2), (2401, 2048, "bfloat16", 1, 1, 0), (9001, 64, "float32", 1, 0, 0),
+    (5003, 500, "float16", 0, 1, 4), (4750, 301, "float32", 0, 1, 3), (700, 8192, "float32", 1, 1, 0),
+    (2600, 1500, "float32", 1, 1, 1),
 ]
 
 
