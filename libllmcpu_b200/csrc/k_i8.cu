@@ -486,7 +486,8 @@ extern "C" int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream)
 extern "C" int nncu_i8_linear_dev(const nncu_i8_linear* l, void* stream)
 {
 	if (!l) return refuse("i8 linear: NULL argument");
-	if (l->n_tok < 0 || l->rows <= 0) return refuse("i8 linear: bad n_tok or rows");
+	if (l->n_tok < 0 || l->rows <= 0 || l->n_tok > 1 << 30 || l->rows > 1 << 30)
+		return refuse("i8 linear: bad n_tok or rows (up to 2^30)");
 	if (l->cols <= 0 || l->cols > 131071) return refuse("i8 linear: cols must be 1 to 131071"); // (2^14 cols < 2^31)
 	if ((long long)l->n_tok * l->rows > (1ll << 36)) return refuse("i8 linear: n_tok * rows passes 2^36");
 	if (l->n_tok == 0) return NNCU_OK;

@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 // (cta_group::2) of both SMs' tensor cores reads both. Two accumulators in TMEM:
 // the epilogue of a tile runs beside the next one's products.
 
-constexpr int P_GROUP = 8; // channel tiles that are walked together, so that their weights stay in L2
+constexpr int P_GROUP = 32; // channel tiles that are walked together: their weights stay in L2 and the rows of y are written whole
 
 __device__ __forceinline__ void pair_tile(const Args& a, int id, int& o0, int& t0)
 {

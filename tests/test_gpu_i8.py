@@ -257,3 +257,64 @@ def test_a_token_does_not_go_by_its_batch(nncu, torch_cuda):
     whole = multiplied(nncu, torch_cuda, x, xs, w, ws, b, None, 0, rng)
     for lo, hi in ((0, 1), (5, 21), (100, 164), (300, 500)):
         np.testing.assert_array_equal(multiplied(nncu, torch_cuda, x[lo:hi], xs[lo:hi], w, ws, b, None, 0, rng), whole[lo:hi])
+
+
+# ---- places past 32 bits ---------------------------------------------------------------------
+
+def test_tables_past_4_gb(nncu, torch_cuda):
+    """A table of 4.5 GB: rows at its end looked up and multiplied, and quantised into."""
+    torch, N = torch_cuda, nncu
+    rows_, cols = 1_100_000, 4096
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randint(-127, 128, (rows_, cols), generator=g, dtype=torch.int8, device="cuda")
+    ws = torch.rand(rows_, generator=g, device="cuda")
+    ids = torch.tensor([rows_ - 1, 0, 1 << 20, 524_287, 524_288], dtype=torch.int32, device="cuda")
+    out = torch.zeros(5, cols, device="cuda")
+    N.i8_lookup_dev(N.i8_lookup(n=5, cols=cols, n_rows=rows_, codes=w, scales=ws, ids=ids, out=out))
+    want = w[ids.long()].double() * ws[ids.long()].double()[:, None]
+    assert bool(((out.double() - want).abs() <= 2.01 * H.U * want.abs()).all())
+    x = torch.randint(-127, 128, (3, cols), generator=g, dtype=torch.int8, device="cuda")
+    y = torch.zeros(3, rows_, device="cuda")
+    N.i8_linear_dev(N.i8_linear(n_tok=3, rows=rows_, cols=cols, x=x, x_scales=torch.ones(3, device="cuda"), w=w, w_scales=ws, y=y))
+    at = torch.cat([torch.arange(0, rows_, 997, device="cuda"), torch.arange(rows_ - 300, rows_, device="cuda")])
+    want = (x.double() @ w[at].double().T) * ws[at].double()
+    assert bool(((y[:, at].double() - want).abs() <= 3.01 * H.U * want.abs()).all())
+    f = torch.randn(2, cols, generator=g, device="cuda")
+    sc = torch.zeros(2, device="cuda")
+    before = w[:2].clone()
+    # two rows, from the table's third to last one on
+    N.i8_quantise_dev(N.i8_rows(n=2, cols=cols, x=f, codes=w[rows_ - 3:], scales=sc))
+    codes, scales = H.quantise(f.cpu().numpy(), None, 0, 0.0)
+    np.testing.assert_array_equal(w[rows_ - 3:rows_ - 1].cpu().numpy(), codes)
+    assert torch.equal(w[:2], before)
+    N.i8_check()
+
+
+def test_rows_past_8_gb_apart(nncu, torch_cuda):
+    """Strides whose product with a row's number passes 2^32: x, y, add and the codes of the second row."""
+    torch, N = torch_cuda, nncu
+    far, cols = 1 << 31, 256
+    flat = torch.zeros(far + cols, device="cuda")
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((2, cols)).astype(np.float32)
+    flat[:cols], flat[far:] = dev(torch, x[0]), dev(torch, x[1])
+    codes, sc = torch.zeros(2, cols, dtype=torch.int8, device="cuda"), torch.zeros(2, device="cuda")
+    N.i8_quantise_dev(N.i8_rows(n=2, cols=cols, x=flat, x_stride=far, codes=codes, scales=sc))
+    check_rows(x, (codes.cpu().numpy().astype(np.int64), sc.cpu().numpy()), None, 0)
+    w = rng.integers(-127, 128, (cols, cols), dtype=np.int8)
+    one = torch.ones(cols, device="cuda")
+    N.i8_linear_dev(N.i8_linear(n_tok=2, rows=cols, cols=cols, x=codes, x_scales=one, w=dev(torch, w), w_scales=one,
+                                add=flat, add_stride=far, y=flat, y_stride=far))
+    p = codes.cpu().numpy().astype(np.float64) @ w.astype(np.float64).T
+    for r, got in enumerate((flat[:cols], flat[far:])):
+        assert (np.abs(got.cpu().numpy() - (p[r] + x[r])) <= 1.01 * H.U * (3 * np.abs(p[r]) + np.abs(p[r] + x[r]))).all()
+    N.i8_lookup_dev(N.i8_lookup(n=2, cols=cols, n_rows=2, codes=codes, scales=one, out=flat, out_stride=far))
+    np.testing.assert_array_equal(flat[far:].cpu().numpy(), codes[1].cpu().numpy().astype(np.float32))
+    logits = flat
+    ent, ids = torch.zeros(2, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    N.logprobs_dev(N.logprobs(n=2, n_vocab=cols, logits=logits, stride=far, entropy=ent, top=3, top_ids=ids))
+    for r in range(2):
+        row = codes[r].cpu().numpy().astype(np.float32)
+        want, off = H.logprobs(row, 1.0, -1, 3)
+        np.testing.assert_array_equal(ids[r].cpu().numpy(), want["top_ids"])
+        assert abs(float(ent[r]) - want["entropy"]) <= off["entropy"]

@@ -58,7 +58,8 @@ def test_lookup_refuses(L, change, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    (dict(n_tok=-1), "n_tok"), (dict(rows=0), "rows"), (dict(cols=0), "cols"), (dict(cols=131072), "cols"),
+    (dict(n_tok=-1), "n_tok"), (dict(rows=0), "rows"), (dict(rows=(1 << 30) + 1, n_tok=1), "rows"),
+    (dict(n_tok=(1 << 30) + 1, rows=1), "n_tok"), (dict(cols=0), "cols"), (dict(cols=131072), "cols"),
     (dict(n_tok=1 << 30, rows=1 << 10), "2^36"), (dict(x=None), "NULL"), (dict(w=None), "NULL"),
     (dict(y=None), "NULL"), (dict(x_scales=None), "NULL"), (dict(w_scales=None), "NULL"),
     (dict(x=at(0) + 8), "16-byte"), (dict(w=at(2) + 1), "16-byte"), (dict(x_stride=100), "16-byte"),
