@@ -319,8 +319,9 @@ int launch_quantise(const nncu_i8_rows& r, cudaStream_t st)
 
 constexpr int L_ITEMS = 4, L_MOST = 256;
 
-// per_row threads of the CTA (x) take 16 values each of a row, blockDim.y rows a CTA; a row's next pieces along the grid's y.
-template <bool ALIGNED>
+// per_row threads of the CTA (x) take 16 values each of a row, blockDim.y rows a CTA; a row's next pieces along the grid's
+// y. FAST: rows out on 16 bytes, a multiple of four long (as where rows are quantised).
+template <bool FAST>
 __global__ void __launch_bounds__(L_MOST) i8_lookup_kernel(const nncu_i8_lookup l)
 {
 	const long long t = (long long)blockIdx.x * blockDim.y + threadIdx.y;
@@ -329,49 +330,55 @@ __global__ void __launch_bounds__(L_MOST) i8_lookup_kernel(const nncu_i8_lookup 
 	if (t >= l.n) return;
 	const int per_row = (int)blockDim.x, id = l.ids ? l.ids[t] : (int)t;
 	const bool in = id >= 0 && id < l.n_rows;
-	const float s = in ? l.scales[id] * l.mult : 0.0f;
-	const int8_t* c = l.codes + (size_t)(in ? id : 0) * l.code_stride;
-	float* out = l.out + (size_t)t * l.out_stride;
-	const int i0 = ((int)blockIdx.y * L_ITEMS * per_row + (int)threadIdx.x) * 4;
+	const int cols = l.cols, i0 = ((int)blockIdx.y * L_ITEMS * per_row + (int)threadIdx.x) * 4;
+	const int8_t* c = l.codes + (size_t)(in ? id : 0) * l.code_stride + i0;
+	float* out = l.out + (size_t)t * l.out_stride + i0;
 	uint32_t w[L_ITEMS];
 #pragma unroll
 	for (int k = 0; k < L_ITEMS; ++k)
 	{
-		const int i = i0 + k * per_row * 4;
+		const int i = k * per_row * 4, left = in ? cols - i0 - i : 0;
 		w[k] = 0;
-		if (!in) continue;
-		if (i + 4 <= l.cols)
-			w[k] = *reinterpret_cast<const uint32_t*>(c + i);
+		if (FAST)
+		{
+			if (left > 0) w[k] = *reinterpret_cast<const uint32_t*>(c + i);
+		}
 		else
 #pragma unroll
 			for (int j = 0; j < 4; ++j)
-				if (i + j < l.cols) w[k] |= (uint32_t)(uint8_t)c[i + j] << (8 * j);
+				if (j < left) w[k] |= (uint32_t)(uint8_t)c[i + j] << (8 * j);
 	}
+	const float s = in ? l.scales[id] * l.mult : 0.0f;
 #pragma unroll
 	for (int k = 0; k < L_ITEMS; ++k)
 	{
-		const int i = i0 + k * per_row * 4;
-		float v[4];
-#pragma unroll
-		for (int j = 0; j < 4; ++j)
-			v[j] = in ? s * (__uint_as_float(__byte_perm(w[k] ^ 0x80808080u, 0x4B000000u, 0x7540 + j)) - 8388736.0f) : 0.0f;
-		if (ALIGNED && i + 4 <= l.cols)
-			*reinterpret_cast<float4*>(out + i) = make_float4(v[0], v[1], v[2], v[3]);
+		const int i = k * per_row * 4, left = cols - i0 - i;
+		const uint32_t u = w[k] ^ 0x80808080u;
+		const auto code = [&](int j) { return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + j)); };
+		const float2 off = make_float2(-8388736.0f, -8388736.0f), s2 = make_float2(s, s);
+		const float2 a = mul2(add2(make_float2(code(0), code(1)), off), s2), b = mul2(add2(make_float2(code(2), code(3)), off), s2);
+		if (FAST)
+		{
+			if (left > 0) *reinterpret_cast<float4*>(out + i) = make_float4(a.x, a.y, b.x, b.y);
+		}
 		else
+		{
+			const float v[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
 			for (int j = 0; j < 4; ++j)
-				if (i + j < l.cols) out[i + j] = v[j];
+				if (j < left) out[i + j] = v[j];
+		}
 	}
 }
 
 int launch_lookup(const nncu_i8_lookup& l, cudaStream_t st)
 {
-	const bool on16 = reinterpret_cast<uintptr_t>(l.out) % 16 == 0 && (l.n == 1 || l.out_stride % 4 == 0);
+	const bool fast = reinterpret_cast<uintptr_t>(l.out) % 16 == 0 && (l.n == 1 || l.out_stride % 4 == 0) && l.cols % 4 == 0;
 	const int need = (l.cols + 4 * L_ITEMS - 1) / (4 * L_ITEMS), pieces = (need + L_MOST - 1) / L_MOST;
 	const int per_row = ((need + pieces - 1) / pieces + 31) / 32 * 32; // the pieces alike: few idle threads
 	const int rows = per_row >= 128 ? 1 : 128 / per_row;
 	const dim3 grid((unsigned)(((long long)l.n + rows - 1) / rows), (unsigned)pieces), block(per_row, rows);
-	return launch_dependent(on16 ? i8_lookup_kernel<true> : i8_lookup_kernel<false>, grid, block, 0, st, l);
+	return launch_dependent(fast ? i8_lookup_kernel<true> : i8_lookup_kernel<false>, grid, block, 0, st, l);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
