@@ -157,6 +157,27 @@ struct Share
 		}
 		return make_float4(v[0], v[1], v[2], v[3]);
 	}
+	// the thread's logits of the group of T * LP_ITEMS vectors from g on
+	template <int T>
+	__device__ __forceinline__ void read(int g, float (&v)[4 * LP_ITEMS]) const
+	{
+		if (g > 0 && g + T * LP_ITEMS < nvec && g + T * LP_ITEMS <= v1)
+		{
+#pragma unroll
+			for (int u = 0; u < LP_ITEMS; ++u)
+			{
+				const float4 q = __ldg(at(g + u * T + (int)threadIdx.x));
+				v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
+			}
+		}
+		else
+#pragma unroll
+			for (int u = 0; u < LP_ITEMS; ++u)
+			{
+				const float4 q = load(g + u * T + (int)threadIdx.x);
+				v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
+			}
+	}
 };
 
 // A thread's largest logits of its share: what the selection goes by.
@@ -183,17 +204,13 @@ __device__ __forceinline__ void lp_select(const Share& sh, const Best& b, int to
 	const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	// The thread's first candidate: the first of its largest logits, in the group that reached them first.
 	float v[4 * LP_ITEMS];
-#pragma unroll
-	for (int u = 0; u < LP_ITEMS; ++u)
-	{
-		const float4 q = b.value > -INFINITY ? sh.load(b.group + u * T + tid) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-		v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
-	}
+	sh.template read<T>(b.group, v);
 	const auto index = [&](int i) { return sh.index(b.group + (i / 4) * T + tid, i % 4); };
-	Key first = 0;
+	int at = 0;
 #pragma unroll
 	for (int i = 4 * LP_ITEMS - 1; i >= 0; --i)
-		if (v[i] == b.value) first = lp_key(b.value, index(i));
+		if (v[i] == b.value) at = (i / 4) * 4 * T + i % 4;
+	const Key first = lp_key(b.value, sh.index(b.group + tid, 0) + at); // (0 where all are masked)
 	// The warp's first few of those, one after another.
 	Key left = first;
 #pragma unroll
@@ -323,25 +340,7 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 
 	const Share sh(l, r, part, a.parts);
 	float v[4 * LP_ITEMS];
-	const auto read = [&](int g) {
-		if (g > 0 && g + GROUP < sh.nvec && g + GROUP <= sh.v1)
-		{
-#pragma unroll
-			for (int u = 0; u < LP_ITEMS; ++u)
-			{
-				const float4 q = __ldg(sh.at(g + u * T + tid));
-				v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
-			}
-		}
-		else
-#pragma unroll
-			for (int u = 0; u < LP_ITEMS; ++u)
-			{
-				const float4 q = sh.load(g + u * T + tid);
-				v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
-			}
-	};
-	read(sh.v0); // (before the token's own logit, which waits for two loads in a row)
+	sh.template read<T>(sh.v0, v); // (before the token's own logit, which waits for two loads in a row)
 	const int n = l.n_vocab, tok = l.tokens ? l.tokens[r] : -1;
 	const bool in = tok >= 0 && tok < n;
 	const float xt = in ? sh.x[tok] : 0.0f;
@@ -393,7 +392,7 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 		s.z += z.x + z.y;
 		s.h += h.x + h.y;
 		g += GROUP;
-		if (g < sh.v1) read(g);
+		if (g < sh.v1) sh.template read<T>(g, v);
 	}
 	if (in && tid == 0)
 	{
