@@ -1,5 +1,6 @@
 // k_i8.cu -- a serving batch's rows in 8 bits: quantised with the norm before
-// a projection, looked up from a table, and multiplied (nncu_i8_*).
+// a projection, looked up from a table, and the entries of these and of the
+// product (k_i8_linear.cu).
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -28,7 +29,10 @@ constexpr float I8_TINY = 1.17549435e-38f; // 2^-126: the least step of a row's 
 // stays in the registers of `per_row` threads (16-byte loads) between its
 // maximum and its codes; longer rows than a CTA holds are read twice. The
 // squares of the norm are summed in 64 bits: float inputs' never overflow, and
-// the scale is rounded once.
+// the scale is rounded once. 8191 x 2560 floats with gain and norm 23.6 us (the
+// copy rate: 16.0), of which the norm's conversions and the exact border are 6;
+// 16 values a thread and five CTAs of 256 threads per SM: with 32 values 51 us,
+// with four CTAs 27, with CTAs that stay and copy ahead 29.
 
 constexpr int Q_MOST = 256, Q_CTAS = 5; // threads of a row, and of a CTA; CTAs per SM
 constexpr int Q_VALUES = 16; // a thread's values of a row (of a piece of it)
@@ -315,7 +319,8 @@ int launch_quantise(const nncu_i8_rows& r, cudaStream_t st)
 // Four bytes written for each one read: bound by the stores. A lane turns four
 // codes into one 16-byte store, so that a warp's is 512 bytes in a row; four
 // such loads are in flight a lane. A code becomes a float by putting it, as
-// code + 128, below the bits of 2^23 and taking 2^23 + 128 off again.
+// code + 128, below the bits of 2^23 and taking 2^23 + 128 off again. 8191 of
+// 128256 x 2048: 15.0 us (the copy rate: 12.8); two loads a lane 16.8, eight 15.7.
 
 constexpr int L_ITEMS = 4, L_MOST = 256;
 
