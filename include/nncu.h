@@ -544,11 +544,13 @@ int nncu_kv4_check(const nncu_kv4_attn* a, void* stream);
  * written. */
 
 /* Rows quantised, with the norm before a projection: z = x * gamma (a float
- * product; gamma NULL: x), s = max(max |z| / 127, 2^-126), code = z / s rounded
- * to the nearest integer, ties to even. The row's scale is s, with `norm` s /
- * sqrt(mean(x^2) + eps): an RMS norm is a factor of the row and leaves its
- * codes alone (where that mean and eps are both zero: s). A row whose z has a NaN or an infinity gets codes of zero and
- * the scale NaN. Weights are laid out by the same call, a row a channel. */
+ * product; gamma NULL: x), s = max(max |z| * (1 / 127), 2^-126) (a float product
+ * with 1 / 127 rounded to float, as tensor libraries divide by a constant), code =
+ * z / s rounded to the nearest integer, ties to even. The row's scale is s, with
+ * `norm` s / sqrt(mean(x^2) + eps): an RMS norm is a factor of the row and leaves
+ * its codes alone (where that mean and eps are both zero: s). A row whose z has a
+ * NaN or an infinity gets codes of zero and the scale NaN. Weights are laid out by
+ * the same call, a row a channel. */
 typedef struct nncu_i8_rows
 {
 	int32_t n, cols;

@@ -120,7 +120,7 @@ constexpr float MAGIC = 12582912.0f; // 1.5 * 2^23: a sum's low bits are the rou
 
 // A thread's codes, x / s rounded to the nearest integer n, ties to even, four to a word. The quotient is corrected once, so
 // that half integers come out as such and round to even. What is left of x, d = x - n s (exact: about s / 2 at most, in units
-// of s's or x's last bit), then says whether n is right: where |d| passes s / 2, x lies closer to a border than a float
+// of s's or x's last bit), then says whether n is right: where 2 |d| passes s (halving the least steps would round), x lies closer to a border than a float
 // quotient tells, and n is one off. Of 32-bit inputs one in a million does: the largest |d| is returned, and i8_codes_exact
 // writes such a thread's codes once more. Of 16-bit inputs one in two thousand does (their scale is a rounded one too):
 // they are put right here.
@@ -142,13 +142,12 @@ __device__ __forceinline__ float i8_codes(const float (&v)[Q_VALUES], float s, f
 	}
 	if (NARROW)
 	{
-		const float h = 0.5f * s;
-		if (__any_sync(0xffffffffu, left > h))
+		if (__any_sync(0xffffffffu, left + left > s))
 #pragma unroll
 			for (int j = 0; j < Q_VALUES; ++j)
 			{
 				const float d = fmaf(-(__uint_as_float(b[j]) - MAGIC), s, v[j]);
-				b[j] += (d > h) - (d < -h);
+				b[j] += (d + d > s) - (d + d < -s);
 			}
 	}
 #pragma unroll
@@ -183,10 +182,12 @@ __device__ __noinline__ void i8_codes_exact(const T* x, const float* gamma, int8
 #pragma unroll
 		for (int j = 0; j < VEC; ++j)
 		{
-			const float z = v[k * VEC + j], t = z * inv + MAGIC, d = fmaf(-(t - MAGIC), s, z), h = 0.5f * s;
+			const float z = v[k * VEC + j], t = z * inv + MAGIC, d = fmaf(-(t - MAGIC), s, z), d2 = d + d;
 			uint32_t c = __float_as_uint(t);
-			if (d > h || (d == h && (c & 1))) ++c;
-			if (d < -h || (d == -h && (c & 1))) --c;
+			if (d2 > s || (d2 == s && (c & 1)))
+				++c;
+			else if (d2 < -s || (d2 == -s && (c & 1)))
+				--c;
 			w[j / 4] |= (c & 0xFFu) << (8 * (j % 4));
 		}
 		store_codes<VEC, FAST>(codes, place(k), cols, w);
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(Q_MOST, Q_CTAS) i8_quantise_kernel(const nncu_
 	else
 		__syncwarp();
 	const bool bad = bits >= 0x7F800000u;
-	const float s = bad ? 1.0f : fmaxf(__fdiv_rn(__uint_as_float(bits), 127.0f), I8_TINY), inv = __frcp_rn(s);
+	const float s = bad ? 1.0f : fmaxf(__fmul_rn(__uint_as_float(bits), 1.0f / 127.0f), I8_TINY), inv = __frcp_rn(s);
 	int8_t* c = r.codes + (size_t)(live ? row : 0) * r.code_stride;
 	for (int p0 = 0; p0 < (LOOP ? cols : 1); p0 += piece)
 	{
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(Q_MOST, Q_CTAS) i8_quantise_kernel(const nncu_
 		const float left = i8_codes<sizeof(T) == 2>(v, s, inv, bad, w);
 #pragma unroll
 		for (int k = 0; k < NV; ++k) store_codes<VEC, FAST>(c, p0 + (k * per_row + tid) * VEC, cols, w + k * (VEC / 4));
-		if (sizeof(T) == 4 && live && left > 0.5f * s) i8_codes_exact<T, FAST>(x, r.gamma, c, cols, p0, s, inv);
+		if (sizeof(T) == 4 && live && left + left > s) i8_codes_exact<T, FAST>(x, r.gamma, c, cols, p0, s, inv);
 	}
 	if (tid < 32) // (one warp, after its codes: nobody waits for it)
 	{

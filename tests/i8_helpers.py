@@ -13,7 +13,8 @@ def quantise(x, gamma, norm, eps):
     with np.errstate(all="ignore"):
         z = x if gamma is None else x * gamma.astype(np.float32)
         bad = ~np.isfinite(z).all(-1)
-        step = np.maximum(np.where(bad, np.float32(1), np.abs(z).max(-1)) / np.float32(127), np.float32(2.0 ** -126))
+        step = np.maximum(np.where(bad, np.float32(1), np.abs(z).max(-1)) * (np.float32(1) / np.float32(127)),
+                          np.float32(2.0 ** -126))
         step = step.astype(np.float32)
         codes = np.rint(np.where(bad[:, None], 0, z).astype(np.float64) / step.astype(np.float64)[:, None])
         scale = step.astype(np.float64)

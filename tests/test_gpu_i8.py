@@ -107,6 +107,25 @@ def test_quantise_at_the_borders(nncu, torch_cuda, cols):
     check_rows(x, quantised(nncu, torch_cuda, x, "float32", None, 0), None, 0)
 
 
+@pytest.mark.parametrize("kind,top", [(k, t) for k in ("float32", "bfloat16", "float16")
+                                      for t in (2.0 ** -119, 1.7 * 2.0 ** -119, 2.0 ** -10, 1.99 * 2.0 ** 120)
+                                      if k != "float16" or t == 2.0 ** -10])  # (the others are past its range)
+def test_quantise_next_to_every_border(nncu, torch_cuda, kind, top):
+    """For many steps (the least, whose halves are no floats, among them) the values at, just below and just above all 254
+    borders between codes; of 16-bit inputs the nearest ones that there are."""
+    import torch as t
+
+    rng = np.random.default_rng(8)
+    most = typed((top * rng.uniform(1, 2, 60)).astype(np.float32), kind)
+    step = (most * (np.float32(1) / np.float32(127))).astype(np.float64)[:, None]
+    border = ((np.arange(-127, 127) + 0.5) * step).astype(np.float32)
+    x = np.concatenate([np.nextafter(border, np.float32(-np.inf)), border, np.nextafter(border, np.float32(np.inf)), most[:, None]], 1)
+    x = t.from_numpy(x).to(getattr(t, kind)).float().numpy()
+    x = np.concatenate([x, np.zeros((60, 5), np.float32)], 1)  # 768 values
+    for cols in (768, 767):  # with and without code for odd ends
+        check_rows(x[:, :cols].copy(), quantised(nncu, torch_cuda, x[:, :cols].copy(), kind, None, 0), None, 0)
+
+
 @pytest.mark.parametrize("cols", [17, 2048, 2051, 70000])
 def test_quantise_odd_rows(nncu, torch_cuda, cols):
     """Rows of zeros, of subnormal and of the largest values, with NaN and infinities, signed zeros."""
@@ -172,6 +191,8 @@ LINEAR = [  # tokens, rows, cols, bias, add (2: y itself), values between rows o
     (64, 640, 8192, 0, 0, 0), (65, 129, 127, 0, 1, 2), (100, 6144, 640, 1, 0, 0), (128, 256, 16384, 0, 0, 0),
     (129, 512, 512, 1, 1, 0), (255, 2561, 1000, 0, 0, 7), (256, 256, 256, 0, 2, 0), (257, 300, 2048, 1, 0, 0),
     (300, 4096, 2560, 0, 1, 0), (777, 2560, 2048, 1, 0, 0), (1000, 100, 96, 0, 0, 0), (1025, 1537, 130, 1, 1, 1),
+    (200, 2560, 10240, 0, 1, 0), (520, 2000, 20000, 1, 0, 1), (333, 515, 9000, 1, 2, 1), (1500, 300, 16384, 0, 0, 0),
+    (200, 20480, 300, 0, 0, 0), (4099, 6200, 300, 1, 0, 3),
     (2500, 40, 700, 0, 0, 0), (2048, 2048, 1024, 0, 0, 0), (5, 40000, 200, 0, 0, 0), (2, 3, 131071, 0, 0, 0),
     (40, 16, 100000, 0, 0, 0), (4100, 130, 16, 1, 2, 2),
 ]
