@@ -582,13 +582,14 @@ struct Plan
 
 // Which kernel, how many tokens a tile, over how many CTAs (pairs) a tile's columns are split, one or two panels a
 // stage, one CTA per SM or two (of half the memory): the least of an estimate in SM cycles. Its constants were
-// fitted to 6700 timings of 140 shapes (1 to 4096 tokens, 128 to 262144 channels, 300 to 16384 columns, weights from
-// HBM); the choices it makes there are 3 % slower than the best of all in the mean, 19 % at worst. What they stand for:
-//  - a stage costs the issue of its copies and products (one panel 500, two together 110 a panel: the second panel's
-//    go along), its products (a pair's 210 + 1.5 a token, a single CTA's the fourth of which is 57 or 44 + 0.36 a
-//    token), its bytes into an SM (62 a cycle) or, over all SMs, out of L2 (8000 a cycle);
+// fitted to 6700 timings of 167 shapes (1 to 4096 tokens, 128 to 262144 channels, 300 to 16384 columns, weights from
+// HBM); the choices it makes there are 2.5 % slower than the best of all in the mean, 16 % at worst. What they stand for:
+//  - a panel costs the issue of its copies and products (500 alone, 82 where two go together), its products (a pair's
+//    81 + 2.17 a token, a single CTA's four of 56.5 or 44 + 0.36 a token), its bytes into an SM (62 a cycle) or, over
+//    all SMs, out of L2 (8250 a cycle), whichever is the most;
 //  - clusters of 4 and more do not fill every SM;
-//  - a launch's start and end, the epilogue by token, and the joining of a split tile through shared memory.
+//  - the weights come from HBM at 3300 bytes a cycle;
+//  - a launch has a start and an end, an epilogue by token, a split tile the joining of its parts.
 // Both sides, microseconds: 1 token, 6144 channels, 4096 columns: whole columns, two panels 7.5, one panel 8.8, split
 // over four 8.3; 1 x 2560 x 10240: split over eight 8.1, whole 12.0; 777 x 2560 x 2048: single CTAs 7.7, pairs 8.6;
 // 1024 x 6144 x 4096: pairs 22.9, single CTAs 30.4.
@@ -608,12 +609,13 @@ Plan make_plan(int n_tok, int rows, int n_kb)
 		const double waves = (double)((tiles + slots - 1) / slots), active = (double)((tiles < slots ? tiles : slots) * ctas);
 		const double per_sm = two && tiles > alone[ctas] ? 2 : 1;
 		const double bytes = (128 + (pair ? bn / 2 : bn)) * 128.0;
-		const double issue = panels > 1 ? 110 : 500;
-		const double products = pair ? 210 + 1.5 * bn : 4 * fmax(57.0, 44 + 0.36 * bn) * per_sm;
-		const double load = fmax(bytes * per_sm / 62, active * bytes / 8000);
+		const double issue = panels > 1 ? 82 : 500;
+		const double products = pair ? 81 + 2.17 * bn : 4 * fmax(56.5, 44 + 0.36 * bn) * per_sm;
+		const double load = fmax(bytes * per_sm / 62, active * bytes / 8250);
 		const double columns = (double)((n_kb + split - 1) / split) * fmax(fmax(issue, products), load);
-		double t = fmax(waves * columns, (double)rows * n_kb * KB / 3300) + (pair ? 6300 : 5400) + 12.0 * bn * waves * (split > 1 ? 0.5 : 1);
-		if (split > 1) t += 3600 + 77 * bn;
+		double t = fmax(waves * columns, (double)rows * n_kb * KB / 3300) + (pair ? 6470 : 4770) +
+		           (pair ? 9.2 : 14.2) * bn * waves * (split > 1 ? 0.5 : 1);
+		if (split > 1) t += 3300 + 82 * bn;
 		if (best.bn == 0 || t < least)
 		{
 			least = t;
