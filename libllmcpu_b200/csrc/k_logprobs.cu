@@ -18,8 +18,11 @@
 //
 // Bound by memory where rows are many (2047 x 128256: 159 us, the copy rate); a
 // row is shared by up to eight CTAs (a cluster, whose parts meet in the first
-// one's shared memory) where they are few: 64 x 151936 with 5 alternatives 14 us
-// (the copy rate: 5.9; 4 of it the selection), 1 x 262144 with 20 8.9 us.
+// one's shared memory) where they are few: 64 x 151936 with 5 alternatives 13.4
+// us (the copy rate: 5.9), 1 x 262144 with 20 8.1 us. Their ends are short chains:
+// the largest first (redux), then sums; every warp's parts straight to the first
+// CTA; a thread's group read again while its sums are joined; runs merged by
+// counting (14.4 and 8.9 us with pairwise joins and bitonic merges of the parts).
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -99,23 +102,30 @@ __device__ __forceinline__ Key lp_merge(Key a, Key b, int lane)
 	return a;
 }
 
+__device__ __forceinline__ float lp_max(float x)
+{
+	float m;
+	asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+	return m;
+}
+
 // What a part of a row knows of its softmax, in base 2: the largest logit, the sum of e = 2^((x - m) k) and that of e
 // times its exponent.
 struct Stat
 {
 	float m, z, h;
 };
-__device__ __forceinline__ Stat lp_join(Stat a, Stat b, float k)
+// A warp's parts as one, in every lane: first the largest logit, then sums.
+__device__ __forceinline__ Stat lp_join(Stat s, float k)
 {
-	const float m = fmaxf(a.m, b.m);
-	// (held above -infinity, so that an empty part adds zeros)
-	const float da = fmaxf((a.m - m) * k, -1e5f), db = fmaxf((b.m - m) * k, -1e5f);
-	const float ca = ex2(da), cb = ex2(db);
-	return {m, a.z * ca + b.z * cb, ca * (a.h + da * a.z) + cb * (b.h + db * b.z)};
-}
-__device__ __forceinline__ Stat lp_shfl(Stat s, int d)
-{
-	return {__shfl_xor_sync(0xffffffffu, s.m, d), __shfl_xor_sync(0xffffffffu, s.z, d), __shfl_xor_sync(0xffffffffu, s.h, d)};
+	const float m = lp_max(s.m);
+	const float d = fmaxf((s.m - m) * k, -1e5f), c = ex2(d); // (held above -infinity, so that an empty part adds zeros)
+	s.h = c * (s.h + d * s.z);
+	s.z *= c;
+	s.m = m;
+#pragma unroll
+	for (int i = 16; i > 0; i >>= 1) s.z += __shfl_xor_sync(0xffffffffu, s.z, i), s.h += __shfl_xor_sync(0xffffffffu, s.h, i);
+	return s;
 }
 
 struct LpArgs
@@ -123,14 +133,6 @@ struct LpArgs
 	nncu_logprobs l;
 	float k; // scale / ln 2
 	int parts; // CTAs that share a row
-};
-
-// What a CTA knows of its part of a row.
-struct Part
-{
-	Key top[LP_TOP];
-	Stat stat;
-	int before;
 };
 
 // A row's share of one CTA, in vectors of four logits that lie on 16 bytes: the row's first and last one may be cut.
@@ -195,77 +197,75 @@ template <int T>
 struct Found
 {
 	static constexpr int WARPS = T / 32, MOST = LP_TOP * 4 * LP_ITEMS + WARPS * LP_TOP;
-	Key keys[MOST], bound[WARPS * LP_FIRST], lists[WARPS][LP_TOP], least;
+	Key keys[MOST], lists[WARPS][LP_TOP];
+	float bound[WARPS * LP_FIRST], least;
 	int n, n_again;
 	short again[T];
 };
 
-// The likeliest tokens of the CTA's share into top[LP_TOP], falling (0: none).
+// The likeliest tokens of the CTA's share into out[LP_TOP], falling (0: none); v: the thread's logits of its best group.
 template <int T>
-__device__ __forceinline__ void lp_select(const Share& sh, const Best& b, int top, Found<T>& f, Key* out)
+__device__ __forceinline__ void lp_select(const Share& sh, const Best& b, const float (&v)[4 * LP_ITEMS], int top, Found<T>& f, Key* out)
 {
-	constexpr int WARPS = Found<T>::WARPS, MOST = Found<T>::MOST;
+	constexpr int WARPS = Found<T>::WARPS, MOST = Found<T>::MOST, BOUNDS = WARPS * LP_FIRST;
 	const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	// The thread's first candidate: the first of its largest logits, in the group that reached them first.
-	float v[4 * LP_ITEMS];
-	sh.template read<T>(b.group, v);
 	const auto index = [&](int i) { return sh.index(b.group + (i / 4) * T + tid, i % 4); };
-	int at = 0;
-#pragma unroll
-	for (int i = 4 * LP_ITEMS - 1; i >= 0; --i)
-		if (v[i] == b.value) at = (i / 4) * 4 * T + i % 4;
-	const Key first = lp_key(b.value, sh.index(b.group + tid, 0) + at); // (0 where all are masked)
-	// The warp's first few of those, one after another.
-	Key left = first;
+	// The warp's first few of its threads' largest, one after another.
+	float left = b.value;
 #pragma unroll
 	for (int i = 0; i < LP_FIRST; ++i)
 	{
-		const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32));
-		const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(left >> 32) == hi ? (uint32_t)left : 0u);
-		const Key k = (Key)hi << 32 | lo;
-		if (left == k) left = 0;
-		if (lane == 0) f.bound[warp * LP_FIRST + i] = k;
+		const float m = lp_max(left);
+		const uint32_t with = __ballot_sync(0xffffffffu, left == m);
+		if (lane == __ffs(with) - 1) left = -INFINITY;
+		if (lane == 0) f.bound[warp * LP_FIRST + i] = m;
 	}
-	if (tid == 0) f.n = f.n_again = 0, f.least = 0;
+	if (tid == 0) f.n = f.n_again = 0, f.least = -INFINITY;
 	if (tid < LP_TOP) out[tid] = 0;
 	__syncthreads();
-	// The top-th of them is a bound: that many tokens are not after it.
-	if (tid < WARPS * LP_FIRST)
+	// The top-th of them is a bound: that many logits are not below it. Eight threads count for each.
 	{
-		const Key k = f.bound[tid];
-		int above = 0;
-#pragma unroll 8
-		for (int j = 0; j < WARPS * LP_FIRST; ++j) above += f.bound[j] > k;
-		if (k != 0 && above == top - 1) f.least = k;
+		static_assert(T == 8 * BOUNDS, "eight threads a bound");
+		const float x = f.bound[tid / 8];
+		int n = 0; // those above x, and in the upper half those not below it
+#pragma unroll
+		for (int j = tid % 8; j < BOUNDS; j += 8) n += (f.bound[j] > x) + ((f.bound[j] >= x) << 16);
+#pragma unroll
+		for (int d = 4; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+		if (x > -INFINITY && (n & 0xFFFF) < top && (n >> 16) >= top) f.least = x; // (equal ones write the same)
 	}
 	__syncthreads();
-	// What is not after it lies with the threads whose first is not, nearly always in that one's group.
-	Key least = f.least;
+	// What is not below it lies with the threads whose largest is not, nearly always in that one's group.
 	const auto push = [&](Key k) {
 		const int i = atomicAdd(&f.n, 1);
 		if (i < MOST) f.keys[i] = k;
 	};
-	const auto owners = [&]() {
-		if (first == 0 || first < least) return;
-		if (least == 0 ? b.second > -INFINITY : b.second >= lp_value(least)) // more may lie in the thread's other groups
-			f.again[atomicAdd(&f.n_again, 1)] = (short)tid;
-		else
+	const auto give = [&](float low, Key least) {
+		if (low == -INFINITY ? b.second > low : b.second >= low) // more may lie in the thread's other groups
 		{
-			push(first);
-			const float low = lp_value(least);
-			int more = 0;
-#pragma unroll
-			for (int i = 0; i < 4 * LP_ITEMS; ++i) more += least == 0 ? v[i] > -INFINITY : v[i] >= low;
-			if (more > 1)
-#pragma unroll
-				for (int i = 0; i < 4 * LP_ITEMS; ++i)
-				{
-					const Key k = lp_key(v[i], index(i));
-					if (k != 0 && k != first && k >= least) push(k);
-				}
+			f.again[atomicAdd(&f.n_again, 1)] = (short)tid;
+			return;
 		}
+		uint32_t those = 0;
+#pragma unroll
+		for (int i = 0; i < 4 * LP_ITEMS; ++i) those |= (v[i] >= low && v[i] > -INFINITY ? 1u : 0u) << i;
+		if ((those & (those - 1)) == 0) // one: the largest
+		{
+			const int i = __ffs(those) - 1;
+			const Key k = lp_key(b.value, index(i));
+			if (k >= least) push(k);
+			return;
+		}
+#pragma unroll
+		for (int i = 0; i < 4 * LP_ITEMS; ++i)
+			if (those >> i & 1)
+			{
+				const Key k = lp_key(v[i], index(i));
+				if (k >= least) push(k);
+			}
 	};
-	owners();
+	const float low = f.least;
+	if (b.value > -INFINITY && b.value >= low) give(low, 0);
 	__syncthreads();
 	for (int w = warp; w < f.n_again; w += WARPS) // those threads' vectors once more, a warp a thread
 		for (int j = sh.v0 + f.again[w] + lane * T; j < sh.v1; j += 32 * T)
@@ -274,16 +274,18 @@ __device__ __forceinline__ void lp_select(const Share& sh, const Best& b, int to
 			const float e[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
 			for (int c = 0; c < 4; ++c)
-			{
-				const Key k = lp_key(e[c], sh.index(j, c));
-				if (k != 0 && k >= least) push(k);
-			}
+				if (e[c] >= low && e[c] > -INFINITY) push(lp_key(e[c], sh.index(j, c)));
 		}
 	__syncthreads();
 	if (f.n > MOST)
 	{
-		// Too many: few warps hold the largest, or most of the row is equal. The top-th of all threads' firsts bounds the
-		// owners to `top` of them, and a warp's list what it takes of each.
+		// Too many: few warps hold the largest, or most of the row is equal. The top-th of all threads' firsts (by value and
+		// index) bounds the owners to `top` of them, and a warp's list what it takes of each.
+		int at = 0; // (the first of the largest, in the group that reached them first)
+#pragma unroll
+		for (int i = 4 * LP_ITEMS - 1; i >= 0; --i)
+			if (v[i] == b.value) at = (i / 4) * 4 * T + i % 4;
+		const Key first = lp_key(b.value, sh.index(b.group + tid, 0) + at); // (0 where all are masked)
 		Key list = lp_sort(first, lane);
 		f.lists[warp][lane] = list;
 		__syncthreads();
@@ -292,10 +294,10 @@ __device__ __forceinline__ void lp_select(const Share& sh, const Best& b, int to
 			if (warp < d) f.lists[warp][lane] = list = lp_merge(list, f.lists[warp + d][lane], lane);
 			__syncthreads();
 		}
-		least = f.lists[0][top - 1];
+		const Key least = f.lists[0][top - 1];
 		if (tid == 0) f.n = f.n_again = 0;
 		__syncthreads();
-		owners();
+		if (first != 0 && first >= least) give(least ? lp_value(least) : -INFINITY, least);
 		__syncthreads();
 		list = 0;
 		for (int w = warp; w < f.n_again; w += WARPS)
@@ -325,13 +327,41 @@ __device__ __forceinline__ void lp_select(const Share& sh, const Best& b, int to
 	}
 }
 
+// What the CTAs that share a row know of it, in the first one's shared memory.
+template <bool TOP, int T>
+struct Row
+{
+	Stat stat[LP_CLUSTER][T / 32];
+	int before[LP_CLUSTER][T / 32];
+	Key top[TOP ? LP_CLUSTER : 1][LP_TOP], all[LP_TOP];
+	float m;
+	double lz;
+};
+
+// The falling runs of `parts` CTAs into one (all: zeros before), each key at the number of keys above it.
+template <class R>
+__device__ __forceinline__ void lp_merge_parts(R& row, int parts, int lane, int warp)
+{
+	if (warp >= parts) return;
+	const Key k = row.top[warp][lane];
+	int above[LP_CLUSTER] = {};
+#pragma unroll
+	for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+		for (int p = 0; p < LP_CLUSTER; ++p) above[p] += row.top[p][above[p] + d - 1] > k ? d : 0; // (past `parts`: not used)
+	int n = 0;
+#pragma unroll
+	for (int p = 0; p < LP_CLUSTER; ++p)
+		if (p < parts) n += above[p] + (row.top[p][above[p]] > k); // (all 32 may be above)
+	if (k != 0 && n < LP_TOP) row.all[n] = k;
+}
+
 template <bool TOP, int T>
 __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTAS) logprobs_kernel(const LpArgs a)
 {
 	constexpr int WARPS = T / 32, GROUP = T * LP_ITEMS; // vectors (of four logits) that the CTA takes at a time
-	__shared__ Part parts[LP_CLUSTER]; // this CTA's own at its number; the first CTA of a cluster gets the others'
-	__shared__ Stat warp_stat[WARPS];
-	__shared__ int warp_before[WARPS];
+	static_assert(WARPS >= LP_CLUSTER && WARPS <= 32, "a warp a part, a lane a warp");
+	__shared__ Row<TOP, T> row;
 	__shared__ std::conditional_t<TOP, Found<T>, int> found;
 	const nncu_logprobs& l = a.l;
 	const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -406,64 +436,66 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 		if (hidden) before += max(0, min(v_first, 4 * sh.v1 - sh.cut) - max(0, 4 * sh.v0 - sh.cut));
 	}
 
-#pragma unroll
-	for (int d = 16; d > 0; d >>= 1) s = lp_join(s, lp_shfl(s, d), k);
+	if constexpr (TOP) sh.template read<T>(best.group, v); // (for the selection, while the sums are joined)
+	s = lp_join(s, k);
 	before = __reduce_add_sync(0xffffffffu, before);
-	if (lane == 0) warp_stat[warp] = s, warp_before[warp] = before;
-	Part& mine = parts[part];
-	if constexpr (TOP) lp_select(sh, best, l.top, found, mine.top);
-	__syncthreads();
-	if (warp == 0)
+	if (a.parts > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); // (the first CTA has begun)
+	Row<TOP, T>& to = a.parts > 1 ? *static_cast<Row<TOP, T>*>(cluster_map(&row, 0)) : row;
+	if (lane == 0) to.stat[part][warp] = s, to.before[part][warp] = before;
+	if constexpr (TOP)
 	{
-		s = lane < WARPS ? warp_stat[lane] : Stat{-FLT_MAX, 0.0f, 0.0f};
-		before = __reduce_add_sync(0xffffffffu, lane < WARPS ? warp_before[lane] : 0);
-#pragma unroll
-		for (int d = WARPS / 2; d > 0; d >>= 1) s = lp_join(s, lp_shfl(s, d), k);
+		if (warp == 0) row.all[lane] = 0;
+		lp_select(sh, best, v, l.top, found, a.parts > 1 ? to.top[part] : row.all);
 	}
+	__syncthreads();
 	if (a.parts > 1)
 	{
-		// to the cluster's first CTA, which finishes the row
-		asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-		if (warp == 0)
-		{
-			Part* to = static_cast<Part*>(cluster_map(&mine, 0));
-			if (TOP) to->top[lane] = mine.top[lane];
-			if (lane == 0) to->stat = s, to->before = before;
-		}
-		__syncthreads();
 		cluster_sync();
 		if (part != 0) return;
-		if (TOP) // the parts' runs into one
-#pragma unroll
-			for (int d = LP_CLUSTER / 2; d > 0; d >>= 1)
-			{
-				if (warp < d && warp + d < a.parts)
-					parts[warp].top[lane] = lp_merge(parts[warp].top[lane], parts[warp + d].top[lane], lane);
-				__syncthreads();
-			}
-		if (warp == 0)
+		if constexpr (TOP) lp_merge_parts(row, a.parts, lane, warp);
+	}
+	if (warp == WARPS - 1) // (the last one: the first ones merge)
+	{
+		s = Stat{-FLT_MAX, 0.0f, 0.0f}, before = 0;
+		if (lane < WARPS)
 		{
-			s = lane < a.parts ? parts[lane].stat : Stat{-FLT_MAX, 0.0f, 0.0f};
-			before = __reduce_add_sync(0xffffffffu, lane < a.parts ? parts[lane].before : 0);
+			Stat of[LP_CLUSTER];
 #pragma unroll
-			for (int d = LP_CLUSTER / 2; d > 0; d >>= 1) s = lp_join(s, lp_shfl(s, d), k);
+			for (int p = 0; p < LP_CLUSTER; ++p)
+			{
+				of[p] = p < a.parts ? row.stat[p][lane] : Stat{-FLT_MAX, 0.0f, 0.0f};
+				s.m = fmaxf(s.m, of[p].m);
+				before += p < a.parts ? row.before[p][lane] : 0;
+			}
+#pragma unroll
+			for (int p = 0; p < LP_CLUSTER; ++p)
+			{
+				const float d = fmaxf((of[p].m - s.m) * k, -1e5f), c = ex2(d);
+				s.z += c * of[p].z;
+				s.h += c * (of[p].h + d * of[p].z);
+			}
+		}
+		s = lp_join(s, k);
+		before = __reduce_add_sync(0xffffffffu, before);
+		const double lz = log((double)s.z);
+		if (lane == 0)
+		{
+			row.m = s.m, row.lz = lz;
+			if (l.logprob) l.logprob[r] = !in ? 0.0f : s.z == 0.0f ? -INFINITY : (float)(((double)xt - (double)s.m) * (double)l.scale - lz);
+			if (l.rank) l.rank[r] = in ? before : -1;
+			if (l.entropy) l.entropy[r] = s.z == 0.0f ? 0.0f : (float)(lz - (double)s.h * 0.69314718055994530942 / (double)s.z);
 		}
 	}
-	if (warp != 0) return;
-	s.m = __shfl_sync(0xffffffffu, s.m, 0), s.z = __shfl_sync(0xffffffffu, s.z, 0), s.h = __shfl_sync(0xffffffffu, s.h, 0);
-	const double lz = log((double)s.z), scale = (double)l.scale;
-	if (lane == 0)
+	if constexpr (TOP)
 	{
-		if (l.logprob) l.logprob[r] = !in ? 0.0f : s.z == 0.0f ? -INFINITY : (float)(((double)xt - (double)s.m) * scale - lz);
-		if (l.rank) l.rank[r] = in ? before : -1;
-		if (l.entropy) l.entropy[r] = s.z == 0.0f ? 0.0f : (float)(lz - (double)s.h * 0.69314718055994530942 / (double)s.z);
-	}
-	if (TOP && lane < l.top)
-	{
-		const Key key = parts[0].top[lane];
-		if (l.top_ids) l.top_ids[r * l.top + lane] = key ? lp_index(key) : -1;
-		if (l.top_logprobs)
-			l.top_logprobs[r * l.top + lane] = key ? (float)(((double)lp_value(key) - (double)s.m) * scale - lz) : -INFINITY;
+		__syncthreads();
+		if (tid < l.top)
+		{
+			const Key key = row.all[tid];
+			if (l.top_ids) l.top_ids[r * l.top + tid] = key ? lp_index(key) : -1;
+			if (l.top_logprobs)
+				l.top_logprobs[r * l.top + tid] = key ? (float)(((double)lp_value(key) - (double)row.m) * (double)l.scale - row.lz) : -INFINITY;
+		}
 	}
 }
 
