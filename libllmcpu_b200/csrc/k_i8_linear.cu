@@ -597,40 +597,42 @@ Plan make_plan(int n_tok, int rows, int n_kb)
 {
 	// how many clusters run at once with one CTA per SM and with two, by CTAs of a cluster
 	static const int alone[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15}, both[9] = {0, 296, 148, 93, 71, 56, 45, 37, 33};
+	const double from_hbm = (double)rows * n_kb * KB * (1 / 3300.0);
+	const auto larger = [](double a, double b) { return a > b ? a : b; };
 	Plan best{};
-	double least = 0;
-	const auto consider = [&](bool pair, int bn, int split, int panels, bool two) {
-		const int stage = (W_BYTES + (pair ? bn / 2 : bn) * KB) * panels, smem = two ? 107 * 1024 : SMEM_MOST;
-		const int ctas = (pair ? 2 : 1) * split;
-		if (split * panels > n_kb || (smem - 1024) / stage < 2 || (panels > 1 && (smem - 1024) / stage < 3)) return;
-		const long long tiles_o = (rows + (pair ? 255 : 127)) / (pair ? 256 : 128), tiles_t = (n_tok + bn - 1) / bn, tiles = tiles_o * tiles_t;
-		const long long slots = two ? both[ctas] : alone[ctas];
-		if ((two || split > 1) && tiles > 2 * slots && split > 1) return;
-		const double waves = (double)((tiles + slots - 1) / slots), active = (double)((tiles < slots ? tiles : slots) * ctas);
-		const double per_sm = two && tiles > alone[ctas] ? 2 : 1;
-		const double bytes = (128 + (pair ? bn / 2 : bn)) * 128.0;
-		const double issue = panels > 1 ? 82 : 500;
-		const double products = pair ? 81 + 2.17 * bn : 4 * fmax(56.5, 44 + 0.36 * bn) * per_sm;
-		const double load = fmax(bytes * per_sm / 62, active * bytes / 8250);
-		const double columns = (double)((n_kb + split - 1) / split) * fmax(fmax(issue, products), load);
-		double t = fmax(waves * columns, (double)rows * n_kb * KB / 3300) + (pair ? 6470 : 4770) +
-		           (pair ? 9.2 : 14.2) * bn * waves * (split > 1 ? 0.5 : 1);
-		if (split > 1) t += 3300 + 82 * bn;
-		if (best.bn == 0 || t < least)
+	double least = INFINITY;
+	// (two hundred estimates a call: what does not go by the innermost choice is worked out outside of it)
+	const auto consider = [&](bool pair, int bn, int tiles_o) {
+		const int tiles_t = (n_tok + bn - 1) / bn;
+		const double tiles = (double)tiles_o * tiles_t;
+		const double bytes = (128 + (pair ? bn / 2 : bn)) * 128.0, ends = pair ? 6470 : 4770, epilogue = (pair ? 9.2 : 14.2) * bn;
+		for (int split = 1; split <= (pair ? 4 : 8) && split <= n_kb; split += pair ? 1 : split)
 		{
-			least = t;
-			best = {pair, bn, split, panels, (int)tiles_o, (int)tiles_t, smem};
+			const int ctas = (pair ? 2 : 1) * split;
+			const double kb = (n_kb + split - 1) / split, join = split > 1 ? 3300 + 82 * bn : 0;
+			for (int two = 0; two < (pair ? 1 : 2); ++two)
+			{
+				const int smem = two ? 107 * 1024 : SMEM_MOST, slots = two ? both[ctas] : alone[ctas];
+				if (split > 1 && tiles > 2 * slots) continue;
+				const double waves = tiles <= slots ? 1 : tiles <= 2 * slots ? 2 : (double)(((long long)tiles + slots - 1) / slots);
+				const double per_sm = two && tiles > alone[ctas] ? 2 : 1;
+				const double products = pair ? 81 + 2.17 * bn : 4 * larger(56.5, 44 + 0.36 * bn) * per_sm;
+				const double load = bytes * larger(per_sm * (1 / 62.0), (tiles < slots ? tiles : slots) * ctas * (1 / 8250.0));
+				const double panel = larger(products, load), rest = ends + epilogue * waves * (split > 1 ? 0.5 : 1) + join;
+				for (int panels = 1; panels <= 2 && split * panels <= n_kb; ++panels)
+				{
+					const int stage = (W_BYTES + (pair ? bn / 2 : bn) * KB) * panels;
+					if (smem - 1024 < (panels > 1 ? 3 : 2) * stage) continue;
+					const double t = larger(waves * kb * larger(panels > 1 ? 82 : 500, panel), from_hbm) + rest;
+					if (t < least) least = t, best = {pair, bn, split, panels, tiles_o, tiles_t, smem};
+				}
+			}
 		}
 	};
 	const int most = n_tok < 256 ? (n_tok + 15) / 16 * 16 : 256;
-	for (int bn = 16; bn <= most; bn += 16)
-		for (int split = 1; split <= 8; split *= 2)
-			for (int panels = 1; panels <= 2; ++panels)
-				for (int two = 0; two < 2; ++two) consider(false, bn, split, panels, two);
+	for (int bn = 16; bn <= most; bn += 16) consider(false, bn, (rows + 127) / 128);
 	if (n_tok > 32 && rows > 128)
-		for (int bn = 64; bn <= (most + 31) / 32 * 32; bn += 32)
-			for (int split = 1; split <= 4; ++split)
-				for (int panels = 1; panels <= 2; ++panels) consider(true, bn, split, panels, false);
+		for (int bn = 64; bn <= (most + 31) / 32 * 32; bn += 32) consider(true, bn, (rows + 255) / 256);
 	return best;
 }
 
