@@ -18,8 +18,8 @@
 //
 // Bound by memory where rows are many (2047 x 128256: 159 us, the copy rate); a
 // row is shared by up to eight CTAs (a cluster, whose parts meet in the first
-// one's shared memory) where they are few: 64 x 151936 with 5 alternatives 13.4
-// us (the copy rate: 5.9), 1 x 262144 with 20 8.1 us. Their ends are short chains:
+// one's shared memory) where they are few: 64 x 151936 with 5 alternatives 13.2
+// us (the copy rate: 5.9), 1 x 262144 with 20 7.9 us. Their ends are short chains:
 // the largest first (redux), then sums; every warp's parts straight to the first
 // CTA; a thread's group read again while its sums are joined; runs merged by
 // counting (14.4 and 8.9 us with pairwise joins and bitonic merges of the parts).
@@ -386,8 +386,13 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 	Stat s{-FLT_MAX, 0.0f, 0.0f};
 	int before = 0;
 	Best best{-INFINITY, -INFINITY, sh.v0};
+	// Wide CTAs have the next group's loads in flight while they count one (64 x 151936 top 5: 13.2 us, without 13.7);
+	// narrow ones, five to an SM, have no registers for it (four to an SM with them: 300 x 50257 17.7 us, 15.9 without).
+	constexpr bool AHEAD = T == LP_WIDE;
+	float next[4 * LP_ITEMS];
 	for (int g = sh.v0; g < sh.v1;)
 	{
+		if (AHEAD && g + GROUP < sh.v1) sh.template read<T>(g + GROUP, next);
 		float top = -INFINITY;
 #pragma unroll
 		for (int i = 0; i < 4 * LP_ITEMS; ++i) top = fmaxf(top, v[i]);
@@ -426,7 +431,11 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 		s.z += z.x + z.y;
 		s.h += h.x + h.y;
 		g += GROUP;
-		if (g < sh.v1) sh.template read<T>(g, v);
+		if (AHEAD)
+#pragma unroll
+			for (int i = 0; i < 4 * LP_ITEMS; ++i) v[i] = next[i];
+		else if (g < sh.v1)
+			sh.template read<T>(g, v);
 	}
 	if (in && tid == 0)
 	{
@@ -508,24 +517,24 @@ struct LpPlan
 // The least of an estimate, in SM cycles: the waves that the CTAs make of what the GPU holds at once (clusters do not
 // fill every SM) times a CTA's start and end and its share, at a pace of its own or, with others on its SM, at a share
 // of the SM's. Its constants were fitted to 1900 timings (1 to 2000 rows of 5000 to 262144 logits, from HBM); its
-// choices are 1.7 % slower there than the best of all in the mean, 20 % at worst. Both sides, microseconds: 64 rows of
-// 151936: wide CTAs, four a row 14.0, narrow ones 17.0; 2000 rows: narrow ones 187, wide ones 194; 1 x 262144: eight
-// wide CTAs 5.3, one 20.6.
+// choices are 0.9 % slower there than the best of all in the mean, 19 % at worst. Both sides, microseconds, with 5
+// alternatives: 64 rows of 151936: wide CTAs, four a row 13.6, narrow ones 17.1; 2000 rows: wide ones 212, narrow ones
+// 216 (without alternatives 202 and 186); 1 x 262144: eight wide CTAs 6.9, one 20.4.
 LpPlan lp_plan(long long n, int n_vocab, bool top)
 {
-	static const int filled[] = {148, 148, 142, 132}; // SMs that clusters of 1, 2, 4, 8 fill
 	LpPlan best{};
 	double least = 0;
 	for (int wide = 1; wide >= 0; --wide)
 		for (int i = 0, parts = 1; parts <= LP_CLUSTER; ++i, parts *= 2)
 		{
+			const int filled[] = {148, 148, 142, wide && top ? 124 : 132}; // SMs that clusters of 1, 2, 4, 8 fill
 			const double slots = filled[i] * (wide ? LP_WIDE_CTAS : LP_NARROW_CTAS), ctas = (double)n * parts;
 			const double beside = fmax(1.0, fmin(ctas, slots) / 148);
-			double ends = wide ? 4000 : 4600;
-			if (top) ends += wide ? 3800 : 2600;
-			if (parts > 1) ends += top ? 1800 : 350;
-			const double pace = fmax(wide ? 0.075 : 0.228, 0.043 * beside); // cycles a logit
-			const double t = ceil(ctas / slots) * (ends * fmax(1.0, 0.13 * beside) + pace * n_vocab / parts);
+			double ends = wide ? 3310 : 3560;
+			if (top) ends += wide ? 1450 : 3600;
+			if (parts > 1) ends += (wide ? 443 : 320) + (top ? 200 : 0);
+			const double pace = fmax(wide ? 0.098 : 0.256, 0.045 * beside); // cycles a logit
+			const double t = ceil(ctas / slots) * (ends * fmax(1.0, 0.163 * beside) + pace * n_vocab / parts);
 			if (best.parts == 0 || t < least) least = t, best = {wide != 0, parts};
 		}
 	return best;
