@@ -167,20 +167,26 @@ __device__ __forceinline__ void land(uint64_t* full, Ring at, int stages)
 
 __device__ __forceinline__ uint32_t pow2_cols(uint32_t n) { return n <= 32 ? 32 : 1u << (32 - __clz(n - 1)); }
 
-// A channel's sums of C tokens from t on, scaled and out; `n` of them are real.
+// What `n` tokens from t on have to add to a channel.
 template <int C>
-__device__ __forceinline__ void put(const Args& a, int t, int o, const int (&acc)[C], const float* xs, float ws, float bias, int n)
+__device__ __forceinline__ void get_add(const Args& a, int t, int o, float (&more)[C], int n)
+{
+	const float* p = a.add + (size_t)t * a.add_stride + o;
+#pragma unroll
+	for (int c = 0; c < C; ++c, p += a.add_stride) more[c] = c < n ? *p : 0.0f;
+}
+
+// A channel's sums of C tokens from t on, scaled and out; `n` of them are real.
+template <bool ADD, int C>
+__device__ __forceinline__ void put(const Args& a, int t, int o, const int (&acc)[C], const float* xs, float ws, float bias,
+                                    const float (&more)[C], int n)
 {
 	float v[C];
 #pragma unroll
 	for (int c = 0; c < C; ++c) v[c] = fmaf(__int2float_rn(acc[c]) * xs[c], ws, bias);
-	if (a.add)
-	{
-		const float* p = a.add + (size_t)t * a.add_stride + o;
+	if (ADD)
 #pragma unroll
-		for (int c = 0; c < C; ++c, p += a.add_stride)
-			if (c < n) v[c] += *p;
-	}
+		for (int c = 0; c < C; ++c) v[c] += more[c];
 	float* y = a.y + (size_t)t * a.y_stride + o;
 	if (n >= C)
 	{
@@ -198,16 +204,37 @@ __device__ __forceinline__ void put(const Args& a, int t, int o, const int (&acc
 constexpr int THREADS = 320; // a warp for the loads, one for the products, eight for the epilogue (two to a quarter of TMEM)
 constexpr int EPI = 256;
 
+// What is added to the tokens first, first + step, ... of a tile's 128 channels, on its way into L2 while its products run
+// (read when they are done, 16 tokens at a time, it took longer than they: 4660 x 2560 to 4096 146 us, so 55, 41 with
+// nothing to add).
+__device__ __forceinline__ void add_ahead(const Args& a, int o0, int t0, int real, int first, int step)
+{
+	for (int i = (int)threadIdx.x - 64; first + step * (i / 4) < real; i += EPI)
+	{
+		const int o = o0 + 32 * (i % 4);
+		if (o >= a.rows) continue;
+		const float* p = a.add + (size_t)(t0 + first + step * (i / 4)) * a.add_stride + o;
+		asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+		if (reinterpret_cast<uintptr_t>(p) & 127) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + min(31, a.rows - 1 - o)));
+	}
+}
+
 // The epilogue of a whole tile from TMEM: this warp's lanes (channels) and its half of the columns, out or, as sums
 // only, into `part` ([token][128 channels]).
+template <bool ADD>
 __device__ __forceinline__ void tile_out(const Args& a, uint32_t tmem, int ch, int o, int t0, int real, const float* xs, float ws,
                                          float bias, int* part)
 {
 	const int side = ((int)threadIdx.x - 64) >> 7, quad = (threadIdx.x >> 5) & 3;
-	const bool in = o < a.rows;
+	const bool in = o < a.rows, adds = ADD && !part && in;
+	float next[16] = {}; // (added: a step ahead)
+	if (adds && 16 * side < real) get_add(a, t0 + 16 * side, o, next, real - 16 * side);
 	for (int c0 = 16 * side; c0 < real; c0 += 32)
 	{
-		float f[16];
+		float f[16], more[16];
+#pragma unroll
+		for (int c = 0; c < 16; ++c) more[c] = next[c];
+		if (adds && c0 + 32 < real) get_add(a, t0 + c0 + 32, o, next, real - c0 - 32);
 		int v[16];
 		tmem_ld16(tmem + ((uint32_t)quad << 21) + c0, f);
 		tmem_wait_ld();
@@ -219,12 +246,13 @@ __device__ __forceinline__ void tile_out(const Args& a, uint32_t tmem, int ch, i
 			for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + ch] = v[c];
 		}
 		else if (in)
-			put<16>(a, t0 + c0, o, v, xs + c0, ws, bias, real - c0);
+			put<ADD>(a, t0 + c0, o, v, xs + c0, ws, bias, more, real - c0);
 	}
 }
 
 // The tokens first, first + step, ... of a tile from the sums of `n` CTAs of the cluster (CTA i's at rank0 + i * rank_step),
 // four channels a lane, a warp a token.
+template <bool ADD>
 __device__ __forceinline__ void join_out(const Args& a, const int* part, int rank0, int rank_step, int n, int first, int step, int o0,
                                          int t0, int real, const float* xs)
 {
@@ -235,9 +263,19 @@ __device__ __forceinline__ void join_out(const Args& a, const int* part, int ran
 	uint32_t from[8];
 #pragma unroll
 	for (int i = 0; i < 8; ++i) from[i] = mapa(smem_u32(part) + 16 * lane, i < n ? rank0 + i * rank_step : rank0);
-	const bool wide = left >= 4 && a.y_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+	const auto in_fours = [&](const float* p, size_t stride) { return left >= 4 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+	const bool wide = in_fours(a.y, a.y_stride), add_wide = ADD && in_fours(a.add, a.add_stride);
 	for (int c = first + step * warp; c < real; c += step * (THREADS / 32))
 	{
+		float4 more = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+		if (ADD)
+		{
+			const float* p = a.add + (size_t)(t0 + c) * a.add_stride + o;
+			if (add_wide)
+				more = *reinterpret_cast<const float4*>(p);
+			else
+				more = make_float4(left > 0 ? p[0] : 0.0f, left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
+		}
 		int4 q[8];
 #pragma unroll
 		for (int i = 0; i < 8; ++i) q[i] = i < n ? ld_cluster4(from[i] + c * 512) : make_int4(0, 0, 0, 0);
@@ -246,12 +284,13 @@ __device__ __forceinline__ void join_out(const Args& a, const int* part, int ran
 		for (int i = 1; i < 8; ++i) sum.x += q[i].x, sum.y += q[i].y, sum.z += q[i].z, sum.w += q[i].w;
 		const int acc[4] = {sum.x, sum.y, sum.z, sum.w};
 		const int t = t0 + c;
+		const float of[4] = {more.x, more.y, more.z, more.w};
 		float v[4];
 #pragma unroll
 		for (int j = 0; j < 4; ++j)
 		{
 			v[j] = fmaf(__int2float_rn(acc[j]) * xs[c], ws[j], bias[j]);
-			if (a.add && j < left) v[j] += a.add[(size_t)t * a.add_stride + o + j];
+			if (ADD) v[j] += of[j];
 		}
 		float* y = a.y + (size_t)t * a.y_stride + o;
 		if (wide)
@@ -269,6 +308,8 @@ __device__ __forceinline__ void join_out(const Args& a, const int* part, int ran
 // share of the columns; their sums meet in shared memory, every CTA adding up
 // the tokens t % split = its rank out of the others' (integers: no order).
 
+// (ADD: its code and registers apart; what adds nothing took one to two percent longer with them.)
+template <bool ADD>
 __global__ void __launch_bounds__(THREADS, 2)
 	i8_split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Args a)
 {
@@ -348,17 +389,18 @@ __global__ void __launch_bounds__(THREADS, 2)
 		const bool in = o < a.rows && split == 1;
 		const float ws = in ? a.ws[o] : 0.0f, bias = in && a.bias ? a.bias[o] : 0.0f;
 		for (int c = (int)threadIdx.x - 64; c < a.bn; c += EPI) xs_s[c] = c < real ? a.xs[t0 + c] : 0.0f;
+		if (ADD) add_ahead(a, o0, t0, real, rank, split);
 		named_sync(1, EPI);
 		const bool ok = wait(&done, 0);
 		tc_fence_after();
-		if (__all_sync(0xffffffffu, ok)) tile_out(a, tmem, ch, o, t0, real, xs_s, ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
+		if (__all_sync(0xffffffffu, ok)) tile_out<ADD>(a, tmem, ch, o, t0, real, xs_s, ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
 		tc_fence_before();
 	}
 	__syncthreads();
 	if (split > 1)
 	{
 		cluster_sync();
-		join_out(a, reinterpret_cast<const int*>(smem), 0, 1, split, rank, split, o0, t0, real, xs_s);
+		join_out<ADD>(a, reinterpret_cast<const int*>(smem), 0, 1, split, rank, split, o0, t0, real, xs_s);
 		cluster_sync(); // nobody reads this CTA's sums any more
 	}
 	if (warp == 1)
@@ -385,6 +427,7 @@ __device__ __forceinline__ void pair_tile(const Args& a, int id, int& o0, int& t
 	t0 = in / size * a.bn;
 }
 
+template <bool ADD>
 __global__ void __launch_bounds__(THREADS, 1)
 	i8_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Args a)
 {
@@ -486,11 +529,19 @@ __global__ void __launch_bounds__(THREADS, 1)
 		const int ch = (warp & 3) * 32 + lane;
 		int n = 0;
 		bool ok = true; // (after a wait that ran out the warp goes on through the barriers, without work)
+		const auto ahead = [&](int id) {
+			if (!ADD || id >= tiles) return;
+			int o0, t0;
+			pair_tile(a, id, o0, t0);
+			add_ahead(a, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), part, split);
+		};
+		ahead(pair);
 		for (int id = pair; id < tiles; id += pairs, ++n)
 		{
 			const int b = n & 1;
 			int o0, t0;
 			pair_tile(a, id, o0, t0);
+			ahead(id + pairs);
 			const int o = o0 + rank * 128 + ch, real = min(a.bn, a.n_tok - t0);
 			const bool in = o < a.rows && split == 1;
 			const float ws = in ? a.ws[o] : 0.0f, bias = in && a.bias ? a.bias[o] : 0.0f;
@@ -500,7 +551,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 			ok = __all_sync(0xffffffffu, ok && wait(&acc_full[b], (uint32_t)(n / 2) & 1));
 			if (!ok) continue;
 			tc_fence_after();
-			tile_out(a, tmem + b * 256, ch, o, t0, real, xs_s[b], ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
+			tile_out<ADD>(a, tmem + b * 256, ch, o, t0, real, xs_s[b], ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
 			tc_fence_before();
 			__syncwarp();
 			if (lane == 0) arrive_cluster(mapa(smem_u32(&acc_empty[b]), first));
@@ -512,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 	{
 		int o0, t0;
 		pair_tile(a, pair, o0, t0);
-		join_out(a, reinterpret_cast<const int*>(smem), rank, 2, split, part, split, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), xs_s[0]);
+		join_out<ADD>(a, reinterpret_cast<const int*>(smem), rank, 2, split, part, split, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), xs_s[0]);
 		cluster_sync(); // nobody reads this CTA's sums any more
 	}
 	if (warp == 1)
@@ -564,9 +615,11 @@ int configure()
 	if (ce != cudaSuccess) return (int)ce;
 	if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
 	if (configured[dev]) return 0;
-	ce = cudaFuncSetAttribute(i8_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
-	if (ce == cudaSuccess) ce = cudaFuncSetAttribute(i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
-	if (ce != cudaSuccess) return (int)ce;
+	for (const auto kernel : {i8_split_kernel<false>, i8_split_kernel<true>, i8_pair_kernel<false>, i8_pair_kernel<true>})
+	{
+		ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST);
+		if (ce != cudaSuccess) return (int)ce;
+	}
 	configured[dev] = true;
 	return 0;
 }
@@ -670,10 +723,10 @@ int launch_i8_linear(const nncu_i8_linear& l, void* stream)
 	if (p.pair)
 	{
 		cfg.gridDim = dim3(2 * (unsigned)(p.split > 1 ? tiles * p.split : min(tiles, (long long)SMS / 2)));
-		return (int)cudaLaunchKernelEx(&cfg, i8_pair_kernel, xm, wm, a);
+		return (int)cudaLaunchKernelEx(&cfg, l.add ? i8_pair_kernel<true> : i8_pair_kernel<false>, xm, wm, a);
 	}
 	cfg.gridDim = dim3((unsigned)(tiles * p.split));
-	return (int)cudaLaunchKernelEx(&cfg, i8_split_kernel, xm, wm, a);
+	return (int)cudaLaunchKernelEx(&cfg, l.add ? i8_split_kernel<true> : i8_split_kernel<false>, xm, wm, a);
 }
 
 int i8_error_word(int* word)
