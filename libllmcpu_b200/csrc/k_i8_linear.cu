@@ -302,6 +302,23 @@ __device__ __forceinline__ void join_out(const Args& a, const int* part, int ran
 	}
 }
 
+// Channel tiles that are walked together: their weights come from HBM once and the rows of y are written whole.
+constexpr int P_GROUP = 32;
+
+// The channels (`wide` a tile) and tokens of tile `id`.
+__device__ __forceinline__ void place(const Args& a, int id, int wide, int& o0, int& t0)
+{
+	if (a.tiles_t == 1)
+	{
+		o0 = id * wide, t0 = 0;
+		return;
+	}
+	const int per = P_GROUP * a.tiles_t, g = id / per, in = id % per;
+	const int size = min(P_GROUP, a.tiles_o - g * P_GROUP);
+	o0 = (g * P_GROUP + in % size) * wide;
+	t0 = in / size * a.bn;
+}
+
 // ---- few tokens ------------------------------------------------------------------------
 //
 // A cluster of `split` CTAs per tile of 128 channels x bn tokens, each with its
@@ -320,7 +337,8 @@ __global__ void __launch_bounds__(THREADS, 2)
 	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	const int split = a.split, rank = (int)blockIdx.x % split; // (clusters lie along x)
-	const int tile = (int)(blockIdx.x / split), o0 = tile % a.tiles_o * 128, t0 = tile / a.tiles_o * a.bn;
+	int o0, t0;
+	place(a, (int)(blockIdx.x / split), 128, o0, t0);
 	const int k0 = (int)((long long)a.n_kb * rank / split), n = (int)((long long)a.n_kb * (rank + 1) / split) - k0;
 	const uint32_t x_at = W_BYTES * a.panels, stage = x_at + a.bn * KB * a.panels, cols = pow2_cols(a.bn);
 	const int real = min(a.bn, a.n_tok - t0);
@@ -417,16 +435,6 @@ __global__ void __launch_bounds__(THREADS, 2)
 // (cta_group::2) of both SMs' tensor cores reads both. Two accumulators in TMEM:
 // the epilogue of a tile runs beside the next one's products.
 
-constexpr int P_GROUP = 32; // channel tiles that are walked together: their weights stay in L2 and the rows of y are written whole
-
-__device__ __forceinline__ void pair_tile(const Args& a, int id, int& o0, int& t0)
-{
-	const int per = P_GROUP * a.tiles_t, g = id / per, in = id % per;
-	const int size = min(P_GROUP, a.tiles_o - g * P_GROUP);
-	o0 = (g * P_GROUP + in % size) * 256;
-	t0 = in / size * a.bn;
-}
-
 template <bool ADD>
 __global__ void __launch_bounds__(THREADS, 1)
 	i8_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Args a)
@@ -473,7 +481,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 		for (int id = pair; id < tiles && ok; id += pairs)
 		{
 			int o0, t0;
-			pair_tile(a, id, o0, t0);
+			place(a, id, 256, o0, t0);
 			for (int k = 0; k < n_kb; ++k, at.next(a.stages))
 			{
 				if (at.round > 0 && !(ok = __all_sync(0xffffffffu, wait(&empty[at.s], (at.round - 1) & 1)))) break;
@@ -532,7 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 		const auto ahead = [&](int id) {
 			if (!ADD || id >= tiles) return;
 			int o0, t0;
-			pair_tile(a, id, o0, t0);
+			place(a, id, 256, o0, t0);
 			add_ahead(a, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), part, split);
 		};
 		ahead(pair);
@@ -540,7 +548,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 		{
 			const int b = n & 1;
 			int o0, t0;
-			pair_tile(a, id, o0, t0);
+			place(a, id, 256, o0, t0);
 			ahead(id + pairs);
 			const int o = o0 + rank * 128 + ch, real = min(a.bn, a.n_tok - t0);
 			const bool in = o < a.rows && split == 1;
@@ -562,7 +570,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 	if (split > 1) // (one tile a cluster)
 	{
 		int o0, t0;
-		pair_tile(a, pair, o0, t0);
+		place(a, pair, 256, o0, t0);
 		join_out<ADD>(a, reinterpret_cast<const int*>(smem), rank, 2, split, part, split, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), xs_s[0]);
 		cluster_sync(); // nobody reads this CTA's sums any more
 	}
@@ -683,9 +691,10 @@ Plan make_plan(int n_tok, int rows, int n_kb)
 		}
 	};
 	const int most = n_tok < 256 ? (n_tok + 15) / 16 * 16 : 256;
-	for (int bn = 16; bn <= most; bn += 16) consider(false, bn, (rows + 127) / 128);
+	// (from the widest: of equal estimates the one with the fewest copies of the weights, 20 x 4096 to 34146 24 us, 43)
+	for (int bn = most; bn >= 16; bn -= 16) consider(false, bn, (rows + 127) / 128);
 	if (n_tok > 32 && rows > 128)
-		for (int bn = 64; bn <= (most + 31) / 32 * 32; bn += 32) consider(true, bn, (rows + 255) / 256);
+		for (int bn = (most + 31) / 32 * 32; bn >= 64; bn -= 32) consider(true, bn, (rows + 255) / 256);
 	return best;
 }
 

@@ -193,6 +193,7 @@ LINEAR = [  # tokens, rows, cols, bias, add (2: y itself), values between rows o
     (300, 4096, 2560, 0, 1, 0), (777, 2560, 2048, 1, 0, 0), (1000, 100, 96, 0, 0, 0), (1025, 1537, 130, 1, 1, 1),
     (200, 2560, 10240, 0, 1, 0), (520, 2000, 20000, 1, 0, 1), (333, 515, 9000, 1, 2, 1), (1500, 300, 16384, 0, 0, 0),
     (200, 20480, 300, 0, 0, 0), (4099, 6200, 300, 1, 0, 3),
+    (600, 5000, 130, 1, 1, 3), (270, 9000, 64, 0, 2, 0), (2050, 1300, 3000, 1, 1, 2), (2050, 1300, 3000, 0, 2, 0), (900, 700, 640, 0, 1, 0),
     (2500, 40, 700, 0, 0, 0), (2048, 2048, 1024, 0, 0, 0), (5, 40000, 200, 0, 0, 0), (2, 3, 131071, 0, 0, 0),
     (40, 16, 100000, 0, 0, 0), (4100, 130, 16, 1, 2, 2),
 ]
