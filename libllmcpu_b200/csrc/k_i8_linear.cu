@@ -643,16 +643,17 @@ struct Plan
 
 // Which kernel, how many tokens a tile, over how many CTAs (pairs) a tile's columns are split, one or two panels a
 // stage, one CTA per SM or two (of half the memory): the least of an estimate in SM cycles. Its constants were
-// fitted to 6700 timings of 167 shapes (1 to 4096 tokens, 128 to 262144 channels, 300 to 16384 columns, weights from
-// HBM); the choices it makes there are 2.5 % slower than the best of all in the mean, 16 % at worst. What they stand for:
+// fitted to 7000 timings of 180 shapes (1 to 4096 tokens, 128 to 262144 channels, 300 to 16384 columns, weights from
+// HBM); the choices it makes there are 1.9 % slower than the best of all in the mean, 14 % at worst. What they stand for:
 //  - a panel costs the issue of its copies and products (500 alone, 82 where two go together), its products (a pair's
 //    81 + 2.17 a token, a single CTA's four of 56.5 or 44 + 0.36 a token), its bytes into an SM (62 a cycle) or, over
 //    all SMs, out of L2 (8250 a cycle), whichever is the most;
 //  - clusters of 4 and more do not fill every SM;
 //  - the weights come from HBM at 3300 bytes a cycle;
-//  - a launch has a start and an end, an epilogue by token, a split tile the joining of its parts.
+//  - a launch has a start and an end, and so has each CTA that runs alone on its SM after another; there is an epilogue
+//    by token, and a split tile has the joining of its parts.
 // Both sides, microseconds: 1 token, 6144 channels, 4096 columns: whole columns, two panels 7.5, one panel 8.8, split
-// over four 8.3; 1 x 2560 x 10240: split over eight 8.1, whole 12.0; 777 x 2560 x 2048: single CTAs 7.7, pairs 8.6;
+// over four 8.3; 1 x 2560 x 10240: split over eight 8.1, whole 12.0; 777 x 2560 x 2048: single CTAs 7.9, pairs 8.7;
 // 1024 x 6144 x 4096: pairs 22.9, single CTAs 30.4.
 Plan make_plan(int n_tok, int rows, int n_kb)
 {
@@ -666,7 +667,7 @@ Plan make_plan(int n_tok, int rows, int n_kb)
 	const auto consider = [&](bool pair, int bn, int tiles_o) {
 		const int tiles_t = (n_tok + bn - 1) / bn;
 		const double tiles = (double)tiles_o * tiles_t;
-		const double bytes = (128 + (pair ? bn / 2 : bn)) * 128.0, ends = pair ? 6470 : 4770, epilogue = (pair ? 9.2 : 14.2) * bn;
+		const double bytes = (128 + (pair ? bn / 2 : bn)) * 128.0, ends = pair ? 7800 : 4770, epilogue = (pair ? 9.2 : 14.2) * bn;
 		for (int split = 1; split <= (pair ? 4 : 8) && split <= n_kb; split += pair ? 1 : split)
 		{
 			const int ctas = (pair ? 2 : 1) * split;
@@ -679,7 +680,7 @@ Plan make_plan(int n_tok, int rows, int n_kb)
 				const double per_sm = two && tiles > alone[ctas] ? 2 : 1;
 				const double products = pair ? 81 + 2.17 * bn : 4 * larger(56.5, 44 + 0.36 * bn) * per_sm;
 				const double load = bytes * larger(per_sm * (1 / 62.0), (tiles < slots ? tiles : slots) * ctas * (1 / 8250.0));
-				const double panel = larger(products, load), rest = ends + epilogue * waves * (split > 1 ? 0.5 : 1) + join;
+				const double panel = larger(products, load), rest = ends + (pair || two ? 0 : 3000 * (waves - 1)) + epilogue * waves * (split > 1 ? 0.5 : 1) + join;
 				for (int panels = 1; panels <= 2 && split * panels <= n_kb; ++panels)
 				{
 					const int stage = (W_BYTES + (pair ? bn / 2 : bn) * KB) * panels;
