@@ -120,10 +120,10 @@ constexpr float MAGIC = 12582912.0f; // 1.5 * 2^23: a sum's low bits are the rou
 
 // A thread's codes, x / s rounded to the nearest integer n, ties to even, four to a word. The quotient is corrected once, so
 // that half integers come out as such and round to even. What is left of x, d = x - n s (exact: about s / 2 at most, in units
-// of s's or x's last bit), then says whether n is right: where 2 |d| passes s (halving the least steps would round), x lies closer to a border than a float
-// quotient tells, and n is one off. Of 32-bit inputs one in a million does: the largest |d| is returned, and i8_codes_exact
-// writes such a thread's codes once more. Of 16-bit inputs one in two thousand does (their scale is a rounded one too):
-// they are put right here.
+// of s's or x's last bit), then says whether n is right: where 2 |d| passes s (halving the least steps would round), x lies
+// closer to a border than a float quotient tells, and n is one off. Of 32-bit inputs one in a million does: the largest |d|
+// is returned, and i8_codes_exact writes such a thread's codes once more. Of 16-bit inputs one in two thousand does (their
+// scale is a rounded one too): they are put right here.
 template <bool NARROW>
 __device__ __forceinline__ float i8_codes(const float (&v)[Q_VALUES], float s, float inv, bool bad, uint32_t (&w)[Q_VALUES / 4])
 {

@@ -313,7 +313,7 @@ __device__ __forceinline__ void place(const Args& a, int id, int wide, int& o0, 
 		o0 = id * wide, t0 = 0;
 		return;
 	}
-	const int per = P_GROUP * a.tiles_t, g = id / per, in = id % per;
+	const int per = min(P_GROUP, a.tiles_o) * a.tiles_t, g = id / per, in = id % per;
 	const int size = min(P_GROUP, a.tiles_o - g * P_GROUP);
 	o0 = (g * P_GROUP + in % size) * wide;
 	t0 = in / size * a.bn;
