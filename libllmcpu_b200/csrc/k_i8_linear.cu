@@ -131,11 +131,9 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank)
 	asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
 	return r;
 }
-__device__ __forceinline__ int4 ld_cluster4(uint32_t addr)
+__device__ __forceinline__ void st_cluster(uint32_t addr, int v)
 {
-	int4 v;
-	asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-	return v;
+	asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar)
 {
@@ -204,29 +202,40 @@ __device__ __forceinline__ void put(const Args& a, int t, int o, const int (&acc
 constexpr int THREADS = 320; // a warp for the loads, one for the products, eight for the epilogue (two to a quarter of TMEM)
 constexpr int EPI = 256;
 
-// What is added to the tokens first, first + step, ... of a tile's 128 channels, on its way into L2 while its products run
+// What is added to a tile's tokens from `from` to `to`, of 128 channels, on its way into L2 while its products run
 // (read when they are done, 16 tokens at a time, it took longer than they: 4660 x 2560 to 4096 146 us, so 55, 41 with
 // nothing to add).
-__device__ __forceinline__ void add_ahead(const Args& a, int o0, int t0, int real, int first, int step)
+__device__ __forceinline__ void add_ahead(const Args& a, int o0, int t0, int from, int to)
 {
-	for (int i = (int)threadIdx.x - 64; first + step * (i / 4) < real; i += EPI)
+	for (int i = (int)threadIdx.x - 64; from + i / 4 < to; i += EPI)
 	{
 		const int o = o0 + 32 * (i % 4);
 		if (o >= a.rows) continue;
-		const float* p = a.add + (size_t)(t0 + first + step * (i / 4)) * a.add_stride + o;
+		const float* p = a.add + (size_t)(t0 + from + i / 4) * a.add_stride + o;
 		asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 		if (reinterpret_cast<uintptr_t>(p) & 127) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + min(31, a.rows - 1 - o)));
 	}
 }
 
+// Where the columns of a tile are split: CTA `at` of `n` finishes the tile's tokens from at * per on, and every CTA puts
+// its sums of them into that one's shared memory ([CTA][token][128 channels] from `base` on), behind its stages, which may
+// still be read. One barrier later they are all there, and nobody looks into another CTA any more.
+struct Join
+{
+	uint32_t base;
+	int n, at, per, rank0, rank_step; // (CTA i is the cluster's rank0 + i * rank_step)
+	__device__ __forceinline__ int from() const { return at * per; }
+	__device__ __forceinline__ int to(int real) const { return min(real, from() + per); }
+};
+
 // The epilogue of a whole tile from TMEM: this warp's lanes (channels) and its half of the columns, out or, as sums
-// only, into `part` ([token][128 channels]).
+// only, to the CTAs that join them.
 template <bool ADD>
 __device__ __forceinline__ void tile_out(const Args& a, uint32_t tmem, int ch, int o, int t0, int real, const float* xs, float ws,
-                                         float bias, int* part)
+                                         float bias, const Join& join)
 {
 	const int side = ((int)threadIdx.x - 64) >> 7, quad = (threadIdx.x >> 5) & 3;
-	const bool in = o < a.rows, adds = ADD && !part && in;
+	const bool in = o < a.rows, adds = ADD && join.n == 1 && in;
 	float next[16] = {}; // (added: a step ahead)
 	if (adds && 16 * side < real) get_add(a, t0 + 16 * side, o, next, real - 16 * side);
 	for (int c0 = 16 * side; c0 < real; c0 += 32)
@@ -240,50 +249,59 @@ __device__ __forceinline__ void tile_out(const Args& a, uint32_t tmem, int ch, i
 		tmem_wait_ld();
 #pragma unroll
 		for (int c = 0; c < 16; ++c) v[c] = __float_as_int(f[c]);
-		if (part)
+		if (join.n > 1)
 		{
+			const uint32_t mine = join.base + (join.at * join.per * 128 + ch) * 4;
+			int to = c0 / join.per, i = c0 - to * join.per;
+			uint32_t there = mapa(mine, join.rank0 + to * join.rank_step);
 #pragma unroll
-			for (int c = 0; c < 16; ++c) part[(c0 + c) * 128 + ch] = v[c];
+			for (int c = 0; c < 16; ++c)
+			{
+				if (i == join.per) i = 0, ++to, there = mapa(mine, join.rank0 + to * join.rank_step);
+				st_cluster(there + i++ * 512, v[c]);
+			}
 		}
 		else if (in)
 			put<ADD>(a, t0 + c0, o, v, xs + c0, ws, bias, more, real - c0);
 	}
 }
 
-// The tokens first, first + step, ... of a tile from the sums of `n` CTAs of the cluster (CTA i's at rank0 + i * rank_step),
-// four channels a lane, a warp a token.
-template <bool ADD>
-__device__ __forceinline__ void join_out(const Args& a, const int* part, int rank0, int rank_step, int n, int first, int step, int o0,
-                                         int t0, int real, const float* xs)
+// The tokens that this CTA joins, from its own shared memory, four channels a lane, a warp a token. `arrive`: the barrier;
+// what does not wait for it is read before. `channel`: the channels' scales and biases.
+template <bool ADD, class Arrive>
+__device__ __forceinline__ void join_out(const Args& a, const Join& join, const int* sums, int o0, int t0, int real, const float* xs,
+                                         const float (*channel)[128], Arrive arrive)
 {
-	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, o = o0 + 4 * lane, left = a.rows - o;
+	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, o = o0 + 4 * lane, left = a.rows - o, end = join.to(real);
 	float ws[4], bias[4];
 #pragma unroll
-	for (int j = 0; j < 4; ++j) ws[j] = j < left ? a.ws[o + j] : 0.0f, bias[j] = j < left && a.bias ? a.bias[o + j] : 0.0f;
-	uint32_t from[8];
-#pragma unroll
-	for (int i = 0; i < 8; ++i) from[i] = mapa(smem_u32(part) + 16 * lane, i < n ? rank0 + i * rank_step : rank0);
+	for (int j = 0; j < 4; ++j) ws[j] = channel[0][4 * lane + j], bias[j] = channel[1][4 * lane + j];
 	const auto in_fours = [&](const float* p, size_t stride) { return left >= 4 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
 	const bool wide = in_fours(a.y, a.y_stride), add_wide = ADD && in_fours(a.add, a.add_stride);
-	for (int c = first + step * warp; c < real; c += step * (THREADS / 32))
+	const auto get = [&](int c) {
+		const float* p = a.add + (size_t)(t0 + c) * a.add_stride + o;
+		if (add_wide) return *reinterpret_cast<const float4*>(p);
+		return make_float4(left > 0 ? p[0] : 0.0f, left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
+	};
+	int c = join.from() + warp;
+	float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+	if (ADD && c < end) next = get(c);
+	__syncwarp();
+	arrive();
+	for (; c < end; c += THREADS / 32)
 	{
-		float4 more = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-		if (ADD)
-		{
-			const float* p = a.add + (size_t)(t0 + c) * a.add_stride + o;
-			if (add_wide)
-				more = *reinterpret_cast<const float4*>(p);
-			else
-				more = make_float4(left > 0 ? p[0] : 0.0f, left > 1 ? p[1] : 0.0f, left > 2 ? p[2] : 0.0f, left > 3 ? p[3] : 0.0f);
-		}
-		int4 q[8];
+		const float4 more = next;
+		if (ADD && c + THREADS / 32 < end) next = get(c + THREADS / 32);
+		const int4* from = reinterpret_cast<const int4*>(sums + (c - join.from()) * 128) + lane;
+		int4 sum = from[0];
 #pragma unroll
-		for (int i = 0; i < 8; ++i) q[i] = i < n ? ld_cluster4(from[i] + c * 512) : make_int4(0, 0, 0, 0);
-		int4 sum = q[0];
-#pragma unroll
-		for (int i = 1; i < 8; ++i) sum.x += q[i].x, sum.y += q[i].y, sum.z += q[i].z, sum.w += q[i].w;
+		for (int i = 1; i < 8; ++i)
+			if (i < join.n)
+			{
+				const int4 q = from[i * join.per * 32];
+				sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+			}
 		const int acc[4] = {sum.x, sum.y, sum.z, sum.w};
-		const int t = t0 + c;
 		const float of[4] = {more.x, more.y, more.z, more.w};
 		float v[4];
 #pragma unroll
@@ -292,7 +310,7 @@ __device__ __forceinline__ void join_out(const Args& a, const int* part, int ran
 			v[j] = fmaf(__int2float_rn(acc[j]) * xs[c], ws[j], bias[j]);
 			if (ADD) v[j] += of[j];
 		}
-		float* y = a.y + (size_t)t * a.y_stride + o;
+		float* y = a.y + (size_t)(t0 + c) * a.y_stride + o;
 		if (wide)
 			*reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
 		else
@@ -322,8 +340,8 @@ __device__ __forceinline__ void place(const Args& a, int id, int wide, int& o0, 
 // ---- few tokens ------------------------------------------------------------------------
 //
 // A cluster of `split` CTAs per tile of 128 channels x bn tokens, each with its
-// share of the columns; their sums meet in shared memory, every CTA adding up
-// the tokens t % split = its rank out of the others' (integers: no order).
+// share of the columns; every CTA adds up the sums of a share of the tokens,
+// which the others have put into its shared memory (integers: no order).
 
 // (ADD: its code and registers apart; what adds nothing took one to two percent longer with them.)
 template <bool ADD>
@@ -333,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 	extern __shared__ uint8_t raw[];
 	__shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], done;
 	__shared__ uint32_t tmem_slot;
-	__shared__ float xs_s[256];
+	__shared__ float xs_s[256], channel_s[2][128];
 	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	const int split = a.split, rank = (int)blockIdx.x % split; // (clusters lie along x)
@@ -342,6 +360,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 	const int k0 = (int)((long long)a.n_kb * rank / split), n = (int)((long long)a.n_kb * (rank + 1) / split) - k0;
 	const uint32_t x_at = W_BYTES * a.panels, stage = x_at + a.bn * KB * a.panels, cols = pow2_cols(a.bn);
 	const int real = min(a.bn, a.n_tok - t0);
+	const Join join{smem_u32(smem) + a.stages * stage, split, rank, (a.bn + split - 1) / split, 0, 1};
 
 	if (threadIdx.x == 0)
 	{
@@ -356,6 +375,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 	__syncthreads();
 	tc_fence_after();
 	const uint32_t tmem = tmem_slot;
+	if (split > 1) cluster_sync(); // all have begun: their memory may be written
 	griddep_launch_dependents();
 	griddep_wait(); // what came before on the stream is done: up to here nothing was read that it may write
 
@@ -404,23 +424,19 @@ __global__ void __launch_bounds__(THREADS, 2)
 	else
 	{
 		const int ch = (warp & 3) * 32 + lane, o = o0 + ch;
-		const bool in = o < a.rows && split == 1;
+		const bool in = o < a.rows;
 		const float ws = in ? a.ws[o] : 0.0f, bias = in && a.bias ? a.bias[o] : 0.0f;
+		if (split > 1 && warp < 6) channel_s[0][ch] = ws, channel_s[1][ch] = bias;
 		for (int c = (int)threadIdx.x - 64; c < a.bn; c += EPI) xs_s[c] = c < real ? a.xs[t0 + c] : 0.0f;
-		if (ADD) add_ahead(a, o0, t0, real, rank, split);
+		if (ADD) add_ahead(a, o0, t0, join.from(), join.to(real));
 		named_sync(1, EPI);
 		const bool ok = wait(&done, 0);
 		tc_fence_after();
-		if (__all_sync(0xffffffffu, ok)) tile_out<ADD>(a, tmem, ch, o, t0, real, xs_s, ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
+		if (__all_sync(0xffffffffu, ok)) tile_out<ADD>(a, tmem, ch, o, t0, real, xs_s, ws, bias, join);
 		tc_fence_before();
 	}
 	__syncthreads();
-	if (split > 1)
-	{
-		cluster_sync();
-		join_out<ADD>(a, reinterpret_cast<const int*>(smem), 0, 1, split, rank, split, o0, t0, real, xs_s);
-		cluster_sync(); // nobody reads this CTA's sums any more
-	}
+	if (split > 1) join_out<ADD>(a, join, reinterpret_cast<const int*>(smem + a.stages * stage), o0, t0, real, xs_s, channel_s, cluster_sync);
 	if (warp == 1)
 	{
 		tc_fence_after();
@@ -442,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 	extern __shared__ uint8_t raw[];
 	__shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2];
 	__shared__ uint32_t tmem_slot;
-	__shared__ float xs_s[2][256];
+	__shared__ float xs_s[2][256], channel_s[2][128];
 	uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
 	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 	const int split = a.split, in_cluster = (int)blockIdx.x % (2 * split), rank = in_cluster & 1, first = in_cluster - rank, part = in_cluster >> 1;
@@ -450,6 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 	const int k0 = (int)((long long)a.n_kb * part / split), n_kb = (int)((long long)a.n_kb * (part + 1) / split) - k0;
 	const int tiles = a.tiles_o * a.tiles_t, half = a.bn / 2;
 	const uint32_t x_at = W_BYTES * a.panels, stage = x_at + half * KB * a.panels;
+	const Join join{smem_u32(smem) + a.stages * stage, split, part, (a.bn + split - 1) / split, rank, 2};
 
 	if (threadIdx.x == 0)
 	{
@@ -541,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 			if (!ADD || id >= tiles) return;
 			int o0, t0;
 			place(a, id, 256, o0, t0);
-			add_ahead(a, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), part, split);
+			add_ahead(a, o0 + rank * 128, t0, join.from(), join.to(min(a.bn, a.n_tok - t0)));
 		};
 		ahead(pair);
 		for (int id = pair; id < tiles; id += pairs, ++n)
@@ -551,29 +568,31 @@ __global__ void __launch_bounds__(THREADS, 1)
 			place(a, id, 256, o0, t0);
 			ahead(id + pairs);
 			const int o = o0 + rank * 128 + ch, real = min(a.bn, a.n_tok - t0);
-			const bool in = o < a.rows && split == 1;
+			const bool in = o < a.rows;
 			const float ws = in ? a.ws[o] : 0.0f, bias = in && a.bias ? a.bias[o] : 0.0f;
+			if (split > 1 && warp < 6) channel_s[0][ch] = ws, channel_s[1][ch] = bias;
 			// (a warp is at most one tile behind another: the barrier below lets none two ahead)
 			for (int c = (int)threadIdx.x - 64; c < a.bn; c += EPI) xs_s[b][c] = c < real ? a.xs[t0 + c] : 0.0f;
 			named_sync(1, EPI);
 			ok = __all_sync(0xffffffffu, ok && wait(&acc_full[b], (uint32_t)(n / 2) & 1));
 			if (!ok) continue;
 			tc_fence_after();
-			tile_out<ADD>(a, tmem + b * 256, ch, o, t0, real, xs_s[b], ws, bias, split > 1 ? reinterpret_cast<int*>(smem) : nullptr);
+			tile_out<ADD>(a, tmem + b * 256, ch, o, t0, real, xs_s[b], ws, bias, join);
 			tc_fence_before();
 			__syncwarp();
 			if (lane == 0) arrive_cluster(mapa(smem_u32(&acc_empty[b]), first));
 		}
 	}
 	__syncthreads();
-	cluster_sync(); // the other CTA's products read this one's memory, its epilogue arrives here
+	// (the barrier also for this: the other CTA's products read this one's memory, its epilogue arrives here)
 	if (split > 1) // (one tile a cluster)
 	{
 		int o0, t0;
 		place(a, pair, 256, o0, t0);
-		join_out<ADD>(a, reinterpret_cast<const int*>(smem), rank, 2, split, part, split, o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), xs_s[0]);
-		cluster_sync(); // nobody reads this CTA's sums any more
+		join_out<ADD>(a, join, reinterpret_cast<const int*>(smem + a.stages * stage), o0 + rank * 128, t0, min(a.bn, a.n_tok - t0), xs_s[0], channel_s, cluster_sync);
 	}
+	else
+		cluster_sync();
 	if (warp == 1)
 	{
 		tc_fence_after();
@@ -634,6 +653,9 @@ int configure()
 
 constexpr int SMS = 148;
 
+// The sums that a CTA takes of its share of a tile's tokens, from all that share the tile's columns.
+constexpr int join_bytes(int bn, int split) { return split > 1 ? (bn + split - 1) / split * split * 512 : 0; }
+
 struct Plan
 {
 	bool pair;
@@ -644,12 +666,12 @@ struct Plan
 // Which kernel, how many tokens a tile, over how many CTAs (pairs) a tile's columns are split, one or two panels a
 // stage, one CTA per SM or two (of half the memory): the least of an estimate in SM cycles. Its constants were
 // fitted to 7000 timings of 180 shapes (1 to 4096 tokens, 128 to 262144 channels, 300 to 16384 columns, weights from
-// HBM); the choices it makes there are 1.9 % slower than the best of all in the mean, 14 % at worst. What they stand for:
-//  - a panel costs the issue of its copies and products (500 alone, 82 where two go together), its products (a pair's
-//    81 + 2.17 a token, a single CTA's four of 56.5 or 44 + 0.36 a token), its bytes into an SM (62 a cycle) or, over
-//    all SMs, out of L2 (8250 a cycle), whichever is the most;
+// HBM); the choices it makes there are 2.2 % slower than the best of all in the mean, 27 % at worst (200 x
+// 4096 to 128: 4.7 us, 3.7 with half the tiles). What they stand for:
+//  - a panel costs the issue of its copies and products (435 alone, 89 where two go together), its products (a pair's
+//    107 + 1.75 a token, a single CTA's four of 49.3 or 44 + 0.36 a token), its bytes into an SM (64 a cycle) or, over
+//    all SMs, out of L2 (10500 a cycle), or a copy's way (2670) by the panels in flight, whichever is the most;
 //  - clusters of 4 and more do not fill every SM;
-//  - the weights come from HBM at 3300 bytes a cycle;
 //  - a launch has a start and an end, and so has each CTA that runs alone on its SM after another; there is an epilogue
 //    by token, and a split tile has the joining of its parts.
 // Both sides, microseconds: 1 token, 6144 channels, 4096 columns: whole columns, two panels 7.5, one panel 8.8, split
@@ -659,33 +681,34 @@ Plan make_plan(int n_tok, int rows, int n_kb)
 {
 	// how many clusters run at once with one CTA per SM and with two, by CTAs of a cluster
 	static const int alone[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15}, both[9] = {0, 296, 148, 93, 71, 56, 45, 37, 33};
-	const double from_hbm = (double)rows * n_kb * KB * (1 / 3300.0);
 	const auto larger = [](double a, double b) { return a > b ? a : b; };
 	Plan best{};
 	double least = INFINITY;
-	// (two hundred estimates a call: what does not go by the innermost choice is worked out outside of it)
+	// (some hundred estimates a call: what does not go by the innermost choice is worked out outside of it)
 	const auto consider = [&](bool pair, int bn, int tiles_o) {
-		const int tiles_t = (n_tok + bn - 1) / bn;
-		const double tiles = (double)tiles_o * tiles_t;
-		const double bytes = (128 + (pair ? bn / 2 : bn)) * 128.0, ends = pair ? 7800 : 4770, epilogue = (pair ? 9.2 : 14.2) * bn;
-		for (int split = 1; split <= (pair ? 4 : 8) && split <= n_kb; split += pair ? 1 : split)
+		const int tiles_t = (n_tok + bn - 1) / bn, one = W_BYTES + (pair ? bn / 2 : bn) * KB; // bytes of a panel
+		const double tiles = (double)tiles_o * tiles_t, ends = pair ? 9600 : 3790, epilogue = (pair ? 9.4 : 18.7) * bn;
+		for (int split = 1; split <= (pair ? 4 : 8) && split <= n_kb; split += split < 4 ? 1 : 2)
 		{
 			const int ctas = (pair ? 2 : 1) * split;
-			const double kb = (n_kb + split - 1) / split, join = split > 1 ? 3300 + 82 * bn : 0;
+			if (split > 1 && tiles > 2 * both[ctas]) break;
+			const double kb = (n_kb + split - 1) / split, join = split > 1 ? 4090 + 43.6 * bn : 0;
+			const int sums = join_bytes(bn, split);
 			for (int two = 0; two < (pair ? 1 : 2); ++two)
 			{
-				const int smem = two ? 107 * 1024 : SMEM_MOST, slots = two ? both[ctas] : alone[ctas];
-				if (split > 1 && tiles > 2 * slots) continue;
+				const int smem = two ? 107 * 1024 : SMEM_MOST, slots = two ? both[ctas] : alone[ctas], fit = min(MAX_STAGES, (smem - 1024 - sums) / one);
+				if (fit < 2 || (split > 1 && tiles > 2 * slots)) continue;
 				const double waves = tiles <= slots ? 1 : tiles <= 2 * slots ? 2 : (double)(((long long)tiles + slots - 1) / slots);
 				const double per_sm = two && tiles > alone[ctas] ? 2 : 1;
-				const double products = pair ? 81 + 2.17 * bn : 4 * larger(56.5, 44 + 0.36 * bn) * per_sm;
-				const double load = bytes * larger(per_sm * (1 / 62.0), (tiles < slots ? tiles : slots) * ctas * (1 / 8250.0));
-				const double panel = larger(products, load), rest = ends + (pair || two ? 0 : 3000 * (waves - 1)) + epilogue * waves * (split > 1 ? 0.5 : 1) + join;
+				const double products = pair ? 107 + 1.75 * bn : 4 * larger(49.3, 44 + 0.36 * bn) * per_sm;
+				const double load = one * larger(per_sm * (1 / 64.0), (tiles < slots ? tiles : slots) * ctas * (1 / 10500.0));
+				const double rest = ends + (pair || two ? 0 : 3390 * (waves - 1)) + epilogue * waves * (split > 1 ? 0.5 : 1) + join;
 				for (int panels = 1; panels <= 2 && split * panels <= n_kb; ++panels)
 				{
-					const int stage = (W_BYTES + (pair ? bn / 2 : bn) * KB) * panels;
-					if (smem - 1024 < (panels > 1 ? 3 : 2) * stage) continue;
-					const double t = larger(waves * kb * larger(panels > 1 ? 82 : 500, panel), from_hbm) + rest;
+					const int stages = panels == 1 ? fit : min(MAX_STAGES, (smem - 1024 - sums) / (2 * one));
+					if (stages < panels + 1) continue;
+					const double panel = larger(larger(products, load), larger(panels > 1 ? 89 : 435, 2670.0 / (panels * stages)));
+					const double t = waves * kb * panel + rest;
 					if (t < least) least = t, best = {pair, bn, split, panels, tiles_o, tiles_t, smem};
 				}
 			}
@@ -712,7 +735,8 @@ int launch_i8_linear(const nncu_i8_linear& l, void* stream)
 	const Plan p = make_plan(l.n_tok, l.rows, (l.cols + KB - 1) / KB);
 	a.bn = p.bn, a.split = p.split, a.panels = p.panels, a.n_kb = (l.cols + KB * p.panels - 1) / (KB * p.panels);
 	const int stage = (W_BYTES + (p.pair ? p.bn / 2 : p.bn) * KB) * p.panels;
-	a.stages = min(MAX_STAGES, (p.smem - 1024) / stage);
+	const int join = join_bytes(p.bn, p.split);
+	a.stages = min(MAX_STAGES, (p.smem - 1024 - join) / stage);
 	CUtensorMap xm, wm;
 	if (!code_map(&xm, l.x, l.n_tok, l.cols, l.x_stride, p.pair ? p.bn / 2 : p.bn) ||
 	    !code_map(&wm, l.w, l.rows, l.cols, l.w_stride, 128))
@@ -728,7 +752,7 @@ int launch_i8_linear(const nncu_i8_linear& l, void* stream)
 	cfg.attrs = at;
 	cfg.numAttrs = at[1].val.clusterDim.x > 1 ? 2 : 1;
 	cfg.blockDim = dim3(THREADS);
-	cfg.dynamicSmemBytes = max(a.stages * stage, p.split > 1 ? p.bn * 512 : 0) + 1024;
+	cfg.dynamicSmemBytes = a.stages * stage + join + 1024;
 	const long long tiles = (long long)p.tiles_o * p.tiles_t;
 	if (p.pair)
 	{
