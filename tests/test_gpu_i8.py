@@ -193,6 +193,10 @@ LINEAR = [  # tokens, rows, cols, bias, add (2: y itself), values between rows o
     (300, 4096, 2560, 0, 1, 0), (777, 2560, 2048, 1, 0, 0), (1000, 100, 96, 0, 0, 0), (1025, 1537, 130, 1, 1, 1),
     (200, 2560, 10240, 0, 1, 0), (520, 2000, 20000, 1, 0, 1), (333, 515, 9000, 1, 2, 1), (1500, 300, 16384, 0, 0, 0),
     (200, 20480, 300, 0, 0, 0), (4099, 6200, 300, 1, 0, 3),
+    (53, 6961, 10665, 1, 1, 0), (1, 5940, 7068, 0, 2, 0), (1, 10436, 9584, 1, 1, 1), (2793, 17, 7489, 0, 1, 0),
+    (1, 2912, 4032, 1, 2, 0), (2538, 20, 6169, 1, 1, 2), (1367, 16, 6873, 0, 0, 0), (1187, 18, 7366, 1, 1, 0),
+    (363, 6513, 2729, 0, 1, 1), (155, 9877, 3828, 1, 2, 0), (383, 1993, 14475, 1, 1, 1), (50, 7333, 14773, 0, 2, 0),
+    (2498, 147, 14681, 1, 1, 0), (49, 4725, 21378, 1, 0, 2), (1910, 165, 14429, 0, 2, 1), (57, 2895, 27905, 1, 1, 0),
     (600, 5000, 130, 1, 1, 3), (270, 9000, 64, 0, 2, 0), (2050, 1300, 3000, 1, 1, 2), (2050, 1300, 3000, 0, 2, 0), (900, 700, 640, 0, 1, 0),
     (2500, 40, 700, 0, 0, 0), (2048, 2048, 1024, 0, 0, 0), (5, 40000, 200, 0, 0, 0), (2, 3, 131071, 0, 0, 0),
     (40, 16, 100000, 0, 0, 0), (4100, 130, 16, 1, 2, 2),
