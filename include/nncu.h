@@ -583,10 +583,10 @@ typedef struct nncu_i8_lookup
 int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream);
 
 /* y[t][o] = x_scales[t] * w_scales[o] * sum_c x[t][c] * w[o][c] + bias[o] +
- * add[t][o] for n_tok tokens and `rows` channels. The sum is exact (32-bit
- * integers: cols up to 131071; n_tok and rows up to 2^30), so nothing of a result goes by the other
- * tokens of its call. bias and add NULL: none; add may be y (a residual stream in
- * place), otherwise y meets none of the inputs. */
+ * add[t][o] for n_tok tokens and `rows` channels (up to 2^30 each, 2^36 as a
+ * product). The sum is exact (32-bit integers: cols up to 131071), so nothing of
+ * a result goes by the other tokens of its call. bias and add NULL: none; add may
+ * be y (a residual stream in place), otherwise y meets none of the inputs. */
 typedef struct nncu_i8_linear
 {
 	int32_t n_tok, rows, cols;

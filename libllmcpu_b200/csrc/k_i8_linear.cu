@@ -13,7 +13,7 @@
 //
 // Few tokens are bound by the weights' bytes (16 x 2560 to 262144 channels: 104
 // us, the copy rate) and, where the weights are small, by the chain of launch,
-// first copies, stages and epilogue (1 x 4096 to 6144: 6.1 us of 3.8); many by
+// first copies, stages and epilogue (1 x 4096 to 6144: 6.0 us of 3.8); many by
 // the products, the copies out of L2 and the card's power (8192 x 4096 to 6144:
 // 140 us, the tensor pipe 80 % busy at 1.66 GHz).
 #include <cuda.h>

@@ -18,8 +18,8 @@
 //
 // Bound by memory where rows are many (2047 x 128256: 159 us, the copy rate); a
 // row is shared by up to eight CTAs (a cluster, whose parts meet in the first
-// one's shared memory) where they are few: 64 x 151936 with 5 alternatives 13.2
-// us (the copy rate: 5.9), 1 x 262144 with 20 7.9 us. Their ends are short chains:
+// one's shared memory) where they are few: 64 x 151936 with 5 alternatives 12.8
+// us (the copy rate: 5.9), 1 x 262144 with 20 8.0 us. Their ends are short chains:
 // the largest first (redux), then sums; every warp's parts straight to the first
 // CTA; a thread's group read again while its sums are joined; runs merged by
 // counting (14.4 and 8.9 us with pairwise joins and bitonic merges of the parts).
