@@ -56,8 +56,9 @@ constexpr int LP_TOP = 32;
 constexpr int LP_ITEMS = 4;   // 16-byte loads a thread has in flight
 constexpr int LP_CLUSTER = 8; // the most CTAs that share a row
 constexpr int LP_FIRST = 4;   // of each warp's candidates, those that bound the others
-constexpr int LP_WIDE = 512, LP_NARROW = 256;      // threads of a CTA: where rows are few, and where they are many
-constexpr int LP_WIDE_CTAS = 2, LP_NARROW_CTAS = 5; // per SM
+constexpr int LP_WIDE = 512, LP_NARROW = 256; // threads of a CTA: where rows are few, and where they are many
+// CTAs per SM.
+constexpr int lp_ctas(int threads, bool ahead) { return threads == LP_WIDE ? 2 : ahead ? 4 : 5; }
 
 using Key = unsigned long long;
 
@@ -356,8 +357,8 @@ __device__ __forceinline__ void lp_merge_parts(R& row, int parts, int lane, int 
 	if (k != 0 && n < LP_TOP) row.all[n] = k;
 }
 
-template <bool TOP, int T>
-__global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTAS) logprobs_kernel(const LpArgs a)
+template <bool TOP, int T, bool AHEAD>
+__global__ void __launch_bounds__(T, lp_ctas(T, AHEAD)) logprobs_kernel(const LpArgs a)
 {
 	constexpr int WARPS = T / 32, GROUP = T * LP_ITEMS; // vectors (of four logits) that the CTA takes at a time
 	static_assert(WARPS >= LP_CLUSTER && WARPS <= 32, "a warp a part, a lane a warp");
@@ -386,9 +387,9 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 	Stat s{-FLT_MAX, 0.0f, 0.0f};
 	int before = 0;
 	Best best{-INFINITY, -INFINITY, sh.v0};
-	// Wide CTAs have the next group's loads in flight while they count one (64 x 151936 top 5: 13.2 us, without 13.7);
-	// narrow ones, five to an SM, have no registers for it (four to an SM with them: 300 x 50257 17.7 us, 15.9 without).
-	constexpr bool AHEAD = T == LP_WIDE;
+	// AHEAD: the next group's loads are in flight while one is counted (wide, 64 x 151936 top 5: 13.2 us, without 13.7;
+	// narrow, 450 x 43807 17.4, without 20.7). The registers for it cost the fifth narrow CTA of an SM (700 x 43807: 29.1 us,
+	// five without it 23.7).
 	float next[4 * LP_ITEMS];
 	for (int g = sh.v0; g < sh.v1;)
 	{
@@ -510,32 +511,41 @@ __global__ void __launch_bounds__(T, T == LP_WIDE ? LP_WIDE_CTAS : LP_NARROW_CTA
 
 struct LpPlan
 {
-	bool wide;
+	bool wide, ahead;
 	int parts; // CTAs that share a row
 };
 
 // The least of an estimate, in SM cycles: the waves that the CTAs make of what the GPU holds at once (clusters do not
 // fill every SM) times a CTA's start and end and its share, at a pace of its own or, with others on its SM, at a share
-// of the SM's. Its constants were fitted to 1900 timings (1 to 2000 rows of 5000 to 262144 logits, from HBM); its
-// choices are 0.9 % slower there than the best of all in the mean, 19 % at worst. Both sides, microseconds, with 5
-// alternatives: 64 rows of 151936: wide CTAs, four a row 13.6, narrow ones 17.1; 2000 rows: wide ones 212, narrow ones
-// 216 (without alternatives 202 and 186); 1 x 262144: eight wide CTAs 6.9, one 20.4.
+// of the SM's. Its constants were fitted to 2600 timings (1 to 2000 rows of 5000 to 162275 logits, from HBM); its
+// choices are 0.3 % slower there than the best of all in the mean, 8 % at worst. Both sides, microseconds, with 5
+// alternatives: 64 rows of 151936: wide CTAs, four a row 13.6, narrow ones 17.1; 1 x 262144: eight wide CTAs 6.9, one
+// 20.4; 450 rows of 43807: narrow CTAs 24.3, with loads ahead 20.2, wide ones 25; 700 rows: 29.2 and 32.8.
 LpPlan lp_plan(long long n, int n_vocab, bool top)
 {
+	struct Kind
+	{
+		bool wide, ahead;
+		double ends, top_ends, join, top_join, pace; // cycles a CTA, and a logit
+		int all_of_8; // SMs that clusters of eight fill
+	};
+	const Kind kinds[] = {{true, true, 3310, 2170, 443, 190, 0.098, top ? 124 : 132},
+	                      {false, true, 3560, 2210, 183, 290, 0.192, top ? 132 : 136},
+	                      {false, false, 3520, 4150, 320, 90, 0.259, 132}};
 	LpPlan best{};
-	double least = 0;
-	for (int wide = 1; wide >= 0; --wide)
+	double least = INFINITY;
+	for (const Kind& k : kinds)
 		for (int i = 0, parts = 1; parts <= LP_CLUSTER; ++i, parts *= 2)
 		{
-			const int filled[] = {148, 148, 142, wide && top ? 124 : 132}; // SMs that clusters of 1, 2, 4, 8 fill
-			const double slots = filled[i] * (wide ? LP_WIDE_CTAS : LP_NARROW_CTAS), ctas = (double)n * parts;
+			const int filled[] = {148, 148, 142, k.all_of_8}; // SMs that clusters of 1, 2, 4, 8 fill
+			const double slots = filled[i] * lp_ctas(k.wide ? LP_WIDE : LP_NARROW, k.ahead), ctas = (double)n * parts;
 			const double beside = fmax(1.0, fmin(ctas, slots) / 148);
-			double ends = wide ? 3310 : 3560;
-			if (top) ends += wide ? 1450 : 3600;
-			if (parts > 1) ends += (wide ? 443 : 320) + (top ? 200 : 0);
-			const double pace = fmax(wide ? 0.098 : 0.256, 0.045 * beside); // cycles a logit
-			const double t = ceil(ctas / slots) * (ends * fmax(1.0, 0.163 * beside) + pace * n_vocab / parts);
-			if (best.parts == 0 || t < least) least = t, best = {wide != 0, parts};
+			double ends = k.ends;
+			if (top) ends += k.top_ends;
+			if (parts > 1) ends += k.join + (top ? k.top_join : 0);
+			const double pace = fmax(k.pace, 0.045 * beside);
+			const double t = ceil(ctas / slots) * (ends * fmax(1.0, 0.145 * beside) + pace * n_vocab / parts);
+			if (t < least) least = t, best = {k.wide, k.ahead, parts};
 		}
 	return best;
 }
@@ -597,8 +607,9 @@ extern "C" int nncu_logprobs_dev(const nncu_logprobs* l, void* stream)
 	{
 		const long long rows = left < most ? left : most;
 		cfg.gridDim = dim3((unsigned)(rows * a.parts));
-		const auto kernel = plan.wide ? (tops ? logprobs_kernel<true, LP_WIDE> : logprobs_kernel<false, LP_WIDE>)
-		                              : (tops ? logprobs_kernel<true, LP_NARROW> : logprobs_kernel<false, LP_NARROW>);
+		const auto kernel = plan.wide    ? (tops ? logprobs_kernel<true, LP_WIDE, true> : logprobs_kernel<false, LP_WIDE, true>)
+		                    : plan.ahead ? (tops ? logprobs_kernel<true, LP_NARROW, true> : logprobs_kernel<false, LP_NARROW, true>)
+		                                 : (tops ? logprobs_kernel<true, LP_NARROW, false> : logprobs_kernel<false, LP_NARROW, false>);
 		e = (int)cudaLaunchKernelEx(&cfg, kernel, a);
 		note_launches(1);
 		a.l.logits += (size_t)rows * a.l.stride;

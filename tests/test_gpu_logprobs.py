@@ -50,6 +50,9 @@ CASES = [  # rows, vocabulary, top, scale, masked, logits in steps of a 16-bit f
     (1, 262144, 32, 1.0, 0, 0, 0, 0), (3, 262144, 20, 1.0, 0.99, 0, 0, 0), (64, 32000, 5, 1.25, 0.9, 1, 0, 0),
     (16, 128256, 0, 1.0, 0, 0, 0, 0), (40, 65537, 32, 1.0, 0, 1, 0, 0), (160, 20000, 1, 1.0, 0, 0, 0, 0),
     (300, 8193, 20, 1.0, 0.2, 0, 3, 1), (1, 500001, 7, 1.0, 0, 0, 0, 0),
+    (450, 5003, 5, 1.0, 0.3, 0, 1, 1), (400, 5000, 0, 0.8, 0, 1, 0, 0), (100, 33990, 0, 1.0, 0.5, 0, 2, 3),
+    (64, 43807, 9, 1.0, 0, 0, 0, 0), (340, 43807, 5, 1.0, 0, 1, 1, 2), (300, 33990, 0, 2.0, 0, 0, 0, 0), (700, 5001, 32, 1.0, 0.9, 1, 0, 0),
+    (150, 43807, 20, 1.0, 0.99, 0, 0, 0),
 ]
 
 
