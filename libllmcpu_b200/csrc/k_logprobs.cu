@@ -137,6 +137,8 @@ struct LpArgs
 };
 
 // A row's share of one CTA, in vectors of four logits that lie on 16 bytes: the row's first and last one may be cut.
+// (Ordinary loads: the kernel before this one may still write the logits when this one begins, so that they are not
+// read-only for its life, which a non-coherent load asks for.)
 struct Share
 {
 	const float* x;
@@ -154,13 +156,13 @@ struct Share
 	// what is not the share's reads as masked
 	__device__ __forceinline__ float4 load(int j) const
 	{
-		if (whole(j)) return __ldg(at(j));
+		if (whole(j)) return *at(j);
 		float v[4];
 #pragma unroll
 		for (int c = 0; c < 4; ++c)
 		{
 			const int i = index(j, c);
-			v[c] = j < v1 && i >= 0 && i < n ? __ldg(x + i) : -INFINITY;
+			v[c] = j < v1 && i >= 0 && i < n ? x[i] : -INFINITY;
 		}
 		return make_float4(v[0], v[1], v[2], v[3]);
 	}
@@ -173,7 +175,7 @@ struct Share
 #pragma unroll
 			for (int u = 0; u < LP_ITEMS; ++u)
 			{
-				const float4 q = __ldg(at(g + u * T + (int)threadIdx.x));
+				const float4 q = *at(g + u * T + (int)threadIdx.x);
 				v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
 			}
 		}
