@@ -735,13 +735,17 @@ def _fill_dev(s, shapes, **kw):
 
 def i8_rows(n: int, cols: int, x, codes, scales, gamma=None, norm: int = 0, eps: float = 1e-6, x_type=None,
             x_stride=None, code_stride=None) -> I8Rows:
-    """An nncu_i8_rows; x float32, bfloat16 or float16 rows (the type of a tensor is its own)."""
-    if hasattr(x, "dtype") and str(x.dtype).rpartition(".")[2] not in _X_TYPES:
-        raise ValueError(f"x: float32, bfloat16 or float16 rows are read, not {x.dtype}")
-    if x_type is None:
-        x_type = _X_TYPES[str(x.dtype).rpartition(".")[2]] if hasattr(x, "dtype") else KV_F32
+    """An nncu_i8_rows; x float32, bfloat16 or float16 rows (the type of a tensor is its own; x_type says it of a raw
+    pointer)."""
+    own = KV_F32 if x_type is None else x_type
+    if hasattr(x, "dtype"):
+        own = _X_TYPES.get(str(x.dtype).rpartition(".")[2])
+        if own is None:
+            raise ValueError(f"x: float32, bfloat16 or float16 rows are read, not {x.dtype}")
+        if x_type not in (None, own):
+            raise ValueError(f"x_type: {x_type} is not the type of x, {x.dtype}")
     return _fill_dev(I8Rows(), dict(x=(n, cols), codes=(n, cols), scales=(n, 1), gamma=(1, cols)), n=n, cols=cols,
-                     x_type=x_type, norm=int(norm), eps=eps, x=x, x_stride=_stride(x, x_stride, cols), gamma=gamma,
+                     x_type=own, norm=int(norm), eps=eps, x=x, x_stride=_stride(x, x_stride, cols), gamma=gamma,
                      codes=codes, code_stride=_stride(codes, code_stride, cols), scales=scales)
 
 
