@@ -730,6 +730,13 @@ def _fill_dev(s, shapes, **kw):
         one = v.ndim == 2 and name in _ROWS
         if (one and n > 0 and (v.shape[0] < n or v.shape[1] < row)) or (not one and v.numel() < n * row):
             raise ValueError(f"{name}: {tuple(v.shape)} is less than {n} x {row}")
+        if name not in _ROWS and v.ndim > 1 and n > 1 and row > 0:  # these are written side by side
+            if name.startswith("top_"):
+                apart = v.shape[-1] != row and v.numel() != n * row
+            else:
+                apart = v.shape[0] >= n and v.numel() != v.shape[0]
+            if apart:
+                raise ValueError(f"{name}: rows of {tuple(v.shape)} are not {row} long; they lie side by side")
     return _fill(s, **kw)
 
 

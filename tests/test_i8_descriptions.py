@@ -86,3 +86,35 @@ def test_a_tensor_says_its_type(dtype, own):
 def test_a_pointer_does_not():
     assert rows(x=1 << 24).x_type == N.KV_F32
     assert rows(x=1 << 24, x_type=N.KV_BF16).x_type == N.KV_BF16
+
+
+# ---- arrays without a stride -------------------------------------------------------------------
+
+def report(**kw):
+    return N.logprobs(**{**dict(n=6, n_vocab=100, logits=floats(6, 100), tokens=whole(6), logprob=floats(6), rank=whole(6),
+                                entropy=floats(6), top=5, top_ids=whole(6, 5), top_logprobs=floats(6, 5)), **kw})
+
+
+@pytest.mark.parametrize("name,make", [("top_ids", whole), ("top_logprobs", floats)])
+def test_rows_of_alternatives_are_as_long_as_asked(name, make):
+    for shape in ((6, 5), (9, 5), (30,), (2, 3, 5), (40,)):
+        report(**{name: make(*shape)})
+    for shape in ((6, 32), (6, 6), (2, 3, 32), (30, 2)):  # rows would be written 5 apart into longer ones
+        with pytest.raises(ValueError, match=name):
+            report(**{name: make(*shape)})
+    with pytest.raises(ValueError, match=name):
+        report(**{name: make(6, 4)})
+    report(**{name: make(6, 32)}, top=0)  # none are written
+    report(n=1, **{name: make(6, 32)})  # one row: at its place
+    report(top=1, top_ids=whole(2, 3), top_logprobs=floats(6, 1))
+    with pytest.raises(ValueError, match=name):
+        report(top=1, **{"top_ids": whole(6, 1), "top_logprobs": floats(6, 1), name: make(2, 3, 32)})
+
+
+@pytest.mark.parametrize("name,make", [("tokens", whole), ("rank", whole), ("logprob", floats), ("entropy", floats)])
+def test_vectors_lie_side_by_side(name, make):
+    for shape in ((6,), (9,), (6, 1), (1, 6), (2, 3), (3, 3)):
+        report(**{name: make(*shape)})
+    for shape in ((6, 2), (7, 32)):
+        with pytest.raises(ValueError, match=name):
+            report(**{name: make(*shape)})
