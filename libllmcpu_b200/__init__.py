@@ -713,10 +713,21 @@ _I8_TYPES = dict(codes="int8", x="int8", w="int8", tokens="int32", rank="int32",
                                   "logprob", "entropy", "top_logprobs"), "float32"))
 
 
-def _fill_dev(s, shapes, **kw):
+def _matrix(x):
+    """Rows as a matrix: without leading dimensions of one."""
+    while hasattr(x, "data_ptr") and x.ndim > 2 and x.shape[0] == 1:
+        x = x[0]
+    return x
+
+
+def _fill_dev(s, shapes, strides, **kw):
     """_fill for device tensors: their types, shapes (where a tensor says them) and devices agree with the call.
-    `shapes`: the rows and the values of a row (or the values, of a vector) that the call reaches."""
+    `shapes`: the rows and the values of a row (or the values, of a vector) that the call reaches. `strides`: of arrays
+    whose rows may lie apart the field that says how far, and what the caller gave for it."""
     device = None
+    for name, (field, given) in strides.items():
+        kw[name] = _matrix(kw[name])
+        kw[field] = _stride(kw[name], given, shapes[name][1])
     for name, v in kw.items():
         if not hasattr(v, "data_ptr"):
             continue
@@ -727,15 +738,15 @@ def _fill_dev(s, shapes, **kw):
             raise ValueError(f"{name}: on {v.device}; the call's arrays lie on one GPU")
         device = v.device
         n, row = shapes[name]
-        one = v.ndim == 2 and name in _ROWS
-        if (one and n > 0 and (v.shape[0] < n or v.shape[1] < row)) or (not one and v.numel() < n * row):
+        apart = v.ndim > 1 and name in strides  # rows: the first dimension's, of all values of the others
+        if (apart and n > 0 and (v.shape[0] < n or v.numel() < v.shape[0] * row)) or (not apart and v.numel() < n * row):
             raise ValueError(f"{name}: {tuple(v.shape)} is less than {n} x {row}")
-        if name not in _ROWS and v.ndim > 1 and n > 1 and row > 0:  # these are written side by side
+        if name not in strides and v.ndim > 1 and n > 1 and row > 0:  # these are written side by side
             if name.startswith("top_"):
-                apart = v.shape[-1] != row and v.numel() != n * row
+                other = v.shape[-1] != row and v.numel() != n * row
             else:
-                apart = v.shape[0] >= n and v.numel() != v.shape[0]
-            if apart:
+                other = v.shape[0] >= n and v.numel() != v.shape[0]
+            if other:
                 raise ValueError(f"{name}: rows of {tuple(v.shape)} are not {row} long; they lie side by side")
     return _fill(s, **kw)
 
@@ -751,9 +762,9 @@ def i8_rows(n: int, cols: int, x, codes, scales, gamma=None, norm: int = 0, eps:
             raise ValueError(f"x: float32, bfloat16 or float16 rows are read, not {x.dtype}")
         if x_type not in (None, own):
             raise ValueError(f"x_type: {x_type} is not the type of x, {x.dtype}")
-    return _fill_dev(I8Rows(), dict(x=(n, cols), codes=(n, cols), scales=(n, 1), gamma=(1, cols)), n=n, cols=cols,
-                     x_type=own, norm=int(norm), eps=eps, x=x, x_stride=_stride(x, x_stride, cols), gamma=gamma,
-                     codes=codes, code_stride=_stride(codes, code_stride, cols), scales=scales)
+    return _fill_dev(I8Rows(), dict(x=(n, cols), codes=(n, cols), scales=(n, 1), gamma=(1, cols)),
+                     dict(x=("x_stride", x_stride), codes=("code_stride", code_stride)), n=n, cols=cols, x_type=own,
+                     norm=int(norm), eps=eps, x=x, gamma=gamma, codes=codes, scales=scales)
 
 
 def i8_quantise_dev(r: I8Rows, stream=None) -> None:
@@ -764,10 +775,9 @@ def i8_quantise_dev(r: I8Rows, stream=None) -> None:
 def i8_lookup(n: int, cols: int, n_rows: int, codes, scales, out, ids=None, mult: float = 1.0, code_stride=None,
               out_stride=None) -> I8Lookup:
     """An nncu_i8_lookup: the rows `ids` (or each in turn) of an 8-bit table."""
-    return _fill_dev(I8Lookup(), dict(codes=(n_rows, cols), scales=(n_rows, 1), out=(n, cols), ids=(n, 1)), n=n,
-                     cols=cols, n_rows=n_rows, mult=mult, ids=ids, codes=codes,
-                     code_stride=_stride(codes, code_stride, cols), scales=scales, out=out,
-                     out_stride=_stride(out, out_stride, cols))
+    return _fill_dev(I8Lookup(), dict(codes=(n_rows, cols), scales=(n_rows, 1), out=(n, cols), ids=(n, 1)),
+                     dict(codes=("code_stride", code_stride), out=("out_stride", out_stride)), n=n, cols=cols,
+                     n_rows=n_rows, mult=mult, ids=ids, codes=codes, scales=scales, out=out)
 
 
 def i8_lookup_dev(l: I8Lookup, stream=None) -> None:
@@ -780,9 +790,10 @@ def i8_linear(n_tok: int, rows: int, cols: int, x, x_scales, w, w_scales, y, bia
     """An nncu_i8_linear: y = x w^T of n_tok tokens and `rows` channels."""
     return _fill_dev(I8Linear(), dict(x=(n_tok, cols), x_scales=(n_tok, 1), w=(rows, cols), w_scales=(rows, 1),
                                       bias=(rows, 1), add=(n_tok, rows), y=(n_tok, rows)),
-                     n_tok=n_tok, rows=rows, cols=cols, x=x, x_stride=_stride(x, x_stride, cols), x_scales=x_scales,
-                     w=w, w_stride=_stride(w, w_stride, cols), w_scales=w_scales, bias=bias, add=add,
-                     add_stride=_stride(add, add_stride, rows), y=y, y_stride=_stride(y, y_stride, rows))
+                     dict(x=("x_stride", x_stride), w=("w_stride", w_stride), add=("add_stride", add_stride),
+                          y=("y_stride", y_stride)),
+                     n_tok=n_tok, rows=rows, cols=cols, x=x, x_scales=x_scales, w=w, w_scales=w_scales, bias=bias,
+                     add=add, y=y)
 
 
 def i8_linear_dev(l: I8Linear, stream=None) -> None:
@@ -800,9 +811,9 @@ def logprobs(n: int, n_vocab: int, logits, scale: float = 1.0, tokens=None, logp
     """An nncu_logprobs: a given token's log probability and rank, the entropy and the `top` likeliest of each row."""
     return _fill_dev(Logprobs(), dict(logits=(n, n_vocab), top_ids=(n, top), top_logprobs=(n, top),
                                       **dict.fromkeys(("tokens", "logprob", "rank", "entropy"), (n, 1))),
-                     n=n, n_vocab=n_vocab, top=top, scale=scale, logits=logits,
-                     stride=_stride(logits, stride, n_vocab), tokens=tokens, logprob=logprob, rank=rank,
-                     entropy=entropy, top_ids=top_ids, top_logprobs=top_logprobs)
+                     dict(logits=("stride", stride)),
+                     n=n, n_vocab=n_vocab, top=top, scale=scale, logits=logits, tokens=tokens, logprob=logprob,
+                     rank=rank, entropy=entropy, top_ids=top_ids, top_logprobs=top_logprobs)
 
 
 def logprobs_dev(l: Logprobs, stream=None) -> None:

@@ -118,3 +118,35 @@ def test_vectors_lie_side_by_side(name, make):
     for shape in ((6, 2), (7, 32)):
         with pytest.raises(ValueError, match=name):
             report(**{name: make(*shape)})
+
+
+# ---- rows -----------------------------------------------------------------------------------------
+
+def lookup(**kw):
+    return N.i8_lookup(**{**dict(n=6, cols=100, n_rows=9, codes=codes(9, 112), scales=floats(9), out=floats(6, 100)), **kw})
+
+
+def linear(**kw):
+    return N.i8_linear(**{**dict(n_tok=6, rows=50, cols=100, x=codes(6, 112), x_scales=floats(6), w=codes(50, 112),
+                                 w_scales=floats(50), y=floats(6, 50), bias=floats(50), add=floats(6, 50)), **kw})
+
+
+# (an array of rows, its stride's field, how it is made, rows, values of a row)
+ROW_ARRAYS = [(rows, "x", "x_stride", floats, 4, 100), (rows, "codes", "code_stride", codes, 4, 112),
+              (lookup, "codes", "code_stride", codes, 9, 112), (lookup, "out", "out_stride", floats, 6, 100),
+              (linear, "x", "x_stride", codes, 6, 112), (linear, "w", "w_stride", codes, 50, 112),
+              (linear, "y", "y_stride", floats, 6, 50), (linear, "add", "add_stride", floats, 6, 50),
+              (report, "logits", "stride", floats, 6, 100)]
+
+
+@pytest.mark.parametrize("call,name,field,make,n,row", ROW_ARRAYS)
+def test_rows_of_more_dimensions(call, name, field, make, n, row):
+    given = lambda t: getattr(call(**{name: t}), field)  # noqa: E731
+    assert given(make(n, row)) == row and given(make(n + 3, row + 48)) == row + 48
+    assert given(make(1, n, row)) == row and given(make(1, 1, n, row)) == row  # a batch of one
+    assert given(make(1, n, row + 48)) == row + 48
+    assert given(make(n, 2, row // 2)) == row  # heads
+    # (a batch's rows would be read as far apart as its prompts are, past their end)
+    for shape in ((n // 2 + 1, 2, row), (n - 1, 3, row), (1, n - 1, row), (1, n, row // 4), (1, 1, n * row)):
+        with pytest.raises(ValueError, match=f"^{name}:"):
+            call(**{name: make(*shape)})
