@@ -741,6 +741,10 @@ def _fill_dev(s, shapes, strides, **kw):
         apart = v.ndim > 1 and name in strides  # rows: the first dimension's, of all values of the others
         if (apart and n > 0 and (v.shape[0] < n or v.numel() < v.shape[0] * row)) or (not apart and v.numel() < n * row):
             raise ValueError(f"{name}: {tuple(v.shape)} is less than {n} x {row}")
+        if name in strides and n > 0:  # (a stride that is given may reach further than a shape says)
+            field = strides[name][0]
+            if (n - 1) * kw[field] + row > v.untyped_storage().nbytes() // v.element_size() - v.storage_offset():
+                raise ValueError(f"{name}: {n} rows with a {field} of {kw[field]} reach past its memory")
         if name not in strides and v.ndim > 1 and n > 1 and row > 0:  # these are written side by side
             if name.startswith("top_"):
                 other = v.shape[-1] != row and v.numel() != n * row

@@ -150,3 +150,17 @@ def test_rows_of_more_dimensions(call, name, field, make, n, row):
     for shape in ((n // 2 + 1, 2, row), (n - 1, 3, row), (1, n - 1, row), (1, n, row // 4), (1, 1, n * row)):
         with pytest.raises(ValueError, match=f"^{name}:"):
             call(**{name: make(*shape)})
+
+
+@pytest.mark.parametrize("call,name,field,make,n,row", ROW_ARRAYS)
+def test_rows_end_within_their_memory(call, name, field, make, n, row):
+    used = 100 if row == 112 else row  # (what a call reads of a row of codes)
+    wide = row + 16
+    call(**{name: make((n - 1) * wide + used), field: wide})
+    call(**{name: make(n, row, stride=(wide, 1))})
+    call(**{name: make(n, used, stride=(row, 1)), field: row})
+    call(**{name: make(n, row, offset=5, memory=make(1).size * (5 + (n - 1) * wide + used)), field: wide})
+    for bad in (make((n - 1) * wide + used - 1), make(n, row), make(n * row),
+                make(n, row, offset=6, memory=make(1).size * (5 + (n - 1) * wide + used))):
+        with pytest.raises(ValueError, match=f"^{name}: .*{field} of {wide}"):
+            call(**{name: bad, field: wide})
