@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include <vector_types.h>
 
 struct nncu_group;  // split.cpp
@@ -222,9 +224,10 @@ struct JobPointers
 	const void* v_cache;
 };
 int check_alignment(const JobPointers& p, int job, const char* what);
-// NNCU_OK where `p` is memory of the current device; a refusal otherwise (a
-// kernel that reads another device's memory would fault the GPU).
-int check_current_device(const void* p, const char* what);
+// NNCU_OK where all `arrays` (NULL: none) are memory of the current device; a
+// refusal otherwise (a kernel that reads the host's or another device's memory
+// would fault the GPU).
+int check_current_device(std::initializer_list<const void*> arrays, const char* what);
 // Count kernels launched outside api.cpp (nncu_launch_count).
 void note_launches(int n);
 

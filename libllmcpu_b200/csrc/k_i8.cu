@@ -406,28 +406,32 @@ bool meet(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
 
 } // namespace
 
-int check_current_device(const void* p, const char* what)
+int check_current_device(std::initializer_list<const void*> arrays, const char* what)
 {
 	int dev = -1;
-	cudaPointerAttributes at;
 	cudaError_t ce = cudaGetDevice(&dev);
-	if (ce == cudaSuccess) ce = cudaPointerGetAttributes(&at, p);
-	if (ce != cudaSuccess)
+	for (const void* p : arrays)
 	{
-		cudaGetLastError();
-		return set_cuda_error((int)ce, what);
-	}
-	if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
-	{
-		char msg[120];
-		snprintf(msg, sizeof msg, "%s: the arrays must be device memory", what);
-		return refuse(msg);
-	}
-	if (at.device != dev)
-	{
-		char msg[120];
-		snprintf(msg, sizeof msg, "%s: the arrays lie on device %d, the current one is %d", what, at.device, dev);
-		return refuse(msg);
+		if (!p) continue;
+		cudaPointerAttributes at;
+		if (ce == cudaSuccess) ce = cudaPointerGetAttributes(&at, p);
+		if (ce != cudaSuccess)
+		{
+			cudaGetLastError();
+			return set_cuda_error((int)ce, what);
+		}
+		if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+		{
+			char msg[120];
+			snprintf(msg, sizeof msg, "%s: the arrays must be device memory", what);
+			return refuse(msg);
+		}
+		if (at.device != dev)
+		{
+			char msg[120];
+			snprintf(msg, sizeof msg, "%s: the arrays lie on device %d, the current one is %d", what, at.device, dev);
+			return refuse(msg);
+		}
 	}
 	return NNCU_OK;
 }
@@ -457,7 +461,7 @@ extern "C" int nncu_i8_quantise_dev(const nncu_i8_rows* r, void* stream)
 	           c = span_bytes(r->codes, r->n, r->code_stride, r->cols), s = span_bytes(r->scales, r->n, 4, 4);
 	if (meet(c, x) || meet(s, x) || meet(c, s) || meet(c, g) || meet(s, g))
 		return refuse("i8 quantise: codes and scales must not meet another array");
-	const int rc = check_current_device(r->codes, "i8 quantise");
+	const int rc = check_current_device({r->x, r->gamma, r->codes, r->scales}, "i8 quantise");
 	if (rc != NNCU_OK) return rc;
 	const auto st = static_cast<cudaStream_t>(stream);
 	const int e = r->x_type == NNCU_KV_F32    ? launch_quantise<float>(*r, st)
@@ -488,7 +492,7 @@ extern "C" int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream)
 	if (meet(o, span_bytes(l->codes, l->n_rows, l->code_stride, l->cols)) || meet(o, span_bytes(l->scales, l->n_rows, 4, 4)) ||
 	    meet(o, span_bytes(l->ids, l->n, 4, 4)))
 		return refuse("i8 lookup: out must not meet another array");
-	const int rc = check_current_device(l->out, "i8 lookup");
+	const int rc = check_current_device({l->ids, l->codes, l->scales, l->out}, "i8 lookup");
 	if (rc != NNCU_OK) return rc;
 	const int e = launch_lookup(*l, static_cast<cudaStream_t>(stream));
 	note_launches(1);
@@ -520,7 +524,7 @@ extern "C" int nncu_i8_linear_dev(const nncu_i8_linear* l, void* stream)
 	    meet(y, span_bytes(l->x_scales, l->n_tok, 4, 4)) || meet(y, span_bytes(l->w_scales, l->rows, 4, 4)) ||
 	    meet(y, span_bytes(l->bias, 1, 0, row)) || (!in_place && meet(y, span_bytes(l->add, l->n_tok, l->add_stride * 4, row))))
 		return refuse("i8 linear: y must not meet an input (add may be y itself)");
-	const int rc = check_current_device(l->y, "i8 linear");
+	const int rc = check_current_device({l->x, l->x_scales, l->w, l->w_scales, l->bias, l->add, l->y}, "i8 linear");
 	if (rc != NNCU_OK) return rc;
 	const int e = launch_i8_linear(*l, stream);
 	if (e) cudaGetLastError();

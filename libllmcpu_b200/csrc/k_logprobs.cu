@@ -587,10 +587,12 @@ extern "C" int nncu_logprobs_dev(const nncu_logprobs* l, void* stream)
 		for (int j = 0; j < i; ++j)
 			if (i > 1 && s[i].lo < s[j].hi && s[j].lo < s[i].hi) return refuse("logprobs: outputs must not meet another array");
 	}
-	const int rc = check_current_device(l->logits, "logprobs");
+	const bool tops = l->top > 0 && (l->top_ids || l->top_logprobs);
+	const int rc = check_current_device({l->logits, l->tokens, l->logprob, l->rank, l->entropy, tops ? l->top_ids : nullptr,
+	                                     tops ? l->top_logprobs : nullptr},
+	                                    "logprobs");
 	if (rc != NNCU_OK) return rc;
 	LpArgs a{*l, (float)fmin((double)l->scale * 1.44269504088896340736, (double)FLT_MAX), 1};
-	const bool tops = l->top > 0 && (l->top_ids || l->top_logprobs);
 	const LpPlan plan = lp_plan(l->n, l->n_vocab, tops);
 	a.parts = plan.parts;
 	cudaLaunchAttribute at[2]{};
