@@ -603,9 +603,12 @@ typedef struct nncu_i8_linear
 	size_t y_stride;
 } nncu_i8_linear;
 int nncu_i8_linear_dev(const nncu_i8_linear* l, void* stream);
-/* Wait for `stream` and report whether a product on the current device since
- * the last check had a bounded wait run out (NNCU_ERR_TIMEOUT: the outputs
- * since then are void); the word is then cleared. */
+/* Wait for `stream` and report whether a bounded wait of a product on the
+ * current device, on whichever stream, has run out since the last check of this
+ * stream (NNCU_ERR_TIMEOUT: what was computed since then is void). Each stream's
+ * check reports it once; none hides it from another's. No other stream is waited
+ * for (but as the legacy default stream does); a stream that is being captured is
+ * refused. */
 int nncu_i8_check(void* stream);
 
 /* Of n rows of logits (`stride` floats apart), p = softmax(scale * logits):

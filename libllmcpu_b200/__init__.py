@@ -806,7 +806,8 @@ def i8_linear_dev(l: I8Linear, stream=None) -> None:
 
 
 def i8_check(stream=None) -> None:
-    """nncu_i8_check: wait for `stream`; raise (ERR_TIMEOUT) if a product on the current device timed out."""
+    """nncu_i8_check: wait for `stream`; raise (ERR_TIMEOUT) if a product on the current device has timed out since the
+    last check of this stream."""
     _check(lib().nncu_i8_check(_stream(stream)))
 
 

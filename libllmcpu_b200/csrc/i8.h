@@ -8,7 +8,7 @@ namespace nncu
 
 // The product of checked arguments (k_i8_linear.cu); a cudaError_t value.
 int launch_i8_linear(const nncu_i8_linear& l, void* stream);
-// The current device's error word of the products, cleared where it is set; a cudaError_t value.
-int i8_error_word(int* word);
+// How many bounded waits of products ran out on the current device, read on `stream` and waited for; a cudaError_t value.
+int i8_waits_out(unsigned* count, void* stream);
 
 } // namespace nncu

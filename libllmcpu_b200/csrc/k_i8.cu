@@ -9,6 +9,7 @@
 
 #include "common.cuh"
 #include "i8.h"
+#include "i8_seen.h"
 
 namespace nncu
 {
@@ -534,9 +535,30 @@ extern "C" int nncu_i8_linear_dev(const nncu_i8_linear* l, void* stream)
 
 extern "C" int nncu_i8_check(void* stream)
 {
-	int word = 0;
-	cudaError_t ce = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
-	if (ce == cudaSuccess) ce = (cudaError_t)i8_error_word(&word);
-	if (ce != cudaSuccess) return set_cuda_error((int)ce, "i8 check");
-	return word ? set_error(NNCU_ERR_TIMEOUT, "an i8 product's bounded wait timed out; the outputs since the last check are void") : NNCU_OK;
+	static I8Seen seen;
+	const auto st = static_cast<cudaStream_t>(stream);
+	cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+	int dev = -1;
+	unsigned long long id = 0;
+	unsigned count = 0;
+	cudaError_t ce = cudaStreamIsCapturing(st, &capturing);
+	if (ce == cudaSuccess && capturing != cudaStreamCaptureStatusNone) return refuse("i8 check: the stream is being captured");
+	if (ce == cudaSuccess) ce = cudaGetDevice(&dev);
+	if (ce == cudaSuccess) ce = cudaStreamGetId(st, &id);
+	// (a capture of another stream, which these calls do not concern, would be ended by them in its mode)
+	cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+	if (ce == cudaSuccess) ce = cudaThreadExchangeStreamCaptureMode(&mode);
+	if (ce == cudaSuccess)
+	{
+		ce = (cudaError_t)i8_waits_out(&count, stream);
+		cudaThreadExchangeStreamCaptureMode(&mode);
+	}
+	if (ce != cudaSuccess)
+	{
+		cudaGetLastError();
+		return set_cuda_error((int)ce, "i8 check");
+	}
+	return seen.more(dev, id, count)
+	           ? set_error(NNCU_ERR_TIMEOUT, "an i8 product's bounded wait timed out; the outputs since this stream's last check are void")
+	           : NNCU_OK;
 }

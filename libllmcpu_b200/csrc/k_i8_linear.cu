@@ -33,7 +33,7 @@ constexpr int KB = 128;           // columns of a panel: one swizzled row
 constexpr int W_BYTES = 128 * KB; // a panel's 128 channels
 constexpr int MAX_STAGES = 12;
 
-__device__ int g_i8_error; // the first bounded wait that ran out
+__device__ unsigned g_i8_waits_out; // bounded waits that ran out
 
 struct Args
 {
@@ -143,7 +143,12 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
 {
 	asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, &g_i8_error, 1); }
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity)
+{
+	const bool ok = mbar_wait_bounded(bar, parity, nullptr, 0);
+	if (!ok) atomicAdd(&g_i8_waits_out, 1u);
+	return ok;
+}
 
 // A place of the ring of stages and the round that it is in (a division by the number of stages costs as much as a stage).
 struct Ring
@@ -763,11 +768,11 @@ int launch_i8_linear(const nncu_i8_linear& l, void* stream)
 	return (int)cudaLaunchKernelEx(&cfg, l.add ? i8_split_kernel<true> : i8_split_kernel<false>, xm, wm, a);
 }
 
-int i8_error_word(int* word)
+int i8_waits_out(unsigned* count, void* stream)
 {
-	cudaError_t ce = cudaMemcpyFromSymbol(word, g_i8_error, sizeof *word);
-	const int zero = 0;
-	if (ce == cudaSuccess && *word) ce = cudaMemcpyToSymbol(g_i8_error, &zero, sizeof zero);
+	const auto st = static_cast<cudaStream_t>(stream);
+	cudaError_t ce = cudaMemcpyFromSymbolAsync(count, g_i8_waits_out, sizeof *count, 0, cudaMemcpyDeviceToHost, st);
+	if (ce == cudaSuccess) ce = cudaStreamSynchronize(st);
 	return (int)ce;
 }
 

@@ -65,3 +65,32 @@ def test_chunks_scored_through_one_buffer_of_logits(nncu, torch_cuda, n, vocab, 
             for k, v in out.items():
                 assert torch.equal(v, one[k]), k
     N.i8_check()
+
+
+def test_a_check_keeps_to_its_stream(nncu, torch_cuda):
+    """While one stream is captured another one is checked; the captured one's own check is refused, and leaves the
+    capture as it is."""
+    torch, N = torch_cuda, nncu
+    rng = np.random.default_rng(1)
+    w, x = (code_rows(torch, rng.integers(-127, 128, (n, 64), dtype=np.int8), rng) for n in (40, 3))
+    y = torch.zeros(3, 40, device="cuda")
+    one = torch.ones(40, device="cuda")
+    call = N.i8_linear(n_tok=3, rows=40, cols=64, x=x, x_scales=one, w=w, w_scales=one, y=y)
+    other, stream = torch.cuda.Stream(), torch.cuda.Stream()
+    N.i8_linear_dev(call, other)
+    N.i8_check(other)
+    want = y.clone()
+    torch.cuda.synchronize()
+    y.zero_()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        N.i8_linear_dev(call, torch.cuda.current_stream())
+        N.i8_check(other)
+        with pytest.raises(N.NnncError, match="captured"):
+            N.i8_check(torch.cuda.current_stream())
+    assert not bool(y.any())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    N.i8_check(stream)
