@@ -393,17 +393,27 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // A stride that rows of `row` values fit, and whose product with a row's number stays far from 64 bits.
 bool fits(size_t stride, int row) { return stride >= (size_t)row && stride <= (size_t)1 << 38; }
 
-// The memory between the first byte of `n` rows and the last.
+// `n` rows of `row` bytes, and the memory between the first byte and the last.
 struct Span
 {
 	uintptr_t lo, hi;
+	size_t n, stride, row;
 };
 Span span_bytes(const void* p, size_t n, size_t stride, size_t row)
 {
 	const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-	return {a, p && n ? a + (n - 1) * stride + row : a};
+	return {a, p && n ? a + (n - 1) * stride + row : a, n, stride, row};
 }
-bool meet(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+// Whether two arrays have bytes in common. Rows equally far apart (or one row) may lie between the other's: columns of one
+// buffer.
+bool meet(const Span& a, const Span& b)
+{
+	if (a.hi <= b.lo || b.hi <= a.lo) return false;
+	const size_t stride = a.n > 1 ? a.stride : b.stride;
+	if ((a.n > 1 && b.n > 1 && a.stride != b.stride) || a.row > stride || b.row > stride) return true;
+	const size_t d = b.lo >= a.lo ? (b.lo - a.lo) % stride : (stride - (a.lo - b.lo) % stride) % stride; // b's place behind a's
+	return d < a.row || d + b.row > stride;
+}
 
 } // namespace
 

@@ -183,3 +183,23 @@ def test_logprobs(nncu, torch_cuda, case):
     some = np.setdiff1d(np.arange(n), some)  # the others: no call leaves one out
     assert np.isfinite(got["entropy"][some]).all() and (got["entropy"][some] > 0).all()
     assert (got["rank"][some] >= 0).all() and (got["rank"][some] < v).all()
+
+
+def test_columns_of_one_buffer(nncu, torch_cuda):
+    """What is added and what comes out in columns of one buffer, looked up into a third part of it, in between its rows."""
+    torch, N = torch_cuda, nncu
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for n, r, c in ((5, 40, 48), (300, 700, 256)):
+        x, w = codes(torch, g, n, c), codes(torch, g, r, c)
+        xs, ws = torch.rand(n, generator=g, device="cuda"), torch.rand(r, generator=g, device="cuda")
+        wide = torch.full((n, 2 * r + c + 10), -7.0, device="cuda")
+        wide[:, r:2 * r] = torch.randn(n, r, generator=g, device="cuda")
+        add, y, out = wide[:, r:2 * r], wide[:, :r], wide[:, 2 * r + 4:2 * r + 4 + c]
+        kept = add.clone()
+        N.i8_lookup_dev(N.i8_lookup(n=n, cols=c, n_rows=n, codes=x, scales=xs, out=out))
+        N.i8_linear_dev(N.i8_linear(n_tok=n, rows=r, cols=c, x=x, x_scales=xs, w=w, w_scales=ws, add=add, y=y))
+        N.i8_check()
+        assert torch.equal(add, kept) and torch.equal(out, x.float() * xs[:, None])
+        assert bool((wide[:, 2 * r:2 * r + 4] == -7).all()) and bool((wide[:, 2 * r + 4 + c:] == -7).all())
+        for a, want, tol in product(torch, x, xs, w, ws, None, kept):
+            assert bool(((y.double() - want).abs() <= tol).all())
