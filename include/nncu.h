@@ -585,8 +585,11 @@ int nncu_i8_lookup_dev(const nncu_i8_lookup* l, void* stream);
 /* y[t][o] = x_scales[t] * w_scales[o] * sum_c x[t][c] * w[o][c] + bias[o] +
  * add[t][o] for n_tok tokens and `rows` channels (up to 2^30 each, 2^36 as a
  * product). The sum is exact (32-bit integers: cols up to 131071), so nothing of
- * a result goes by the other tokens of its call. bias and add NULL: none; add may
- * be y (a residual stream in place), otherwise y meets none of the inputs. */
+ * a result goes by the other tokens of its call; it is rounded to a float, times
+ * x_scales, then (with bias, rounded once) times w_scales, so that it is infinite
+ * where sum * x_scales passes the range of floats. bias and add NULL: none; add may
+ * be y (a residual stream in place), otherwise no row of y meets an input (columns
+ * of one buffer, whose rows are equally far apart, do not meet). */
 typedef struct nncu_i8_linear
 {
 	int32_t n_tok, rows, cols;
@@ -620,8 +623,8 @@ int nncu_i8_check(void* stream);
  * -1 and their log probabilities -infinity. A row that is masked whole has
  * the entropy 0. A NaN or +infinity makes its row's log probabilities and entropy
  * NaN. A given token outside the vocabulary (a padded buffer's) gets
- * logprob 0 and rank -1. Outputs that are NULL are left out (tokens is needed
- * for logprob and rank). Device pointers, asynchronous on `stream`. */
+ * logprob 0 and rank -1. Outputs that are NULL are not written (tokens is needed
+ * for logprob and rank); a call takes about as long without them. Device pointers, asynchronous on `stream`. */
 typedef struct nncu_logprobs
 {
 	int32_t n, n_vocab, top; /* n_vocab: up to 2^30 */

@@ -23,16 +23,16 @@ constexpr float I8_TINY = 1.17549435e-38f; // 2^-126: the least step of a row's 
 
 // ---- quantise -------------------------------------------------------------------------
 //
-// Reads each value once and writes a byte: bound by memory, and by issue slots
-// as soon as a value costs more than a dozen instructions, so that values go
+// Reads each value once and writes a byte; a value costs more than a dozen
+// instructions, which memory does not hide, so that values go
 // in pairs (one instruction for two), borders are settled for all of a thread's
 // values at once, and the edges of a row are looked for once a thread. A row
 // stays in the registers of `per_row` threads (16-byte loads) between its
 // maximum and its codes; longer rows than a CTA holds are read twice. The
 // squares of the norm are summed in 64 bits: float inputs' never overflow, and
-// the scale is rounded once. 8191 x 2560 floats with gain and norm 23.6 us (the
-// copy rate: 16.0), of which the norm's conversions and the exact border are 6;
-// 16 values a thread and five CTAs of 256 threads per SM: with 32 values 51 us,
+// the scale is rounded once. 8191 x 2560 floats 18.8 us, with gain and norm 24.7
+// (the copy rate: 16.0), bf16 17.6 and 22.3 (9.6): 23 instructions a value, issue
+// slots 59 % busy. 16 values a thread and five CTAs of 256 threads per SM: with 32 values 51 us,
 // with four CTAs 27, with CTAs that stay and copy ahead 29.
 
 constexpr int Q_MOST = 256, Q_CTAS = 5; // threads of a row, and of a CTA; CTAs per SM
